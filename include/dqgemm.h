@@ -350,6 +350,64 @@ enum dq_dtype { DQ_DT_F16 = 0, DQ_DT_BF16 = 1, DQ_DT_I8 = 2, DQ_DT_F32 = 3, DQ_D
 int call_gemm_plain(const void* A, const void* B, void* C, void* Workspace, int M, int N, int K, int in_dtype,
                     int out_dtype, int trans_A, int trans_B, dq_stream_t stream);
 
+/* ---- around the projections: rotary positions, the paged key-value cache, attention of one new token -------- */
+
+/* The cache: keys and values [pages][kv_heads][page_size][head_dim], a head's page one contiguous piece; page_size a power
+ * of two from 8 to 1024, head_dim a multiple of 8, at most 256.  dtype (DQ_DT_F16 or DQ_DT_BF16) is that of everything
+ * outside of it; a 16-bit cache is of the same type.  An 8-bit cache has fp32 scales KScale / VScale
+ * [pages][kv_heads][page_size], one a token and head (NULL for 16 bit): value = code * scale.
+ * A slot is page * page_size + place; a sequence's row of PageTable [sequences][max_pages] (int32) names its pages in
+ * order.  Positions, slots, starts and lengths are int32 on the device.  What is out of range there never leaves the
+ * buffers: a slot outside of the cache is not written, a page id outside of it means that its tokens are not there, a
+ * position outside of the table gives NaN, a length counts up to max_pages * page_size. */
+enum dq_cache_format { DQ_CACHE_F16 = 0, DQ_CACHE_BF16 = 1, DQ_CACHE_FP8 = 2 /* OCP e4m3 */, DQ_CACHE_I8 = 3 };
+
+/* Rotary positions: Out = X rotated, X [tokens][row_stride] with heads * head_dim elements a row that count (row_stride a
+ * multiple of 8), Out [tokens][heads][head_dim], or X itself: then in place, with X's stride.  head_dim a multiple of 8, at
+ * most 512; the first rotary_dim (even) elements of a head turn, the others are copied.  Table [positions][rotary_dim] fp32:
+ * the cosines of a position's rotary_dim / 2 angles, then their sines (times a magnitude, where a scaled table has one).
+ * Half layout (interleaved 0): element i turns with i + rotary_dim / 2; interleaved: 2 i with 2 i + 1.  inverse: the sines
+ * negated, which is the gradient with respect to X, given that with respect to Out. */
+int call_rotary(const void* X, const void* Table, const void* Positions, void* Out, int tokens, int heads, int head_dim,
+                int rotary_dim, int positions, int row_stride, int interleaved, int inverse, int dtype, dq_stream_t stream);
+
+/* K, V [tokens][kv_heads][head_dim] into the cache at Slots [tokens].  8 bit: scale = a / top with a = max |x| of a token's
+ * head and top = 448 (fp8) or 127 (int8), code = round to nearest even of x * (top / a); a head with a < 2^-100 is stored as
+ * zeros with scale 0, one with an infinity or a NaN with a NaN scale.  Tokens of one call with the same slot: one of them. */
+int call_kv_cache_write(const void* K, const void* V, const void* Slots, void* KCache, void* VCache, void* KScale, void* VScale,
+                        int tokens, int kv_heads, int head_dim, int pages, int page_size, int dtype, int cache_format,
+                        dq_stream_t stream);
+
+/* call_rotary and call_kv_cache_write in one launch on the rows of a fused projection, QKV [tokens][heads + 2 * kv_heads]
+ * [head_dim]: Q [tokens][heads][head_dim] = the rotated queries; the rotated keys (quantised from fp32) and the values go
+ * into the cache. */
+int call_rotary_kv_cache_write(const void* QKV, const void* Table, const void* Positions, const void* Slots, void* Q, void* KCache,
+                               void* VCache, void* KScale, void* VScale, int tokens, int heads, int kv_heads, int head_dim,
+                               int rotary_dim, int positions, int pages, int page_size, int interleaved, int dtype,
+                               int cache_format, dq_stream_t stream);
+
+/* The cache read back: KV [2][tokens][kv_heads][head_dim] (keys, then values) = the first Starts[b + 1] - Starts[b] tokens of
+ * every sequence b, packed: rows Starts[b] .. Starts[b + 1] - 1, Starts [sequences + 1] ascending.  Rows that belong to no
+ * sequence, and tokens that are not there, are zeros. */
+int call_kv_cache_read(const void* KCache, const void* VCache, const void* KScale, const void* VScale, const void* PageTable,
+                       const void* Starts, void* KV, int sequences, int tokens, int kv_heads, int head_dim, int pages,
+                       int page_size, int max_pages, int dtype, int cache_format, dq_stream_t stream);
+
+/* Attention of one new token a sequence: Out [sequences][heads][head_dim] = softmax(scale * Q . K^T) V over the sequence's
+ * tokens Lengths[b] - window .. Lengths[b] - 1 (window 0: all), head h on key-value head h / (heads / kv_heads), head_dim 64,
+ * 80, 96, 112, 128, 160, 192 or 256.  Sinks [heads] fp32 or NULL: one more score a head, whose value is nothing.  Lse
+ * [sequences][heads] fp32 or NULL: the natural logarithm of the sum of e^score (sinks among them).  A sequence that sees no
+ * token gives zeros and Lse -inf (with a sink: the sink).  What lies in the cache beyond a sequence's length is never used,
+ * NaN or not.  Softmax and sums in fp32; results do not depend on timing.
+ * Workspace: dq_paged_attention_workspace_bytes(...) bytes, 16-byte aligned (0: none), contents undefined before and after,
+ * not to be shared by calls that overlap in time. */
+size_t dq_paged_attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim, int page_size, int max_pages);
+int call_paged_attention_decode(const void* Q, const void* KCache, const void* VCache, const void* KScale, const void* VScale,
+                                const void* PageTable, const void* Lengths, const void* Sinks, void* Out, void* Lse, void* Workspace,
+                                size_t workspace_bytes, int sequences, int heads, int kv_heads, int head_dim, int pages,
+                                int page_size, int max_pages, int window, int dtype, int cache_format, float scale,
+                                dq_stream_t stream);
+
 /* ---- diagnostics ------------------------------------------------------------------------------------- */
 
 /* The rate the matrix pipe sustains on the caller's operands, with no memory, LDS or decode work beside it: every

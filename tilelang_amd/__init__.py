@@ -26,6 +26,14 @@ from .kernels import (  # noqa: F401
     matmul_w4a16,
     quantize_bf16_mxfp4,
 )
+from .kv_kernels import (  # noqa: F401
+    kv_cache_read,
+    kv_cache_write,
+    paged_attention_decode,
+    rotary,
+    rotary_kv_cache_write,
+    rotary_table,
+)
 from .bitlinear import BitLinear  # noqa: F401
 from .w4linear import W4A16Linear  # noqa: F401
 from .profiler import Profiler, TensorSupplyType, do_bench  # noqa: F401

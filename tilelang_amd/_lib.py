@@ -51,6 +51,11 @@ SIGNATURES = {
     "call_mfma_rate": [_vp, _vp, _i, _i, _i, _vp],
     "dq_tile_rows": [_i, _i, _i, _i, _i, _i],
     "dq_kwaves_form": [_i, _i, _i, _i, _i, _i, _i],
+    "call_rotary": [_vp] * 4 + [_i] * 9 + [_vp],
+    "call_kv_cache_write": [_vp] * 7 + [_i] * 7 + [_vp],
+    "call_rotary_kv_cache_write": [_vp] * 9 + [_i] * 11 + [_vp],
+    "call_kv_cache_read": [_vp] * 7 + [_i] * 9 + [_vp],
+    "call_paged_attention_decode": [_vp] * 11 + [ctypes.c_size_t] + [_i] * 10 + [ctypes.c_float, _vp],
     "call_gemm_mxfp4_mxfp4": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
 }
 
@@ -62,6 +67,7 @@ SIZE_QUERIES = {
     "dq_w4a16_workspace_bytes": [_i, _i, _i, _i, _i],
     "dq_mxfp4_workspace_bytes": [_i, _i, _i],
     "dq_bitlinear_workspace_bytes": [_i, _i, _i, _i],
+    "dq_paged_attention_workspace_bytes": [_i] * 6,
 }
 
 

@@ -33,6 +33,13 @@ class KernelParam:
     shape: tuple
     #: packed sub-byte storage: the strict dtype check accepts int8 and uint8 alike
     packed: bool = False
+    #: element strides of a view that the kernel takes as it lies; None: contiguous
+    strides: tuple | None = None
+
+    def lies_as(self, t: torch.Tensor) -> bool:
+        if self.strides is None:
+            return t.is_contiguous()
+        return all(n == 1 or have == want for n, have, want in zip(self.shape, t.stride(), self.strides))
 
 
 #: torch's private call for the current stream of a GPU; None in a build of torch that has none
@@ -98,7 +105,7 @@ class KernelAdapter:
             return None
         entry, slots, ints, f, ws_bytes = self._native_spec
         roles = [2 if i in self.workspace_idx else 1 if i in result_idx else 0 for i in range(len(self.params))]
-        return host.bind(entry, tuple((p.dtype, int(p.packed), tuple(p.shape), role) for p, role in zip(self.params, roles)),
+        return host.bind(entry, tuple((p.dtype, int(p.packed), tuple(p.shape), tuple(p.strides or ()), role) for p, role in zip(self.params, roles)),
                          tuple(-1 if i is None else i for i in slots), tuple(ints), float(f), ws_bytes)
 
     # -- validation, same order and wording as the reference ------------------------------
@@ -111,7 +118,7 @@ class KernelAdapter:
             if isinstance(t, torch.Tensor) and not (
                 t.device.type == device_type
                 and (t.dtype == p.dtype or (p.packed and t.dtype in (torch.int8, torch.uint8)))
-                and t.shape == p.shape and 0 not in p.shape and t.is_contiguous()
+                and t.shape == p.shape and 0 not in p.shape and p.lies_as(t)
             ):
                 break
         else:
@@ -146,13 +153,15 @@ class KernelAdapter:
                 continue
             expected = 1
             for i in range(len(p.shape) - 1, -1, -1):
+                if p.strides is not None:
+                    expected = p.strides[i]
                 if t.shape[i] != 1 and t.stride(i) != expected:
                     raise ValueError(
                         f"Static stride mismatch for parameter {p.name}: expected {expected} at index {i}, got {t.stride(i)}"
                     )
                 expected *= t.shape[i]
         for p, t in zip(self.params, tensors):
-            if isinstance(t, torch.Tensor) and not t.is_contiguous():
+            if isinstance(t, torch.Tensor) and not p.lies_as(t):
                 raise ValueError(f"Expected parameter {p.name} to be a contiguous tensor")
 
     def into_new(self, out_idx: int, *inputs):

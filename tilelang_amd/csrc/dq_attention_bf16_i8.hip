@@ -1,0 +1,6 @@
+// Attention of one new token, bf16 queries on an int8 cache.
+#include "dq_attention.h"
+
+namespace dq {
+int attention_bf16_i8(const AttnArgs& a, hipStream_t stream) { return attention_of_type<bf16_t, CACHE_I8>(a, stream); }
+}  // namespace dq

@@ -1,0 +1,6 @@
+// Attention of one new token, fp16 queries on an fp16 cache.
+#include "dq_attention.h"
+
+namespace dq {
+int attention_f16(const AttnArgs& a, hipStream_t stream) { return attention_of_type<half_t, CACHE_F16>(a, stream); }
+}  // namespace dq

@@ -1,0 +1,332 @@
+// Rotary positions, and the paged key-value cache as it is written and read back (layout: dq_kv.h).
+//
+// Rotation of a head x at position p, r = rotary_dim, h = r / 2, (c_i, s_i) = Table[p][i], Table[p][h + i]:
+//   half layout:        y_i = x_i c_i - x_{i+h} s_i,      y_{i+h} = x_{i+h} c_i + x_i s_i        (i < h)
+//   interleaved layout: y_{2i} = x_{2i} c_i - x_{2i+1} s_i, y_{2i+1} = x_{2i+1} c_i + x_{2i} s_i
+// and y_j = x_j from r on; with s negated it is the transpose, which is the gradient.  The table is the caller's, in fp32
+// from angles in 64 bits: position times frequency loses the angle in fp32 from some ten thousand positions on.
+//
+// Quantised: a = max_j |y_j| of a token's head, code_j = rne(y_j * (top / a)), scale = a / top (top 448 or 127); the
+// rotated key is quantised from fp32, not from a rounded 16-bit key.  A head with an infinity or a NaN gets a NaN scale,
+// so it reads back as NaN and not as plausible numbers.
+//
+// All three operators only move memory.  A group of lanes owns a head's row, eight elements (16 bytes) a lane; the
+// partner half of a row comes from the caches by a second load of the same lines.
+#include "dq_kv.h"
+
+namespace dq {
+
+namespace {
+
+enum RotaryLayout : int {
+  ROTARY_NONE = 0,
+  ROTARY_HALF = 1,         // rotary_dim % 16 == 0: a lane's eight elements have one partner piece
+  ROTARY_INTERLEAVED = 2,  // rotary_dim % 8 == 0: pairs inside a lane's piece
+  ROTARY_ANY = 3,          // either layout, any even rotary_dim: element by element
+};
+
+struct RowArgs {
+  const void* x;     // [tokens][row_stride]: heads (q, or q and k and v) of head_dim
+  const void* v;     // values where they do not lie behind the keys in x; else null
+  const float* table;
+  const int* positions;
+  const int* slots;
+  void* out;         // rotated heads, [tokens][out_stride]
+  void* cache[2];
+  float* scale[2];
+  long row_stride, out_stride;
+  int tokens, q_heads, head_dim, rotary_dim, table_rows, interleaved, inverse;
+  CacheShape shape;
+};
+
+template <int LANES>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  v = max(v, dpp_move<0xB1>(v));                          // xor 1
+  v = max(v, dpp_move<0x4E>(v));                          // xor 2
+  if constexpr (LANES >= 8) v = max(v, dpp_move<0x141>(v));   // mirror in eight lanes
+  if constexpr (LANES >= 16) v = max(v, dpp_move<0x140>(v));  // mirror in sixteen
+  if constexpr (LANES >= 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+  return v;
+}
+
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  const auto h = *reinterpret_cast<const typename Vec8<T>::type*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
+}
+
+template <class T>
+__device__ __forceinline__ typename Vec8<T>::type round8(const float (&f)[8]) {
+  typename Vec8<T>::type h;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = (T)f[i];
+  return h;
+}
+
+// LANES lanes a row (head), the lane's piece at 8 * (lane % LANES); U rows of one token a lane group, so that the row of
+// the table is read once for them.  FORMAT < 0: rotation alone.
+template <class T, int LANES, int LAYOUT, int FORMAT, int U>
+__global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
+  const int lane = threadIdx.x % LANES;
+  const int heads = a.q_heads + (FORMAT >= 0 ? 2 * a.shape.kv_heads : 0);
+  const int blocks = (heads + U - 1) / U;
+  const unsigned group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int token = group / blocks, first = (group - token * blocks) * U;
+  if (token >= a.tokens) return;
+  const int d = lane * 8;
+  const bool inside = d < a.head_dim;
+  const int keys_end = a.q_heads + (FORMAT >= 0 ? a.shape.kv_heads : 0);  // rows that are rotated
+  const int r = a.rotary_dim, h = r >> 1;
+  const bool turns = LAYOUT != ROTARY_NONE && inside && d < r && first < keys_end;
+
+  const T* const row = reinterpret_cast<const T*>(a.x) + (size_t)token * a.row_stride;
+  const T* const vrow = FORMAT >= 0 && a.v ? reinterpret_cast<const T*>(a.v) + ((size_t)token * a.shape.kv_heads) * a.head_dim : nullptr;
+  float x[U][8], partner[U][8];
+  // a piece's partner: the other half's piece of the same row
+  const int other = LAYOUT == ROTARY_HALF ? (d < h ? d + h : d - h) : 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int head = first + u;
+    if (inside && head < heads) {
+      load8(vrow && head >= keys_end ? vrow + (head - keys_end) * a.head_dim + d : row + head * a.head_dim + d, x[u]);
+    }
+    if constexpr (LAYOUT == ROTARY_HALF) {
+      if (turns && head < keys_end) load8(row + head * a.head_dim + other, partner[u]);
+    }
+    if constexpr (LAYOUT == ROTARY_ANY) {
+      if (turns && head < keys_end) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = d + i, p = a.interleaved ? j ^ 1 : (j < h ? j + h : j - h);
+          partner[u][i] = j < r ? (float)row[head * a.head_dim + p] : 0.f;
+        }
+      }
+    }
+  }
+  // in place: what other lanes of the row read is read before any lane of it writes
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+
+  if constexpr (LAYOUT != ROTARY_NONE) {
+    if (turns) {
+      const int position = a.positions[token];
+      const bool known = (unsigned)position < (unsigned)a.table_rows;  // else NaN
+      const float* const angle = a.table + (size_t)(known ? position : 0) * r;
+      float c[8], s[8];
+      if constexpr (LAYOUT == ROTARY_HALF) {
+        const int i = d < h ? d : d - h;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float4_t cq = *reinterpret_cast<const float4_t*>(angle + i + 4 * q), sq = *reinterpret_cast<const float4_t*>(angle + h + i + 4 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) c[4 * q + j] = cq[j], s[4 * q + j] = d < h ? -sq[j] : sq[j];
+        }
+      } else if constexpr (LAYOUT == ROTARY_INTERLEAVED) {
+        const float4_t cq = *reinterpret_cast<const float4_t*>(angle + (d >> 1)), sq = *reinterpret_cast<const float4_t*>(angle + h + (d >> 1));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = cq[j >> 1], s[j] = (j & 1) ? sq[j >> 1] : -sq[j >> 1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = d + i, at = a.interleaved ? j >> 1 : (j < h ? j : j - h);
+          const bool low = a.interleaved ? !(j & 1) : j < h;
+          c[i] = j < r ? angle[at] : 1.f;
+          s[i] = j < r ? (low ? -angle[h + at] : angle[h + at]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (a.inverse) s[i] = -s[i];
+        if (!known && (LAYOUT != ROTARY_ANY || d + i < r)) c[i] = __builtin_nanf("");
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (first + u >= keys_end) continue;
+        if constexpr (LAYOUT == ROTARY_INTERLEAVED) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) partner[u][i] = x[u][i ^ 1];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[u][i] = x[u][i] * c[i] + partner[u][i] * s[i];
+      }
+    }
+  }
+
+  int place = 0, page = -1;
+  if constexpr (FORMAT >= 0) {
+    const int slot = a.slots[token];
+    page = slot >> a.shape.page_shift;  // negative: not written
+    place = slot & ((1 << a.shape.page_shift) - 1);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int head = first + u;
+    if (head >= heads) continue;
+    if (FORMAT < 0 || head < a.q_heads) {
+      if (inside) *reinterpret_cast<typename Vec8<T>::type*>(reinterpret_cast<T*>(a.out) + (size_t)token * a.out_stride + head * a.head_dim + d) = round8<T>(x[u]);
+      continue;
+    }
+    if constexpr (FORMAT >= 0) {
+      if ((unsigned)page >= (unsigned)a.shape.pages) continue;
+      const int which = head >= keys_end;
+      const size_t at = cache_row(a.shape, page, head - (which ? keys_end : a.q_heads), place);
+      void* const cache = which ? a.cache[1] : a.cache[0];
+      if constexpr (cache_is_16bit(FORMAT)) {
+        if (inside) *reinterpret_cast<typename Vec8<T>::type*>(reinterpret_cast<T*>(cache) + at * a.head_dim + d) = round8<T>(x[u]);
+      } else {
+        constexpr float kTop = FORMAT == CACHE_FP8 ? 448.f : 127.f;
+        uint32_t most = 0;  // magnitudes order like their bits, infinities and NaN above every number
+        if (inside) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = max(most, __builtin_bit_cast(uint32_t, x[u][i]) & 0x7FFFFFFFu);
+        }
+        most = row_max<LANES>(most);
+        const float amax = __builtin_bit_cast(float, most);
+        const bool finite = most < 0x7F800000u, some = finite && amax >= kSmallestHead;
+        const float factor = some ? kTop / amax : 0.f;
+        if (inside) {
+          uint2_t codes = {0u, 0u};
+          if (finite) {
+            codes[0] = quantise4<FORMAT>(x[u][0] * factor, x[u][1] * factor, x[u][2] * factor, x[u][3] * factor);
+            codes[1] = quantise4<FORMAT>(x[u][4] * factor, x[u][5] * factor, x[u][6] * factor, x[u][7] * factor);
+          }
+          *reinterpret_cast<uint2_t*>(reinterpret_cast<uint8_t*>(cache) + at * a.head_dim + d) = codes;
+          if (lane == 0) (which ? a.scale[1] : a.scale[0])[at] = finite ? (some ? amax / kTop : 0.f) : __builtin_nanf("");
+        }
+      }
+    }
+  }
+}
+
+template <class T, int LANES, int LAYOUT, int FORMAT>
+int launch_rows(const RowArgs& a, hipStream_t stream) {
+  const int heads = a.q_heads + (FORMAT >= 0 ? 2 * a.shape.kv_heads : 0);
+  const long rows = (long)a.tokens * heads;
+  auto grid = [&](int u) { return dim3((unsigned)(((long)a.tokens * ((heads + u - 1) / u) + 256 / LANES - 1) / (256 / LANES))); };
+  if (rows * LANES >= 256 * 1024 * 4) rows_kernel<T, LANES, LAYOUT, FORMAT, 4><<<grid(4), 256, 0, stream>>>(a);
+  else rows_kernel<T, LANES, LAYOUT, FORMAT, 1><<<grid(1), 256, 0, stream>>>(a);
+  DQ_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+template <class T, int LANES, int FORMAT>
+int launch_rows_layout(const RowArgs& a, hipStream_t stream) {
+  if (a.rotary_dim == 0) return launch_rows<T, LANES, ROTARY_NONE, FORMAT>(a, stream);
+  if (a.interleaved && a.rotary_dim % 8 == 0) return launch_rows<T, LANES, ROTARY_INTERLEAVED, FORMAT>(a, stream);
+  if (!a.interleaved && a.rotary_dim % 16 == 0) return launch_rows<T, LANES, ROTARY_HALF, FORMAT>(a, stream);
+  return launch_rows<T, LANES, ROTARY_ANY, FORMAT>(a, stream);
+}
+
+template <class T, int FORMAT>
+int launch_rows_lanes(const RowArgs& a, hipStream_t stream) {
+  if (a.head_dim <= 64) return launch_rows_layout<T, 8, FORMAT>(a, stream);
+  if (a.head_dim <= 128) return launch_rows_layout<T, 16, FORMAT>(a, stream);
+  if (a.head_dim <= 256) return launch_rows_layout<T, 32, FORMAT>(a, stream);
+  if constexpr (FORMAT < 0) return launch_rows_layout<T, 64, FORMAT>(a, stream);
+  DQ_FAIL("a head of %d is beyond the cache's %d", a.head_dim, kMaxHeadDim);
+}
+
+// Row (token of the packed result, head): the sequence whose tokens it is among, its page, its codes times its scale.
+struct ReadArgs {
+  const void* cache[2];
+  const float* scale[2];
+  const int* table;
+  const int* starts;
+  void* out;  // [2][tokens][kv_heads][head_dim]
+  int sequences, tokens, max_pages;
+  CacheShape shape;
+};
+
+template <class T, int LANES, int FORMAT>
+__global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
+  const int lane = threadIdx.x % LANES, d = lane * 8;
+  const unsigned group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int token = group / a.shape.kv_heads, head = group - token * a.shape.kv_heads;
+  if (token >= a.tokens || d >= a.shape.head_dim) return;
+  // the last sequence that starts at or before the token
+  int lo = 0, hi = a.sequences;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.starts[mid] <= token) lo = mid;
+    else hi = mid;
+  }
+  const int position = token - a.starts[lo];
+  const int column = position >> a.shape.page_shift;
+  int page = -1;
+  if (position >= 0 && token < a.starts[lo + 1] && column < a.max_pages) page = a.table[(size_t)lo * a.max_pages + column];
+  const bool there = (unsigned)page < (unsigned)a.shape.pages;
+  const size_t at = cache_row(a.shape, there ? page : 0, head, position & ((1 << a.shape.page_shift) - 1));
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float x[8] = {};
+    if (there) {
+      if constexpr (cache_is_16bit(FORMAT)) {
+        load8(reinterpret_cast<const T*>(a.cache[which]) + at * a.shape.head_dim + d, x);
+      } else {
+        const float s = a.scale[which][at];
+        codes8_to_float<FORMAT>(*reinterpret_cast<const uint2_t*>(reinterpret_cast<const uint8_t*>(a.cache[which]) + at * a.shape.head_dim + d), x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= s;
+      }
+    }
+    T* const out = reinterpret_cast<T*>(a.out) + (((size_t)which * a.tokens + token) * a.shape.kv_heads + head) * a.shape.head_dim + d;
+    *reinterpret_cast<typename Vec8<T>::type*>(out) = round8<T>(x);
+  }
+}
+
+template <class T, int FORMAT>
+int launch_read(const ReadArgs& a, hipStream_t stream) {
+  const long rows = (long)a.tokens * a.shape.kv_heads;
+  auto grid = [&](int lanes) { return dim3((unsigned)((rows + 256 / lanes - 1) / (256 / lanes))); };
+  if (a.shape.head_dim <= 64) read_kernel<T, 8, FORMAT><<<grid(8), 256, 0, stream>>>(a);
+  else if (a.shape.head_dim <= 128) read_kernel<T, 16, FORMAT><<<grid(16), 256, 0, stream>>>(a);
+  else read_kernel<T, 32, FORMAT><<<grid(32), 256, 0, stream>>>(a);
+  DQ_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+}  // namespace
+
+int rotary(const void* X, const float* Table, const int* Positions, void* Out, int tokens, int heads, int head_dim, int rotary_dim,
+           int positions, long row_stride, long out_stride, int interleaved, int inverse, int bf16, hipStream_t stream) {
+  RowArgs a = {};
+  a.x = X, a.table = Table, a.positions = Positions, a.out = Out, a.row_stride = row_stride, a.out_stride = out_stride;
+  a.tokens = tokens, a.q_heads = heads, a.head_dim = head_dim, a.rotary_dim = rotary_dim, a.table_rows = positions;
+  a.interleaved = interleaved, a.inverse = inverse;
+  return bf16 ? launch_rows_lanes<bf16_t, -1>(a, stream) : launch_rows_lanes<half_t, -1>(a, stream);
+}
+
+int kv_cache_write(const void* X, const void* V, const float* Table, const int* Positions, const int* Slots, void* Q, void* KCache,
+                   void* VCache, float* KScale, float* VScale, int tokens, int heads, int kv_heads, int head_dim, int rotary_dim,
+                   int positions, int pages, int page_shift, int interleaved, int bf16, int format, hipStream_t stream) {
+  RowArgs a = {};
+  a.x = X, a.v = V, a.table = Table, a.positions = Positions, a.slots = Slots, a.out = Q;
+  a.cache[0] = KCache, a.cache[1] = VCache, a.scale[0] = KScale, a.scale[1] = VScale;
+  a.row_stride = (long)(heads + (V ? 1 : 2) * kv_heads) * head_dim, a.out_stride = (long)heads * head_dim;
+  a.tokens = tokens, a.q_heads = heads, a.head_dim = head_dim, a.rotary_dim = rotary_dim, a.table_rows = positions;
+  a.interleaved = interleaved;
+  a.shape = {pages, kv_heads, page_shift, head_dim};
+  switch (format) {
+    case CACHE_FP8: return bf16 ? launch_rows_lanes<bf16_t, CACHE_FP8>(a, stream) : launch_rows_lanes<half_t, CACHE_FP8>(a, stream);
+    case CACHE_I8: return bf16 ? launch_rows_lanes<bf16_t, CACHE_I8>(a, stream) : launch_rows_lanes<half_t, CACHE_I8>(a, stream);
+    default: return bf16 ? launch_rows_lanes<bf16_t, CACHE_BF16>(a, stream) : launch_rows_lanes<half_t, CACHE_F16>(a, stream);
+  }
+}
+
+int kv_cache_read(const void* KCache, const void* VCache, const float* KScale, const float* VScale, const int* PageTable,
+                  const int* Starts, void* KV, int sequences, int tokens, int kv_heads, int head_dim, int pages, int page_shift,
+                  int max_pages, int bf16, int format, hipStream_t stream) {
+  ReadArgs a = {};
+  a.cache[0] = KCache, a.cache[1] = VCache, a.scale[0] = KScale, a.scale[1] = VScale;
+  a.table = PageTable, a.starts = Starts, a.out = KV;
+  a.sequences = sequences, a.tokens = tokens, a.max_pages = max_pages;
+  a.shape = {pages, kv_heads, page_shift, head_dim};
+  switch (format) {
+    case CACHE_FP8: return bf16 ? launch_read<bf16_t, CACHE_FP8>(a, stream) : launch_read<half_t, CACHE_FP8>(a, stream);
+    case CACHE_I8: return bf16 ? launch_read<bf16_t, CACHE_I8>(a, stream) : launch_read<half_t, CACHE_I8>(a, stream);
+    default: return bf16 ? launch_read<bf16_t, CACHE_BF16>(a, stream) : launch_read<half_t, CACHE_F16>(a, stream);
+  }
+}
+
+}  // namespace dq

@@ -22,7 +22,8 @@
 namespace {
 
 constexpr int kMaxDevices = 64;
-constexpr int kMaxPointers = 8;
+constexpr int kMaxPointers = 12;
+constexpr int kMaxParams = 16;
 bool g_initialised[kMaxDevices];  // the library's init() ran there; written and read under the interpreter's lock
 const char* (*g_last_error)() = nullptr;
 PyObject* g_raw_stream = nullptr;  // torch's private call for the current stream of a GPU
@@ -69,6 +70,26 @@ const Entry kEntries[] = {
      [](void* fn, const Args& a) {
        return DQ_CALL(call_gemm_int8xint4)(a.p[0], a.p[1], a.p[2], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.stream);
      }},
+    {"call_rotary", 4, 9,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_rotary)(a.p[0], a.p[1], a.p[2], a.p[3], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.i[8], a.stream);
+     }},
+    {"call_kv_cache_write", 7, 7,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_kv_cache_write)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.stream);
+     }},
+    {"call_rotary_kv_cache_write", 9, 11,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_rotary_kv_cache_write)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.p[7], a.p[8], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.i[8], a.i[9], a.i[10], a.stream);
+     }},
+    {"call_kv_cache_read", 7, 9,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_kv_cache_read)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.i[8], a.stream);
+     }},
+    {"call_paged_attention_decode", 11, 10,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_paged_attention_decode)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.p[7], a.p[8], a.p[9], a.p[10], a.ws, a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.i[8], a.i[9], a.f, a.stream);
+     }},
 };
 #undef DQ_CALL
 
@@ -76,6 +97,7 @@ struct Param {
   at::ScalarType dtype;
   bool packed;
   std::vector<int64_t> shape;
+  std::vector<int64_t> strides;  // empty: contiguous
   int role;  // 0: the caller's; 1: allocated and returned; 2: workspace
 };
 
@@ -94,6 +116,13 @@ struct Call {
 
 PyObject* not_settled() { Py_RETURN_NOTIMPLEMENTED; }
 
+bool lies_as(const at::Tensor& t, const Param& p) {
+  if (p.strides.empty()) return t.is_contiguous();
+  for (size_t d = 0; d < p.strides.size(); ++d)
+    if (p.shape[d] != 1 && t.stride(d) != p.strides[d]) return false;
+  return true;
+}
+
 // Other threads run while blocks are allocated and the kernel is launched, either of which may have to wait.
 struct WithoutInterpreter {
   PyThreadState* const state = PyEval_SaveThread();
@@ -108,7 +137,7 @@ PyObject* call_call(PyObject* self_, PyObject* args, PyObject* kwargs) {
   // a mode that sees torch's calls is to see the ones that the adapter makes
   if (at::impl::PythonTorchFunctionTLS::stack_len() != 0 || c10::impl::TorchDispatchModeTLS::any_modes_set()) return not_settled();
   const size_t n = self->params->size();
-  void* pointers[16] = {};
+  void* pointers[kMaxParams] = {};
   int device = -1;
   size_t at_input = 0;
   for (size_t k = 0; k < n; ++k) {
@@ -122,7 +151,7 @@ PyObject* call_call(PyObject* self_, PyObject* args, PyObject* kwargs) {
     if (device < 0) device = t.device().index();
     const at::ScalarType dtype = t.scalar_type();
     if (t.device().index() != device || !(dtype == p.dtype || (p.packed && (dtype == at::kChar || dtype == at::kByte))) ||
-        t.sizes() != at::IntArrayRef(p.shape) || t.numel() == 0 || !t.is_contiguous())
+        t.sizes() != at::IntArrayRef(p.shape) || t.numel() == 0 || !lies_as(t, p))
       return not_settled();
     pointers[k] = t.data_ptr();
   }
@@ -175,7 +204,7 @@ void call_dealloc(PyObject* self_) {
 
 PyTypeObject CallType = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
-// bind(entry, ((dtype, packed, shape, role), ...), slots, ints, f, ws) -> callable, or None where there is no such entry
+// bind(entry, ((dtype, packed, shape, strides (none: contiguous), role), ...), slots, ints, f, ws) -> callable, or None where there is no such entry
 PyObject* bind(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
   const char* name;
@@ -188,7 +217,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     if (!strcmp(e.name, name)) entry = &e;
   void* const fn = entry && g_library ? dlsym(g_library, name) : nullptr;
   const Py_ssize_t n = PyTuple_GET_SIZE(params);
-  if (!fn || PyTuple_GET_SIZE(slots) != entry->pointers || PyTuple_GET_SIZE(ints) != entry->ints || n > 16) Py_RETURN_NONE;
+  if (!fn || PyTuple_GET_SIZE(slots) != entry->pointers || PyTuple_GET_SIZE(ints) != entry->ints || n > kMaxParams) Py_RETURN_NONE;
   Call* const self = PyObject_New(Call, &CallType);
   if (!self) return nullptr;
   self->entry = entry;
@@ -202,14 +231,16 @@ PyObject* bind(PyObject*, PyObject* args) {
   bool good = true;
   int workspaces = 0;
   for (Py_ssize_t k = 0; k < n && good; ++k) {
-    PyObject *dtype, *shape;
+    PyObject *dtype, *shape, *strides;
     int packed, role;
-    if (!PyArg_ParseTuple(PyTuple_GET_ITEM(params, k), "OpO!i", &dtype, &packed, &PyTuple_Type, &shape, &role) || !THPDtype_Check(dtype)) {
+    if (!PyArg_ParseTuple(PyTuple_GET_ITEM(params, k), "OpO!O!i", &dtype, &packed, &PyTuple_Type, &shape, &PyTuple_Type, &strides, &role) || !THPDtype_Check(dtype)) {
       good = false;
       break;
     }
-    Param p{reinterpret_cast<THPDtype*>(dtype)->scalar_type, packed != 0, {}, role};
+    Param p{reinterpret_cast<THPDtype*>(dtype)->scalar_type, packed != 0, {}, {}, role};
     for (Py_ssize_t d = 0; d < PyTuple_GET_SIZE(shape); ++d) p.shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(shape, d)));
+    for (Py_ssize_t d = 0; d < PyTuple_GET_SIZE(strides); ++d) p.strides.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(strides, d)));
+    good = good && (p.strides.empty() || p.strides.size() == p.shape.size());
     self->inputs += role == 0;
     workspaces += role == 2;
     if (role == 1) {
