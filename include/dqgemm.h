@@ -401,7 +401,8 @@ int call_kv_cache_read(const void* KCache, const void* VCache, const void* KScal
  * NaN or not.  Softmax and sums in fp32; results do not depend on timing.
  * Workspace: dq_paged_attention_workspace_bytes(...) bytes, 16-byte aligned (0: none), contents undefined before and after,
  * not to be shared by calls that overlap in time. */
-size_t dq_paged_attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim, int page_size, int max_pages);
+size_t dq_paged_attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim, int page_size, int max_pages,
+                                          int window, int cache_format);
 int call_paged_attention_decode(const void* Q, const void* KCache, const void* VCache, const void* KScale, const void* VScale,
                                 const void* PageTable, const void* Lengths, const void* Sinks, void* Out, void* Lse, void* Workspace,
                                 size_t workspace_bytes, int sequences, int heads, int kv_heads, int head_dim, int pages,

@@ -181,5 +181,6 @@ def test_table():
 
 def test_workspace_is_named_without_a_gpu():
     room = _lib.load_library().dq_paged_attention_workspace_bytes
-    assert room(1, 32, 8, 128, 16, 1) == 0  # one tile: nothing to join
-    assert room(1, 32, 8, 128, 16, 1000) > 0 and room(0, 32, 8, 128, 16, 1) == 0 and room(1, 33, 8, 128, 16, 1) == 0
+    assert room(1, 32, 8, 128, 16, 1, 0, CACHE_F16) == 0  # one tile: nothing to join
+    assert room(1, 32, 8, 128, 16, 1000, 0, CACHE_F16) > 0
+    assert room(0, 32, 8, 128, 16, 1000, 0, CACHE_F16) == 0 and room(1, 33, 8, 128, 16, 1000, 0, CACHE_F16) == 0

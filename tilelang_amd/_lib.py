@@ -67,7 +67,7 @@ SIZE_QUERIES = {
     "dq_w4a16_workspace_bytes": [_i, _i, _i, _i, _i],
     "dq_mxfp4_workspace_bytes": [_i, _i, _i],
     "dq_bitlinear_workspace_bytes": [_i, _i, _i, _i],
-    "dq_paged_attention_workspace_bytes": [_i] * 6,
+    "dq_paged_attention_workspace_bytes": [_i] * 8,
 }
 
 

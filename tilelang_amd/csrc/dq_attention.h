@@ -27,6 +27,9 @@ namespace dq {
 constexpr int kAttnWaves = 4;
 constexpr int kAttnTile = 32;  // tokens a wave takes at once
 
+constexpr int kAttnUnit = kAttnTile * kAttnWaves;  // tokens that a workgroup takes at once
+constexpr int kComputeUnits = 256;
+
 struct AttnArgs {
   const void* q;           // [sequences][heads][head_dim]
   const void* cache[2];
@@ -36,14 +39,43 @@ struct AttnArgs {
   const float* sinks;      // [heads] or null
   void* out;               // [sequences][heads][head_dim]
   float* lse;              // [sequences][heads] or null
-  float* part_o;           // [sequences][heads][splits][head_dim]
-  float* part_ml;          // [sequences][heads][splits][2]
+  float* part_o;           // [workgroups][2][rows][head_dim]
+  float* part_ml;          // [workgroups][2][rows][2]
+  int* pieces;             // [sequences][kv_heads * head_blocks][2]: the first and last workgroup that has a piece
   float score_scale;       // scale * log2(e)
-  int sequences, heads, max_pages, window, splits, head_blocks;
+  int sequences, heads, max_pages, window, head_blocks, rows, workgroups;
   CacheShape shape;
 };
 
-typedef float float2_t_ __attribute__((ext_vector_type(2)));
+// The tokens of a sequence: [first, length), in tiles from tile0 on, in units of kAttnUnit tokens.
+struct Span {
+  int length, first, tile0, tiles, units;
+};
+__device__ __forceinline__ Span span_of(int length, int capacity, int window) {
+  Span s;
+  s.length = min(max(length, 0), capacity);
+  s.first = window > 0 ? max(0, s.length - window) : 0;
+  s.tile0 = s.first / kAttnTile;
+  s.tiles = (s.length + kAttnTile - 1) / kAttnTile - s.tile0;
+  s.units = (s.tiles + kAttnWaves - 1) / kAttnWaves;
+  return s;
+}
+
+// How the work is shared out.  The tokens that a key-value head (a column) has of a sequence cost their units and one more: what
+// a workgroup does before the first and after the last takes about as long.  All costs in a row, sequence by
+// sequence and in a sequence column by column, are cut into equal shares, one a workgroup, whatever the lengths are; a
+// cut inside a column makes pieces of it, which the join adds up.  A column of up to two units is not worth a
+// join: a cut there moves to its nearer end.
+constexpr int kWholeUnits = 2;
+struct Shares {
+  unsigned each, more;  // the first `more` workgroups have one more
+  __device__ __forceinline__ Shares(unsigned total, unsigned workgroups) : each(total / workgroups), more(total - total / workgroups * workgroups) {}
+  __device__ __forceinline__ unsigned begin(unsigned w) const { return w * each + min(w, more); }
+  __device__ __forceinline__ unsigned owner(unsigned u) const {
+    const unsigned large = more * (each + 1);
+    return u < large ? u / (each + 1) : more + (u - large) / max(each, 1u);
+  }
+};
 
 // ---- which elements of a row a lane holds ----------------------------------------------------------------------
 // Keys (and queries): k-step s of 32 elements, group g has eight of them.  16 bit: 32 s + 8 g.  8 bit: a lane loads 16
@@ -108,9 +140,14 @@ __device__ __forceinline__ void codes4_to_half(uint32_t w, uint32_t& lo, uint32_
   }
 }
 
+// Rows of 16 lanes change places pairwise, then the halves of the wave.  In assembly: of a builtin's two results the compiler
+// uses one for both where a value is swapped with itself.  (Two wait states between a result and its swap.)
 __device__ __forceinline__ float max_over_groups(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  float y = x;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  x = fmaxf(x, y), y = x;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  return fmaxf(x, y);
 }
 __device__ __forceinline__ float sum_over_groups(float x) {
   x += __shfl_xor(x, 16);
@@ -120,9 +157,18 @@ __device__ __forceinline__ float sum_over_groups(float x) {
 // 2^(m - to), 0 where there is nothing (m = -inf), whatever `to` is
 __device__ __forceinline__ float weight(float m, float to) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to); }
 
+// How many workgroups (of four waves) a compute unit holds: by the registers that a kernel needs, and the LDS of the join.
+constexpr int attention_per_unit(int head_dim, int format) { return head_dim <= 64 ? 4 : 2; }
+
+// A wave's LDS: 32 keys on their way into the operand's order, later 16 rows of its result.
+constexpr int attention_wave_lds(int head_dim, int format) {
+  const int bytes = head_dim * (cache_is_16bit(format) ? 2 : 1), keys = kAttnTile * (bytes / 16 | 1) * 16, result = 16 * (head_dim + 4) * 4;
+  return keys > result ? keys : result;
+}
+
 // T: queries and output; FORMAT: the cache; D: head_dim; NT: blocks of 16 heads that a workgroup takes
 template <class T, int FORMAT, int D, int NT>
-__global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) void attention_kernel(const AttnArgs a) {
   constexpr bool kWide = cache_is_16bit(FORMAT);
   using C = typename std::conditional<kWide, T, half_t>::type;  // what the products are taken in
   typedef typename Vec8<C>::type C8;
@@ -131,336 +177,469 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_kernel(const Att
   using VB = ValueBlocks<D>;
   constexpr int kVDwords = VB::dword(VB::count(), kBytes);
   constexpr int kAcc = D / 16;
-  constexpr int kKeyDwords = kWide ? 4 : 2;  // of one k-step
+  constexpr int kKeyPieces = D * kBytes / 2;              // of 16 bytes, of eight tokens
+  constexpr int kKeyLoads = (4 * kKeyPieces + 63) / 64;
+  constexpr int kKeyPitch = (D * kBytes / 16 | 1) * 16;   // an odd number of pieces: 16 rows on 64 banks
+  constexpr int kWaveLds = attention_wave_lds(D, FORMAT);
 
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x, kv_head = blockIdx.y / a.head_blocks, head_block = blockIdx.y - kv_head * a.head_blocks;
-  const int sequence = blockIdx.z;
-  const int group = a.heads / a.shape.kv_heads;  // heads that share kv_head
+  __shared__ float sm[kAttnWaves][16 * NT][3];
+  __shared__ int s_scan[kAttnWaves];
+  __shared__ unsigned s_cut[2][3];  // where the share begins and ends: cost, sequence, the sequence's first cost
+  extern __shared__ __align__(16) char lds[];
+  constexpr int kRow = D + 4;
 
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  char* const keys = lds + wave * kWaveLds;
+  auto result = [&](int w, int row) { return reinterpret_cast<float*>(lds + w * kWaveLds) + row * kRow; };
+  const int group = a.heads / a.shape.kv_heads;  // heads that share a key-value head
+  const int columns = a.shape.kv_heads * a.head_blocks;
   const int capacity = a.max_pages << a.shape.page_shift;
-  const int length = min(max(a.lengths[sequence], 0), capacity);
-  const int first_token = a.window > 0 ? max(0, length - a.window) : 0;
-  const int tile0 = first_token / kAttnTile, tiles_all = (length + kAttnTile - 1) / kAttnTile - tile0;
-  // this split's tiles, whole rounds of the workgroup's waves
-  const int per = ((tiles_all + a.splits - 1) / a.splits + kAttnWaves - 1) / kAttnWaves * kAttnWaves;
-  const int begin = tile0 + split * per, end = min(begin + per, tile0 + tiles_all);
-
-  // ---- queries: the second operand of the first product, held for the whole walk -----------------------------
-  C8 q[NT][kSteps];
-  float q_scale[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int row = (head_block * NT + t) * 16 + n;
-    const T* const qrow = reinterpret_cast<const T*>(a.q) + ((size_t)sequence * a.heads + (size_t)kv_head * group + row) * D;
-    float f[kSteps][8];
-    float most = 0.f;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int d = key_element<D, kWide>(s, g);
-      typename Vec8<T>::type h = {};
-      if (row < group && d < D) h = *reinterpret_cast<const typename Vec8<T>::type*>(qrow + d);
-      if constexpr (kWide) {
-        q[t][s] = h;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[s][i] = (float)h[i], most = fmaxf(most, fabsf(f[s][i]));
-      }
-    }
-    q_scale[t] = a.score_scale;
-    if constexpr (!kWide) {
-      most = max_over_groups(most);
-      const int e = most > 0.f ? 14 - ilogbf(most) : 0;  // 2^e * most in [2^14, 2^15)
-      const int shift = min(max(e, -126), 126);
-      q_scale[t] = ldexpf(a.score_scale, -shift);
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[t][s][i] = (C)ldexpf(f[s][i], shift);
-    }
-  }
-
-  float4_t acc[NT][kAcc];
-  float m[NT], l[NT];
-  float o_ref[NT];  // acc is o / 2^o_ref (quantised caches; else 2^m)
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    m[t] = -INFINITY, l[t] = 0.f, o_ref[t] = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kAcc; ++i) acc[t][i] = float4_t{0.f, 0.f, 0.f, 0.f};
-  }
-
   const int place_mask = (1 << a.shape.page_shift) - 1;
-  const int* const table = a.table + (size_t)sequence * a.max_pages;
 
-  for (int tile = begin + wave; tile < end; tile += kAttnWaves) {
-    // the eight tokens whose keys (values) this lane reads, their page, whether it is there
-    const int k_first = tile * kAttnTile + (n >> 2) * 8, v_first = tile * kAttnTile + g * 8;
-    int k_page = -1, v_page = -1;
-    if (k_first < length) k_page = table[k_first >> a.shape.page_shift];
-    if (v_first < length) v_page = table[v_first >> a.shape.page_shift];
-    const bool k_there = (unsigned)k_page < (unsigned)a.shape.pages, v_there = (unsigned)v_page < (unsigned)a.shape.pages;
-    const size_t k_row = cache_row(a.shape, k_there ? k_page : 0, kv_head, (k_first & place_mask) + (n & 3));
-    const size_t v_row = cache_row(a.shape, v_there ? v_page : 0, kv_head, v_first & place_mask);
-    const char* const kp = reinterpret_cast<const char*>(a.cache[0]) + k_row * (D * kBytes);
-    const char* const vp = reinterpret_cast<const char*>(a.cache[1]) + v_row * (D * kBytes);
-
-    uint32_t kr[2][kSteps][kKeyDwords];
+  // ---- this workgroup's share: a running sum of the sequences' costs ---------------------------------------------
+  const int per_thread = (a.sequences + 64 * kAttnWaves - 1) / (64 * kAttnWaves);
+  const int seq_begin = min((int)threadIdx.x * per_thread, a.sequences), seq_end = min(seq_begin + per_thread, a.sequences);
+  int mine = 0;
+  for (int b = seq_begin; b < seq_end; ++b) mine += span_of(a.lengths[b], capacity, a.window).units + 1;
+  int sum = mine;  // inclusive
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(sum, o);
+    if (lane >= o) sum += up;
+  }
+  if (lane == 63) s_scan[wave] = sum;
+  __syncthreads();
+  int total = 0;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const char* const p = kp + t * 4 * D * kBytes + key_element<D, kWide>(s, g) * kBytes;
-        if constexpr (!kWide) {
-          if (64 * ((s >> 1) + 1) <= D) {
-            if (s & 1) continue;
-            const uint4_t w = *reinterpret_cast<const uint4_t*>(p);
-            kr[t][s][0] = w[0], kr[t][s][1] = w[1], kr[t][s + 1][0] = w[2], kr[t][s + 1][1] = w[3];
-            continue;
-          }
-          uint2_t w = {0u, 0u};
-          if (32 * (s + 1) <= D || key_element<D, kWide>(s, g) < D) w = *reinterpret_cast<const uint2_t*>(p);
-          kr[t][s][0] = w[0], kr[t][s][1] = w[1];
-        } else {
-          uint4_t w = {0u, 0u, 0u, 0u};
-          if (32 * (s + 1) <= D || key_element<D, kWide>(s, g) < D) w = *reinterpret_cast<const uint4_t*>(p);
+  for (int w = 0; w < kAttnWaves; ++w) {
+    if (w < wave) sum += s_scan[w];
+    total += s_scan[w];
+  }
+  const Shares shares((unsigned)total * columns, a.workgroups);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) kr[t][s][i] = w[i];
-        }
+  for (int side = 0; side < 2; ++side) {
+    const unsigned cut = shares.begin(blockIdx.x + side);
+    const int at = cut / columns;
+    if (threadIdx.x == 0 && at >= total) s_cut[side][0] = cut;  // behind everything
+    if (!(sum - mine <= at && at < sum)) continue;
+    int b = seq_begin, before = sum - mine;
+    for (;; ++b) {
+      const int units = span_of(a.lengths[b], capacity, a.window).units, cost = units + 1;
+      if (at >= before + cost) {
+        before += cost;
+        continue;
       }
+      const unsigned begin = (unsigned)before * columns;
+      const unsigned off = (cut - begin) % cost;
+      const unsigned moved = units <= kWholeUnits ? cut - off + (2 * off >= (unsigned)cost ? cost : 0) : cut;
+      const bool next = moved == begin + (unsigned)cost * columns;
+      s_cut[side][0] = moved, s_cut[side][1] = b + next, s_cut[side][2] = next ? moved : begin;
+      break;
+    }
+  }
+  __syncthreads();
+  unsigned u = __builtin_amdgcn_readfirstlane(s_cut[0][0]);
+  const unsigned u_end = __builtin_amdgcn_readfirstlane(s_cut[1][0]);
+  int sequence = __builtin_amdgcn_readfirstlane(s_cut[0][1]);
+  unsigned sequence_begin = __builtin_amdgcn_readfirstlane(s_cut[0][2]);
+
+  while (u < u_end) {
+    const Span span = span_of(a.lengths[sequence], capacity, a.window);
+    const int cost = span.units + 1;
+    const int column = (u - sequence_begin) / cost, from = (u - sequence_begin) - column * cost;
+    const int to = min((unsigned)cost, from + (u_end - u));
+    const unsigned column_begin = u - from;
+    u += to - from;
+    const int this_sequence = sequence;
+    if (u == sequence_begin + (unsigned)cost * columns) sequence_begin = u, ++sequence;
+    // the first of a column's cost stands for no tokens; a share that ends there leaves it all to the next
+    const int unit0 = max(from - 1, 0), units_here = to - 1 - unit0;
+    const bool complete = unit0 == 0 && to == cost;
+    if (to == 1 && !complete) continue;
+    const int kv_head = column / a.head_blocks, head_block = column - kv_head * a.head_blocks;
+    const int begin = span.tile0 + unit0 * kAttnWaves, end = span.tile0 + min((unit0 + units_here) * kAttnWaves, span.tiles);
+    const int length = span.length, first_token = span.first;
+    const int* const table = a.table + (size_t)this_sequence * a.max_pages;
+
+    // the page of a token
+    auto page_of = [&](int token) {
+      int page = -1;
+      if (token < length) page = table[token >> a.shape.page_shift];
+      return page;
+    };
+    auto row_of = [&](int page, int token) { return cache_row(a.shape, (unsigned)page < (unsigned)a.shape.pages ? page : 0, kv_head, token & place_mask); };
+
+    uint4_t kraw[kKeyLoads];
     uint32_t vr[8][kVDwords];
+    float ks[8], vs[8];
+    // Eight tokens' keys are one piece of memory: a load takes 64 times 16 bytes of the tile as they lie, whole lines.
+    auto load_keys = [&](int page, int tile) {  // page: that of the tokens 8 g ..
+      const char* base[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+      for (int e = 0; e < 4; ++e)
+        base[e] = reinterpret_cast<const char*>(a.cache[0]) + row_of(__builtin_amdgcn_readlane(page, 16 * e), tile * kAttnTile + 8 * e) * (D * kBytes);
 #pragma unroll
-      for (int b = 0; b < VB::count(); ++b) {
-        constexpr int kNone = 0;
-        (void)kNone;
-        const int e = VB::e(b), at = VB::dword(b, kBytes);
-        const char* const p = vp + (j * D + VB::start(b) + n * e) * kBytes;
-        const int bytes = e * kBytes;
-        if (bytes == 16) {
-          const uint4_t w = *reinterpret_cast<const uint4_t*>(p);
-          vr[j][at] = w[0], vr[j][at + 1] = w[1], vr[j][at + 2] = w[2], vr[j][at + 3] = w[3];
-        } else if (bytes == 8) {
-          const uint2_t w = *reinterpret_cast<const uint2_t*>(p);
-          vr[j][at] = w[0], vr[j][at + 1] = w[1];
-        } else if (bytes == 4) {
-          vr[j][at] = *reinterpret_cast<const uint32_t*>(p);
-        } else if (bytes == 2) {
-          vr[j][at] = *reinterpret_cast<const uint16_t*>(p);
-        } else {
-          vr[j][at] = *reinterpret_cast<const uint8_t*>(p);
+      for (int k = 0; k < kKeyLoads; ++k) {
+        const int i = 64 * k + lane, lo = 64 * k / kKeyPieces, hi = min((64 * k + 63) / kKeyPieces, 3);
+        const char* p = base[lo];
+        int e = lo;
+#pragma unroll
+        for (int more = lo + 1; more <= hi; ++more)
+          if (i >= more * kKeyPieces) p = base[more], e = more;
+        if (64 * (k + 1) <= 4 * kKeyPieces || i < 4 * kKeyPieces)
+          kraw[k] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p + (i - e * kKeyPieces) * 16));
+      }
+    };
+    // ... and goes through the wave's own LDS into the operand's order: row 16 t + n is that of lane n in product t.
+    auto keys_to_lds = [&] {
+#pragma unroll
+      for (int k = 0; k < kKeyLoads; ++k) {
+        const int i = 64 * k + lane;
+        const int token = i / (D * kBytes / 16), piece = i - token * (D * kBytes / 16), r = token & 7;
+        if (64 * (k + 1) <= 4 * kKeyPieces || i < 4 * kKeyPieces)
+          *reinterpret_cast<uint4_t*>(keys + ((r >> 2) * 16 + (token >> 3) * 4 + (r & 3)) * kKeyPitch + piece * 16) = kraw[k];
+      }
+      asm volatile("" ::: "memory");  // read by other lanes; a wave's LDS accesses keep their order
+    };
+    auto load_values = [&](size_t row) {
+      const char* const vp = reinterpret_cast<const char*>(a.cache[1]) + row * (D * kBytes);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int b = 0; b < VB::count(); ++b) {
+          const int e = VB::e(b), at = VB::dword(b, kBytes), bytes = e * kBytes;
+          const char* const p = vp + (j * D + VB::start(b) + n * e) * kBytes;
+          if (bytes == 16) {
+            const uint4_t w = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p));
+            vr[j][at] = w[0], vr[j][at + 1] = w[1], vr[j][at + 2] = w[2], vr[j][at + 3] = w[3];
+          } else if (bytes == 8) {
+            const uint2_t w = __builtin_nontemporal_load(reinterpret_cast<const uint2_t*>(p));
+            vr[j][at] = w[0], vr[j][at + 1] = w[1];
+          } else if (bytes == 4) {
+            vr[j][at] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+          } else if (bytes == 2) {
+            vr[j][at] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(p));
+          } else {
+            vr[j][at] = __builtin_nontemporal_load(reinterpret_cast<const uint8_t*>(p));
+          }
+        }
+    };
+    auto load_scales = [&](size_t row) {
+      if constexpr (!kWide) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4_t kq = *reinterpret_cast<const float4_t*>(a.scale[0] + row + 4 * i), vq = *reinterpret_cast<const float4_t*>(a.scale[1] + row + 4 * i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ks[4 * i + j] = kq[j], vs[4 * i + j] = vq[j];
         }
       }
-    float ks[8], vs[8];
-    if constexpr (!kWide) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float4_t kq = *reinterpret_cast<const float4_t*>(a.scale[0] + v_row + 4 * i), vq = *reinterpret_cast<const float4_t*>(a.scale[1] + v_row + 4 * i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ks[4 * i + j] = kq[j], vs[4 * i + j] = vq[j];
-      }
-    }
+    };
 
-    // the tokens v_first + j that take part
-    const int low = max(first_token - v_first, 0), high = v_there ? min(length - v_first, 8) : 0;
-    const bool whole = __all(low == 0 && high == 8);
-    if (!whole) {
-      // what lies in dead places may be anything: its values count as zeros, not as zero times them
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j >= low && j < high) continue;
-#pragma unroll
-        for (int i = 0; i < kVDwords; ++i) vr[j][i] = 0u;
-        if constexpr (!kWide) ks[j] = 0.f, vs[j] = 0.f;
-      }
+    // The first tile's loads, and the page ids of the second: from here on keys, values and page ids are asked for a tile
+    // ahead, each as soon as its registers are free.
+    int tile = begin + wave;
+    int page = page_of(tile * kAttnTile + g * 8);
+    if (tile < end) {
+      load_keys(page, tile);
+      const size_t row = row_of(page, tile * kAttnTile + g * 8);
+      load_scales(row);
+      load_values(row);
     }
+    int page_next = page_of((tile + kAttnWaves) * kAttnTile + g * 8);
 
-    // ---- scores ---------------------------------------------------------------------------------------------
-    float p[NT][8];
+    // ---- queries: the second operand of the first product, held for the whole walk -----------------------------
+    C8 q[NT][kSteps];
+    float q_scale[NT];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      C8 kf[kSteps];
+    for (int t = 0; t < NT; ++t) {
+      const int row = (head_block * NT + t) * 16 + n;
+      const T* const qrow = reinterpret_cast<const T*>(a.q) + ((size_t)this_sequence * a.heads + (size_t)kv_head * group + row) * D;
+      typename Vec8<T>::type h[kSteps];
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        uint4_t w;
-        if constexpr (kWide) {
-          w = uint4_t{kr[t][s][0], kr[t][s][1], kr[t][s][2], kr[t][s][3]};
-        } else {
-          uint32_t h[4];
-          codes4_to_half<FORMAT>(kr[t][s][0], h[0], h[1]);
-          codes4_to_half<FORMAT>(kr[t][s][1], h[2], h[3]);
-          w = uint4_t{h[0], h[1], h[2], h[3]};
+        const int d = key_element<D, kWide>(s, g);
+        h[s] = typename Vec8<T>::type{};
+        if (row < group && d < D) h[s] = *reinterpret_cast<const typename Vec8<T>::type*>(qrow + d);
+      }
+      q_scale[t] = a.score_scale;
+      if constexpr (kWide) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) q[t][s] = h[s];
+      } else {
+        float most = 0.f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf((float)h[s][i]));
+        most = max_over_groups(most);
+        const int e = most > 0.f ? 14 - ilogbf(most) : 0;  // 2^e * most in [2^14, 2^15)
+        const int shift = min(max(e, -126), 126);
+        q_scale[t] = ldexpf(a.score_scale, -shift);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) q[t][s][i] = (C)ldexpf((float)h[s][i], shift);
+      }
+    }
+
+    float4_t acc[NT][kAcc];
+    float m[NT], l[NT];
+    float o_ref[NT];  // acc is o / 2^o_ref (quantised caches; else 2^m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t] = -INFINITY, l[t] = 0.f, o_ref[t] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kAcc; ++i) acc[t][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    auto take = [&](auto last) {
+      const int next = tile + kAttnWaves;
+      const int v_first = tile * kAttnTile + g * 8;
+      // the tokens v_first + j that take part
+      const int low = max(first_token - v_first, 0), high = (unsigned)page < (unsigned)a.shape.pages ? min(length - v_first, 8) : 0;
+      const bool whole = __all(low <= 0 && high == 8);
+
+      // ---- scores ---------------------------------------------------------------------------------------------
+      keys_to_lds();
+      float p[NT][8];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        C8 kf[kSteps];
+        uint4_t pair = {};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const int d = key_element<D, kWide>(s, g);
+          const char* const p = keys + (16 * t + n) * kKeyPitch + d * kBytes;
+          uint4_t w = {0u, 0u, 0u, 0u};
+          if constexpr (kWide) {
+            if (32 * (s + 1) <= D || d < D) w = *reinterpret_cast<const uint4_t*>(p);
+          } else {
+            uint2_t c = {0u, 0u};
+            if (64 * ((s >> 1) + 1) <= D) {
+              if (s & 1) c = uint2_t{pair[2], pair[3]};
+              else pair = *reinterpret_cast<const uint4_t*>(p), c = uint2_t{pair[0], pair[1]};
+            } else if (32 * (s + 1) <= D || d < D) {
+              c = *reinterpret_cast<const uint2_t*>(p);
+            }
+            uint32_t h[4];
+            codes4_to_half<FORMAT>(c[0], h[0], h[1]);
+            codes4_to_half<FORMAT>(c[1], h[2], h[3]);
+            w = uint4_t{h[0], h[1], h[2], h[3]};
+          }
+          kf[s] = __builtin_bit_cast(C8, w);
         }
-        kf[s] = __builtin_bit_cast(C8, w);
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+          float4_t sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) sc = mfma16<C>(kf[s], q[b][s], sc);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[b][4 * t + i] = sc[i];
+        }
+      }
+      asm volatile("" ::: "memory");  // the next keys come behind these
+      size_t next_row = 0;
+      if constexpr (!decltype(last)::value) {
+        load_keys(page_next, next);
+        next_row = row_of(page_next, next * kAttnTile + g * 8);
+      }
+
+      // ---- running maximum and sum ----------------------------------------------------------------------------
+      if constexpr (!kWide) {
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < low || j >= high) ks[j] = 0.f, vs[j] = 0.f;
+        }
       }
 #pragma unroll
       for (int b = 0; b < NT; ++b) {
-        float4_t sc = {0.f, 0.f, 0.f, 0.f};
+        float most = -INFINITY;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) sc = mfma16<C>(kf[s], q[b][s], sc);
+        for (int j = 0; j < 8; ++j) {
+          p[b][j] *= q_scale[b];
+          if constexpr (!kWide) p[b][j] *= ks[j];
+        }
+        if (!whole) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[b][4 * t + i] = sc[i];
+          for (int j = 0; j < 8; ++j)
+            if (j < low || j >= high) p[b][j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, p[b][j]);
+        most = fmaxf(m[b], max_over_groups(most));
+        const float base = most == -INFINITY ? 0.f : most;
+        float shrink = weight(m[b], base);
+        m[b] = most;
+        l[b] *= shrink;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          p[b][j] = __builtin_amdgcn_exp2f(p[b][j] - base);
+          l[b] += p[b][j];
+        }
+        if constexpr (!kWide) {
+          float top = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[b][j] *= vs[j], top = fmaxf(top, p[b][j]);
+          top = max_over_groups(top);
+          const float ref = fmaxf(o_ref[b], top > 0.f ? base + (float)__builtin_amdgcn_frexp_expf(top) : -INFINITY);
+          const float factor = ref == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base - ref);
+          shrink = weight(o_ref[b], ref);
+          o_ref[b] = ref;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[b][j] *= factor;
+        }
+        // (a head of no tokens yet has nothing to scale: 0 by whatever)
+        if (__any(shrink != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < kAcc; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[b][i][k] *= shrink;
+        }
       }
+      C8 pf[NT];
+#pragma unroll
+      for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[b][j] = (C)p[b][j];
+      if constexpr (!decltype(last)::value) load_scales(next_row);
+
+      // ---- values ---------------------------------------------------------------------------------------------
+      if (!whole) {
+        // what lies in dead places may be anything: its values count as zeros, not as zero times them
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j >= low && j < high) continue;
+#pragma unroll
+          for (int i = 0; i < kVDwords; ++i) vr[j][i] = 0u;
+        }
+      }
+      int at_acc = 0;
+#pragma unroll
+      for (int blk = 0; blk < VB::count(); ++blk) {
+        const int e_count = VB::e(blk), at = VB::dword(blk, kBytes);
+        if constexpr (kWide) {
+#pragma unroll
+          for (int e = 0; e < e_count; ++e) {
+            uint4_t w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][at + (e >> 1)], vr[2 * i][at + (e >> 1)], (e & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int b = 0; b < NT; ++b) acc[b][at_acc + e] = mfma16<C>(__builtin_bit_cast(C8, w), pf[b], acc[b][at_acc + e]);
+          }
+        } else {
+#pragma unroll
+          for (int dw = 0; dw < (e_count + 3) / 4; ++dw) {
+            uint4_t tr[2];  // byte e of four tokens
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint4_t w = {vr[4 * half][at + dw], vr[4 * half + 1][at + dw], vr[4 * half + 2][at + dw], vr[4 * half + 3][at + dw]};
+              tr[half] = transpose4x4_bytes(w);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (4 * dw + e >= e_count) break;
+              uint32_t h[4];
+              codes4_to_half<FORMAT>(tr[0][e], h[0], h[1]);
+              codes4_to_half<FORMAT>(tr[1][e], h[2], h[3]);
+              const uint4_t w = {h[0], h[1], h[2], h[3]};
+#pragma unroll
+              for (int b = 0; b < NT; ++b)
+                acc[b][at_acc + 4 * dw + e] = mfma16<C>(__builtin_bit_cast(C8, w), pf[b], acc[b][at_acc + 4 * dw + e]);
+            }
+          }
+        }
+        at_acc += e_count;
+      }
+      if constexpr (!decltype(last)::value) {
+        load_values(next_row);
+        page = page_next;
+        page_next = page_of((next + kAttnWaves) * kAttnTile + g * 8);
+      }
+    };
+    if (tile < end) {
+      for (; tile + kAttnWaves < end; tile += kAttnWaves) take(std::false_type{});
+      take(std::true_type{});
     }
-    // ---- running maximum and sum ----------------------------------------------------------------------------
+
+    // ---- the waves' results, joined in their order -------------------------------------------------------------
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
-      float most = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[b][j] *= q_scale[b];
-        if constexpr (!kWide) p[b][j] *= ks[j];
-        if (!whole && (j < low || j >= high)) p[b][j] = -INFINITY;
-        most = fmaxf(most, p[b][j]);
-      }
-      most = fmaxf(m[b], max_over_groups(most));
-      const float base = most == -INFINITY ? 0.f : most;
-      float shrink = weight(m[b], base);
-      m[b] = most;
-      l[b] *= shrink;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[b][j] = __builtin_amdgcn_exp2f(p[b][j] - base);
-        l[b] += p[b][j];
-      }
-      if constexpr (!kWide) {
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[b][j] *= vs[j], top = fmaxf(top, p[b][j]);
-        top = max_over_groups(top);
-        const float ref = fmaxf(o_ref[b], top > 0.f ? base + (float)__builtin_amdgcn_frexp_expf(top) : -INFINITY);
-        const float factor = ref == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base - ref);
-        shrink = weight(o_ref[b], ref);
-        o_ref[b] = ref;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[b][j] *= factor;
-      }
-#pragma unroll
-      for (int i = 0; i < kAcc; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[b][i][k] *= shrink;
+      l[b] = sum_over_groups(l[b]);
+      if (g == 0) sm[wave][16 * b + n][0] = m[b], sm[wave][16 * b + n][1] = l[b], sm[wave][16 * b + n][2] = kWide ? m[b] : o_ref[b];
     }
-    C8 pf[NT];
 #pragma unroll
-    for (int b = 0; b < NT; ++b)
+    for (int b = 0; b < NT; ++b) {
+      if (b > 0) __syncthreads();
+      int at_acc = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pf[b][j] = (C)p[b][j];
-    // ---- values ---------------------------------------------------------------------------------------------
-    int at_acc = 0;
+      for (int blk = 0; blk < VB::count(); ++blk) {
 #pragma unroll
-    for (int blk = 0; blk < VB::count(); ++blk) {
-      const int e_count = VB::e(blk), at = VB::dword(blk, kBytes);
-      if constexpr (kWide) {
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < e_count; ++e) {
-          uint4_t w;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][at + (e >> 1)], vr[2 * i][at + (e >> 1)], (e & 1) ? 0x07060302u : 0x05040100u);
-#pragma unroll
-          for (int b = 0; b < NT; ++b) acc[b][at_acc + e] = mfma16<C>(__builtin_bit_cast(C8, w), pf[b], acc[b][at_acc + e]);
-        }
-      } else {
-#pragma unroll
-        for (int dw = 0; dw < (e_count + 3) / 4; ++dw) {
-          uint4_t tr[2];  // byte e of four tokens
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint4_t w = {vr[4 * half][at + dw], vr[4 * half + 1][at + dw], vr[4 * half + 2][at + dw], vr[4 * half + 3][at + dw]};
-            tr[half] = transpose4x4_bytes(w);
+          for (int e = 0; e < VB::e(blk); ++e) {
+            const int d = VB::start(blk) + (4 * g + i) * VB::e(blk) + e;
+            result(wave, n)[d] = acc[b][at_acc + e][i];
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (4 * dw + e >= e_count) break;
-            uint32_t h[4];
-            codes4_to_half<FORMAT>(tr[0][e], h[0], h[1]);
-            codes4_to_half<FORMAT>(tr[1][e], h[2], h[3]);
-            const uint4_t w = {h[0], h[1], h[2], h[3]};
-#pragma unroll
-            for (int b = 0; b < NT; ++b)
-              acc[b][at_acc + 4 * dw + e] = mfma16<C>(__builtin_bit_cast(C8, w), pf[b], acc[b][at_acc + 4 * dw + e]);
-          }
-        }
+        at_acc += VB::e(blk);
       }
-      at_acc += e_count;
-    }
-  }
-
-  // ---- the waves' results, joined in their order -----------------------------------------------------------------
-  __shared__ float sm[kAttnWaves][16 * NT][3];
-  extern __shared__ float so[];  // [waves][16 heads][D + 4]
-  constexpr int kRow = D + 4;
+      __syncthreads();
+      // 16 lanes a head
+      const int row = threadIdx.x >> 4, head_in_group = (head_block * NT + b) * 16 + row;
+      if (head_in_group < group) {
+        const int head = kv_head * group + head_in_group;
+        float most = -INFINITY;
 #pragma unroll
-  for (int b = 0; b < NT; ++b) {
-    l[b] = sum_over_groups(l[b]);
-    if (g == 0) sm[wave][16 * b + n][0] = m[b], sm[wave][16 * b + n][1] = l[b], sm[wave][16 * b + n][2] = kWide ? m[b] : o_ref[b];
-  }
-  for (int b = 0; b < NT; ++b) {
-    __syncthreads();
-    int at_acc = 0;
+        for (int w = 0; w < kAttnWaves; ++w) most = fmaxf(most, sm[w][16 * b + row][0]);
+        const float sink = complete && a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
+        const float base = fmaxf(most, sink);
+        float factor[kAttnWaves], total_weight = weight(sink, base);
 #pragma unroll
-    for (int blk = 0; blk < VB::count(); ++blk) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < VB::e(blk); ++e) {
-          const int d = VB::start(blk) + (4 * g + i) * VB::e(blk) + e;
-          so[(wave * 16 + n) * kRow + d] = acc[b][at_acc + e][i];
+        for (int w = 0; w < kAttnWaves; ++w) {
+          factor[w] = weight(sm[w][16 * b + row][2], base);
+          total_weight += weight(sm[w][16 * b + row][0], base) * sm[w][16 * b + row][1];
         }
-      at_acc += VB::e(blk);
-    }
-    __syncthreads();
-    // 16 lanes a head
-    const int row = threadIdx.x >> 4, head_in_group = (head_block * NT + b) * 16 + row;
-    if (head_in_group < group) {
-      const int head = kv_head * group + head_in_group;
-      float most = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kAttnWaves; ++w) most = fmaxf(most, sm[w][16 * b + row][0]);
-      const float sink = a.splits == 1 && a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
-      const float base = fmaxf(most, sink);
-      float factor[kAttnWaves], sum = weight(sink, base);
-#pragma unroll
-      for (int w = 0; w < kAttnWaves; ++w) {
-        factor[w] = weight(sm[w][16 * b + row][2], base);
-        sum += weight(sm[w][16 * b + row][0], base) * sm[w][16 * b + row][1];
-      }
-      const size_t at = (size_t)sequence * a.heads + head;
-      if (a.splits == 1) {
-        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-        for (int d = threadIdx.x & 15; d < D; d += 16) {
-          float x = 0.f;
-#pragma unroll
-          for (int w = 0; w < kAttnWaves; ++w) x += factor[w] * so[(w * 16 + row) * kRow + d];
-          reinterpret_cast<T*>(a.out)[at * D + d] = (T)(x * inv);
-        }
-        if (a.lse && (threadIdx.x & 15) == 0)
-          a.lse[at] = base == -INFINITY ? -INFINITY : (base + log2f(sum)) * 0.693147180559945309f;
-      } else {
-        const size_t part = at * a.splits + split;
-        if (most != -INFINITY) {
+        if (complete) {
+          const size_t at = (size_t)this_sequence * a.heads + head;
+          const float inv = total_weight > 0.f ? 1.f / total_weight : (total_weight == 0.f ? 0.f : total_weight);
           for (int d = threadIdx.x & 15; d < D; d += 16) {
             float x = 0.f;
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) x += factor[w] * so[(w * 16 + row) * kRow + d];
+            for (int w = 0; w < kAttnWaves; ++w) x += factor[w] * result(w, row)[d];
+            reinterpret_cast<T*>(a.out)[at * D + d] = (T)(x * inv);
+          }
+          if (a.lse && (threadIdx.x & 15) == 0)
+            a.lse[at] = base == -INFINITY ? -INFINITY : (base + log2f(total_weight)) * 0.693147180559945309f;
+        } else {
+          // the piece that a head begins with is a workgroup's second, any other its first
+          const size_t part = ((size_t)blockIdx.x * 2 + (unit0 == 0)) * a.rows + 16 * b + row;
+          for (int d = threadIdx.x & 15; d < D; d += 16) {
+            float x = 0.f;
+#pragma unroll
+            for (int w = 0; w < kAttnWaves; ++w) x += factor[w] * result(w, row)[d];
             a.part_o[part * D + d] = x;
           }
+          if ((threadIdx.x & 15) == 0) a.part_ml[2 * part] = most, a.part_ml[2 * part + 1] = total_weight;
         }
-        if ((threadIdx.x & 15) == 0) a.part_ml[2 * part] = most, a.part_ml[2 * part + 1] = sum;
       }
     }
+    if (unit0 == 0 && threadIdx.x == 0 && a.pieces) {
+      int* const pieces = a.pieces + 2 * ((size_t)this_sequence * columns + column);
+      pieces[0] = blockIdx.x, pieces[1] = complete ? blockIdx.x : shares.owner(column_begin + cost - 1);
+    }
+    __syncthreads();  // the LDS is free again
   }
 }
 
 template <class T, int FORMAT, int D, int NT>
 int launch_attention(const AttnArgs& a, hipStream_t stream) {
-  constexpr int kLds = kAttnWaves * 16 * (D + 4) * 4;
+  constexpr int kLds = kAttnWaves * attention_wave_lds(D, FORMAT);
   if constexpr (kLds > 65536 - 4096) {
     static bool raised[kMaxDevices];
     if (raise_lds_limit<kLds>(attention_kernel<T, FORMAT, D, NT>, raised) != 0) return -1;
   }
-  attention_kernel<T, FORMAT, D, NT><<<dim3(a.splits, a.shape.kv_heads * a.head_blocks, a.sequences), 64 * kAttnWaves, kLds, stream>>>(a);
+  attention_kernel<T, FORMAT, D, NT><<<a.workgroups, 64 * kAttnWaves, kLds, stream>>>(a);
   DQ_CHECK_HIP(hipGetLastError());
   return 0;
 }

@@ -16,7 +16,8 @@ int kv_cache_write(const void* X, const void* V, const float* Table, const int* 
 int kv_cache_read(const void* KCache, const void* VCache, const float* KScale, const float* VScale, const int* PageTable,
                   const int* Starts, void* KV, int sequences, int tokens, int kv_heads, int head_dim, int pages, int page_shift,
                   int max_pages, int bf16, int format, hipStream_t stream);
-size_t attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim, long capacity);
+size_t attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim, int format, long capacity, int window);
+bool attention_fits(int sequences, int heads, int kv_heads, long capacity);
 bool attention_head_dim(int d);
 int attention_decode(const void* Q, const void* KCache, const void* VCache, const float* KScale, const float* VScale,
                      const int* PageTable, const int* Lengths, const float* Sinks, void* Out, float* Lse, void* Workspace,
@@ -148,9 +149,10 @@ extern "C" int call_kv_cache_read(const void* KCache, const void* VCache, const 
                        (hipStream_t)stream);
 }
 
-extern "C" size_t dq_paged_attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim, int page_size, int max_pages) {
-  if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || page_size <= 0 || max_pages <= 0 || heads % kv_heads != 0) return 0;
-  return attention_workspace_bytes(sequences, heads, kv_heads, head_dim, (long)max_pages * page_size);
+extern "C" size_t dq_paged_attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim, int page_size, int max_pages,
+                                                     int window, int cache_format) {
+  if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || page_size <= 0 || max_pages <= 0 || window < 0 || heads % kv_heads != 0) return 0;
+  return attention_workspace_bytes(sequences, heads, kv_heads, head_dim, cache_format, (long)max_pages * page_size, window);
 }
 
 extern "C" int call_paged_attention_decode(const void* Q, const void* KCache, const void* VCache, const void* KScale, const void* VScale,
@@ -165,12 +167,14 @@ extern "C" int call_paged_attention_decode(const void* Q, const void* KCache, co
   if (!attention_head_dim(head_dim)) DQ_FAIL("%s: head_dim must be 64, 80, 96, 112, 128, 160, 192 or 256 (got %d)", fn, head_dim);
   if (heads <= 0 || heads % kv_heads != 0) DQ_FAIL("%s: heads must be a multiple of kv_heads=%d (got %d)", fn, kv_heads, heads);
   if (sequences > 65535 || heads > 65535) DQ_FAIL("%s: at most 65535 sequences and heads (got %d and %d)", fn, sequences, heads);
+  if (!attention_fits(sequences, heads, kv_heads, (long)max_pages * page_size))
+    DQ_FAIL("%s: %d sequences of %d heads and up to %ld tokens: more than 2^31 pieces of %d tokens", fn, sequences, heads, (long)max_pages * page_size, 128);
   if (window < 0) DQ_FAIL("%s: window must be 0 (none) or positive (got %d)", fn, window);
   if (!isfinite(scale)) DQ_FAIL("%s: scale must be finite", fn);
   if (!Q || !Lengths || !Out) DQ_FAIL("%s: Q, Lengths and Out are expected to have non-NULL data pointers", fn);
   if (!on_16(Q) || !on_16(Out) || !on_4(Lengths) || !on_4(Sinks) || !on_4(Lse))
     DQ_FAIL("%s: Q and Out must be 16-byte, Lengths, Sinks and Lse 4-byte aligned", fn);
-  const size_t need = dq_paged_attention_workspace_bytes(sequences, heads, kv_heads, head_dim, page_size, max_pages);
+  const size_t need = dq_paged_attention_workspace_bytes(sequences, heads, kv_heads, head_dim, page_size, max_pages, window, cache_format);
   if (need && (!Workspace || !on_16(Workspace) || workspace_bytes < need))
     DQ_FAIL("%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, Workspace ? workspace_bytes : (size_t)0);
   return attention_decode(Q, KCache, VCache, (const float*)KScale, (const float*)VScale, (const int*)PageTable, (const int*)Lengths,

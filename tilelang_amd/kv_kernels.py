@@ -259,7 +259,7 @@ def paged_attention_decode(sequences: int, heads: int, kv_heads: int, head_dim: 
     params.append(KernelParam("out", pool.dtype, (sequences, heads, head_dim)))
     if with_lse:
         params.append(KernelParam("lse", torch.float32, (sequences, heads)))
-    room = int(_lib.load_library().dq_paged_attention_workspace_bytes(sequences, heads, kv_heads, head_dim, page_size, max_pages))
+    room = int(_lib.load_library().dq_paged_attention_workspace_bytes(sequences, heads, kv_heads, head_dim, page_size, max_pages, window, pool.ints[1]))
     if room:
         params.append(KernelParam("Workspace", torch.uint8, (room,)))
     slots = (0, *pool.slots(1), n, n + 1, n + 2 if sinks else None, out, out + 1 if with_lse else None, len(params) - 1 if room else None)
