@@ -335,42 +335,46 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
       }
     };
 
+    int tile = begin + wave;
+    int page = page_of(tile * kAttnTile + g * 8), page_next = -1, page_after = -1;
+    typename Vec8<T>::type q_raw[NT][kSteps];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int row = (head_block * NT + t) * 16 + n;
+      const T* const qrow = reinterpret_cast<const T*>(a.q) + ((size_t)this_sequence * a.heads + (size_t)kv_head * group + row) * D;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int d = key_element<D, kWide>(s, g);
+        q_raw[t][s] = typename Vec8<T>::type{};
+        if (row < group && d < D) q_raw[t][s] = *reinterpret_cast<const typename Vec8<T>::type*>(qrow + d);
+      }
+    }
+
     // The first tile's loads, and the page ids of the second: from here on keys, values and page ids are asked for a tile
     // ahead, each as soon as its registers are free.
-    int tile = begin + wave;
-    int page = page_of(tile * kAttnTile + g * 8);
     if (tile < end) {
       load_keys(page, tile);
+      page_next = page_of((tile + kAttnWaves) * kAttnTile + g * 8);
       const size_t row = row_of(page, tile * kAttnTile + g * 8);
       load_scales(row);
       load_values(row);
     }
-    int page_next = page_of((tile + kAttnWaves) * kAttnTile + g * 8);
 
     // ---- queries: the second operand of the first product, held for the whole walk -----------------------------
     C8 q[NT][kSteps];
     float q_scale[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int row = (head_block * NT + t) * 16 + n;
-      const T* const qrow = reinterpret_cast<const T*>(a.q) + ((size_t)this_sequence * a.heads + (size_t)kv_head * group + row) * D;
-      typename Vec8<T>::type h[kSteps];
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int d = key_element<D, kWide>(s, g);
-        h[s] = typename Vec8<T>::type{};
-        if (row < group && d < D) h[s] = *reinterpret_cast<const typename Vec8<T>::type*>(qrow + d);
-      }
       q_scale[t] = a.score_scale;
       if constexpr (kWide) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) q[t][s] = h[s];
+        for (int s = 0; s < kSteps; ++s) q[t][s] = q_raw[t][s];
       } else {
         float most = 0.f;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf((float)h[s][i]));
+          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf((float)q_raw[t][s][i]));
         most = max_over_groups(most);
         const int e = most > 0.f ? 14 - ilogbf(most) : 0;  // 2^e * most in [2^14, 2^15)
         const int shift = min(max(e, -126), 126);
@@ -378,7 +382,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) q[t][s][i] = (C)ldexpf((float)h[s][i], shift);
+          for (int i = 0; i < 8; ++i) q[t][s][i] = (C)ldexpf((float)q_raw[t][s][i], shift);
       }
     }
 
@@ -441,6 +445,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
       size_t next_row = 0;
       if constexpr (!decltype(last)::value) {
         load_keys(page_next, next);
+        // (before the values, so that the wait for it waits for none of them)
+        page_after = page_of((next + kAttnWaves) * kAttnTile + g * 8);
         next_row = row_of(page_next, next * kAttnTile + g * 8);
       }
 
@@ -554,8 +560,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
       }
       if constexpr (!decltype(last)::value) {
         load_values(next_row);
-        page = page_next;
-        page_next = page_of((next + kAttnWaves) * kAttnTile + g * 8);
+        page = page_next, page_next = page_after;
       }
     };
     if (tile < end) {

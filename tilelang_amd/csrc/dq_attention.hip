@@ -19,6 +19,7 @@ namespace {
 // pieces): a workgroup a head, its groups take the pieces in turn and are added at the end.  Else (many columns, few
 // pieces): a workgroup a column, a group a head.
 constexpr int kJoinGroups = 8;
+typedef float float2_t __attribute__((ext_vector_type(2)));
 template <class T, bool SPREAD>
 __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs a) {
   const int columns = a.shape.kv_heads * a.head_blocks, sequence = blockIdx.x / columns, column = blockIdx.x - sequence * columns;
@@ -26,51 +27,69 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs a) {
   if (count <= 1) return;  // written by the workgroup that had it whole
   const int D = a.shape.head_dim, group = a.heads / a.shape.kv_heads, kv_head = column / a.head_blocks, block = column - kv_head * a.head_blocks;
   __shared__ float4_t so[SPREAD ? kJoinGroups : 1][kMaxHeadDim / 4];
-  __shared__ float ss[kJoinGroups];
+  __shared__ float2_t ss[kJoinGroups];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int rows = min(a.rows, group - block * a.rows);
   for (int row = SPREAD ? blockIdx.y : part; row < rows; row += SPREAD ? gridDim.y : kJoinGroups) {
     const int head = kv_head * group + block * a.rows + row;
-    auto at = [&](int i) { return ((size_t)(first + i) * 2 + (i == 0)) * a.rows + row; };
-    float most = -INFINITY;
-    for (int i = lane; i < count; i += 32) most = fmaxf(most, a.part_ml[2 * at(i)]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-    const float sink = a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
-    const float base = fmaxf(most, sink);
+    // four pieces at a time: their loads together, then the running maximum and sums
+    float m = -INFINITY, sum = 0.f;
     float4_t x[2] = {};
-    float sum = 0.f;
-#pragma unroll 4
-    for (int i = SPREAD ? part : 0; i < count; i += SPREAD ? kJoinGroups : 1) {
-      const size_t k = at(i);
-      const float w = weight(a.part_ml[2 * k], base);
-      sum += w * a.part_ml[2 * k + 1];
+    constexpr int kStep = SPREAD ? kJoinGroups : 1;
+    for (int i0 = SPREAD ? part : 0; i0 < count; i0 += 4 * kStep) {
+      float2_t ml[4];
+      float4_t o[4][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int d = 4 * lane + 128 * j;
-        if (d < D) x[j] += w * *reinterpret_cast<const float4_t*>(a.part_o + k * D + d);
+      for (int p = 0; p < 4; ++p) {
+        const int i = min(i0 + p * kStep, count - 1);
+        const size_t k = ((size_t)(first + i) * 2 + (i == 0)) * a.rows + row;
+        ml[p] = *reinterpret_cast<const float2_t*>(a.part_ml + 2 * k);
+        if (i0 + p * kStep >= count) ml[p] = float2_t{-INFINITY, 0.f};
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (4 * lane + 128 * j < D) o[p][j] = *reinterpret_cast<const float4_t*>(a.part_o + k * D + 4 * lane + 128 * j);
+      }
+      const float to = fmaxf(fmaxf(m, fmaxf(ml[0][0], ml[1][0])), fmaxf(ml[2][0], ml[3][0]));
+      const float keep = weight(m, to);
+      m = to, sum *= keep;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) x[j] *= keep;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float w = weight(ml[p][0], to);
+        sum += w * ml[p][1];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (4 * lane + 128 * j < D && i0 + p * kStep < count) x[j] += w * o[p][j];
       }
     }
     if constexpr (SPREAD) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         if (4 * lane + 128 * j < D) so[part][lane + 32 * j] = x[j];
-      if (lane == 0) ss[part] = sum;
+      if (lane == 0) ss[part] = float2_t{m, sum};
       __syncthreads();
       if (part == 0) {
-        sum = 0.f;
+        m = -INFINITY, sum = 0.f;
         x[0] = x[1] = float4_t{};
 #pragma unroll
+        for (int p = 0; p < kJoinGroups; ++p) m = fmaxf(m, ss[p][0]);
+#pragma unroll
         for (int p = 0; p < kJoinGroups; ++p) {
-          sum += ss[p];
+          const float w = weight(ss[p][0], m);
+          sum += w * ss[p][1];
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            if (4 * lane + 128 * j < D) x[j] += so[p][lane + 32 * j];
+            if (4 * lane + 128 * j < D) x[j] += w * so[p][lane + 32 * j];
         }
       }
     }
     if (!SPREAD || part == 0) {
-      sum += weight(sink, base);
+      const float sink = a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
+      const float base = fmaxf(m, sink), keep = weight(m, base);
+      sum = sum * keep + weight(sink, base);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) x[j] *= keep;
       const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
       const size_t to = (size_t)sequence * a.heads + head;
       typedef T T4 __attribute__((ext_vector_type(4)));
