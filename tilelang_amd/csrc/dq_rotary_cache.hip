@@ -14,6 +14,8 @@
 // partner half of a row comes from the caches by a second load of the same lines.
 #include "dq_kv.h"
 
+#include <algorithm>
+
 namespace dq {
 
 namespace {
@@ -227,7 +229,9 @@ int launch_rows_lanes(const RowArgs& a, hipStream_t stream) {
   DQ_FAIL("a head of %d is beyond the cache's %d", a.head_dim, kMaxHeadDim);
 }
 
-// Row (token of the packed result, head): the sequence whose tokens it is among, its page, its codes times its scale.
+// Reading back: a workgroup has kReadTokens(...) tokens of the packed result.  It first finds each one's sequence, page and place,
+// then its threads take the tokens' pieces of eight elements in the order of the result, which is written as one run, 16 bytes
+// a lane side by side (16 codes a lane, two stores 32 bytes apart, fill no line at once: 290 against XXX us).
 struct ReadArgs {
   const void* cache[2];
   const float* scale[2];
@@ -236,52 +240,94 @@ struct ReadArgs {
   void* out;  // [2][tokens][kv_heads][head_dim]
   int sequences, tokens, max_pages;
   CacheShape shape;
+  int tokens_each;             // of a workgroup, at most kReadTokens
+  int row_pieces, all_pieces;  // of a head, of a token
+  unsigned row_magic, all_magic;  // ceil(2^32 / row_pieces), ceil(2^32 / all_pieces)
 };
+constexpr int kReadTokens = 64;
+constexpr int kReadStarts = 1024;  // starts of so many sequences are looked through in LDS
 
-template <class T, int LANES, int FORMAT>
+// i / n by its magic number: right for i < 2^16, as i * (magic * n - 2^32) < 2^32 there (n <= 2^16); n = 1 has none
+__device__ __forceinline__ int divided(int i, int n, unsigned magic) { return n == 1 ? i : (int)__umulhi((unsigned)i, magic); }
+
+template <class T, int FORMAT>
 __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
-  const int lane = threadIdx.x % LANES, d = lane * 8;
-  const unsigned group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  const int token = group / a.shape.kv_heads, head = group - token * a.shape.kv_heads;
-  if (token >= a.tokens || d >= a.shape.head_dim) return;
-  // the last sequence that starts at or before the token
-  int lo = 0, hi = a.sequences;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.starts[mid] <= token) lo = mid;
-    else hi = mid;
+  constexpr bool kWide = cache_is_16bit(FORMAT);
+  constexpr int kElements = 8, PIECE = kWide ? 16 : 8;
+  __shared__ int s_starts[kReadStarts + 1];
+  __shared__ int s_page[kReadTokens], s_place[kReadTokens];
+  const int token0 = blockIdx.x * a.tokens_each, count = min(a.tokens_each, a.tokens - token0);
+  const bool staged = a.sequences <= kReadStarts;
+  if (staged) {
+    for (int i = threadIdx.x; i <= a.sequences; i += 256) s_starts[i] = a.starts[i];
+    __syncthreads();
   }
-  const int position = token - a.starts[lo];
-  const int column = position >> a.shape.page_shift;
-  int page = -1;
-  if (position >= 0 && token < a.starts[lo + 1] && column < a.max_pages) page = a.table[(size_t)lo * a.max_pages + column];
-  const bool there = (unsigned)page < (unsigned)a.shape.pages;
-  const size_t at = cache_row(a.shape, there ? page : 0, head, position & ((1 << a.shape.page_shift) - 1));
+  if ((int)threadIdx.x < count) {
+    const int token = token0 + threadIdx.x;
+    auto start = [&](int b) { return staged ? s_starts[b] : a.starts[b]; };
+    // the last sequence that starts at or before the token
+    int lo = 0, hi = a.sequences;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start(mid) <= token) lo = mid;
+      else hi = mid;
+    }
+    const int position = token - start(lo), column = position >> a.shape.page_shift;
+    int page = -1;
+    if (position >= 0 && token < start(lo + 1) && column < a.max_pages) page = a.table[(size_t)lo * a.max_pages + column];
+    s_page[threadIdx.x] = (unsigned)page < (unsigned)a.shape.pages ? page : -1;
+    s_place[threadIdx.x] = position & ((1 << a.shape.page_shift) - 1);
+  }
+  __syncthreads();
+  const int which = blockIdx.y;
+  const char* const cache = reinterpret_cast<const char*>(which ? a.cache[1] : a.cache[0]);
+  const float* const scale = which ? a.scale[1] : a.scale[0];
+  T* const out = reinterpret_cast<T*>(a.out) + ((size_t)which * a.tokens + token0) * ((size_t)a.all_pieces * kElements);
+  typedef uint32_t Raw __attribute__((ext_vector_type(PIECE / 4)));
+  const int pieces = count * a.all_pieces;
+  constexpr int U = 4;
+  for (int i0 = threadIdx.x; i0 < pieces; i0 += 256 * U) {
+    Raw raw[U];
+    float s[U];
+    bool there[U];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    float x[8] = {};
-    if (there) {
-      if constexpr (cache_is_16bit(FORMAT)) {
-        load8(reinterpret_cast<const T*>(a.cache[which]) + at * a.shape.head_dim + d, x);
+    for (int k = 0; k < U; ++k) {  // (without branches, so that the loads are in flight together)
+      const int i = min(i0 + 256 * k, pieces - 1);
+      const int token = divided(i, a.all_pieces, a.all_magic), piece = i - token * a.all_pieces;
+      const int head = divided(piece, a.row_pieces, a.row_magic), in_row = piece - head * a.row_pieces;
+      const int page = s_page[token];
+      there[k] = page >= 0;
+      const size_t row = cache_row(a.shape, max(page, 0), head, s_place[token]);
+      raw[k] = __builtin_nontemporal_load(reinterpret_cast<const Raw*>(cache + (row * a.row_pieces + in_row) * PIECE));
+      if constexpr (!kWide) s[k] = scale[row];
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + 256 * k;
+      if (i >= pieces) break;
+      if constexpr (kWide) {
+        __builtin_nontemporal_store(there[k] ? raw[k] : Raw{}, reinterpret_cast<Raw*>(out + (size_t)i * kElements));
       } else {
-        const float s = a.scale[which][at];
-        codes8_to_float<FORMAT>(*reinterpret_cast<const uint2_t*>(reinterpret_cast<const uint8_t*>(a.cache[which]) + at * a.shape.head_dim + d), x);
+        float x[8];
+        codes8_to_float<FORMAT>(raw[k], x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= s;
+        for (int j = 0; j < 8; ++j) x[j] = there[k] ? x[j] * s[k] : 0.f;
+        __builtin_nontemporal_store(round8<T>(x), reinterpret_cast<typename Vec8<T>::type*>(out + (size_t)i * kElements));
       }
     }
-    T* const out = reinterpret_cast<T*>(a.out) + (((size_t)which * a.tokens + token) * a.shape.kv_heads + head) * a.shape.head_dim + d;
-    *reinterpret_cast<typename Vec8<T>::type*>(out) = round8<T>(x);
   }
 }
 
 template <class T, int FORMAT>
-int launch_read(const ReadArgs& a, hipStream_t stream) {
-  const long rows = (long)a.tokens * a.shape.kv_heads;
-  auto grid = [&](int lanes) { return dim3((unsigned)((rows + 256 / lanes - 1) / (256 / lanes))); };
-  if (a.shape.head_dim <= 64) read_kernel<T, 8, FORMAT><<<grid(8), 256, 0, stream>>>(a);
-  else if (a.shape.head_dim <= 128) read_kernel<T, 16, FORMAT><<<grid(16), 256, 0, stream>>>(a);
-  else read_kernel<T, 32, FORMAT><<<grid(32), 256, 0, stream>>>(a);
+int launch_read(ReadArgs a, hipStream_t stream) {
+  a.row_pieces = a.shape.head_dim / 8, a.all_pieces = a.row_pieces * a.shape.kv_heads;
+  auto magic = [](int n) { return (unsigned)(((1ull << 32) + n - 1) / n); };
+  a.row_magic = magic(a.row_pieces), a.all_magic = magic(a.all_pieces);
+  // eight pieces a thread, fewer where that leaves compute units idle
+  int each = std::max(1, std::min(kReadTokens, 2048 / a.all_pieces));
+  while (each > 1 && (long)(a.tokens + each - 1) / each * 2 < 4 * 256) each = (each + 1) / 2;
+  a.tokens_each = each;
+  read_kernel<T, FORMAT><<<dim3((a.tokens + each - 1) / each, 2), 256, 0, stream>>>(a);
   DQ_CHECK_HIP(hipGetLastError());
   return 0;
 }
