@@ -61,12 +61,13 @@ __device__ __forceinline__ Span span_of(int length, int capacity, int window) {
   return s;
 }
 
-// How the work is shared out.  The tokens that a key-value head (a column) has of a sequence cost their units and one more: what
-// a workgroup does before the first and after the last takes about as long.  All costs in a row, sequence by
+// How the work is shared out.  The tokens that a key-value head (a column) has of a sequence cost their units and two more: what
+// a workgroup does before the first and after the last takes about as long (64 sequences of 0 to 16000 tokens, fp8: 158 us
+// without, 127 with one, 124 with two or three; short windows 11.7, with three 13.0).  All costs in a row, sequence by
 // sequence and in a sequence column by column, are cut into equal shares, one a workgroup, whatever the lengths are; a
 // cut inside a column makes pieces of it, which the join adds up.  A column of up to two units is not worth a
 // join: a cut there moves to its nearer end.
-constexpr int kWholeUnits = 2;
+constexpr int kWholeUnits = 2, kColumnCost = 2;
 struct Shares {
   unsigned each, more;  // the first `more` workgroups have one more
   __device__ __forceinline__ Shares(unsigned total, unsigned workgroups) : each(total / workgroups), more(total - total / workgroups * workgroups) {}
@@ -125,8 +126,9 @@ __device__ __forceinline__ float4_t mfma16(typename Vec8<T>::type a, typename Ve
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Four codes (a dword) -> four fp16, exact.
-template <int FORMAT>
+// Four codes (a dword) -> four fp16, exact; int8 with kKeyBias on top where BIASED.
+constexpr float kKeyBias = 1152.f;
+template <int FORMAT, bool BIASED = false>
 __device__ __forceinline__ void codes4_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (FORMAT == CACHE_FP8) {
     lo = as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
@@ -134,9 +136,11 @@ __device__ __forceinline__ void codes4_to_half(uint32_t w, uint32_t& lo, uint32_
   } else {
     // code + 128 in the last byte of an fp16 whose last place is 1: 1024 + 128 + code
     const uint32_t u = w ^ 0x80808080u;
-    const half2_t bias = {(half_t)1152.f, (half_t)1152.f};
-    lo = as_u32(as_half2(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
-    hi = as_u32(as_half2(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
+    lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u), hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    if constexpr (!BIASED) {
+      const half2_t bias = {(half_t)kKeyBias, (half_t)kKeyBias};
+      lo = as_u32(as_half2(lo) - bias), hi = as_u32(as_half2(hi) - bias);
+    }
   }
 }
 
@@ -172,6 +176,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
   constexpr bool kWide = cache_is_16bit(FORMAT);
   using C = typename std::conditional<kWide, T, half_t>::type;  // what the products are taken in
   typedef typename Vec8<C>::type C8;
+  constexpr bool kBiased = FORMAT == CACHE_I8;  // int8 keys are multiplied as code + kKeyBias, of which kKeyBias * sum q is taken off
   constexpr int kBytes = kWide ? 2 : 1;
   constexpr int kSteps = (D + 31) / 32;
   using VB = ValueBlocks<D>;
@@ -184,7 +189,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
 
   __shared__ float sm[kAttnWaves][16 * NT][3];
   __shared__ int s_scan[kAttnWaves];
-  __shared__ unsigned s_cut[2][3];  // where the share begins and ends: cost, sequence, the sequence's first cost
+  __shared__ unsigned s_cut[2][4];  // where the share begins and ends: cost, sequence, the sequence's first cost, its length
   extern __shared__ __align__(16) char lds[];
   constexpr int kRow = D + 4;
 
@@ -199,8 +204,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
   // ---- this workgroup's share: a running sum of the sequences' costs ---------------------------------------------
   const int per_thread = (a.sequences + 64 * kAttnWaves - 1) / (64 * kAttnWaves);
   const int seq_begin = min((int)threadIdx.x * per_thread, a.sequences), seq_end = min(seq_begin + per_thread, a.sequences);
-  int mine = 0;
-  for (int b = seq_begin; b < seq_end; ++b) mine += span_of(a.lengths[b], capacity, a.window).units + 1;
+  int mine = 0, length_here = 0;  // (of the last of this thread's sequences: of its one, where a thread has one)
+  for (int b = seq_begin; b < seq_end; ++b) length_here = a.lengths[b], mine += span_of(length_here, capacity, a.window).units + kColumnCost;
   int sum = mine;  // inclusive
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -224,7 +229,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
     if (!(sum - mine <= at && at < sum)) continue;
     int b = seq_begin, before = sum - mine;
     for (;; ++b) {
-      const int units = span_of(a.lengths[b], capacity, a.window).units, cost = units + 1;
+      const int length = per_thread == 1 ? length_here : a.lengths[b];
+      const int units = span_of(length, capacity, a.window).units, cost = units + kColumnCost;
       if (at >= before + cost) {
         before += cost;
         continue;
@@ -234,6 +240,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
       const unsigned moved = units <= kWholeUnits ? cut - off + (2 * off >= (unsigned)cost ? cost : 0) : cut;
       const bool next = moved == begin + (unsigned)cost * columns;
       s_cut[side][0] = moved, s_cut[side][1] = b + next, s_cut[side][2] = next ? moved : begin;
+      s_cut[side][3] = next && b + 1 < a.sequences ? a.lengths[b + 1] : length;
       break;
     }
   }
@@ -242,31 +249,33 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
   const unsigned u_end = __builtin_amdgcn_readfirstlane(s_cut[1][0]);
   int sequence = __builtin_amdgcn_readfirstlane(s_cut[0][1]);
   unsigned sequence_begin = __builtin_amdgcn_readfirstlane(s_cut[0][2]);
+  int sequence_length = __builtin_amdgcn_readfirstlane(s_cut[0][3]);
 
   while (u < u_end) {
-    const Span span = span_of(a.lengths[sequence], capacity, a.window);
-    const int cost = span.units + 1;
+    const Span span = span_of(sequence_length, capacity, a.window);
+    const int cost = span.units + kColumnCost;
     const int column = (u - sequence_begin) / cost, from = (u - sequence_begin) - column * cost;
     const int to = min((unsigned)cost, from + (u_end - u));
     const unsigned column_begin = u - from;
     u += to - from;
     const int this_sequence = sequence;
-    if (u == sequence_begin + (unsigned)cost * columns) sequence_begin = u, ++sequence;
-    // the first of a column's cost stands for no tokens; a share that ends there leaves it all to the next
-    const int unit0 = max(from - 1, 0), units_here = to - 1 - unit0;
+    if (u == sequence_begin + (unsigned)cost * columns) {
+      sequence_begin = u, ++sequence;
+      if (u < u_end) sequence_length = a.lengths[sequence];
+    }
+    // the first kColumnCost of a column stand for no tokens; a share that ends there leaves it all to the next
+    const int unit0 = max(from - kColumnCost, 0), units_here = max(to - kColumnCost, 0) - unit0;
     const bool complete = unit0 == 0 && to == cost;
-    if (to == 1 && !complete) continue;
+    if (to <= kColumnCost && !complete) continue;
     const int kv_head = column / a.head_blocks, head_block = column - kv_head * a.head_blocks;
     const int begin = span.tile0 + unit0 * kAttnWaves, end = span.tile0 + min((unit0 + units_here) * kAttnWaves, span.tiles);
     const int length = span.length, first_token = span.first;
     const int* const table = a.table + (size_t)this_sequence * a.max_pages;
 
-    // the page of a token
-    auto page_of = [&](int token) {
-      int page = -1;
-      if (token < length) page = table[token >> a.shape.page_shift];
-      return page;
-    };
+    // The page of a token; beyond the last one's, the last one's.  (Without a branch: the compiler counts the loads in flight
+    // behind one as the fewer, and waits for the next keys before it uses these values.)
+    const int last_token = max(length - 1, 0);
+    auto page_of = [&](int token) { return table[min(token, last_token) >> a.shape.page_shift]; };
     auto row_of = [&](int page, int token) { return cache_row(a.shape, (unsigned)page < (unsigned)a.shape.pages ? page : 0, kv_head, token & place_mask); };
 
     uint4_t kraw[kKeyLoads];
@@ -337,6 +346,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
 
     int tile = begin + wave;
     int page = page_of(tile * kAttnTile + g * 8), page_next = -1, page_after = -1;
+    float sink_here[NT];  // (of the head that this thread joins at the end)
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+      const int in_group = (head_block * NT + b) * 16 + (int)(threadIdx.x >> 4);
+      sink_here[b] = a.sinks && in_group < group ? a.sinks[kv_head * group + in_group] * 1.44269504088896341f : -INFINITY;
+    }
     typename Vec8<T>::type q_raw[NT][kSteps];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -362,10 +377,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
 
     // ---- queries: the second operand of the first product, held for the whole walk -----------------------------
     C8 q[NT][kSteps];
-    float q_scale[NT];
+    float q_scale[NT], unbias[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      q_scale[t] = a.score_scale;
+      q_scale[t] = a.score_scale, unbias[t] = 0.f;
       if constexpr (kWide) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) q[t][s] = q_raw[t][s];
@@ -383,6 +398,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
           for (int i = 0; i < 8; ++i) q[t][s][i] = (C)ldexpf((float)q_raw[t][s][i], shift);
+        if constexpr (kBiased) {
+          float sum_q = 0.f;
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum_q += (float)q[t][s][i];
+          unbias[t] = -kKeyBias * sum_over_groups(sum_q);
+        }
       }
     }
 
@@ -426,15 +449,15 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
               c = *reinterpret_cast<const uint2_t*>(p);
             }
             uint32_t h[4];
-            codes4_to_half<FORMAT>(c[0], h[0], h[1]);
-            codes4_to_half<FORMAT>(c[1], h[2], h[3]);
+            codes4_to_half<FORMAT, kBiased>(c[0], h[0], h[1]);
+            codes4_to_half<FORMAT, kBiased>(c[1], h[2], h[3]);
             w = uint4_t{h[0], h[1], h[2], h[3]};
           }
           kf[s] = __builtin_bit_cast(C8, w);
         }
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-          float4_t sc = {0.f, 0.f, 0.f, 0.f};
+          float4_t sc = {unbias[b], unbias[b], unbias[b], unbias[b]};
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) sc = mfma16<C>(kf[s], q[b][s], sc);
 #pragma unroll
@@ -503,11 +526,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
             for (int k = 0; k < 4; ++k) acc[b][i][k] *= shrink;
         }
       }
-      C8 pf[NT];
+      C8 pf[NT], pl[NT];
 #pragma unroll
       for (int b = 0; b < NT; ++b)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pf[b][j] = (C)p[b][j];
+        for (int j = 0; j < 8; ++j) pf[b][j] = (C)p[b][j], pl[b][j] = (C)(p[b][j] - (float)pf[b][j]);
       if constexpr (!decltype(last)::value) load_scales(next_row);
 
       // ---- values ---------------------------------------------------------------------------------------------
@@ -532,7 +555,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
             for (int i = 0; i < 4; ++i)
               w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][at + (e >> 1)], vr[2 * i][at + (e >> 1)], (e & 1) ? 0x07060302u : 0x05040100u);
 #pragma unroll
-            for (int b = 0; b < NT; ++b) acc[b][at_acc + e] = mfma16<C>(__builtin_bit_cast(C8, w), pf[b], acc[b][at_acc + e]);
+            for (int b = 0; b < NT; ++b)
+              acc[b][at_acc + e] = mfma16<C>(__builtin_bit_cast(C8, w), pf[b], mfma16<C>(__builtin_bit_cast(C8, w), pl[b], acc[b][at_acc + e]));
           }
         } else {
 #pragma unroll
@@ -552,7 +576,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
               const uint4_t w = {h[0], h[1], h[2], h[3]};
 #pragma unroll
               for (int b = 0; b < NT; ++b)
-                acc[b][at_acc + 4 * dw + e] = mfma16<C>(__builtin_bit_cast(C8, w), pf[b], acc[b][at_acc + 4 * dw + e]);
+                acc[b][at_acc + 4 * dw + e] =
+                    mfma16<C>(__builtin_bit_cast(C8, w), pf[b], mfma16<C>(__builtin_bit_cast(C8, w), pl[b], acc[b][at_acc + 4 * dw + e]));
             }
           }
         }
@@ -597,7 +622,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) voi
         float most = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kAttnWaves; ++w) most = fmaxf(most, sm[w][16 * b + row][0]);
-        const float sink = complete && a.sinks ? a.sinks[head] * 1.44269504088896341f : -INFINITY;
+        const float sink = complete ? sink_here[b] : -INFINITY;
         const float base = fmaxf(most, sink);
         float factor[kAttnWaves], total_weight = weight(sink, base);
 #pragma unroll
