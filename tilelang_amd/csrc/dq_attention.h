@@ -161,8 +161,22 @@ __device__ __forceinline__ float sum_over_groups(float x) {
 // 2^(m - to), 0 where there is nothing (m = -inf), whatever `to` is
 __device__ __forceinline__ float weight(float m, float to) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to); }
 
-// How many workgroups (of four waves) a compute unit holds: by the registers that a kernel needs, and the LDS of the join.
-constexpr int attention_per_unit(int head_dim, int format) { return head_dim <= 64 ? 4 : 2; }
+// How many workgroups (of four waves) a compute unit is to have where the work is shared out: as few as keep enough of the
+// cache in flight, for every one more is a column cut once more and has less in a row.  One of 16-bit rows of 160 bytes
+// and more (32 sequences of 4096 tokens, 128 wide: one 84 us, two 90, three 106; 256 wide 91 and 122), two of shorter ones, whose
+// tiles are small (64 wide 99, 91, 92, four 95; fp8 128 wide, 64 sequences, 113, 91, 106), and of 8 bits, whose waves have codes
+// to convert, up to 256 wide (92 and 103).
+constexpr int attention_per_unit(int head_dim, int format) { return head_dim > 64 && (cache_is_16bit(format) || head_dim > 192) ? 1 : 2; }
+
+// How many of them the registers are to leave room for: more where they fit without spills, for columns that stay whole.
+constexpr int attention_room(int head_dim, int row_blocks) {
+  if (head_dim <= 64) return row_blocks == 1 ? 4 : 3;
+  return head_dim > 192 ? 1 : 2;
+}
+
+// Blocks of 16 heads that a workgroup takes, with one read of the keys and values: two where more than 16 heads share them, but not
+// with the registers of wide heads.
+constexpr int attention_row_blocks(int heads_a_column, int head_dim) { return heads_a_column > 16 && head_dim <= 128 ? 2 : 1; }
 
 // A wave's LDS: 32 keys on their way into the operand's order, later 16 rows of its result.
 constexpr int attention_wave_lds(int head_dim, int format) {
@@ -172,7 +186,7 @@ constexpr int attention_wave_lds(int head_dim, int format) {
 
 // T: queries and output; FORMAT: the cache; D: head_dim; NT: blocks of 16 heads that a workgroup takes
 template <class T, int FORMAT, int D, int NT>
-__global__ __launch_bounds__(64 * kAttnWaves, attention_per_unit(D, FORMAT)) void attention_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attention_kernel(const AttnArgs a) {
   constexpr bool kWide = cache_is_16bit(FORMAT);
   using C = typename std::conditional<kWide, T, half_t>::type;  // what the products are taken in
   typedef typename Vec8<C>::type C8;
@@ -676,12 +690,13 @@ int launch_attention(const AttnArgs& a, hipStream_t stream) {
 
 template <class T, int FORMAT>
 int attention_of_type(const AttnArgs& a, hipStream_t stream) {
+  const bool two = attention_row_blocks(a.heads / a.shape.kv_heads, a.shape.head_dim) == 2;
   switch (a.shape.head_dim) {
-    case 64: return launch_attention<T, FORMAT, 64, 1>(a, stream);
-    case 80: return launch_attention<T, FORMAT, 80, 1>(a, stream);
-    case 96: return launch_attention<T, FORMAT, 96, 1>(a, stream);
-    case 112: return launch_attention<T, FORMAT, 112, 1>(a, stream);
-    case 128: return launch_attention<T, FORMAT, 128, 1>(a, stream);
+    case 64: return two ? launch_attention<T, FORMAT, 64, 2>(a, stream) : launch_attention<T, FORMAT, 64, 1>(a, stream);
+    case 80: return two ? launch_attention<T, FORMAT, 80, 2>(a, stream) : launch_attention<T, FORMAT, 80, 1>(a, stream);
+    case 96: return two ? launch_attention<T, FORMAT, 96, 2>(a, stream) : launch_attention<T, FORMAT, 96, 1>(a, stream);
+    case 112: return two ? launch_attention<T, FORMAT, 112, 2>(a, stream) : launch_attention<T, FORMAT, 112, 1>(a, stream);
+    case 128: return two ? launch_attention<T, FORMAT, 128, 2>(a, stream) : launch_attention<T, FORMAT, 128, 1>(a, stream);
     case 160: return launch_attention<T, FORMAT, 160, 1>(a, stream);
     case 192: return launch_attention<T, FORMAT, 192, 1>(a, stream);
     case 256: return launch_attention<T, FORMAT, 256, 1>(a, stream);

@@ -114,8 +114,8 @@ void launch_join(const AttnArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// A launch's workgroups and what they need to leave pieces of heads: as many as the chip holds at once, and no more than
-// pay.  tokens: that a sequence can have, or that its window shows.
+// A launch's workgroups and what they need to leave pieces of heads: attention_per_unit a compute unit, and no more than there
+// can be units; where no column can be cut, one a column.  tokens: that a sequence can have, or that its window shows.
 struct AttnPlan {
   int head_blocks, rows, workgroups;
   bool joins;
@@ -124,13 +124,14 @@ struct AttnPlan {
 static AttnPlan attention_plan(int sequences, int heads, int kv_heads, int head_dim, int format, long capacity, int window) {
   AttnPlan p;
   const int group = heads / kv_heads;
-  p.head_blocks = (group + 15) / 16;
-  p.rows = std::min(group, 16);
+  const int row_blocks = attention_row_blocks(group, head_dim);
+  p.head_blocks = (group + 16 * row_blocks - 1) / (16 * row_blocks);
+  p.rows = std::min(group, 16 * row_blocks);
   // (a window may begin and end inside a tile)
   const long tokens = window > 0 && window + kAttnTile - 1 < capacity ? window + kAttnTile - 1 : capacity;
   const long units = ((tokens + kAttnTile - 1) / kAttnTile + kAttnWaves - 1) / kAttnWaves, columns = (long)sequences * kv_heads * p.head_blocks;
   p.joins = units > kWholeUnits;
-  p.workgroups = (int)std::min<long>(kComputeUnits * attention_per_unit(head_dim, format), p.joins ? columns * units : columns);
+  p.workgroups = (int)(p.joins ? std::min<long>(kComputeUnits * attention_per_unit(head_dim, format), columns * units) : columns);
   return p;
 }
 
