@@ -65,9 +65,9 @@ __device__ __forceinline__ Span span_of(int length, int capacity, int window) {
 // a workgroup does before the first and after the last takes about as long (64 sequences of 0 to 16000 tokens, fp8: 158 us
 // without, 127 with one, 124 with two or three; short windows 11.7, with three 13.0).  All costs in a row, sequence by
 // sequence and in a sequence column by column, are cut into equal shares, one a workgroup, whatever the lengths are; a
-// cut inside a column makes pieces of it, which the join adds up.  A column of up to two units is not worth a
-// join: a cut there moves to its nearer end.
-constexpr int kWholeUnits = 2, kColumnCost = 2;
+// cut inside a column makes pieces of it, which the join adds up.  A column of up to kWholeUnits is not worth a join (one
+// sequence of 512 tokens: cut 11.7 us, whole 7.5; of 1000 11.2 and 13.9): a cut there moves to its nearer end.
+constexpr int kWholeUnits = 4, kColumnCost = 2;
 struct Shares {
   unsigned each, more;  // the first `more` workgroups have one more
   __device__ __forceinline__ Shares(unsigned total, unsigned workgroups) : each(total / workgroups), more(total - total / workgroups * workgroups) {}
@@ -77,6 +77,72 @@ struct Shares {
     return u < large ? u / (each + 1) : more + (u - large) / max(each, 1u);
   }
 };
+
+struct Share {
+  unsigned at, end;         // in costs
+  int sequence, length;     // of the column at `at`
+  unsigned sequence_begin;  // the sequence's first cost
+};
+struct ShareSearch {
+  int scan[kAttnWaves];
+  unsigned cut[2];
+  int sequence, length;
+  unsigned sequence_begin;
+};
+
+// The workgroup's share: a running sum of the sequences' costs, and the two cuts in it.  For all threads of the workgroup.
+__device__ __forceinline__ Share find_share(const AttnArgs& a, int capacity, int columns, int wave, int lane, ShareSearch& s, Shares& shares) {
+  const int per_thread = (a.sequences + 64 * kAttnWaves - 1) / (64 * kAttnWaves);
+  const int seq_begin = min((int)threadIdx.x * per_thread, a.sequences), seq_end = min(seq_begin + per_thread, a.sequences);
+  int mine = 0, length_here = 0;  // (of the last of this thread's sequences: of its one, where a thread has one)
+  for (int b = seq_begin; b < seq_end; ++b) length_here = a.lengths[b], mine += span_of(length_here, capacity, a.window).units + kColumnCost;
+  int sum = mine;  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(sum, o);
+    if (lane >= o) sum += up;
+  }
+  if (lane == 63) s.scan[wave] = sum;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < kAttnWaves; ++w) {
+    if (w < wave) sum += s.scan[w];
+    total += s.scan[w];
+  }
+  shares = Shares((unsigned)total * columns, a.workgroups);
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const unsigned cut = shares.begin(blockIdx.x + side);
+    const int at = cut / columns;
+    if (threadIdx.x == 0 && at >= total) s.cut[side] = cut;  // behind everything
+    if (!(sum - mine <= at && at < sum)) continue;
+    int b = seq_begin, before = sum - mine;
+    for (;; ++b) {
+      const int length = per_thread == 1 ? length_here : a.lengths[b];
+      const int units = span_of(length, capacity, a.window).units, cost = units + kColumnCost;
+      if (at >= before + cost) {
+        before += cost;
+        continue;
+      }
+      const unsigned begin = (unsigned)before * columns, off = (cut - begin) % cost;
+      const unsigned moved = units <= kWholeUnits ? cut - off + (2 * off >= (unsigned)cost ? cost : 0) : cut;
+      s.cut[side] = moved;
+      if (side == 0) {
+        const bool next = moved == begin + (unsigned)cost * columns;
+        s.sequence = b + next, s.sequence_begin = next ? moved : begin;
+        s.length = !next ? length : b + 1 < a.sequences ? a.lengths[b + 1] : 0;
+      }
+      break;
+    }
+  }
+  __syncthreads();
+  Share share;
+  share.at = __builtin_amdgcn_readfirstlane(s.cut[0]), share.end = __builtin_amdgcn_readfirstlane(s.cut[1]);
+  share.sequence = __builtin_amdgcn_readfirstlane(s.sequence), share.length = __builtin_amdgcn_readfirstlane(s.length);
+  share.sequence_begin = __builtin_amdgcn_readfirstlane(s.sequence_begin);
+  return share;
+}
 
 // ---- which elements of a row a lane holds ----------------------------------------------------------------------
 // Keys (and queries): k-step s of 32 elements, group g has eight of them.  16 bit: 32 s + 8 g.  8 bit: a lane loads 16
@@ -202,8 +268,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
   constexpr int kWaveLds = attention_wave_lds(D, FORMAT);
 
   __shared__ float sm[kAttnWaves][16 * NT][3];
-  __shared__ int s_scan[kAttnWaves];
-  __shared__ unsigned s_cut[2][4];  // where the share begins and ends: cost, sequence, the sequence's first cost, its length
   extern __shared__ __align__(16) char lds[];
   constexpr int kRow = D + 4;
 
@@ -215,67 +279,27 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
   const int capacity = a.max_pages << a.shape.page_shift;
   const int place_mask = (1 << a.shape.page_shift) - 1;
 
-  // ---- this workgroup's share: a running sum of the sequences' costs ---------------------------------------------
-  const int per_thread = (a.sequences + 64 * kAttnWaves - 1) / (64 * kAttnWaves);
-  const int seq_begin = min((int)threadIdx.x * per_thread, a.sequences), seq_end = min(seq_begin + per_thread, a.sequences);
-  int mine = 0, length_here = 0;  // (of the last of this thread's sequences: of its one, where a thread has one)
-  for (int b = seq_begin; b < seq_end; ++b) length_here = a.lengths[b], mine += span_of(length_here, capacity, a.window).units + kColumnCost;
-  int sum = mine;  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int up = __shfl_up(sum, o);
-    if (lane >= o) sum += up;
+  __shared__ ShareSearch search;
+  Share share;
+  Shares shares(0, 1);
+  if (a.pieces) {
+    share = find_share(a, capacity, columns, wave, lane, search, shares);
+  } else {  // no column can be cut: one a workgroup
+    share.sequence = blockIdx.x / columns, share.length = a.lengths[share.sequence], share.sequence_begin = 0;
+    const unsigned cost = span_of(share.length, capacity, a.window).units + kColumnCost;
+    share.at = (blockIdx.x - share.sequence * columns) * cost, share.end = share.at + cost;
   }
-  if (lane == 63) s_scan[wave] = sum;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < kAttnWaves; ++w) {
-    if (w < wave) sum += s_scan[w];
-    total += s_scan[w];
-  }
-  const Shares shares((unsigned)total * columns, a.workgroups);
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const unsigned cut = shares.begin(blockIdx.x + side);
-    const int at = cut / columns;
-    if (threadIdx.x == 0 && at >= total) s_cut[side][0] = cut;  // behind everything
-    if (!(sum - mine <= at && at < sum)) continue;
-    int b = seq_begin, before = sum - mine;
-    for (;; ++b) {
-      const int length = per_thread == 1 ? length_here : a.lengths[b];
-      const int units = span_of(length, capacity, a.window).units, cost = units + kColumnCost;
-      if (at >= before + cost) {
-        before += cost;
-        continue;
-      }
-      const unsigned begin = (unsigned)before * columns;
-      const unsigned off = (cut - begin) % cost;
-      const unsigned moved = units <= kWholeUnits ? cut - off + (2 * off >= (unsigned)cost ? cost : 0) : cut;
-      const bool next = moved == begin + (unsigned)cost * columns;
-      s_cut[side][0] = moved, s_cut[side][1] = b + next, s_cut[side][2] = next ? moved : begin;
-      s_cut[side][3] = next && b + 1 < a.sequences ? a.lengths[b + 1] : length;
-      break;
-    }
-  }
-  __syncthreads();
-  unsigned u = __builtin_amdgcn_readfirstlane(s_cut[0][0]);
-  const unsigned u_end = __builtin_amdgcn_readfirstlane(s_cut[1][0]);
-  int sequence = __builtin_amdgcn_readfirstlane(s_cut[0][1]);
-  unsigned sequence_begin = __builtin_amdgcn_readfirstlane(s_cut[0][2]);
-  int sequence_length = __builtin_amdgcn_readfirstlane(s_cut[0][3]);
 
-  while (u < u_end) {
-    const Span span = span_of(sequence_length, capacity, a.window);
-    const int cost = span.units + kColumnCost;
-    const int column = (u - sequence_begin) / cost, from = (u - sequence_begin) - column * cost;
-    const int to = min((unsigned)cost, from + (u_end - u));
-    const unsigned column_begin = u - from;
-    u += to - from;
-    const int this_sequence = sequence;
-    if (u == sequence_begin + (unsigned)cost * columns) {
-      sequence_begin = u, ++sequence;
-      if (u < u_end) sequence_length = a.lengths[sequence];
+  while (share.at < share.end) {
+    const Span span = span_of(share.length, capacity, a.window);
+    const int sequence = share.sequence, cost = span.units + kColumnCost;
+    const int column = (share.at - share.sequence_begin) / cost, from = (share.at - share.sequence_begin) - column * cost;
+    const int to = min((unsigned)cost, from + (share.end - share.at));
+    const unsigned column_begin = share.at - from;
+    share.at += to - from;
+    if (share.at == share.sequence_begin + (unsigned)cost * columns) {
+      share.sequence_begin = share.at, ++share.sequence;
+      if (share.at < share.end) share.length = a.lengths[share.sequence];
     }
     // the first kColumnCost of a column stand for no tokens; a share that ends there leaves it all to the next
     const int unit0 = max(from - kColumnCost, 0), units_here = max(to - kColumnCost, 0) - unit0;
@@ -284,7 +308,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
     const int kv_head = column / a.head_blocks, head_block = column - kv_head * a.head_blocks;
     const int begin = span.tile0 + unit0 * kAttnWaves, end = span.tile0 + min((unit0 + units_here) * kAttnWaves, span.tiles);
     const int length = span.length, first_token = span.first;
-    const int* const table = a.table + (size_t)this_sequence * a.max_pages;
+    const int* const table = a.table + (size_t)sequence * a.max_pages;
 
     // The page of a token; beyond the last one's, the last one's.  (Without a branch: the compiler counts the loads in flight
     // behind one as the fewer, and waits for the next keys before it uses these values.)
@@ -370,7 +394,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int row = (head_block * NT + t) * 16 + n;
-      const T* const qrow = reinterpret_cast<const T*>(a.q) + ((size_t)this_sequence * a.heads + (size_t)kv_head * group + row) * D;
+      const T* const qrow = reinterpret_cast<const T*>(a.q) + ((size_t)sequence * a.heads + (size_t)kv_head * group + row) * D;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const int d = key_element<D, kWide>(s, g);
@@ -645,7 +669,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
           total_weight += weight(sm[w][16 * b + row][0], base) * sm[w][16 * b + row][1];
         }
         if (complete) {
-          const size_t at = (size_t)this_sequence * a.heads + head;
+          const size_t at = (size_t)sequence * a.heads + head;
           const float inv = total_weight > 0.f ? 1.f / total_weight : (total_weight == 0.f ? 0.f : total_weight);
           for (int d = threadIdx.x & 15; d < D; d += 16) {
             float x = 0.f;
@@ -669,7 +693,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
       }
     }
     if (unit0 == 0 && threadIdx.x == 0 && a.pieces) {
-      int* const pieces = a.pieces + 2 * ((size_t)this_sequence * columns + column);
+      int* const pieces = a.pieces + 2 * ((size_t)sequence * columns + column);
       pieces[0] = blockIdx.x, pieces[1] = complete ? blockIdx.x : shares.owner(column_begin + cost - 1);
     }
     __syncthreads();  // the LDS is free again
