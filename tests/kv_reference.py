@@ -52,15 +52,15 @@ def stale(cache, scale, page, place):
 def tokens_of(cache, scale, pages, length):
     """The first tokens of a sequence in 64 bits, [length, kv_heads, head_dim]; pages that are not there: NaN."""
     size = cache.shape[2]
-    x = cache.float().cpu().double()
+    ids = torch.as_tensor(pages)[: -(-length // size)].long().cpu()
+    there = (ids >= 0) & (ids < cache.shape[0])
+    at = ids.clamp(0, cache.shape[0] - 1).to(cache.device)
+    raw = cache.view(torch.uint8 if cache.dtype.itemsize == 1 else torch.int16)
+    x = raw[at].view(cache.dtype).float().cpu().double()
     if scale is not None:
-        x = x * scale.cpu().double()[..., None]
-    out = torch.full((length, cache.shape[1], cache.shape[3]), math.nan, dtype=torch.float64)
-    for t in range(0, length, size):
-        page, n = int(pages[t // size]), min(size, length - t)
-        if 0 <= page < cache.shape[0]:
-            out[t : t + n] = x[page, :, :n].transpose(0, 1)
-    return out
+        x = x * scale[at].cpu().double()[..., None]
+    x[~there] = math.nan
+    return x.transpose(1, 2).reshape(-1, cache.shape[1], cache.shape[3])[:length]
 
 
 def attention(q, keys, values, scale, window=0, sinks=None, there=None):
@@ -68,22 +68,21 @@ def attention(q, keys, values, scale, window=0, sinks=None, there=None):
     values.  Returns out, lse and sum_t p_t |v_t| / sum p, which rounded weights are off by in proportion."""
     heads, dim = q.shape
     length, kv_heads = keys.shape[:2]
-    out, spread = torch.zeros((heads, dim), dtype=torch.float64), torch.zeros((heads, dim), dtype=torch.float64)
-    lse = torch.full((heads,), -math.inf, dtype=torch.float64)
-    first = max(0, length - window) if window else 0
-    live = torch.arange(length) >= first
+    live = torch.arange(length) >= (max(0, length - window) if window else 0)
     if there is not None:
         live &= there
-    for h in range(heads):
-        k, v = keys[live][:, h * kv_heads // heads], values[live][:, h * kv_heads // heads]
-        s = (k @ q[h].cpu().double()) * scale
-        extra = s.new_tensor([float(sinks[h])]) if sinks is not None else s.new_empty(0)
-        both = torch.cat([s, extra])
-        if not len(both):
+    out, spread = torch.zeros((heads, dim), dtype=torch.float64), torch.zeros((heads, dim), dtype=torch.float64)
+    lse = torch.full((heads,), -math.inf, dtype=torch.float64)
+    group = heads // kv_heads
+    for j in range(kv_heads):
+        k, v, own = keys[live, j], values[live, j], slice(j * group, (j + 1) * group)
+        scores = (q[own].cpu().double() @ k.T) * scale
+        both = scores if sinks is None else torch.cat([scores, sinks[own].double()[:, None]], dim=1)
+        if not both.shape[1]:
             continue
-        lse[h] = torch.logsumexp(both, 0)
-        p = torch.exp(s - lse[h])
-        out[h], spread[h] = p @ v, p @ v.abs()
+        lse[own] = torch.logsumexp(both, 1)
+        p = torch.exp(scores - lse[own, None])
+        out[own], spread[own] = p @ v, p @ v.abs()
     return out, lse, spread
 
 

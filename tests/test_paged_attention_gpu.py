@@ -238,3 +238,42 @@ def test_offsets_beyond_32_bits(cuda):
     out = tl.paged_attention_decode(1, 16, max_pages=1, **pool)(q, kc, vc, ks, vs, table, torch.tensor([tokens], dtype=torch.int32, device=cuda))
     want, _, spread = attention(q[0], *(tokens_of(c[-1:], s[-1:], [0], tokens) for c, s in ((kc, ks), (vc, vs))), dim**-0.5)
     assert ((out[0].cpu().double() - want).abs() <= attention_bound(want, spread, out.dtype, torch.int8)).all()
+
+
+def _ragged(n, longest, seed):
+    gen = torch.Generator().manual_seed(seed)
+    lengths = (torch.rand(n, generator=gen) ** 3 * longest).int().tolist()
+    lengths[n // 2], lengths[n // 3] = longest, 0
+    return lengths
+
+
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page_size,cache,window,sinks", [
+    # more sequences than a workgroup has threads, several a thread; nothing that can be cut
+    (_ragged(700, 120, 1), 2, 1, 64, 8, "same", 0, False),
+    # ... and one among them that is
+    (_ragged(530, 6000, 2), 2, 2, 64, 16, "int8", 0, True),
+    # few columns cut into hundreds of pieces, more than a lane group takes at once
+    ([70000, 3], 6, 2, 64, 128, "float8_e4m3fn", 0, True),
+    ([33000], 3, 1, 128, 64, "same", 0, False),
+    # many columns, some cut: the join of a group a head
+    (_ragged(150, 3000, 3), 48, 16, 64, 16, "same", 0, True),
+    # whole columns of several units, and of one more unit than that
+    ([2048, 1, 2047, 700] * 4, 32, 32, 64, 64, "same", 0, False),
+    ([2049, 1, 2048, 700] * 4, 32, 32, 64, 64, "same", 0, False),
+    ([512, 513, 511] * 3, 4, 4, 80, 32, "float8_e4m3fn", 0, False),
+    # two blocks of 16 heads, and three, and a wide head that takes them one by one
+    ([900, 20], 71, 1, 64, 16, "same", 0, True),
+    ([5000], 33, 1, 128, 16, "int8", 0, False),
+    ([1300, 0, 77], 40, 1, 192, 16, "same", 0, False),
+    # windows that are cut and windows that are not
+    ([9000, 300, 40], 8, 2, 128, 16, "int8", 3001, True),
+    ([9000, 300, 40], 8, 2, 128, 16, "same", 481, False),
+], ids=lambda v: f"{len(v)}x{max(v)}" if isinstance(v, list) else str(v))
+def test_shares(cuda, lengths, heads, kv_heads, dim, page_size, cache, window, sinks):
+    """Batches whose work is cut in every way that there is."""
+    print(f"shares n={len(lengths)} longest={max(lengths)} {heads}/{kv_heads}x{dim} page {page_size} {cache} window {window}", flush=True)
+    case = _Case(cuda, lengths, heads, kv_heads, dim, page_size, "bfloat16", cache)
+    case.check(window=window, sinks=sinks)
+    first, _ = case.run(window, sinks)
+    for _ in range(2):
+        assert torch.equal(case.run(window, sinks)[0], first)
