@@ -34,7 +34,7 @@ def _type16(fn: str, dtype) -> torch.dtype:
 def _cache_type(fn: str, cache_dtype, dtype: torch.dtype) -> torch.dtype:
     if cache_dtype is None:
         return dtype
-    d = torch.float8_e4m3fn if cache_dtype == "float8_e4m3fn" else _dtype(cache_dtype)
+    d = torch.float8_e4m3fn if cache_dtype in ("float8_e4m3fn", torch.float8_e4m3fn) else _dtype(cache_dtype)
     if d not in (dtype, torch.float8_e4m3fn, torch.int8):
         raise ValueError(f"{fn}: cache_dtype must be dtype itself, float8_e4m3fn or int8 (got {cache_dtype!r} with {dtype})")
     return d
