@@ -167,6 +167,20 @@ def test_infinities_and_nan_that_live(cuda):
     assert torch.isnan(out[1, :2]).all() and torch.isnan(lse[1, :2]).all() and not torch.isnan(out[1, 2:]).any()
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_infinite_values(cuda, dtype):
+    """An infinity among a head's values is one in its result, in that element alone; two of both signs are no number."""
+    case = _Case(cuda, [100, 2000], 4, 2, 64, 16, dtype)
+    values = case.buffers[1][0]
+    values[int(case.table[0, 2]), 1, 3, 9] = math.inf
+    values[int(case.table[1, 5]), 0, 3, 7] = -math.inf
+    values[int(case.table[1, 90]), 0, 1, 8], values[int(case.table[1, 3]), 0, 1, 8] = math.inf, -math.inf
+    out, lse = case.run()
+    assert (out[0, 2:, 9] == math.inf).all() and (out[1, :2, 7] == -math.inf).all() and torch.isnan(out[1, :2, 8]).all()
+    out[0, 2:, 9] = out[1, :2, 7] = out[1, :2, 8] = 0
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
 @pytest.mark.parametrize("cache", ["same", "int8"])
 def test_parts_join(cuda, cache):
     """Results over a context's first and second half, joined by their logarithms, are those over the whole."""

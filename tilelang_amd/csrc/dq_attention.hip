@@ -137,10 +137,10 @@ static AttnPlan attention_plan(int sequences, int heads, int kv_heads, int head_
   return p;
 }
 
-// Units are counted in 31 bits.
+// Costs are counted in 31 bits, and a column may be a workgroup.
 bool attention_fits(int sequences, int heads, int kv_heads, long capacity) {
-  const double units = (double)sequences * kv_heads * ((heads / kv_heads + 15) / 16) * (capacity / kAttnUnit + 3);
-  return units < 2147483647.0;
+  const double columns = (double)sequences * kv_heads * ((heads / kv_heads + 15) / 16);
+  return columns < 8388608.0 && columns * (capacity / kAttnUnit + 1 + kColumnCost) < 2147483647.0;
 }
 
 size_t attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim, int format, long capacity, int window) {

@@ -81,7 +81,8 @@ int check_cache(const char* fn, const void* K, const void* V, const void* KS, co
 int check_table(const char* fn, const void* PageTable, int sequences, int max_pages, int page_size) {
   if (sequences <= 0 || max_pages <= 0) DQ_FAIL("%s: sequences and max_pages must be positive (got %d and %d)", fn, sequences, max_pages);
   if (!PageTable || !on_4(PageTable)) DQ_FAIL("%s: PageTable must be a 4-byte aligned, non-NULL data pointer", fn);
-  if ((long)max_pages * page_size > 0x7FFFFFC0l) DQ_FAIL("%s: %d pages of %d tokens a sequence: lengths are 32-bit", fn, max_pages, page_size);
+  // (some tiles more than a sequence's tokens are counted ahead)
+  if ((long)max_pages * page_size > 0x7FFFF000l) DQ_FAIL("%s: %d pages of %d tokens a sequence: lengths are 32-bit", fn, max_pages, page_size);
   return 0;
 }
 
@@ -168,7 +169,7 @@ extern "C" int call_paged_attention_decode(const void* Q, const void* KCache, co
   if (heads <= 0 || heads % kv_heads != 0) DQ_FAIL("%s: heads must be a multiple of kv_heads=%d (got %d)", fn, kv_heads, heads);
   if (sequences > 65535 || heads > 65535) DQ_FAIL("%s: at most 65535 sequences and heads (got %d and %d)", fn, sequences, heads);
   if (!attention_fits(sequences, heads, kv_heads, (long)max_pages * page_size))
-    DQ_FAIL("%s: %d sequences of %d heads and up to %ld tokens: more than 2^31 pieces of %d tokens", fn, sequences, heads, (long)max_pages * page_size, 128);
+    DQ_FAIL("%s: %d sequences of %d heads and up to %ld tokens: more than the work that a call counts", fn, sequences, heads, (long)max_pages * page_size);
   if (window < 0) DQ_FAIL("%s: window must be 0 (none) or positive (got %d)", fn, window);
   if (!isfinite(scale)) DQ_FAIL("%s: scale must be finite", fn);
   if (!Q || !Lengths || !Out) DQ_FAIL("%s: Q, Lengths and Out are expected to have non-NULL data pointers", fn);
