@@ -130,9 +130,12 @@ ODD = ctypes.c_void_p((1 << 20) + 2)
     ("call_kv_cache_read", dict(PageTable=None), "PageTable"),
     ("call_kv_cache_read", dict(max_pages=1 << 28), "lengths are 32-bit"),
     ("call_kv_cache_read", dict(KV=ODD), "16-byte"),
+    ("call_kv_cache_read", dict(kv_heads=8192), "524280 elements"),
     ("call_paged_attention_decode", dict(heads=5), "multiple of kv_heads"),
     ("call_paged_attention_decode", dict(head_dim=72), "head_dim must be"),
     ("call_paged_attention_decode", dict(window=-1), "window must be"),
+    ("call_paged_attention_decode", dict(sequences=60000, max_pages=1 << 26), "the work that a call counts"),
+    ("call_paged_attention_decode", dict(max_pages=(1 << 27) - 1), "lengths are 32-bit"),
     ("call_paged_attention_decode", dict(scale=math.nan), "scale must be finite"),
     ("call_paged_attention_decode", dict(sequences=70000), "at most 65535"),
     ("call_paged_attention_decode", dict(Lengths=None), "non-NULL"),

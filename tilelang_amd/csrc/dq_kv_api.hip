@@ -143,6 +143,7 @@ extern "C" int call_kv_cache_read(const void* KCache, const void* VCache, const 
   int shift;
   if (check_cache(fn, KCache, VCache, KScale, VScale, kv_heads, head_dim, pages, page_size, dtype, cache_format, &shift) != 0) return -1;
   if (check_rows(fn, tokens, kv_heads) != 0 || check_table(fn, PageTable, sequences, max_pages, page_size) != 0) return -1;
+  if ((long)kv_heads * head_dim > 8 * 65535l) DQ_FAIL("%s: %d heads of %d: at most 524280 elements a token", fn, kv_heads, head_dim);
   if (!Starts || !KV) DQ_FAIL("%s: Starts and KV are expected to have non-NULL data pointers", fn);
   if (!on_4(Starts) || !on_16(KV)) DQ_FAIL("%s: Starts must be 4-byte and KV 16-byte aligned", fn);
   return kv_cache_read(KCache, VCache, (const float*)KScale, (const float*)VScale, (const int*)PageTable, (const int*)Starts, KV,

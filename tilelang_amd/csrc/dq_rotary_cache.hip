@@ -67,7 +67,8 @@ __device__ __forceinline__ typename Vec8<T>::type round8(const float (&f)[8]) {
 // A group of LANES lanes has a row (a head of a token), a lane two pieces of eight elements of it: in the half layout two that turn
 // with each other, so that every element is read once.  One row a group: four of one token, with one look at the table,
 // take as long on whole lines and longer where rows are none (7999 tokens of 64 heads of 80: 34 against 40 us).  Nothing is
-// streamed here: what comes in is fresh from the projection, what goes out is read next.
+// streamed here: what comes in is fresh from the projection, what goes out is read next.  Bound by memory: 4096 tokens of 40
+// heads of 128 in 15.3 us, 5.6 TB/s read and written of the 6.6 that a copy of that size reaches; one token is a launch.
 template <class T, int LANES, int LAYOUT, int FORMAT>
 __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
   const int lane = threadIdx.x % LANES;
@@ -220,10 +221,13 @@ int launch_rows_lanes(const RowArgs& a, hipStream_t stream) {
   DQ_FAIL("a head of %d is beyond the cache's %d", a.head_dim, kMaxHeadDim);
 }
 
-// Reading back: a workgroup has kReadTokens(...) tokens of the packed result.  It first finds each one's sequence, page and place,
-// then its threads take the tokens' pieces of eight elements in the order of the result, which is written as one run, 16 bytes
-// a lane side by side (131071 tokens of 8 heads of 128, fp8: 138 us, 5.9 TB/s of the 6.7 that a large copy reaches; 16 codes a lane, two stores 32 bytes apart, fill no line at
-// once: 290).  Loads and stores are streamed: such a result is larger than the caches (197 us without, and without the runs).
+// Reading back: a workgroup has some tokens of the packed result, 1024 pieces of eight elements or at most kReadTokens tokens.  It
+// first finds each one's sequence, page and place, then its threads take the pieces in the order of the result, which is
+// written as one run, 16 bytes a lane side by side.  Stores are streamed: such a result is larger than the caches.  Loads are not:
+// what was just written still lies there, and a line of narrow heads or of scales is another workgroup's too (48 sequences of
+// up to 1100 tokens, 12 heads of 96, int8: 22 us, streamed 29.7).  131071 tokens of 8 heads of 128, fp8: 138 us, 5.9 TB/s of
+// the 6.7 that a large copy reaches (a row a lane group, nothing streamed: 197; 16 codes a lane, whose two stores lie 32
+// bytes apart and fill no line at once: 290).
 struct ReadArgs {
   const void* cache[2];
   const float* scale[2];
@@ -290,7 +294,7 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
       const int page = s_page[token];
       there[k] = page >= 0;
       const size_t row = cache_row(a.shape, max(page, 0), head, s_place[token]);
-      raw[k] = __builtin_nontemporal_load(reinterpret_cast<const Raw*>(cache + (row * a.row_pieces + in_row) * PIECE));
+      raw[k] = *reinterpret_cast<const Raw*>(cache + (row * a.row_pieces + in_row) * PIECE);
       if constexpr (!kWide) s[k] = scale[row];
     }
 #pragma unroll
