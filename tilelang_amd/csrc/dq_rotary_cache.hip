@@ -225,7 +225,7 @@ int launch_rows_lanes(const RowArgs& a, hipStream_t stream) {
 // first finds each one's sequence, page and place, then its threads take the pieces in the order of the result, which is
 // written as one run, 16 bytes a lane side by side.  Stores are streamed: such a result is larger than the caches.  Loads are not:
 // what was just written still lies there, and a line of narrow heads or of scales is another workgroup's too (48 sequences of
-// up to 1100 tokens, 12 heads of 96, int8: 22 us, streamed 29.7).  131071 tokens of 8 heads of 128, fp8: 138 us, 5.9 TB/s of
+// up to 1100 tokens, 12 heads of 96, int8: 23 us, streamed 29.7).  131071 tokens of 8 heads of 128, fp8: 138 us, 5.9 TB/s of
 // the 6.7 that a large copy reaches (a row a lane group, nothing streamed: 197; 16 codes a lane, whose two stores lie 32
 // bytes apart and fill no line at once: 290).
 struct ReadArgs {
@@ -237,10 +237,12 @@ struct ReadArgs {
   int sequences, tokens, max_pages;
   CacheShape shape;
   int tokens_each;             // of a workgroup, at most kReadTokens
+  bool runs;                   // neighbouring workgroups by sixteens on one of the eight L2 caches
   int row_pieces, all_pieces;  // of a head, of a token
   unsigned row_magic, all_magic;  // ceil(2^32 / row_pieces), ceil(2^32 / all_pieces)
 };
 constexpr int kReadTokens = 64;
+constexpr int kReadRun = 16;
 constexpr int kReadStarts = 1024;  // starts of so many sequences are looked through in LDS
 
 // i / n by its magic number: right for i < 2^16, as i * (magic * n - 2^32) < 2^32 there (n <= 2^16); n = 1 has none
@@ -252,7 +254,13 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
   constexpr int kElements = 8, PIECE = kWide ? 16 : 8;
   __shared__ int s_starts[kReadStarts + 1];
   __shared__ int s_page[kReadTokens], s_place[kReadTokens];
-  const int token0 = blockIdx.x * a.tokens_each, count = min(a.tokens_each, a.tokens - token0);
+  int block = blockIdx.x;
+  if (a.runs) {  // sixteen neighbours on one of the eight L2 caches, which share the lines between them (31.5 -> 29.5 us at 12 heads of 96)
+    const int run = block / (8 * kReadRun) * (8 * kReadRun), in_run = block - run;
+    block = run + (in_run & 7) * kReadRun + (in_run >> 3);
+  }
+  const int token0 = block * a.tokens_each, count = min(a.tokens_each, a.tokens - token0);
+  if (count <= 0) return;
   const bool staged = a.sequences <= kReadStarts;
   if (staged) {
     for (int i = threadIdx.x; i <= a.sequences; i += 256) s_starts[i] = a.starts[i];
@@ -323,7 +331,10 @@ int launch_read(ReadArgs a, hipStream_t stream) {
   int each = std::max(1, std::min(kReadTokens, 1024 / a.all_pieces));
   while (each > 1 && (long)(a.tokens + each - 1) / each * 2 < 4 * 256) each = (each + 1) / 2;
   a.tokens_each = each;
-  read_kernel<T, FORMAT><<<dim3((a.tokens + each - 1) / each, 2), 256, 0, stream>>>(a);
+  unsigned blocks = (a.tokens + each - 1) / each;
+  a.runs = blocks >= 16 * kReadRun;
+  if (a.runs) blocks = (blocks + 8 * kReadRun - 1) / (8 * kReadRun) * (8 * kReadRun);
+  read_kernel<T, FORMAT><<<dim3(blocks, 2), 256, 0, stream>>>(a);
   DQ_CHECK_HIP(hipGetLastError());
   return 0;
 }
