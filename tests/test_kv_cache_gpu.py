@@ -15,6 +15,7 @@ SHAPES = [  # tokens, heads, kv_heads, head_dim, rotary_dim, interleaved, pages,
     (1, 1, 1, 64, 64, False, 1, 8),
     (16, 32, 8, 128, 128, False, 5, 16),
     (37, 6, 3, 96, 48, True, 9, 64),
+    (53, 5, 1, 112, 56, False, 7, 16),
     (23, 4, 4, 80, 32, False, 4, 32),
     (70, 2, 1, 256, 256, True, 2, 1024),
     (9, 3, 1, 72, 20, False, 3, 8),

@@ -22,6 +22,7 @@ def _inputs(seed, tokens, heads, dim, dtype, device, wide=0):
 @pytest.mark.parametrize("tokens,heads,dim,rotary_dim,wide", [
     (1, 1, 8, 2, 0), (1, 40, 128, 128, 0), (3, 5, 64, 64, 2), (37, 3, 80, 32, 1), (7, 9, 96, 24, 0), (5, 4, 256, 256, 4),
     (2, 3, 512, 512, 0), (19, 2, 40, 6, 0), (1500, 20, 128, 64, 8), (900, 7, 72, 70, 0), (2, 1, 264, 136, 1),
+    (123, 6, 80, 40, 2),
 ])
 def test_rotary(cuda, tokens, heads, dim, rotary_dim, wide, interleaved, dtype):
     print(f"rotary {tokens}x{heads}x{dim} r={rotary_dim} wide={wide} {interleaved} {dtype}", flush=True)
@@ -42,7 +43,7 @@ def test_rotary(cuda, tokens, heads, dim, rotary_dim, wide, interleaved, dtype):
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
-@pytest.mark.parametrize("rotary_dim", [128, 48, 20])
+@pytest.mark.parametrize("rotary_dim", [128, 48, 56, 20])
 def test_rotary_in_place_in_a_fused_projection(cuda, interleaved, rotary_dim):
     tokens, heads, wide, dim = 700, 10, 3, 128
     x, gen = _inputs(3, tokens, heads, dim, "bfloat16", cuda, wide)
