@@ -303,9 +303,31 @@ constexpr int attention_wave_lds(int head_dim, int format) {
   return keys > result ? keys : result;
 }
 
-// T: queries and output; FORMAT: the cache; D: head_dim; NT: blocks of 16 heads that a workgroup takes
-template <class T, int FORMAT, int D, int NT>
+// Whether a workgroup's heads are taken PACKED, see there: up to eight, where instructions and not memory bound the kernel, which
+// is in narrow heads of 8 bits (64 sequences of 4000 tokens, eight key-value heads: int8, 64 wide, 68 -> 60 us, 80 wide 78 -> 72;
+// fp8, 96 wide, 77 -> 73; 128 wide 180 -> 177 and 167 -> 167; 16 bits, 64 wide, 83 -> 83).
+constexpr bool attention_packs(int heads_a_column, int head_dim, int format) { return heads_a_column <= 8 && head_dim < 128 && !cache_is_16bit(format); }
+
+// What lane n ^ 8 of the 16 has; into lane n < 8 its four elements, behind its own four.
+template <class T>
+__device__ __forceinline__ T other_half(T x) { return dpp_move<0x128>(x); }
+__device__ __forceinline__ float into_upper_half(float x, float upper) {  // lanes n >= 8 get lane n - 8's `upper`
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, x), __builtin_bit_cast(int, upper), 0x128, 0xF, 0xC, false));
+}
+template <class C8>
+__device__ __forceinline__ void both_halves(C8& x) {
+  uint4_t w = __builtin_bit_cast(uint4_t, x);
+  w[2] = other_half((uint32_t)w[0]), w[3] = other_half((uint32_t)w[1]);
+  x = __builtin_bit_cast(C8, w);
+}
+
+// T: queries and output; FORMAT: the cache; D: head_dim; NT: blocks of 16 heads that a workgroup takes.  PACKED: of its 16
+// columns at most eight are heads, so between the products lane n has the scores of head n & 7: n < 8 of its lane group's first
+// four tokens, n >= 8 of the other four, and the softmax half the instructions.
+template <class T, int FORMAT, int D, int NT, bool PACKED>
 __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attention_kernel(const AttnArgs a) {
+  static_assert(NT == 1 || !PACKED, "");
+  constexpr int kEach = PACKED ? 4 : 8;  // tokens of a tile whose scores a lane has
   constexpr bool kWide = cache_is_16bit(FORMAT);
   using C = typename std::conditional<kWide, T, half_t>::type;  // what the products are taken in
   typedef typename Vec8<C>::type C8;
@@ -327,6 +349,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
   extern __shared__ __align__(16) char lds[];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int lane_tokens = PACKED ? (n & 8) >> 1 : 0;  // where the kEach of eight begin
   char* const keys = lds + wave * kWaveLds;
   auto result = [&](int w, int row) { return reinterpret_cast<float*>(lds + w * kWaveLds) + row * kRow; };
   const int group = a.heads / a.shape.kv_heads;  // heads that share a key-value head
@@ -372,7 +395,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 
     uint4_t kraw[kKeyLoads];
     uint32_t vr[8][kVDwords];
-    float ks[8], vs[8];
+    float ks[kEach], vs[kEach];
     // Eight tokens' keys are one piece of memory: a load takes 64 times 16 bytes of the tile as they lie, whole lines.
     auto load_keys = [&](int page, int tile) {  // page: that of the tokens 8 g ..
       const char* base[4];
@@ -424,8 +447,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
     };
     auto load_scales = [&](size_t row) {
       if constexpr (!kWide) {
+        if constexpr (PACKED) row += lane_tokens;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kEach / 4; ++i) {
           const float4_t kq = *reinterpret_cast<const float4_t*>(a.scale[0] + row + 4 * i), vq = *reinterpret_cast<const float4_t*>(a.scale[1] + row + 4 * i);
 #pragma unroll
           for (int j = 0; j < 4; ++j) ks[4 * i + j] = kq[j], vs[4 * i + j] = vq[j];
@@ -495,6 +519,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
             for (int i = 0; i < 8; ++i) sum_q += (float)q[t][s][i];
           unbias[t] = -kKeyBias * sum_over_groups(sum_q);
         }
+        if constexpr (PACKED) {
+          const float there = other_half(q_scale[t]);
+          if (n >= 8) q_scale[t] = there;
+        }
       }
     }
 
@@ -517,7 +545,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 
       // ---- scores ---------------------------------------------------------------------------------------------
       keys_to_lds();
-      float p[NT][8];
+      float p[NT][kEach];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         C8 kf[kSteps];
@@ -550,7 +578,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) sc = mfma16<C>(kf[s], q[b][s], sc);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[b][4 * t + i] = sc[i];
+          for (int i = 0; i < 4; ++i) {
+            const float x = sc[i];
+            if constexpr (!PACKED) p[b][4 * t + i] = x;
+            else p[b][i] = t == 0 ? x : into_upper_half(p[b][i], x);
+          }
         }
       }
       asm volatile("" ::: "memory");  // the next keys come behind these
@@ -566,46 +598,49 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
       if constexpr (!kWide) {
         if (!whole) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < low || j >= high) ks[j] = 0.f, vs[j] = 0.f;
+          for (int j = 0; j < kEach; ++j)
+            if (lane_tokens + j < low || lane_tokens + j >= high) ks[j] = 0.f, vs[j] = 0.f;
         }
       }
 #pragma unroll
       for (int b = 0; b < NT; ++b) {
         float most = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kEach; ++j) {
           p[b][j] *= q_scale[b];
           if constexpr (!kWide) p[b][j] *= ks[j];
         }
         if (!whole) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < low || j >= high) p[b][j] = -INFINITY;
+          for (int j = 0; j < kEach; ++j)
+            if (lane_tokens + j < low || lane_tokens + j >= high) p[b][j] = -INFINITY;
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, p[b][j]);
-        most = fmaxf(m[b], max_over_groups(most));
+        for (int j = 0; j < kEach; ++j) most = fmaxf(most, p[b][j]);
+        most = max_over_groups(most);
+        if constexpr (PACKED) most = fmaxf(most, other_half(most));
+        most = fmaxf(m[b], most);
         const float base = most == -INFINITY ? 0.f : most;
         float shrink = weight(m[b], base);
         m[b] = most;
         l[b] *= shrink;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kEach; ++j) {
           p[b][j] = __builtin_amdgcn_exp2f(p[b][j] - base);
           l[b] += p[b][j];
         }
         if constexpr (!kWide) {
           float top = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) p[b][j] *= vs[j], top = fmaxf(top, p[b][j]);
+          for (int j = 0; j < kEach; ++j) p[b][j] *= vs[j], top = fmaxf(top, p[b][j]);
           top = max_over_groups(top);
+          if constexpr (PACKED) top = fmaxf(top, other_half(top));
           const float ref = fmaxf(o_ref[b], top > 0.f ? base + (float)__builtin_amdgcn_frexp_expf(top) : -INFINITY);
           const float factor = ref == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base - ref);
           shrink = weight(o_ref[b], ref);
           o_ref[b] = ref;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) p[b][j] *= factor;
+          for (int j = 0; j < kEach; ++j) p[b][j] *= factor;
         }
         // (a head of no tokens yet has nothing to scale: 0 by whatever)
         if (__any(shrink != 1.f)) {
@@ -617,12 +652,17 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
       }
       C8 pf[NT], rest[NT];  // the weights, and what their rounding left (codes only)
 #pragma unroll
-      for (int b = 0; b < NT; ++b)
+      for (int b = 0; b < NT; ++b) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kEach; ++j) {
           pf[b][j] = (C)p[b][j];
           if constexpr (!kWide) rest[b][j] = (C)(p[b][j] - (float)pf[b][j]);
         }
+        if constexpr (PACKED) {  // the columns from 8 on are no heads': whatever they sum up is not read
+          both_halves(pf[b]);
+          if constexpr (!kWide) both_halves(rest[b]);
+        }
+      }
       if constexpr (!decltype(last)::value) load_scales(next_row);
 
       // ---- values ---------------------------------------------------------------------------------------------
@@ -685,6 +725,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
       l[b] = sum_over_groups(l[b]);
+      if constexpr (PACKED) l[b] += other_half(l[b]);
       if (g == 0) sm[wave][16 * b + n][0] = m[b], sm[wave][16 * b + n][1] = l[b], sm[wave][16 * b + n][2] = kWide ? m[b] : o_ref[b];
     }
 #pragma unroll
@@ -747,30 +788,39 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
   }
 }
 
-template <class T, int FORMAT, int D, int NT>
+template <class T, int FORMAT, int D, int NT, bool PACKED>
 int launch_attention(const AttnArgs& a, hipStream_t stream) {
   constexpr int kLds = kAttnWaves * attention_wave_lds(D, FORMAT);
   if constexpr (kLds > 65536 - 4096) {
     static bool raised[kMaxDevices];
-    if (raise_lds_limit<kLds>(attention_kernel<T, FORMAT, D, NT>, raised) != 0) return -1;
+    if (raise_lds_limit<kLds>(attention_kernel<T, FORMAT, D, NT, PACKED>, raised) != 0) return -1;
   }
-  attention_kernel<T, FORMAT, D, NT><<<a.workgroups, 64 * kAttnWaves, kLds, stream>>>(a);
+  attention_kernel<T, FORMAT, D, NT, PACKED><<<a.workgroups, 64 * kAttnWaves, kLds, stream>>>(a);
   DQ_CHECK_HIP(hipGetLastError());
   return 0;
 }
 
+template <class T, int FORMAT, int D>
+int attention_of_width(const AttnArgs& a, hipStream_t stream) {
+  const int group = a.heads / a.shape.kv_heads;
+  if constexpr (attention_packs(1, D, FORMAT))
+    if (attention_packs(group, D, FORMAT)) return launch_attention<T, FORMAT, D, 1, true>(a, stream);
+  if constexpr (attention_row_blocks(32, D) == 2)
+    if (attention_row_blocks(group, D) == 2) return launch_attention<T, FORMAT, D, 2, false>(a, stream);
+  return launch_attention<T, FORMAT, D, 1, false>(a, stream);
+}
+
 template <class T, int FORMAT>
 int attention_of_type(const AttnArgs& a, hipStream_t stream) {
-  const bool two = attention_row_blocks(a.heads / a.shape.kv_heads, a.shape.head_dim) == 2;
   switch (a.shape.head_dim) {
-    case 64: return two ? launch_attention<T, FORMAT, 64, 2>(a, stream) : launch_attention<T, FORMAT, 64, 1>(a, stream);
-    case 80: return two ? launch_attention<T, FORMAT, 80, 2>(a, stream) : launch_attention<T, FORMAT, 80, 1>(a, stream);
-    case 96: return two ? launch_attention<T, FORMAT, 96, 2>(a, stream) : launch_attention<T, FORMAT, 96, 1>(a, stream);
-    case 112: return two ? launch_attention<T, FORMAT, 112, 2>(a, stream) : launch_attention<T, FORMAT, 112, 1>(a, stream);
-    case 128: return two ? launch_attention<T, FORMAT, 128, 2>(a, stream) : launch_attention<T, FORMAT, 128, 1>(a, stream);
-    case 160: return launch_attention<T, FORMAT, 160, 1>(a, stream);
-    case 192: return launch_attention<T, FORMAT, 192, 1>(a, stream);
-    case 256: return launch_attention<T, FORMAT, 256, 1>(a, stream);
+    case 64: return attention_of_width<T, FORMAT, 64>(a, stream);
+    case 80: return attention_of_width<T, FORMAT, 80>(a, stream);
+    case 96: return attention_of_width<T, FORMAT, 96>(a, stream);
+    case 112: return attention_of_width<T, FORMAT, 112>(a, stream);
+    case 128: return attention_of_width<T, FORMAT, 128>(a, stream);
+    case 160: return attention_of_width<T, FORMAT, 160>(a, stream);
+    case 192: return attention_of_width<T, FORMAT, 192>(a, stream);
+    case 256: return attention_of_width<T, FORMAT, 256>(a, stream);
     default: DQ_FAIL("attention: no kernel for a head of %d", a.shape.head_dim);
   }
 }
