@@ -72,7 +72,8 @@ struct alignas(8) Quad {
 
 // A group of LANES lanes has a row (a head of a token), a lane two pieces of eight elements of it: in the half layout two that turn
 // with each other, so that every element is read once.  One row a group: four of one token, with one look at the table,
-// take as long on whole lines and longer where rows are none (7999 tokens of 64 heads of 80: 34 against 40 us).  Nothing is
+// take as long on whole lines and longer where rows are none (7999 tokens of 64 heads of 80: 33 against 40 us); two and four
+// rows side by side longer too (4000 tokens of 64 heads of 128: 24.9, 26.7, 28.9 us).  Nothing is
 // streamed here: what comes in is fresh from the projection, what goes out is read next.  Bound by memory: 4096 tokens of 40
 // heads of 128 in 15.3 us, 5.6 TB/s read and written of the 6.6 that a copy of that size reaches; one token is a launch.
 template <class T, int LANES, int LAYOUT, int FORMAT>
@@ -251,7 +252,7 @@ int launch_rows_lanes(const RowArgs& a, hipStream_t stream) {
 // first finds each one's sequence, page and place, then its threads take the pieces in the order of the result, which is
 // written as one run, 16 bytes a lane side by side.  Stores are streamed: such a result is larger than the caches.  Loads are not:
 // what was just written still lies there, and a line of narrow heads or of scales is another workgroup's too (48 sequences of
-// up to 1100 tokens, 12 heads of 96, int8: 23 us, streamed 29.7).  131071 tokens of 8 heads of 128, fp8: 138 us, 5.9 TB/s of
+// up to 1100 tokens, 12 heads of 96, int8: 21.2 us, streamed 29.7).  131071 tokens of 8 heads of 128, fp8: 138 us, 5.9 TB/s of
 // the 6.7 that a large copy reaches (a row a lane group, nothing streamed: 197; 16 codes a lane, whose two stores lie 32
 // bytes apart and fill no line at once: 290).
 struct ReadArgs {
@@ -281,7 +282,7 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
   __shared__ int s_starts[kReadStarts + 1];
   __shared__ int s_page[kReadTokens], s_place[kReadTokens];
   int block = blockIdx.x;
-  if (a.runs) {  // sixteen neighbours on one of the eight L2 caches, which share the lines between them (31.5 -> 29.5 us at 12 heads of 96)
+  if (a.runs) {  // sixteen neighbours on one of the eight L2 caches, which share the lines between them (with the write 31.5 -> 29.4 us at 12 heads of 96)
     const int run = block / (8 * kReadRun) * (8 * kReadRun), in_run = block - run;
     block = run + (in_run & 7) * kReadRun + (in_run >> 3);
   }
@@ -358,7 +359,7 @@ int launch_read(ReadArgs a, hipStream_t stream) {
   while (each > 1 && (long)(a.tokens + each - 1) / each * 2 < 4 * 256) each = (each + 1) / 2;
   a.tokens_each = each;
   unsigned blocks = (a.tokens + each - 1) / each;
-  a.runs = blocks >= 16 * kReadRun;
+  a.runs = blocks >= 16 * kReadRun;  // (of fewer the last, incomplete round of eight runs is too large a part)
   if (a.runs) blocks = (blocks + 8 * kReadRun - 1) / (8 * kReadRun) * (8 * kReadRun);
   read_kernel<T, FORMAT><<<dim3(blocks, 2), 256, 0, stream>>>(a);
   DQ_CHECK_HIP(hipGetLastError());
