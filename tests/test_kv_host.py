@@ -187,3 +187,13 @@ def test_workspace_is_named_without_a_gpu():
     assert room(1, 32, 8, 128, 16, 1, 0, CACHE_F16) == 0  # one tile: nothing to join
     assert room(1, 32, 8, 128, 16, 1000, 0, CACHE_F16) > 0
     assert room(0, 32, 8, 128, 16, 1000, 0, CACHE_F16) == 0 and room(1, 33, 8, 128, 16, 1000, 0, CACHE_F16) == 0
+
+
+def test_a_window_beyond_every_length():
+    room = _lib.load_library().dq_paged_attention_workspace_bytes
+    sizes = (1, 32, 8, 128, 16, 1000)
+    for window in (16000 - 31, 16000, 2**31 - 32, 2**31 - 1):
+        assert room(*sizes, window, CACHE_F16) == room(*sizes, 0, CACHE_F16)
+    pool = dict(kv_heads=2, head_dim=64, pages=8, page_size=16, max_pages=4)
+    for window in (64, 2**31, 2**32 + 5):  # 32 bits of the last are 5
+        assert tl.paged_attention_decode(1, 4, window=window, **pool)._native_spec[2][7] == 64

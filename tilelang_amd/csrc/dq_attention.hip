@@ -128,7 +128,7 @@ static AttnPlan attention_plan(int sequences, int heads, int kv_heads, int head_
   p.head_blocks = (group + 16 * row_blocks - 1) / (16 * row_blocks);
   p.rows = std::min(group, 16 * row_blocks);
   // (a window may begin and end inside a tile)
-  const long tokens = window > 0 && window + kAttnTile - 1 < capacity ? window + kAttnTile - 1 : capacity;
+  const long tokens = window > 0 ? std::min((long)window + kAttnTile - 1, capacity) : capacity;
   const long units = ((tokens + kAttnTile - 1) / kAttnTile + kAttnWaves - 1) / kAttnWaves, columns = (long)sequences * kv_heads * p.head_blocks;
   // Columns of up to 16 units stay whole where there are enough of them: 1024 of 2000 tokens, fp8, 86 us, cut 114; 256 of 2000,
   // bf16, 43 and 46; 128 of 1000 17 and 20; 64 of 1000 as before, 8 of 1000 13.9 and 11.2.

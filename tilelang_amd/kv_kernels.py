@@ -247,6 +247,7 @@ def paged_attention_decode(sequences: int, heads: int, kv_heads: int, head_dim: 
         raise ValueError(f"{fn}: head_dim={head_dim} must be one of {ATTENTION_HEAD_DIMS}")
     if window < 0:
         raise ValueError(f"{fn}: window={window} must be 0 (none) or positive")
+    window = min(window, max_pages * page_size)  # (32 bits in the library)
     scale = head_dim**-0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{fn}: scale must be finite")
