@@ -75,7 +75,7 @@ class _Case:
     ([515, 130], 16, 2, 256, 1024),
     ([5000, 40], 7, 1, 128, 32),
     ([77, 4, 5, 300], 16, 2, 64, 16),  # eight heads share one, and nine
-    ([77, 300], 18, 2, 64, 16), ([36, 1000], 8, 1, 112, 32), ([12, 640], 9, 1, 96, 8),
+    ([90, 700], 20, 1, 256, 16), ([33, 500, 0], 50, 2, 192, 32), ([77, 300], 18, 2, 64, 16), ([36, 1000], 8, 1, 112, 32), ([12, 640], 9, 1, 96, 8),
 ])
 def test_lengths_heads_types(cuda, lengths, heads, kv_heads, dim, page_size, cache, dtype):
     print(f"attention {lengths} {heads}/{kv_heads}x{dim} page {page_size} {cache} {dtype}", flush=True)

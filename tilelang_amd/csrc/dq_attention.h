@@ -285,17 +285,20 @@ __device__ __forceinline__ float weight(float m, float to) { return m == -INFINI
 // and more (32 sequences of 4096 tokens, 128 wide: one 84 us, two 90, three 106; 256 wide 91 and 122), two of shorter ones, whose
 // tiles are small (64 wide 99, 91, 92, four 95; fp8 128 wide, 64 sequences, 113, 91, 106), and of 8 bits, whose waves have codes
 // to convert, up to 256 wide (92 and 103).
-constexpr int attention_per_unit(int head_dim, int format) { return head_dim > 64 && (cache_is_16bit(format) || head_dim > 192) ? 1 : 2; }
+constexpr int attention_per_unit(int head_dim, int row_blocks, int format) {
+  return head_dim > 64 && (cache_is_16bit(format) || head_dim > (row_blocks == 2 ? 128 : 192)) ? 1 : 2;
+}
 
 // How many of them the registers are to leave room for: more where they fit without spills, for columns that stay whole.
 constexpr int attention_room(int head_dim, int row_blocks) {
   if (head_dim <= 64) return row_blocks == 1 ? 3 : 2;
-  return head_dim > 192 ? 1 : 2;
+  return head_dim > (row_blocks == 2 ? 128 : 192) ? 1 : 2;
 }
 
-// Blocks of 16 heads that a workgroup takes, with one read of the keys and values: two where more than 16 heads share them, but not
-// with the registers of wide heads.
-constexpr int attention_row_blocks(int heads_a_column, int head_dim) { return heads_a_column > 16 && head_dim <= 128 ? 2 : 1; }
+// Blocks of 16 heads that a workgroup takes, with one read of the keys and values: two where more than 16 heads share them (32
+// heads on one, 48 sequences of 6000 tokens, bf16, one block and two: 160 wide 67 and 45 us, 256 wide 104 and 81, some registers
+// of which lie in memory; int8, with one workgroup a compute unit in place of two: 160 wide 46.9 and 45.7, 256 wide 63 and 58).
+constexpr int attention_row_blocks(int heads_a_column) { return heads_a_column > 16 ? 2 : 1; }
 
 // A wave's LDS: 32 keys on their way into the operand's order, later 16 rows of its result.
 constexpr int attention_wave_lds(int head_dim, int format) {
@@ -805,8 +808,7 @@ int attention_of_width(const AttnArgs& a, hipStream_t stream) {
   const int group = a.heads / a.shape.kv_heads;
   if constexpr (attention_packs(1, D, FORMAT))
     if (attention_packs(group, D, FORMAT)) return launch_attention<T, FORMAT, D, 1, true>(a, stream);
-  if constexpr (attention_row_blocks(32, D) == 2)
-    if (attention_row_blocks(group, D) == 2) return launch_attention<T, FORMAT, D, 2, false>(a, stream);
+  if (attention_row_blocks(group) == 2) return launch_attention<T, FORMAT, D, 2, false>(a, stream);
   return launch_attention<T, FORMAT, D, 1, false>(a, stream);
 }
 

@@ -124,7 +124,7 @@ struct AttnPlan {
 static AttnPlan attention_plan(int sequences, int heads, int kv_heads, int head_dim, int format, long capacity, int window) {
   AttnPlan p;
   const int group = heads / kv_heads;
-  const int row_blocks = attention_row_blocks(group, head_dim);
+  const int row_blocks = attention_row_blocks(group);
   p.head_blocks = (group + 16 * row_blocks - 1) / (16 * row_blocks);
   p.rows = std::min(group, 16 * row_blocks);
   // (a window may begin and end inside a tile)
@@ -133,7 +133,7 @@ static AttnPlan attention_plan(int sequences, int heads, int kv_heads, int head_
   // Columns of up to 16 units stay whole where there are enough of them: 1024 of 2000 tokens, fp8, 86 us, cut 114; 256 of 2000,
   // bf16, 43 and 46; 128 of 1000 17 and 20; 64 of 1000 as before, 8 of 1000 13.9 and 11.2.
   p.joins = units > (columns >= 128 ? 16 : kWholeUnits);
-  p.workgroups = (int)(p.joins ? std::min<long>(kComputeUnits * attention_per_unit(head_dim, format), columns * units) : columns);
+  p.workgroups = (int)(p.joins ? std::min<long>(kComputeUnits * attention_per_unit(head_dim, row_blocks, format), columns * units) : columns);
   return p;
 }
 
