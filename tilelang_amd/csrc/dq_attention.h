@@ -307,8 +307,8 @@ constexpr int attention_wave_lds(int head_dim, int format) {
 }
 
 // Whether a workgroup's heads are taken PACKED, see there: up to eight, where instructions and not memory bound the kernel, which
-// is in narrow heads of 8 bits (64 sequences of 4000 tokens, eight key-value heads: int8, 64 wide, 68 -> 60 us, 80 wide 78 -> 72;
-// fp8, 96 wide, 77 -> 73; 128 wide 180 -> 177 and 167 -> 167; 16 bits, 64 wide, 83 -> 83).
+// is in narrow heads of 8 bits (64 sequences of 4000 tokens, eight key-value heads: int8, 64 wide, 55 -> 52 us, 80 wide 74 -> 71,
+// 96 wide 77 -> 75; fp8, 112 wide, 84 -> 82; 128 wide 88 -> 88; 16 bits, 64 wide, 83 -> 83).
 constexpr bool attention_packs(int heads_a_column, int head_dim, int format) { return heads_a_column <= 8 && head_dim < 128 && !cache_is_16bit(format); }
 
 // What lane n ^ 8 of the 16 has; into lane n < 8 its four elements, behind its own four.
