@@ -38,6 +38,7 @@ struct RowArgs {
   float* scale[2];
   long row_stride, out_stride;
   int tokens, q_heads, head_dim, rotary_dim, table_rows, interleaved, inverse;
+  int row_end;       // elements of a row that are read and written: in place no more pieces than turn (64 of 128: 27.4 -> 13.2 us)
   CacheShape shape;
 };
 
@@ -84,15 +85,15 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
   const int token = group / heads, head = group - token * heads;
   if (token >= a.tokens) return;
   const int keys_end = a.q_heads + (FORMAT >= 0 ? a.shape.kv_heads : 0);  // rows that are rotated
-  const int r = a.rotary_dim, h = r >> 1, pieces = a.head_dim >> 3, half = (pieces + 1) >> 1;
+  const int r = a.rotary_dim, h = r >> 1, pieces = a.row_end >> 3, half = (pieces + 1) >> 1;
   // this lane's pieces, as their first elements; one that lies behind the row is not there
-  int d[2] = {lane < half ? 8 * lane : a.head_dim, lane < half ? 8 * (lane + half) : a.head_dim};
+  int d[2] = {lane < half ? 8 * lane : a.row_end, lane < half ? 8 * (lane + half) : a.row_end};
   if (LAYOUT == ROTARY_HALF) {
     const bool pair = lane < r >> 4;
     d[0] = pair ? 8 * lane : 16 * lane;  // (the pieces behind the rotated ones two by two: lane r / 16 begins at r)
     d[1] = pair ? 8 * lane + h : 16 * lane + 8;
   }
-  const bool inside[2] = {d[0] < a.head_dim, d[1] < a.head_dim};
+  const bool inside[2] = {d[0] < a.row_end, d[1] < a.row_end};
   const bool turns = LAYOUT != ROTARY_NONE && head < keys_end;
 
   const T* const row = FORMAT >= 0 && a.v && head >= keys_end
@@ -241,11 +242,11 @@ int launch_rows_layout(const RowArgs& a, hipStream_t stream) {
 
 template <class T, int FORMAT>
 int launch_rows_lanes(const RowArgs& a, hipStream_t stream) {
-  if (a.head_dim <= 64) return launch_rows_layout<T, 4, FORMAT>(a, stream);
-  if (a.head_dim <= 128) return launch_rows_layout<T, 8, FORMAT>(a, stream);
-  if (a.head_dim <= 256) return launch_rows_layout<T, 16, FORMAT>(a, stream);
+  if (a.row_end <= 64) return launch_rows_layout<T, 4, FORMAT>(a, stream);
+  if (a.row_end <= 128) return launch_rows_layout<T, 8, FORMAT>(a, stream);
+  if (a.row_end <= 256) return launch_rows_layout<T, 16, FORMAT>(a, stream);
   if constexpr (FORMAT < 0) return launch_rows_layout<T, 32, FORMAT>(a, stream);
-  DQ_FAIL("a head of %d is beyond the cache's %d", a.head_dim, kMaxHeadDim);
+  DQ_FAIL("a head of %d is beyond the cache's %d", a.row_end, kMaxHeadDim);
 }
 
 // Reading back: a workgroup has some tokens of the packed result, 1024 pieces of eight elements or at most kReadTokens tokens.  It
@@ -374,6 +375,7 @@ int rotary(const void* X, const float* Table, const int* Positions, void* Out, i
   a.x = X, a.table = Table, a.positions = Positions, a.out = Out, a.row_stride = row_stride, a.out_stride = out_stride;
   a.tokens = tokens, a.q_heads = heads, a.head_dim = head_dim, a.rotary_dim = rotary_dim, a.table_rows = positions;
   a.interleaved = interleaved, a.inverse = inverse;
+  a.row_end = X == Out ? (rotary_dim + 7) & ~7 : head_dim;
   return bf16 ? launch_rows_lanes<bf16_t, -1>(a, stream) : launch_rows_lanes<half_t, -1>(a, stream);
 }
 
@@ -385,7 +387,7 @@ int kv_cache_write(const void* X, const void* V, const float* Table, const int* 
   a.cache[0] = KCache, a.cache[1] = VCache, a.scale[0] = KScale, a.scale[1] = VScale;
   a.row_stride = (long)(heads + (V ? 1 : 2) * kv_heads) * head_dim, a.out_stride = (long)heads * head_dim;
   a.tokens = tokens, a.q_heads = heads, a.head_dim = head_dim, a.rotary_dim = rotary_dim, a.table_rows = positions;
-  a.interleaved = interleaved;
+  a.interleaved = interleaved, a.row_end = head_dim;
   a.shape = {pages, kv_heads, page_shift, head_dim};
   switch (format) {
     case CACHE_FP8: return bf16 ? launch_rows_lanes<bf16_t, CACHE_FP8>(a, stream) : launch_rows_lanes<half_t, CACHE_FP8>(a, stream);
