@@ -284,7 +284,7 @@ __device__ __forceinline__ float weight(float m, float to) { return m == -INFINI
 // cache in flight, for every one more is a column cut once more and has less in a row.  One of 16-bit rows of 160 bytes
 // and more (32 sequences of 4096 tokens, 128 wide: one 84 us, two 90, three 106; 256 wide 91 and 122), two of shorter ones, whose
 // tiles are small (64 wide 99, 91, 92, four 95; fp8 128 wide, 64 sequences, 113, 91, 106), and of 8 bits, whose waves have codes
-// to convert, up to 256 wide (92 and 103).
+// to convert, up to 256 wide (92 and 103; two blocks of 16 heads of more than 128 elements leave registers for one).
 constexpr int attention_per_unit(int head_dim, int row_blocks, int format) {
   return head_dim > 64 && (cache_is_16bit(format) || head_dim > (row_blocks == 2 ? 128 : 192)) ? 1 : 2;
 }
