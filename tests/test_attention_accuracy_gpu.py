@@ -1,0 +1,83 @@
+"""Attention of one new token where its numbers are far apart: scores, value scales and weights over the whole range that fp32 holds."""
+
+import math
+
+import pytest
+import torch
+
+import tilelang_amd as tl
+from kv_reference import attention, attention_bound, tokens_of
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float8_e4m3fn": torch.float8_e4m3fn, "int8": torch.int8}
+#: heads, kv_heads, head_dim: heads that share lanes, one block of 16 and two of them
+HEADS = [(4, 1, 64), (12, 1, 64), (6, 2, 128), (20, 1, 128), (5, 1, 256), (18, 1, 160)]
+
+
+class _Sequence:
+    """One sequence in pages in order: keys and values [length, kv_heads, head_dim] as numbers of the cache's type, scales
+    [length] or None, queries [heads, head_dim]."""
+
+    def __init__(self, cuda, q, keys, values, held, key_scale=None, value_scale=None, page_size=16):
+        length, kv_heads, dim = keys.shape
+        self.length, self.q, self.dim, self.held = length, q.to(cuda)[None], dim, held
+        pages = -(-length // page_size)
+        self.buffers = []
+        for x, s in ((keys, key_scale), (values, value_scale)):
+            whole = torch.zeros((pages * page_size, kv_heads, dim))
+            whole[:length] = x.float()
+            cache = whole.view(pages, page_size, kv_heads, dim).transpose(1, 2).contiguous().to(held).to(cuda)
+            scale = None
+            if s is not None:
+                scale = torch.zeros((pages * page_size, kv_heads))
+                scale[:length] = s[:, None]
+                scale = scale.view(pages, page_size, kv_heads).transpose(1, 2).contiguous().to(cuda)
+            self.buffers.append((cache, scale))
+        self.table = torch.arange(pages, dtype=torch.int32, device=cuda)[None]
+        name = {v: k for k, v in DTYPES.items()}
+        self.sizes = dict(kv_heads=kv_heads, head_dim=dim, pages=pages, page_size=page_size, max_pages=pages, dtype=name[q.dtype],
+                          cache_dtype=None if held == q.dtype else name[held])
+
+    def run(self, scale, length=None, max_pages=None):
+        (kc, ks), (vc, vs) = self.buffers
+        n = torch.tensor([self.length if length is None else length], dtype=torch.int32, device=kc.device)
+        table = self.table if max_pages is None else torch.nn.functional.pad(self.table, (0, max_pages - self.table.shape[1]), value=-1)
+        sizes = self.sizes | dict(max_pages=table.shape[1])
+        kernel = tl.paged_attention_decode(1, self.q.shape[1], scale=scale, with_lse=True, **sizes)
+        out, lse = kernel(self.q, *((kc, vc) if ks is None else (kc, vc, ks, vs)), table, n)
+        return out[0].cpu().double(), lse[0].cpu().double()
+
+    def exact(self, scale):
+        k, v = (tokens_of(c, s, self.table[0].cpu(), self.length) for c, s in self.buffers)
+        return attention(self.q[0], k, v, scale)
+
+
+def _coded(cuda, heads, kv_heads, dim, held, scores, value_scale, codes=None, dtype=torch.bfloat16):
+    """A quantised sequence whose tokens' scores are `scores` for every head: queries of ones on codes of 16, scale 1 / (16 head_dim)."""
+    n = len(scores)
+    q = torch.ones((heads, dim), dtype=dtype)
+    keys = torch.full((n, kv_heads, dim), 16.0)
+    if codes is None:
+        codes = torch.randint(-120, 121, (n, kv_heads, dim), generator=torch.Generator().manual_seed(n + dim)).float()
+    return _Sequence(cuda, q, keys, codes, held, torch.tensor(scores), torch.tensor(value_scale)), 1 / (16 * dim)
+
+
+@pytest.mark.parametrize("cache", ["float8_e4m3fn", "int8"])
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("length", [20, 300])
+@pytest.mark.parametrize("best", ["first", "later"])
+def test_best_token_without_a_value(cuda, best, length, heads, kv_heads, dim, cache):
+    """The token that outweighs all others has a value scale of zero, as a head of zeros is stored: what the others leave is tiny, and a
+    number.  First: among the first tokens, the others 86 below (times their scale out of fp32's normal range).  Later: 200 above those
+    that came before."""
+    print(f"best token {best} of {length}, {heads}/{kv_heads}x{dim} {cache}", flush=True)
+    scores, scales = [0.0] * length, [2.0**-5] * length
+    for t in (3,) if best == "first" else range(min(140, length - 5), length):
+        scores[t], scales[t] = (86.0 if best == "first" else 200.0), 0.0
+    case, scale = _coded(cuda, heads, kv_heads, dim, DTYPES[cache], scores, scales)
+    out, lse = case.run(scale)
+    want, want_lse, spread = case.exact(scale)
+    assert torch.isfinite(out).all()
+    assert ((out - want).abs() <= attention_bound(want, spread, torch.bfloat16, case.held)).all()
+    assert ((lse - want_lse).abs() <= 2.0**-16 * (1 + want_lse.abs())).all()

@@ -18,7 +18,8 @@
 // A quantised cache is multiplied as fp16: a code is exact there; a query is scaled by a power of two so that its largest element
 // lies in [2^14, 2^15), where bf16's range is no issue; a token's scale multiplies its score in fp32.  A weight times its
 // value's scale, w_t = p_t c_t, may lie anywhere: o is kept relative to a power of two of its own, the running maximum of a
-// head's w_t, as the sum is relative to the running maximum of its scores.  w_t goes into the second product in two parts, what
+// head's w_t, as the sum is relative to the running maximum of its scores; it is counted from that maximum, and from 2^-126 on, so
+// that no factor is infinite where the token of the largest score has a value of zero.  w_t goes into the second product in two parts, what
 // fp16 holds of it and what that rounding left, so that the result is rounded once, at the end.  Of a 16-bit cache p_t is
 // rounded to the cache's type alone: the largest are near 1, where that costs least, and a part of zero or below would make an
 // infinity among the values a NaN.
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 
   constexpr int kRow = D + 4;                             // of a wave's result: 16 rows on 64 banks
 
-  __shared__ float sm[kAttnWaves][16 * NT][3];  // a wave's m, l and the power of two that its o is relative to
+  __shared__ float sm[kAttnWaves][16 * NT][3];  // a wave's m, l and the power of two, from 2^m, that its o is relative to
   __shared__ ShareSearch search;
   extern __shared__ __align__(16) char lds[];
 
@@ -531,10 +532,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 
     float4_t acc[NT][kAcc];
     float m[NT], l[NT];
-    float o_ref[NT];  // acc is o / 2^o_ref (quantised caches; else 2^m)
+    float o_exp[NT];  // acc is o / 2^(m + o_exp) (quantised caches; else 2^m)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      m[t] = -INFINITY, l[t] = 0.f, o_ref[t] = -INFINITY;
+      m[t] = -INFINITY, l[t] = 0.f, o_exp[t] = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kAcc; ++i) acc[t][i] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
@@ -625,6 +626,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
         most = fmaxf(m[b], most);
         const float base = most == -INFINITY ? 0.f : most;
         float shrink = weight(m[b], base);
+        const float grown = m[b] - base;
         m[b] = most;
         l[b] *= shrink;
 #pragma unroll
@@ -638,10 +640,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
           for (int j = 0; j < kEach; ++j) p[b][j] *= vs[j], top = fmaxf(top, p[b][j]);
           top = max_over_groups(top);
           if constexpr (PACKED) top = fmaxf(top, other_half(top));
-          const float ref = fmaxf(o_ref[b], top > 0.f ? base + (float)__builtin_amdgcn_frexp_expf(top) : -INFINITY);
-          const float factor = ref == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(base - ref);
-          shrink = weight(o_ref[b], ref);
-          o_ref[b] = ref;
+          // (smaller ones than 2^kLowest are small beside it; where o_exp lies below it, these weights are all zero)
+          constexpr int kLowest = -126;
+          const float before = o_exp[b] + grown;
+          o_exp[b] = fmaxf(before, top > 0.f ? (float)max(__builtin_amdgcn_frexp_expf(top), kLowest) : -INFINITY);
+          const float factor = __builtin_amdgcn_exp2f(fminf(-o_exp[b], -kLowest));
+          shrink = weight(before, o_exp[b]);
 #pragma unroll
           for (int j = 0; j < kEach; ++j) p[b][j] *= factor;
         }
@@ -729,7 +733,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
     for (int b = 0; b < NT; ++b) {
       l[b] = sum_over_groups(l[b]);
       if constexpr (PACKED) l[b] += other_half(l[b]);
-      if (g == 0) sm[wave][16 * b + n][0] = m[b], sm[wave][16 * b + n][1] = l[b], sm[wave][16 * b + n][2] = kWide ? m[b] : o_ref[b];
+      if (g == 0) sm[wave][16 * b + n][0] = m[b], sm[wave][16 * b + n][1] = l[b], sm[wave][16 * b + n][2] = kWide ? (m[b] == -INFINITY ? m[b] : 0.f) : o_exp[b];
     }
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
@@ -753,10 +757,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
         for (int w = 0; w < kAttnWaves; ++w) most = fmaxf(most, sm[w][16 * b + row][0]);
         const float sink = complete ? sink_here[b] : -INFINITY;
         const float base = fmaxf(most, sink);
-        float factor[kAttnWaves], total_weight = weight(sink, base);
+        float root[kAttnWaves], total_weight = weight(sink, base);
 #pragma unroll
         for (int w = 0; w < kAttnWaves; ++w) {
-          factor[w] = weight(sm[w][16 * b + row][2], base);
+          // (-inf: nothing summed up.  The root: a factor may lie below fp32's range where factor times sum does not)
+          const float power = sm[w][16 * b + row][2];
+          root[w] = power == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (sm[w][16 * b + row][0] - base + power));
           total_weight += weight(sm[w][16 * b + row][0], base) * sm[w][16 * b + row][1];
         }
         if (complete) {
@@ -765,7 +771,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
           for (int d = threadIdx.x & 15; d < D; d += 16) {
             float x = 0.f;
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) x += factor[w] * result(w, row)[d];
+            for (int w = 0; w < kAttnWaves; ++w) x += root[w] * result(w, row)[d] * root[w];
             reinterpret_cast<T*>(a.out)[at * D + d] = (T)(x * inv);
           }
           if (a.lse && (threadIdx.x & 15) == 0)
@@ -776,7 +782,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
           for (int d = threadIdx.x & 15; d < D; d += 16) {
             float x = 0.f;
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) x += factor[w] * result(w, row)[d];
+            for (int w = 0; w < kAttnWaves; ++w) x += root[w] * result(w, row)[d] * root[w];
             a.part_o[part * D + d] = x;
           }
           if ((threadIdx.x & 15) == 0) a.part_ml[2 * part] = most, a.part_ml[2 * part + 1] = total_weight;
