@@ -81,3 +81,19 @@ def test_best_token_without_a_value(cuda, best, length, heads, kv_heads, dim, ca
     assert torch.isfinite(out).all()
     assert ((out - want).abs() <= attention_bound(want, spread, torch.bfloat16, case.held)).all()
     assert ((lse - want_lse).abs() <= 2.0**-16 * (1 + want_lse.abs())).all()
+
+
+@pytest.mark.parametrize("cache", ["float8_e4m3fn", "int8"])
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("sign", ["all", "some"])
+def test_negative_value_scales(cuda, sign, heads, kv_heads, dim, cache):
+    """value = code * scale, whatever the scale's sign and size."""
+    print(f"negative scales ({sign}) {heads}/{kv_heads}x{dim} {cache}", flush=True)
+    n, gen = 333, torch.Generator().manual_seed(dim)
+    for exponent in (-40, 0, 30):
+        scales = torch.exp2(exponent + 4 * torch.rand(n, generator=gen))
+        scales = -scales if sign == "all" else scales * torch.where(torch.rand(n, generator=gen) < 0.3, -64.0, 1.0)
+        case, scale = _coded(cuda, heads, kv_heads, dim, DTYPES[cache], torch.randn(n, generator=gen).tolist(), scales.tolist())
+        out, _ = case.run(scale)
+        want, _, spread = case.exact(scale)
+        assert ((out - want).abs() <= attention_bound(want, spread, torch.bfloat16, case.held)).all(), exponent

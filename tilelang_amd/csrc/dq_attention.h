@@ -18,7 +18,7 @@
 // A quantised cache is multiplied as fp16: a code is exact there; a query is scaled by a power of two so that its largest element
 // lies in [2^14, 2^15), where bf16's range is no issue; a token's scale multiplies its score in fp32.  A weight times its
 // value's scale, w_t = p_t c_t, may lie anywhere: o is kept relative to a power of two of its own, the running maximum of a
-// head's w_t, as the sum is relative to the running maximum of its scores; it is counted from that maximum, and from 2^-126 on, so
+// head's |w_t|, as the sum is relative to the running maximum of its scores; it is counted from that maximum, and from 2^-126 on, so
 // that no factor is infinite where the token of the largest score has a value of zero.  w_t goes into the second product in two parts, what
 // fp16 holds of it and what that rounding left, so that the result is rounded once, at the end.  Of a 16-bit cache p_t is
 // rounded to the cache's type alone: the largest are near 1, where that costs least, and a part of zero or below would make an
@@ -637,7 +637,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
         if constexpr (!kWide) {
           float top = 0.f;
 #pragma unroll
-          for (int j = 0; j < kEach; ++j) p[b][j] *= vs[j], top = fmaxf(top, p[b][j]);
+          for (int j = 0; j < kEach; ++j) p[b][j] *= vs[j], top = fmaxf(top, fabsf(p[b][j]));
           top = max_over_groups(top);
           if constexpr (PACKED) top = fmaxf(top, other_half(top));
           // (smaller ones than 2^kLowest are small beside it; where o_exp lies below it, these weights are all zero)
