@@ -97,3 +97,33 @@ def test_negative_value_scales(cuda, sign, heads, kv_heads, dim, cache):
         out, _ = case.run(scale)
         want, _, spread = case.exact(scale)
         assert ((out - want).abs() <= attention_bound(want, spread, torch.bfloat16, case.held)).all(), exponent
+
+
+def _one_and_many(cuda, heads, kv_heads, dim, dtype, cache, n, gap):
+    """One early token of a value of zero, and n others whose scores lie `gap` to `gap` - 1 below its score."""
+    gen = torch.Generator().manual_seed(n + dim)
+    below = gap - torch.rand(n, generator=gen)
+    values = 0.5 + torch.rand((n, kv_heads, dim), generator=gen)  # (of one sign, so that what is lost adds up)
+    values[5] = 0.0
+    if cache != "same":
+        scores = gap - below
+        scores[5] = gap
+        return _coded(cuda, heads, kv_heads, dim, DTYPES[cache], scores.tolist(), [2.0**-6] * n, (values * 60).round(), DTYPES[dtype])
+    keys = (gap - below)[:, None, None].expand(n, kv_heads, dim).clone()
+    keys[5] = gap
+    held = DTYPES[dtype]
+    return _Sequence(cuda, torch.ones((heads, dim), dtype=held), keys.to(held), values.to(held), held), 1 / dim
+
+
+@pytest.mark.parametrize("dtype,cache", [("float16", "same"), ("float16", "float8_e4m3fn"), ("bfloat16", "int8"), ("bfloat16", "same")])
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("gap", [12.0, 18.5])
+def test_many_light_tokens_beside_a_heavy_one(cuda, gap, heads, kv_heads, dim, dtype, cache):
+    """Weights of e^-18 and less of the largest, below what fp16 holds beside 1, whose values are all that there is."""
+    print(f"light tokens {gap} below, {heads}/{kv_heads}x{dim} {dtype} {cache}", flush=True)
+    case, scale = _one_and_many(cuda, heads, kv_heads, dim, dtype, cache, 3000, gap)
+    out, _ = case.run(scale)
+    want, _, spread = case.exact(scale)
+    # the output's rounding (fp16's smallest steps among them), fp32 scores of up to 20 and sums: 2^-14
+    half = 2.0**-11 if dtype == "float16" else 2.0**-8
+    assert ((out - want).abs() <= half * want.abs() + 2.0**-25 + 2.0**-14 * spread).all(), ((out - want).abs() / spread).max()

@@ -18,11 +18,13 @@
 // A quantised cache is multiplied as fp16: a code is exact there; a query is scaled by a power of two so that its largest element
 // lies in [2^14, 2^15), where bf16's range is no issue; a token's scale multiplies its score in fp32.  A weight times its
 // value's scale, w_t = p_t c_t, may lie anywhere: o is kept relative to a power of two of its own, the running maximum of a
-// head's |w_t|, as the sum is relative to the running maximum of its scores; it is counted from that maximum, and from 2^-126 on, so
-// that no factor is infinite where the token of the largest score has a value of zero.  w_t goes into the second product in two parts, what
-// fp16 holds of it and what that rounding left, so that the result is rounded once, at the end.  Of a 16-bit cache p_t is
+// head's |w_t|, as the sum is relative to the running maximum of its scores; it is counted from that maximum, and from 2^-112 on, so
+// that no factor is infinite where the token of the largest score has a value of zero.  w_t goes into the second product in two
+// parts, what fp16 holds of it and what that rounding left, so that the result is rounded once, at the end.  Of a 16-bit cache p_t is
 // rounded to the cache's type alone: the largest are near 1, where that costs least, and a part of zero or below would make an
-// infinity among the values a NaN.
+// infinity among the values a NaN.  Weights that are rounded to fp16 are taken times 2^kLift, the largest then about 2^15 of the
+// 65504 that fp16 ends at: a weight of 2^-29 of the largest keeps 11 bits and one of 2^-39 is not lost, where at 1 that was 2^-14 and 2^-24
+// and thousands of tokens that light beside a heavy one of a small value (all that the result is made of) were.
 //
 // Bound by memory: eight heads on one key-value head do 8 operations a byte of a 16-bit cache, where the chip has some 300.
 // 128 sequences of 8192 tokens, 8 heads of 128, int8: 334 us, 6.6 TB/s of the 6.9 that plain streamed reads of such pieces
@@ -335,6 +337,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
   constexpr bool kWide = cache_is_16bit(FORMAT);
   using C = typename std::conditional<kWide, T, half_t>::type;  // what the products are taken in
   typedef typename Vec8<C>::type C8;
+  constexpr float kLift = __is_same(C, half_t) ? 15.f : 0.f;  // weights are taken times 2^kLift
   constexpr bool kBiased = FORMAT == CACHE_I8;  // int8 keys are multiplied as code + kKeyBias, of which kKeyBias * sum q is taken off
   constexpr int kBytes = kWide ? 2 : 1;
   constexpr int kSteps = (D + 31) / 32;
@@ -348,7 +351,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 
   constexpr int kRow = D + 4;                             // of a wave's result: 16 rows on 64 banks
 
-  __shared__ float sm[kAttnWaves][16 * NT][3];  // a wave's m, l and the power of two, from 2^m, that its o is relative to
+  __shared__ float sm[kAttnWaves][16 * NT][3];  // a wave's m, l and the power of two, from 2^m, that its o is relative to (or -inf)
   __shared__ ShareSearch search;
   extern __shared__ __align__(16) char lds[];
 
@@ -532,7 +535,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 
     float4_t acc[NT][kAcc];
     float m[NT], l[NT];
-    float o_exp[NT];  // acc is o / 2^(m + o_exp) (quantised caches; else 2^m)
+    float o_exp[NT];  // acc is o / 2^(m + o_exp - kLift) (quantised caches; else 2^(m - kLift))
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t] = -INFINITY, l[t] = 0.f, o_exp[t] = -INFINITY;
@@ -641,13 +644,17 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
           top = max_over_groups(top);
           if constexpr (PACKED) top = fmaxf(top, other_half(top));
           // (smaller ones than 2^kLowest are small beside it; where o_exp lies below it, these weights are all zero)
-          constexpr int kLowest = -126;
+          constexpr int kLowest = -112;
           const float before = o_exp[b] + grown;
           o_exp[b] = fmaxf(before, top > 0.f ? (float)max(__builtin_amdgcn_frexp_expf(top), kLowest) : -INFINITY);
-          const float factor = __builtin_amdgcn_exp2f(fminf(-o_exp[b], -kLowest));
+          const float factor = __builtin_amdgcn_exp2f(fminf(kLift - o_exp[b], kLift - kLowest));
           shrink = weight(before, o_exp[b]);
 #pragma unroll
           for (int j = 0; j < kEach; ++j) p[b][j] *= factor;
+        }
+        if constexpr (kWide && kLift != 0.f) {
+#pragma unroll
+          for (int j = 0; j < kEach; ++j) p[b][j] *= 0x1p15f;
         }
         // (a head of no tokens yet has nothing to scale: 0 by whatever)
         if (__any(shrink != 1.f)) {
@@ -733,7 +740,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
     for (int b = 0; b < NT; ++b) {
       l[b] = sum_over_groups(l[b]);
       if constexpr (PACKED) l[b] += other_half(l[b]);
-      if (g == 0) sm[wave][16 * b + n][0] = m[b], sm[wave][16 * b + n][1] = l[b], sm[wave][16 * b + n][2] = kWide ? (m[b] == -INFINITY ? m[b] : 0.f) : o_exp[b];
+      if (g == 0) sm[wave][16 * b + n][0] = m[b], sm[wave][16 * b + n][1] = l[b], sm[wave][16 * b + n][2] = (kWide ? (m[b] == -INFINITY ? m[b] : 0.f) : o_exp[b]) - kLift;
     }
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
