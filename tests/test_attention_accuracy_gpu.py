@@ -127,3 +127,26 @@ def test_many_light_tokens_beside_a_heavy_one(cuda, gap, heads, kv_heads, dim, d
     # the output's rounding (fp16's smallest steps among them), fp32 scores of up to 20 and sums: 2^-14
     half = 2.0**-11 if dtype == "float16" else 2.0**-8
     assert ((out - want).abs() <= half * want.abs() + 2.0**-25 + 2.0**-14 * spread).all(), ((out - want).abs() / spread).max()
+
+
+@pytest.mark.parametrize("cache", ["float8_e4m3fn", "int8"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 1, 128), (16, 1, 256), (4, 1, 64), (20, 2, 128)])
+@pytest.mark.parametrize("mean,width", [(3.0, 2.0), (12.0, 8.0)])
+def test_queries_that_are_not_centred(cuda, mean, width, heads, kv_heads, dim, cache):
+    """Queries whose elements have a mean, keys with one channel far out: the score is a small part of what such queries would sum up to
+    with every code moved by a constant."""
+    print(f"queries around {mean} {heads}/{kv_heads}x{dim} {cache}", flush=True)
+    gen, n = torch.Generator().manual_seed(dim + int(mean)), 200
+    q = (mean + width * torch.randn((heads, dim), generator=gen)).to(torch.float16)
+    keys, values = torch.randn((2, n, kv_heads, dim), generator=gen)
+    keys[..., 7] = 30.0
+    top = 127.0 if cache == "int8" else 448.0
+    most = keys.abs().amax(dim=(1, 2))
+    codes = keys * (top / most)[:, None, None]
+    case = _Sequence(cuda, q, codes.round() if cache == "int8" else codes, (values * 30).round(), DTYPES[cache], most / top,
+                     torch.full((n,), 1 / 30))
+    out, lse = case.run(dim**-0.5)
+    want, want_lse, spread = case.exact(dim**-0.5)
+    assert ((lse - want_lse).abs() <= 2.0**-16 * (1 + want_lse.abs())).all(), (lse - want_lse).abs().max()
+    # a score's error is a weight's, relative: as above, of scores of up to a hundred
+    assert ((out - want).abs() <= 2.0**-11 * want.abs() + 2.0**-25 + 2.0**-13 * spread).all(), ((out - want).abs() / spread).max()

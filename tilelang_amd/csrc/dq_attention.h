@@ -248,21 +248,19 @@ __device__ __forceinline__ float4_t mfma16(typename Vec8<T>::type a, typename Ve
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Four codes (a dword) -> four fp16, exact; int8 with kKeyBias on top where BIASED.
-constexpr float kKeyBias = 1152.f;
-template <int FORMAT, bool BIASED = false>
+// Four codes (a dword) -> four fp16, exact.
+template <int FORMAT>
 __device__ __forceinline__ void codes4_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (FORMAT == CACHE_FP8) {
     lo = as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
     hi = as_u32(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
   } else {
-    // code + 128 in the last byte of an fp16 whose last place is 1: 1024 + 128 + code
+    // code + 128 in the last byte of an fp16 whose last place is 1: 1024 + 128 + code, and 1152 off.  (Keys too: with the 1152 left in, and
+    // 1152 * sum q taken off the product, the fp32 sum of queries with a mean runs so high that the score is what its rounding leaves.)
     const uint32_t u = w ^ 0x80808080u;
     lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u), hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-    if constexpr (!BIASED) {
-      const half2_t bias = {(half_t)kKeyBias, (half_t)kKeyBias};
-      lo = as_u32(as_half2(lo) - bias), hi = as_u32(as_half2(hi) - bias);
-    }
+    const half2_t bias = {(half_t)1152.f, (half_t)1152.f};
+    lo = as_u32(as_half2(lo) - bias), hi = as_u32(as_half2(hi) - bias);
   }
 }
 
@@ -338,7 +336,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
   using C = typename std::conditional<kWide, T, half_t>::type;  // what the products are taken in
   typedef typename Vec8<C>::type C8;
   constexpr float kLift = __is_same(C, half_t) ? 15.f : 0.f;  // weights are taken times 2^kLift
-  constexpr bool kBiased = FORMAT == CACHE_I8;  // int8 keys are multiplied as code + kKeyBias, of which kKeyBias * sum q is taken off
   constexpr int kBytes = kWide ? 2 : 1;
   constexpr int kSteps = (D + 31) / 32;
   using VB = ValueBlocks<D>;
@@ -497,10 +494,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
 
     // ---- queries: the second operand of the first product, held for the whole walk -----------------------------
     C8 q[NT][kSteps];
-    float q_scale[NT], unbias[NT];
+    float q_scale[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      q_scale[t] = a.score_scale, unbias[t] = 0.f;
+      q_scale[t] = a.score_scale;
       if constexpr (kWide) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) q[t][s] = q_raw[t][s];
@@ -518,14 +515,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
           for (int i = 0; i < 8; ++i) q[t][s][i] = (C)ldexpf((float)q_raw[t][s][i], shift);
-        if constexpr (kBiased) {
-          float sum_q = 0.f;
-#pragma unroll
-          for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum_q += (float)q[t][s][i];
-          unbias[t] = -kKeyBias * sum_over_groups(sum_q);
-        }
         if constexpr (PACKED) {
           const float there = other_half(q_scale[t]);
           if (n >= 8) q_scale[t] = there;
@@ -573,15 +562,15 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
               c = *reinterpret_cast<const uint2_t*>(p);
             }
             uint32_t h[4];
-            codes4_to_half<FORMAT, kBiased>(c[0], h[0], h[1]);
-            codes4_to_half<FORMAT, kBiased>(c[1], h[2], h[3]);
+            codes4_to_half<FORMAT>(c[0], h[0], h[1]);
+            codes4_to_half<FORMAT>(c[1], h[2], h[3]);
             w = uint4_t{h[0], h[1], h[2], h[3]};
           }
           kf[s] = __builtin_bit_cast(C8, w);
         }
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-          float4_t sc = {unbias[b], unbias[b], unbias[b], unbias[b]};
+          float4_t sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) sc = mfma16<C>(kf[s], q[b][s], sc);
 #pragma unroll
