@@ -129,6 +129,28 @@ def test_many_light_tokens_beside_a_heavy_one(cuda, gap, heads, kv_heads, dim, d
     assert ((out - want).abs() <= half * want.abs() + 2.0**-25 + 2.0**-14 * spread).all(), ((out - want).abs() / spread).max()
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("cache", ["same", "float8_e4m3fn", "int8"])
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("length", [3, 17, 70])
+def test_weights_keep_their_bits(cuda, length, heads, kv_heads, dim, cache, dtype):
+    """The weights' rounding does not show beside the output's: 2^-16 of each where they go into the product in two parts of bf16 (less in
+    fp16), and 2^-14 from fp32 scores, exponentials and sums."""
+    print(f"weights' bits {length} {heads}/{kv_heads}x{dim} {dtype} {cache}", flush=True)
+    held = DTYPES[dtype if cache == "same" else cache]
+    gen = torch.Generator().manual_seed(length * dim)
+    q = torch.randn((heads, dim), generator=gen).to(DTYPES[dtype])
+    keys, values = torch.randn((2, length, kv_heads, dim), generator=gen)
+    scales = (None, None)
+    if cache != "same":
+        keys, values, scales = (keys * 40).round(), (values * 40).round(), (torch.rand((2, length), generator=gen) + 0.5) / 40
+    case = _Sequence(cuda, q, keys, values, held, *scales)
+    out, _ = case.run(dim**-0.5)
+    want, _, spread = case.exact(dim**-0.5)
+    half = 2.0**-11 if dtype == "float16" else 2.0**-8
+    assert ((out - want).abs() <= half * want.abs() + 2.0**-25 + (2.0**-14 + 2.0**-16) * spread).all(), ((out - want).abs() / spread).max()
+
+
 @pytest.mark.parametrize("cache", ["float8_e4m3fn", "int8"])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 1, 128), (16, 1, 256), (4, 1, 64), (20, 2, 128)])
 @pytest.mark.parametrize("mean,width", [(3.0, 2.0), (12.0, 8.0)])

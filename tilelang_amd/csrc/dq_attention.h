@@ -19,12 +19,15 @@
 // lies in [2^14, 2^15), where bf16's range is no issue; a token's scale multiplies its score in fp32.  A weight times its
 // value's scale, w_t = p_t c_t, may lie anywhere: o is kept relative to a power of two of its own, the running maximum of a
 // head's |w_t|, as the sum is relative to the running maximum of its scores; it is counted from that maximum, and from 2^-112 on, so
-// that no factor is infinite where the token of the largest score has a value of zero.  w_t goes into the second product in two
-// parts, what fp16 holds of it and what that rounding left, so that the result is rounded once, at the end.  Of a 16-bit cache p_t is
-// rounded to the cache's type alone: the largest are near 1, where that costs least, and a part of zero or below would make an
-// infinity among the values a NaN.  Weights that are rounded to fp16 are taken times 2^kLift, the largest then about 2^15 of the
-// 65504 that fp16 ends at: a weight of 2^-29 of the largest keeps 11 bits and one of 2^-39 is not lost, where at 1 that was 2^-14 and 2^-24
-// and thousands of tokens that light beside a heavy one of a small value (all that the result is made of) were.
+// that no factor is infinite where the token of the largest score has a value of zero.
+//
+// Weights go into the second product in two parts, what the product's type holds of one and what that left (some 22 bits in fp16, 16
+// in bf16), so that they are rounded far below the result, which is rounded once, at the end.  Codes are finite, so there the first
+// part is the nearest number; of a 16-bit cache it is the one toward zero, and the second is not zero where the first is not, so
+// that an infinity among the values stays one.  (In one part, rounded to the cache's type: 1.6e-3 of the result off that of fp32
+// weights, in two 1.9e-4; 131071 tokens, bf16, 88 us either way.)  In fp16 weights are taken times 2^kLift, the largest then about
+// 2^15 of the 65504 that fp16 ends at: all are held to 2^-40 of the largest.  At 1 that was 2^-25, and thousands of tokens that
+// light, beside a heavy one of a small value all that the result is made of, were lost.
 //
 // Bound by memory: eight heads on one key-value head do 8 operations a byte of a 16-bit cache, where the chip has some 300.
 // 128 sequences of 8192 tokens, 8 heads of 128, int8: 334 us, 6.6 TB/s of the 6.9 that plain streamed reads of such pieces
@@ -276,6 +279,26 @@ __device__ __forceinline__ float max_over_groups(float x) {
 __device__ __forceinline__ float sum_over_groups(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
+}
+
+// Eight weights as two parts that add up to them; of a weight above 0 (2^-24 in fp16) both are, if the second has to be made so.
+template <class C>
+__device__ __forceinline__ void positive_parts(const float (&p)[8], typename Vec8<C>::type& first, typename Vec8<C>::type& second) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    float low[2];
+    if constexpr (__is_same(C, half_t)) {
+      const auto z = __builtin_amdgcn_cvt_pkrtz(p[j], p[j + 1]);
+      first[j] = (half_t)z[0], first[j + 1] = (half_t)z[1];
+      low[0] = fminf(p[j], 0x1p-24f), low[1] = fminf(p[j + 1], 0x1p-24f);
+    } else {
+      first[j] = __builtin_bit_cast(bf16_t, (uint16_t)(__builtin_bit_cast(uint32_t, p[j]) >> 16));
+      first[j + 1] = __builtin_bit_cast(bf16_t, (uint16_t)(__builtin_bit_cast(uint32_t, p[j + 1]) >> 16));
+      low[0] = p[j] * 0x1p-20f, low[1] = p[j + 1] * 0x1p-20f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) second[j + i] = (C)fmaxf(p[j + i] - (float)first[j + i], low[i]);
+  }
 }
 
 // 2^(m - to), 0 where there is nothing (m = -inf), whatever `to` is
@@ -653,17 +676,17 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
             for (int k = 0; k < 4; ++k) acc[b][i][k] *= shrink;
         }
       }
-      C8 pf[NT], rest[NT];  // the weights, and what their rounding left (codes only)
+      C8 pf[NT], rest[NT];  // the weights' two parts
 #pragma unroll
       for (int b = 0; b < NT; ++b) {
+        if constexpr (kWide) {
+          positive_parts<C>(p[b], pf[b], rest[b]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          pf[b][j] = (C)p[b][j];
-          if constexpr (!kWide) rest[b][j] = (C)(p[b][j] - (float)pf[b][j]);
+          for (int j = 0; j < kEach; ++j) pf[b][j] = (C)p[b][j], rest[b][j] = (C)(p[b][j] - (float)pf[b][j]);
         }
         if constexpr (PACKED) {  // the columns from 8 on are no heads': whatever they sum up is not read
-          both_halves(pf[b]);
-          if constexpr (!kWide) both_halves(rest[b]);
+          both_halves(pf[b]), both_halves(rest[b]);
         }
       }
       if constexpr (!decltype(last)::value) load_scales(next_row);
@@ -682,13 +705,20 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
         constexpr int blk = decltype(block)::value, e_count = VB::e(blk), at = VB::dword(blk, kBytes), at_acc = VB::rows(blk);
         if constexpr (kWide) {
 #pragma unroll
-          for (int e = 0; e < e_count; ++e) {
-            uint4_t w;
+          for (int e = 0; e < e_count; e += 2) {  // (two at a time: a product that another waits for lies further back)
+            uint4_t w[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][at + (e >> 1)], vr[2 * i][at + (e >> 1)], (e & 1) ? 0x07060302u : 0x05040100u);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t odd = vr[2 * i + 1][at + (e >> 1)], even = vr[2 * i][at + (e >> 1)];
+              w[0][i] = __builtin_amdgcn_perm(odd, even, 0x05040100u), w[1][i] = __builtin_amdgcn_perm(odd, even, 0x07060302u);
+            }
 #pragma unroll
-            for (int b = 0; b < NT; ++b) acc[b][at_acc + e] = mfma16<C>(__builtin_bit_cast(C8, w), pf[b], acc[b][at_acc + e]);
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+              for (int b = 0; b < NT; ++b)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                  acc[b][at_acc + e + k] = mfma16<C>(__builtin_bit_cast(C8, w[k]), part == 0 ? rest[b] : pf[b], acc[b][at_acc + e + k]);
           }
         } else {
 #pragma unroll
