@@ -172,3 +172,32 @@ def test_queries_that_are_not_centred(cuda, mean, width, heads, kv_heads, dim, c
     assert ((lse - want_lse).abs() <= 2.0**-16 * (1 + want_lse.abs())).all(), (lse - want_lse).abs().max()
     # a score's error is a weight's, relative: as above, of scores of up to a hundred
     assert ((out - want).abs() <= 2.0**-11 * want.abs() + 2.0**-25 + 2.0**-13 * spread).all(), ((out - want).abs() / spread).max()
+
+
+@pytest.mark.parametrize("cache", ["same", "int8"])
+@pytest.mark.parametrize("length,max_pages", [(1, 1), (40, 3), (700, 60), (2000, 200)])
+@pytest.mark.parametrize("what", ["query", "keys"])
+def test_nothing_but_nan(cuda, what, length, max_pages, cache):
+    """A head all of whose scores are NaN has no logarithm of a sum: NaN, not the -inf of a head that sees no token."""
+    print(f"nan {what} {length} of {max_pages} pages {cache}", flush=True)
+    heads, kv_heads, dim = 6, 2, 64
+    gen = torch.Generator().manual_seed(length)
+    q = torch.randn((heads, dim), generator=gen).half()
+    keys, values = torch.randn((2, length, kv_heads, dim), generator=gen)
+    scales = (None, None) if cache == "same" else (torch.full((length,), 1 / 40), torch.full((length,), 1 / 40))
+    if what == "query":
+        q[4] = math.nan
+    elif cache == "same":
+        keys[:, 1] = math.nan
+    else:
+        keys, values = (keys * 40).round(), (values * 40).round()
+    case = _Sequence(cuda, q, keys, values, torch.float16 if cache == "same" else torch.int8, *scales)
+    if what == "keys" and cache == "int8":
+        case.buffers[0][1][:, 1] = math.nan
+    out, lse = case.run(0.125, max_pages=max(max_pages, -(-length // 16)))
+    lost = torch.zeros(heads, dtype=torch.bool)
+    lost[4 if what == "query" else slice(3, 6)] = True
+    assert torch.isnan(out[lost]).all() and torch.isnan(lse[lost]).all()
+    assert torch.isfinite(out[~lost]).all() and torch.isfinite(lse[~lost]).all()
+    out, lse = case.run(0.125, length=0, max_pages=max(max_pages, -(-length // 16)))
+    assert (out == 0).all() and (lse == -math.inf).all()

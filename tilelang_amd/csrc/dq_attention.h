@@ -304,6 +304,12 @@ __device__ __forceinline__ void positive_parts(const float (&p)[8], typename Vec
 // 2^(m - to), 0 where there is nothing (m = -inf), whatever `to` is
 __device__ __forceinline__ float weight(float m, float to) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to); }
 
+// The natural logarithm of 2^m * sum.  NaN where the sum is: scores that are NaN are no maximum, so m alone cannot tell a head all of
+// whose scores are NaN (m = -inf, sum NaN) from one that sees no token (m = -inf, sum 0).
+__device__ __forceinline__ float log_of_sum(float m, float sum) {
+  return m == -INFINITY && sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+}
+
 // How many workgroups (of four waves) a compute unit is to have where the work is shared out: as few as keep enough of the
 // cache in flight, for every one more is a column cut once more and has less in a row.  One of 16-bit rows of 160 bytes
 // and more (32 sequences of 4096 tokens, 128 wide: one 84 us, two 90, three 106; 256 wide 91 and 122), two of shorter ones, whose
@@ -800,8 +806,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attention_room(D, NT)) void attent
             for (int w = 0; w < kAttnWaves; ++w) x += root[w] * result(w, row)[d] * root[w];
             reinterpret_cast<T*>(a.out)[at * D + d] = (T)(x * inv);
           }
-          if (a.lse && (threadIdx.x & 15) == 0)
-            a.lse[at] = base == -INFINITY ? -INFINITY : (base + log2f(total_weight)) * 0.693147180559945309f;
+          if (a.lse && (threadIdx.x & 15) == 0) a.lse[at] = log_of_sum(base, total_weight);
         } else {
           // the piece that a head begins with is a workgroup's second, any other its first
           const size_t part = ((size_t)blockIdx.x * 2 + (unit0 == 0)) * a.rows + 16 * b + row;

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs a) {
         const int d = 4 * lane + 128 * j;
         if (d < D) *reinterpret_cast<T4*>(reinterpret_cast<T*>(a.out) + to * D + d) = T4{(T)(x[j][0] * inv), (T)(x[j][1] * inv), (T)(x[j][2] * inv), (T)(x[j][3] * inv)};
       }
-      if (a.lse && lane == 0) a.lse[to] = base == -INFINITY ? -INFINITY : (base + log2f(sum)) * 0.693147180559945309f;
+      if (a.lse && lane == 0) a.lse[to] = log_of_sum(base, sum);
     }
     if (SPREAD) __syncthreads();
   }
