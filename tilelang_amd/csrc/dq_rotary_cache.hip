@@ -79,6 +79,9 @@ struct alignas(8) Quad {
 // heads of 128 in 15.3 us, 5.6 TB/s read and written of the 6.6 that a copy of that size reaches; one token is a launch.
 template <class T, int LANES, int LAYOUT, int FORMAT>
 __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
+  // Every product and sum rounded by itself, as the formula stands in fp32.  Which of two products of a sum goes unrounded into a
+  // fused one is the compiler's choice, another in each layout's kernel, and moves codes over ties; it would save no time here.
+#pragma clang fp contract(off)
   const int lane = threadIdx.x % LANES;
   const int heads = a.q_heads + (FORMAT >= 0 ? 2 * a.shape.kv_heads : 0);
   const unsigned group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
