@@ -66,3 +66,22 @@ def test_codes(cuda, dim, rotary_dim, interleaved, cache):
         code = code.round().clamp(-127, 127).to(held) if cache == "int8" else code.clamp(-448, 448).to(held)
         got = codes.view(torch.uint8).transpose(1, 2).reshape(tokens, kv_heads, dim).cpu()
         assert torch.equal(got, code.view(torch.uint8)) and torch.equal(scale.transpose(1, 2).reshape(tokens, kv_heads).cpu(), most / tops)
+
+
+def test_more_heads_than_31_bits_of_elements(cuda):
+    """A token of 2^23 heads of 256: the keys and values behind them begin beyond 2^31 elements."""
+    heads, dim, rows = 2**23, 256, 4
+    if torch.cuda.mem_get_info()[0] < 20 * 2**30:
+        pytest.skip("not enough memory")
+    print(f"one token of {heads} heads of {dim}", flush=True)
+    qkv = torch.zeros((1, heads + 2, dim), dtype=torch.float16, device=cuda)
+    gen = torch.Generator().manual_seed(1)
+    some = torch.randn((1, 3, dim), generator=gen).half().to(cuda)
+    qkv[:, heads - 1 :] = some
+    table = tl.rotary_table(rows, dim, device=cuda)
+    positions, slots = (torch.full((1,), n, dtype=torch.int32, device=cuda) for n in (3, 9))
+    kc, vc = (torch.zeros((2, 1, 8, dim), dtype=torch.float16, device=cuda) for _ in range(2))
+    q = tl.rotary_kv_cache_write(1, heads, kv_heads=1, head_dim=dim, pages=2, page_size=8, positions=rows)(qkv, table, positions, slots, kc, vc)
+    turned = _turned(some[:, :2], table, positions, dim, False).half()
+    assert torch.equal(q[:, -1], turned[:, 0]) and torch.equal(kc[1, :, 1], turned[:, 1]) and torch.equal(vc[1, :, 1], some[:, 2])
+    assert not q[:, :-1].any() and (kc != 0).any(dim=-1).sum() == 1 and (vc != 0).any(dim=-1).sum() == 1

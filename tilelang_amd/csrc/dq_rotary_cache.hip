@@ -101,7 +101,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
 
   const T* const row = FORMAT >= 0 && a.v && head >= keys_end
                            ? reinterpret_cast<const T*>(a.v) + ((size_t)token * a.shape.kv_heads + (head - keys_end)) * a.head_dim
-                           : reinterpret_cast<const T*>(a.x) + (size_t)token * a.row_stride + head * a.head_dim;
+                           : reinterpret_cast<const T*>(a.x) + (size_t)token * a.row_stride + (size_t)head * a.head_dim;
   float x[2][8], partner[2][8] = {};
 #pragma unroll
   for (int k = 0; k < 2; ++k) load8(row + (inside[k] ? d[k] : 0), x[k]);
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
   }
 
   if (FORMAT < 0 || head < a.q_heads) {
-    T* const out = reinterpret_cast<T*>(a.out) + (size_t)token * a.out_stride + head * a.head_dim;
+    T* const out = reinterpret_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)head * a.head_dim;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (inside[k]) *reinterpret_cast<typename Vec8<T>::type*>(out + d[k]) = round8<T>(x[k]);
