@@ -373,14 +373,15 @@ int call_rotary(const void* X, const void* Table, const void* Positions, void* O
 
 /* K, V [tokens][kv_heads][head_dim] into the cache at Slots [tokens].  8 bit: scale = a / top with a = max |x| of a token's
  * head and top = 448 (fp8) or 127 (int8), code = round to nearest even of x * (top / a); a head with a < 2^-100 is stored as
- * zeros with scale 0, one with an infinity or a NaN with a NaN scale.  Tokens of one call with the same slot: one of them. */
+ * zeros with scale 0, one with an infinity or a NaN with a NaN scale.  The slots of a call have to be distinct (those outside of the
+ * cache aside): a place that two of its tokens name holds parts of both, the codes of one beside the scale of the other. */
 int call_kv_cache_write(const void* K, const void* V, const void* Slots, void* KCache, void* VCache, void* KScale, void* VScale,
                         int tokens, int kv_heads, int head_dim, int pages, int page_size, int dtype, int cache_format,
                         dq_stream_t stream);
 
 /* call_rotary and call_kv_cache_write in one launch on the rows of a fused projection, QKV [tokens][heads + 2 * kv_heads]
  * [head_dim]: Q [tokens][heads][head_dim] = the rotated queries; the rotated keys (quantised from fp32) and the values go
- * into the cache. */
+ * into the cache at distinct slots. */
 int call_rotary_kv_cache_write(const void* QKV, const void* Table, const void* Positions, const void* Slots, void* Q, void* KCache,
                                void* VCache, void* KScale, void* VScale, int tokens, int heads, int kv_heads, int head_dim,
                                int rotary_dim, int positions, int pages, int page_size, int interleaved, int dtype,

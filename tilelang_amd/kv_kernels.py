@@ -175,7 +175,7 @@ def rotary(tokens: int, heads: int, head_dim: int, positions: int, rotary_dim: i
 def kv_cache_write(tokens: int, kv_heads: int, head_dim: int, pages: int, page_size: int, dtype="float16", cache_dtype=None) -> KernelAdapter:
     """New keys and values into the cache: ``kernel(k, v, Slots, KCache, VCache[, KScale, VScale])``, ``k`` and ``v``
     ``[tokens, kv_heads, head_dim]``, ``Slots`` int32 ``[tokens]`` = page * page_size + place (one that is negative or beyond
-    the cache is not written).
+    the cache is not written).  A call's slots have to be distinct: a place that two tokens name holds parts of both.
 
     ``cache_dtype``: ``dtype`` itself (default), or ``"float8_e4m3fn"`` / ``"int8"`` with one fp32 scale a token and head:
     ``scale = max|x| / top``, ``code = round(x * (top / max|x|))``, top 448 / 127.  A head with an infinity or a NaN reads back
@@ -194,7 +194,7 @@ def rotary_kv_cache_write(tokens: int, heads: int, kv_heads: int, head_dim: int,
     """:func:`rotary` and :func:`kv_cache_write` in one launch on the rows of a fused projection:
     ``q = kernel(qkv, Table, Positions, Slots, KCache, VCache[, KScale, VScale])``, ``qkv`` ``[tokens, heads + 2 * kv_heads,
     head_dim]`` (queries, keys, values), ``q`` ``[tokens, heads, head_dim]`` the rotated queries; the rotated keys, quantised
-    from fp32, and the values go into the cache.
+    from fp32, and the values go into the cache, at slots that are distinct.
     """
     fn = "rotary_kv_cache_write"
     _positive(fn, tokens=tokens, heads=heads)
