@@ -30,3 +30,19 @@ def test_slots_of_a_call_are_distinct():
         if len(held[2]) > 20:
             cache.release(3)
             held[3] = []
+
+
+@pytest.mark.parametrize("make", [
+    lambda: tl.rotary(2, 2, 64, positions=5, row_stride=2**32 + 128),
+    lambda: tl.rotary(2, 2, 64, positions=2**32 + 5),
+    lambda: tl.rotary(2**32 + 1, 2, 64, positions=5),
+    lambda: tl.kv_cache_write(2**32 + 1, kv_heads=2, head_dim=64, pages=3, page_size=16),
+    lambda: tl.kv_cache_write(1, kv_heads=2**32 + 2, head_dim=64, pages=3, page_size=16),
+    lambda: tl.rotary_kv_cache_write(1, 2**32 + 4, positions=5, kv_heads=2, head_dim=64, pages=3, page_size=16),
+    lambda: tl.kv_cache_read(1, 2**32 + 9, kv_heads=2, head_dim=64, pages=3, page_size=16, max_pages=2),
+    lambda: tl.kv_cache_read(1, 9, kv_heads=2, head_dim=64, pages=3, page_size=16, max_pages=2**32 + 2),
+])
+def test_sizes_beyond_32_bits(make):
+    """Refused, and not taken by their lower 32 bits."""
+    with pytest.raises(ValueError, match="32-bit"):
+        make()

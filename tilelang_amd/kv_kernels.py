@@ -86,6 +86,8 @@ def _kernel(name: str, entry: str, params: list, result_idx: list, slots: tuple,
             workspace_bytes: int | None = None, workspace_idx=()) -> KernelAdapter:
     """The kernel object of an entry point whose arguments are ``slots`` (a parameter each; None: NULL), the workspace's
     bytes where it takes one, ``ints``, a float where it takes one, and the stream."""
+    if not all(-(2**31) <= i < 2**31 for i in ints):  # (ctypes would keep the lower 32 bits)
+        raise ValueError(f"{name}: sizes are 32-bit (got {max(ints, key=abs)})")
 
     def launch(ptrs, stream):
         middle = () if workspace_bytes is None else (workspace_bytes,)
