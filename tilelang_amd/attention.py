@@ -4,6 +4,8 @@
 A step has rows: the new tokens of every sequence, one sequence behind the other.  One token a sequence is a decode step; several
 are a prompt or a part of one, and each of them sees the tokens before it and itself.  ``rows = cache.extend(counts)`` finds their
 places once for all layers, ``layer(x, cache, rows)`` projects, rotates and writes, attends and projects back.
+
+The attention is that of one new token: every row reads its whole context, so a prompt of n tokens reads n / 2 of them n times.
 """
 
 from __future__ import annotations
@@ -20,13 +22,23 @@ from .w4linear import W4A16Linear
 
 @dataclass(frozen=True)
 class Rows:
-    """The new tokens of a step, on the device: of each its position, its slot in the cache, its sequence's row of the page
-    table and how many tokens it sees."""
+    """The new tokens of a step, on the device, a sequence's one behind the other in their order: of each its position, its slot in the
+    cache, its sequence's row of the page table and how many tokens it sees.  ``owners``: where a row of ``pages`` for every token would
+    take too much memory, ``pages`` has one for every sequence, and this is the one of each token."""
 
     positions: torch.Tensor
     slots: torch.Tensor
     pages: torch.Tensor
     lengths: torch.Tensor
+    owners: torch.Tensor | None = None
+
+    def pages_of(self, part: slice) -> torch.Tensor:
+        """The rows of the page table of some of the tokens."""
+        return self.pages[part] if self.owners is None else self.pages[self.owners[part]]
+
+
+#: page ids (256 MiB) of a step's tokens that are held at once
+MAX_PAGE_IDS = 2**26
 
 
 class PagedKVCache:
@@ -91,8 +103,12 @@ class PagedKVCache:
             self.lengths[b] += c
         both = torch.tensor([positions, slots], dtype=torch.int32).to(self.device)
         # (one token of every sequence: the table as it stands)
-        pages = self.page_table if owners == list(range(self.sequences)) else self.page_table[torch.tensor(owners, device=self.device)]
-        return Rows(both[0], both[1], pages, both[0] + 1)
+        if owners == list(range(self.sequences)):
+            return Rows(both[0], both[1], self.page_table, both[0] + 1)
+        owner = torch.tensor(owners, device=self.device)
+        if len(owners) * self.max_pages > MAX_PAGE_IDS:
+            return Rows(both[0], both[1], self.page_table, both[0] + 1, owner)
+        return Rows(both[0], both[1], self.page_table[owner], both[0] + 1)
 
     def release(self, sequence: int) -> None:
         """The sequence has no tokens any more; its pages are free."""
@@ -137,6 +153,19 @@ class W4Attention(nn.Module):
 
     def attend(self, qkv: torch.Tensor, cache: PagedKVCache, rows: Rows, layer: int = 0) -> torch.Tensor:
         """``qkv`` ``[rows, heads + 2 kv_heads, head_dim]`` -> ``[rows, heads, head_dim]``; its keys and values go into the cache."""
+        n, at_once = qkv.shape[0], self._rows_at_once(cache)
+        if n <= at_once and rows.owners is None:
+            return self._attend(qkv, cache, rows, layer)
+        # (a row sees tokens of its own part and of those before it only, as a sequence's rows come in their order)
+        parts = [slice(at, min(at + at_once, n)) for at in range(0, n, at_once)]
+        return torch.cat([self._attend(qkv[p], cache, Rows(rows.positions[p], rows.slots[p], rows.pages_of(p), rows.lengths[p]), layer) for p in parts])
+
+    def _rows_at_once(self, cache: PagedKVCache) -> int:
+        """What one call of the write and of the attention takes."""
+        return max(1, min(kv_kernels.attention_sequences(self.heads, self.kv_heads, cache.max_pages * cache.page_size),
+                          kv_kernels.MAX_HEADS // (self.heads + 2 * self.kv_heads), MAX_PAGE_IDS // cache.max_pages))
+
+    def _attend(self, qkv: torch.Tensor, cache: PagedKVCache, rows: Rows, layer: int) -> torch.Tensor:
         n, (positions, rotary_dim) = qkv.shape[0], self.rotary.shape
         write = cache.kernel(kv_kernels.rotary_kv_cache_write, n, self.heads, positions=positions, rotary_dim=rotary_dim, interleaved=self.interleaved)
         attend = cache.kernel(kv_kernels.paged_attention_decode, n, self.heads, max_pages=cache.max_pages, window=self.window,

@@ -9,6 +9,7 @@ does), in the activations' type or in 8 bits with fp32 scales ``[pages, kv_heads
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -47,6 +48,23 @@ def _positive(fn: str, **sizes) -> None:
     for name, value in sizes.items():
         if value <= 0:
             raise ValueError(f"{fn}: {name} must be positive (got {value})")
+
+
+#: heads of all tokens that a call of the rotation, the write and the read takes
+MAX_HEADS = 2**25
+
+
+def _heads(fn: str, tokens: int, heads: int) -> None:
+    if tokens * heads > MAX_HEADS and max(tokens, heads) < 2**31:  # (beyond: no size at all, see _kernel)
+        raise ValueError(f"{fn}: {tokens} tokens of {heads} heads: at most {MAX_HEADS} heads in a call")
+
+
+@functools.lru_cache(maxsize=64)
+def attention_sequences(heads: int, kv_heads: int, tokens: int) -> int:
+    """How many sequences a call of :func:`paged_attention_decode` takes whose page tables have room for ``tokens`` tokens: the library
+    counts its work, a unit 128 tokens of a key-value head and 16 query heads and three more, in 31 bits, and such columns in 23."""
+    columns = kv_heads * -(-(heads // kv_heads) // 16)
+    return min(65535, (2**23 - 1) // columns, (2**31 - 2) // (columns * (tokens // 128 + 3)))
 
 
 def _rotation(fn: str, head_dim: int, rotary_dim: int | None, positions: int) -> int:
@@ -159,6 +177,7 @@ def rotary(tokens: int, heads: int, head_dim: int, positions: int, rotary_dim: i
     """
     fn = "rotary"
     _positive(fn, tokens=tokens, heads=heads)
+    _heads(fn, tokens, heads)
     if head_dim <= 0 or head_dim % 8 or head_dim > 512:
         raise ValueError(f"{fn}: head_dim={head_dim} must be a multiple of 8, at most 512")
     rotary_dim = _rotation(fn, head_dim, rotary_dim, positions)
@@ -186,6 +205,7 @@ def kv_cache_write(tokens: int, kv_heads: int, head_dim: int, pages: int, page_s
     fn = "kv_cache_write"
     _positive(fn, tokens=tokens)
     pool = _Pool(fn, kv_heads, head_dim, pages, page_size, dtype, cache_dtype)
+    _heads(fn, tokens, 2 * kv_heads)
     shape = (tokens, kv_heads, head_dim)
     params = [KernelParam("k", pool.dtype, shape), KernelParam("v", pool.dtype, shape), KernelParam("Slots", torch.int32, (tokens,)), *pool.params]
     return _kernel(fn, "call_kv_cache_write", params, [], (0, 1, 2, *pool.slots(3)), (tokens, kv_heads, head_dim, pages, page_size, *pool.ints))
@@ -201,6 +221,7 @@ def rotary_kv_cache_write(tokens: int, heads: int, kv_heads: int, head_dim: int,
     fn = "rotary_kv_cache_write"
     _positive(fn, tokens=tokens, heads=heads)
     pool = _Pool(fn, kv_heads, head_dim, pages, page_size, dtype, cache_dtype)
+    _heads(fn, tokens, heads + 2 * kv_heads)
     rotary_dim = _rotation(fn, head_dim, rotary_dim, positions)
     params = [KernelParam("qkv", pool.dtype, (tokens, heads + 2 * kv_heads, head_dim)),
               KernelParam("Table", torch.float32, (positions, rotary_dim)), KernelParam("Positions", torch.int32, (tokens,)),
@@ -220,6 +241,7 @@ def kv_cache_read(sequences: int, tokens: int, kv_heads: int, head_dim: int, pag
     fn = "kv_cache_read"
     _positive(fn, sequences=sequences, tokens=tokens, max_pages=max_pages)
     pool = _Pool(fn, kv_heads, head_dim, pages, page_size, dtype, cache_dtype)
+    _heads(fn, tokens, kv_heads)
     n = len(pool.params)
     params = [*pool.params, KernelParam("PageTable", torch.int32, (sequences, max_pages)), KernelParam("Starts", torch.int32, (sequences + 1,)),
               KernelParam("kv", pool.dtype, (2, tokens, kv_heads, head_dim))]
@@ -247,6 +269,9 @@ def paged_attention_decode(sequences: int, heads: int, kv_heads: int, head_dim: 
         raise ValueError(f"{fn}: heads={heads} must be a multiple of kv_heads={kv_heads}")
     if head_dim not in ATTENTION_HEAD_DIMS:
         raise ValueError(f"{fn}: head_dim={head_dim} must be one of {ATTENTION_HEAD_DIMS}")
+    if heads > 65535 or sequences > attention_sequences(heads, kv_heads, max_pages * page_size):
+        raise ValueError(f"{fn}: {sequences} sequences of {heads} heads and up to {max_pages * page_size} tokens: more than a call takes, at most "
+                         f"{attention_sequences(heads, kv_heads, max_pages * page_size)} sequences and 65535 heads")
     if window < 0:
         raise ValueError(f"{fn}: window={window} must be 0 (none) or positive")
     window = min(window, max_pages * page_size)  # (32 bits in the library)
