@@ -105,3 +105,18 @@ def test_a_prompt_of_many_rows(monkeypatch):
     assert most * cache.max_pages <= 2**26 and most < 65536
     starts = range(0, 70000, most)
     assert seen == [(name, min(most, 70000 - at), at if at < 69000 else at - 69000) for at in starts for name in ("rotary_kv_cache_write", "paged_attention_decode")]
+
+
+def test_rows_keep_their_pages():
+    """What a step was given stays as it was when a sequence grows or goes, one token a sequence or several."""
+    cache = tl.PagedKVCache(2, pages=20, kv_heads=1, head_dim=64, page_size=8, max_tokens=64, device="cpu")
+    for counts in ([7, 8], [1, 1], [1, 1], [3, 0], [20, 20]):
+        rows, table = cache.extend(counts), cache.page_table.tolist()
+        owners = [b for b, c in enumerate(counts) for _ in range(c)]
+        kept = rows.pages.tolist()
+        assert kept == [table[b] for b in owners]
+        cache.extend([8, 8])
+        assert rows.pages.tolist() == kept
+        for b in range(2):
+            cache.release(b)
+        assert rows.pages.tolist() == kept and (cache.page_table == -1).all()

@@ -46,6 +46,7 @@ class PagedKVCache:
 
     ``cache_dtype``: ``dtype`` itself, ``"float8_e4m3fn"`` or ``"int8"`` (one fp32 scale a token and head).  ``pages`` are shared by
     the sequences as they grow; ``extend`` takes what it needs, or raises and takes nothing, and ``release`` gives a sequence's back.
+    ``page_table`` is another tensor after each change, so the :class:`Rows` of a step keep the pages that they were made with.
     """
 
     def __init__(self, sequences: int, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, max_tokens: int | None = None,
@@ -93,7 +94,7 @@ class PagedKVCache:
             self._pages[b] += [self._free.pop() for _ in range(wanted[b])]
         if changed:
             rows = torch.tensor([self._pages[b] + [-1] * (self.max_pages - len(self._pages[b])) for b in changed], dtype=torch.int32)
-            self.page_table[torch.tensor(changed, device=self.device)] = rows.to(self.device)
+            self.page_table = self.page_table.index_copy(0, torch.tensor(changed, device=self.device), rows.to(self.device))
         positions, slots, owners = [], [], []
         for b, c in enumerate(counts):
             for t in range(self.lengths[b], self.lengths[b] + c):
@@ -114,6 +115,7 @@ class PagedKVCache:
         """The sequence has no tokens any more; its pages are free."""
         self._free += reversed(self._pages[sequence])
         self._pages[sequence], self.lengths[sequence] = [], 0
+        self.page_table = self.page_table.clone()
         self.page_table[sequence] = -1
 
     def read(self, layer: int = 0) -> tuple:
