@@ -120,3 +120,14 @@ def test_rows_keep_their_pages():
         for b in range(2):
             cache.release(b)
         assert rows.pages.tolist() == kept and (cache.page_table == -1).all()
+
+
+def test_kernels_that_a_cache_keeps():
+    """Not one for every number of rows that there ever was; those in use stay."""
+    cache = tl.PagedKVCache(1, pages=2, kv_heads=2, head_dim=64, page_size=8, device="cpu")
+    step = cache.kernel(tl.kv_cache_write, 1)
+    for n in range(2, 1000):
+        prompt = cache.kernel(tl.kv_cache_write, n)
+        assert prompt.params[0].shape[0] == n and cache.kernel(tl.kv_cache_write, n) is prompt
+        assert cache.kernel(tl.kv_cache_write, 1) is step
+    assert len(cache._kernels) == 64

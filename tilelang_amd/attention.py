@@ -37,6 +37,8 @@ class Rows:
         return self.pages[part] if self.owners is None else self.pages[self.owners[part]]
 
 
+#: kernel objects that a cache keeps: prompts come in any number of rows
+MAX_KERNELS = 64
 #: page ids (256 MiB) of a step's tokens that are held at once
 MAX_PAGE_IDS = 2**26
 
@@ -130,11 +132,14 @@ class PagedKVCache:
         return k, v
 
     def kernel(self, make, *args, **kwargs):
-        """The kernel object ``make(*args, **kwargs, **sizes())``, made once for all layers."""
+        """The kernel object ``make(*args, **kwargs, **sizes())``, made once for all layers; the last :data:`MAX_KERNELS` used are kept."""
         key = (make, args, tuple(sorted(kwargs.items())))
-        found = self._kernels.get(key)
+        found = self._kernels.pop(key, None)
         if found is None:
-            found = self._kernels[key] = make(*args, **kwargs, **self.sizes())
+            found = make(*args, **kwargs, **self.sizes())
+            while len(self._kernels) >= MAX_KERNELS:
+                del self._kernels[next(iter(self._kernels))]
+        self._kernels[key] = found  # (the last in the order)
         return found
 
 
