@@ -131,3 +131,22 @@ def test_kernels_that_a_cache_keeps():
         assert prompt.params[0].shape[0] == n and cache.kernel(tl.kv_cache_write, n) is prompt
         assert cache.kernel(tl.kv_cache_write, 1) is step
     assert len(cache._kernels) == 64
+
+
+@pytest.mark.parametrize("turned", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.to(torch.float16), lambda m: m.double(), lambda m: m.half().float()])
+def test_table_and_sinks_stay_in_32_bits(turned):
+    """A model is turned into another type as a whole; its positions' table and its sinks are not."""
+    table = tl.rotary_table(50000, 64)
+    layer = tl.W4Attention(128, 4, 1, 64, table, sinks=True)
+    layer.sinks.copy_(torch.randn(4, generator=torch.Generator().manual_seed(0)))
+    sinks = layer.sinks.clone()
+    model = torch.nn.Sequential(layer, torch.nn.Linear(8, 8))
+    turned(model)
+    assert layer.rotary.dtype == layer.sinks.dtype == torch.float32
+    assert torch.equal(layer.rotary, table) and torch.equal(layer.sinks, sinks)
+    assert layer.to("meta").rotary.device.type == "meta"
+
+
+def test_table_and_sinks_where_there_are_none():
+    layer = tl.W4Attention(128, 4, 1, 64, tl.rotary_table(10, 64)).half()
+    assert layer.sinks is None and layer.rotary.dtype == torch.float32

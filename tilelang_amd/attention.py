@@ -158,6 +158,16 @@ class W4Attention(nn.Module):
         self.register_buffer("rotary", rotary, persistent=False)
         self.register_buffer("sinks", torch.zeros((heads,), dtype=torch.float32) if sinks else None)
 
+    def _apply(self, fn, *args, **kwargs):
+        # The kernels read both in fp32 whatever type a model is turned into, and a table rounded in between has lost its angles: they
+        # are moved, not converted.
+        kept = {name: b for name in ("rotary", "sinks") if (b := self._buffers[name]) is not None and b.dtype == torch.float32}
+        super()._apply(fn, *args, **kwargs)
+        for name, b in kept.items():
+            if self._buffers[name].dtype != torch.float32:
+                self._buffers[name] = b.to(self._buffers[name].device)
+        return self
+
     def attend(self, qkv: torch.Tensor, cache: PagedKVCache, rows: Rows, layer: int = 0) -> torch.Tensor:
         """``qkv`` ``[rows, heads + 2 kv_heads, head_dim]`` -> ``[rows, heads, head_dim]``; its keys and values go into the cache."""
         n, at_once = qkv.shape[0], self._rows_at_once(cache)
