@@ -398,7 +398,7 @@ int call_kv_cache_read(const void* KCache, const void* VCache, const void* KScal
  * tokens Lengths[b] - window .. Lengths[b] - 1 (window 0: all), head h on key-value head h / (heads / kv_heads), head_dim 64,
  * 80, 96, 112, 128, 160, 192 or 256.  Sinks [heads] fp32 or NULL: one more score a head, whose value is nothing.  Lse
  * [sequences][heads] fp32 or NULL: the natural logarithm of the sum of e^score (sinks among them).  A sequence that sees no
- * token gives zeros and Lse -inf (with a sink: the sink).  What lies in the cache beyond a sequence's length is never used,
+ * token gives zeros and Lse -inf (with a sink: the sink); where scores are NaN, Out and Lse are.  What lies in the cache beyond a sequence's length is never used,
  * NaN or not.  Softmax and sums in fp32; results do not depend on timing.
  * Workspace: dq_paged_attention_workspace_bytes(...) bytes, 16-byte aligned (0: none), contents undefined before and after,
  * not to be shared by calls that overlap in time. */

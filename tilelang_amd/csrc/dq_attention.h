@@ -30,8 +30,8 @@
 // light, beside a heavy one of a small value all that the result is made of, were lost.
 //
 // Bound by memory: eight heads on one key-value head do 8 operations a byte of a 16-bit cache, where the chip has some 300.
-// 128 sequences of 8192 tokens, 8 heads of 128, int8: 334 us, 6.6 TB/s of the 6.9 that plain streamed reads of such pieces
-// reach (keys and values not streamed 397, K's operand straight from memory 400); one sequence of 131071 tokens, bf16: 88 us,
+// 128 sequences of 8192 tokens, 8 heads of 128, int8: 347 us, 6.4 TB/s of the 6.9 that plain streamed reads of such pieces
+// reach (when it took 355, keys and values not streamed took 397 and K's operand straight from memory 400); one sequence of 131071 tokens, bf16: 88 us,
 // 5 of them the join.  Short calls are two launches of 4.3 us, or one where no column can be cut.
 #pragma once
 
@@ -326,8 +326,10 @@ constexpr int attention_room(int head_dim, int row_blocks) {
 }
 
 // Blocks of 16 heads that a workgroup takes, with one read of the keys and values: two where more than 16 heads share them (32
-// heads on one, 48 sequences of 6000 tokens, bf16, one block and two: 160 wide 67 and 45 us, 256 wide 104 and 81, some registers
-// of which lie in memory; int8, with one workgroup a compute unit in place of two: 160 wide 46.9 and 45.7, 256 wide 63 and 58).
+// heads on one, 48 sequences of 6000 tokens, bf16, one block and two: 128 wide 55 and 37 us, 160 wide 67 and 45, 256 wide 103 and 82,
+// some registers of which lie in memory; int8, from 160 wide on with one workgroup a compute unit in place of two: 128 wide 42 and 36,
+// 160 wide 48 and 47, 256 wide 64 and 58).  One wave has both blocks: from 160 wide on that is one wave a SIMD, and nothing covers the way
+// from keys through scores and exponentials to values, so these cases stay at 1.6 to 3.3 times their bytes.
 constexpr int attention_row_blocks(int heads_a_column) { return heads_a_column > 16 ? 2 : 1; }
 
 // A wave's LDS: 32 keys on their way into the operand's order, later 16 rows of its result.
@@ -337,8 +339,9 @@ constexpr int attention_wave_lds(int head_dim, int format) {
 }
 
 // Whether a workgroup's heads are taken PACKED, see there: up to eight, where instructions and not memory bound the kernel, which
-// is in narrow heads of 8 bits (64 sequences of 4000 tokens, eight key-value heads: int8, 64 wide, 55 -> 52 us, 80 wide 74 -> 71,
-// 96 wide 77 -> 75; fp8, 112 wide, 84 -> 82; 128 wide 88 -> 88; 16 bits, 64 wide, 83 -> 83).
+// is in narrow heads of 8 bits (64 sequences of 4000 tokens, eight heads on each of eight: int8, 64 wide, 66.6 -> 65.6 us, 80 wide 82 -> 78,
+// 96 wide 82 -> 78, 112 wide 89 -> 86; fp8, 64 wide 54 -> 51, 112 wide 85 -> 83; with four heads on each, fp8, 128 wide 88 -> 88 and 16
+// bits, 64 wide, 83 -> 83).
 constexpr bool attention_packs(int heads_a_column, int head_dim, int format) { return heads_a_column <= 8 && head_dim < 128 && !cache_is_16bit(format); }
 
 // What lane n ^ 8 of the 16 has; into lane n < 8 its four elements, behind its own four.

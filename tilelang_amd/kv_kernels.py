@@ -130,7 +130,7 @@ def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, scaling
       turns more than ``high`` times is kept, between them the share of each goes linearly with the turns;
     * ``"ramp"``: as ``"bands"``, but the share goes linearly with the index ``i`` between the (rounded out) indices whose
       angles turn ``high`` and ``low`` times, and cosines and sines are multiplied by ``0.1 ln(factor) + 1``, which
-      sharpens the attention of a longer context.
+      sharpens the attention of a longer context.  Models that were trained with it mostly have ``high=32``: give their own.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_table: rotary_dim={rotary_dim} must be even and at least 2")
