@@ -410,6 +410,68 @@ int call_paged_attention_decode(const void* Q, const void* KCache, const void* V
                                 int page_size, int max_pages, int window, int dtype, int cache_format, float scale,
                                 dq_stream_t stream);
 
+/* ---- the rest of a decoder block: norm, routing to experts, the experts' products ---------------------------- */
+
+/* Root-mean-square norm with the residual's addition: h = x + r, y = weight * h / sqrt(mean(h^2) + eps), for X [rows][row_stride]
+ * (dim elements a row count; both multiples of 8, dim at most 32768), Residual [rows][dim] or NULL, Weight [dim], all of dtype
+ * (DQ_DT_F16 or DQ_DT_BF16).  Sum [rows][dim] takes h rounded (NULL without a residual); the norm is of h before that.  int8 0:
+ * Y [rows][dim] = y.  int8 1: Y [rows][dim] int8 = round(y * s), Scale [rows] = s = 127 / max(max|y|, 1e-5), what
+ * call_gemm_int8xint2 takes as s_a; a row with an infinity or a NaN gives codes of zero and a scale that is NaN.  Sums in fp32;
+ * eps positive.  Y and Sum overlap no input. */
+int call_rms_norm(const void* X, const void* Residual, const void* Weight, void* Y, void* Sum, void* Scale, int rows, int dim,
+                  int row_stride, int int8, int dtype, float eps, dq_stream_t stream);
+
+enum dq_scores { DQ_SCORES_SOFTMAX = 0, DQ_SCORES_SIGMOID = 1 };
+enum dq_group_score { DQ_GROUP_MAX = 0, DQ_GROUP_SUM2 = 1 /* the sum of a group's two largest */ };
+
+/* Routing: Logits [tokens][experts] (dtype: DQ_DT_F16, DQ_DT_BF16 or DQ_DT_F32) -> of every token its top_k experts,
+ * Ids [tokens][top_k] int32, the best first, and Weights [tokens][top_k] fp32; and the pairs sorted by expert (see below).
+ * A score is the softmax over the token's experts or the logistic function of its logit.  A key is the score plus Bias [experts]
+ * (fp32), or without one (NULL) the logit; of equal keys the lowest index comes first.  groups > 1: of the groups of
+ * experts / groups neighbours only the top_groups best count, by the largest key of each or the sum of its two largest (without a
+ * bias: scores).  Weights are scores (without the bias), renormalize: divided by their sum over the token's choices (a sum of zero
+ * leaves zeros), times factor.  Logits of -inf mask experts: score 0, chosen last.  A NaN counts as the largest, and shows in the
+ * weights.  Choices do not depend on how an exponential is rounded: where fp32 cannot tell two scores apart, 64 bits do.
+ * experts at most 1024, top_k at most 32, groups at most 64, tokens * top_k at most 2^23.
+ * Workspace: dq_experts_order_workspace_bytes(...) bytes, 16-byte aligned (0: none), contents undefined before and after, not to
+ * be shared by calls that overlap in time. */
+size_t dq_experts_order_workspace_bytes(int tokens, int top_k, int experts);
+int call_route_experts(const void* Logits, const void* Bias, void* Weights, void* Ids, void* Order, void* Starts, void* Workspace,
+                       size_t workspace_bytes, int tokens, int experts, int top_k, int scores, int groups, int top_groups,
+                       int group_score, int renormalize, int dtype, float factor, dq_stream_t stream);
+
+/* The pairs (token, choice) of Ids [tokens][top_k] sorted by expert: Order [tokens * top_k] int32 names pairs, token * top_k +
+ * choice, those of expert first + e at Starts[e] .. Starts[e + 1] - 1 (Starts [experts + 1]) in ascending order.  Pairs of other
+ * ids (experts that another GPU has; -1: no token) are in none; the places behind Starts[experts] hold -1.  The same workspace. */
+int call_experts_order(const void* Ids, void* Order, void* Starts, void* Workspace, size_t workspace_bytes, int tokens, int top_k,
+                       int experts, int first, dq_stream_t stream);
+
+enum dq_experts_format { DQ_EXPERTS_UINT4 = 0 /* fp16 x uint4 */, DQ_EXPERTS_MXFP4 = 1 /* bf16 x MXFP4 */ };
+enum dq_activation { DQ_ACT_SILU = 0, DQ_ACT_GELU = 1 /* the tanh form */ };
+
+/* The experts' gate and up projections, row p of the sorted order with token t = Order[p] / top_k and its expert e:
+ * H[p] = act(X[t] . G_e^T + gate bias) * (X[t] . U_e^T + up bias).  X [tokens][K], H [tokens * top_k][N]; rows behind
+ * Starts[experts] are left as they were.  B [experts][2 N][K / 2]: an expert's N gate rows, then its N up rows, even k in the
+ * low nibble; Scale [experts][2 N][K / group_size]; Bias [experts][2 N] or NULL.
+ * DQ_EXPERTS_UINT4: fp16; weights as call_dequantize_gemv_w4a16's, fp16((q - 8) * s), or with Zeros (fp16, as Scale)
+ * fp16(fp16(q - z) * s); group_size 32, 64 or 128; K % 128 == 0.  DQ_EXPERTS_MXFP4: bf16; e2m1 codes times 2^(Scale - 127), Scale
+ * uint8, group_size 32; K % 64 == 0.  N % 32 == 0.  Sums in fp32.  Order and Starts are what the calls above write; whatever they
+ * hold, nothing outside of the buffers is read or written. */
+int call_experts_up(const void* X, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,
+                    const void* Starts, void* H, int tokens, int experts, int top_k, int N, int K, int group_size, int format,
+                    int activation, dq_stream_t stream);
+
+/* The way back: C[t] = Residual[t] + sum over the token's choices j of Weights[t][j] * (H[p] . D_e^T + bias), p the pair's row in
+ * the sorted order and e its expert.  H [tokens * top_k][K], C [tokens][N], Residual [tokens][N] or NULL, Weights fp32 and Ids
+ * [tokens][top_k]; B [experts][N][K / 2] and so on as above.  Pairs whose id is not one of first .. first + experts - 1 add
+ * nothing.  Sums in fp32, a token's choices in their order whatever the timing.
+ * Workspace: dq_experts_down_workspace_bytes(...) bytes, as above. */
+size_t dq_experts_down_workspace_bytes(int tokens, int top_k, int N);
+int call_experts_down(const void* H, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,
+                      const void* Starts, const void* Ids, const void* Weights, const void* Residual, void* C, void* Workspace,
+                      size_t workspace_bytes, int tokens, int experts, int top_k, int N, int K, int group_size, int format, int first,
+                      dq_stream_t stream);
+
 /* ---- diagnostics ------------------------------------------------------------------------------------- */
 
 /* The rate the matrix pipe sustains on the caller's operands, with no memory, LDS or decode work beside it: every

@@ -34,6 +34,13 @@ from .kv_kernels import (  # noqa: F401
     rotary_kv_cache_write,
     rotary_table,
 )
+from .block_kernels import (  # noqa: F401
+    experts_down,
+    experts_order,
+    experts_up,
+    rms_norm,
+    route_experts,
+)
 from .bitlinear import BitLinear  # noqa: F401
 from .w4linear import W4A16Linear  # noqa: F401
 from .attention import PagedKVCache, W4Attention  # noqa: F401

@@ -56,6 +56,11 @@ SIGNATURES = {
     "call_rotary_kv_cache_write": [_vp] * 9 + [_i] * 11 + [_vp],
     "call_kv_cache_read": [_vp] * 7 + [_i] * 9 + [_vp],
     "call_paged_attention_decode": [_vp] * 11 + [ctypes.c_size_t] + [_i] * 10 + [ctypes.c_float, _vp],
+    "call_rms_norm": [_vp] * 6 + [_i] * 5 + [ctypes.c_float, _vp],
+    "call_route_experts": [_vp] * 7 + [ctypes.c_size_t] + [_i] * 9 + [ctypes.c_float, _vp],
+    "call_experts_order": [_vp] * 4 + [ctypes.c_size_t] + [_i] * 4 + [_vp],
+    "call_experts_up": [_vp] * 8 + [_i] * 8 + [_vp],
+    "call_experts_down": [_vp] * 12 + [ctypes.c_size_t] + [_i] * 8 + [_vp],
     "call_gemm_mxfp4_mxfp4": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
 }
 
@@ -68,6 +73,8 @@ SIZE_QUERIES = {
     "dq_mxfp4_workspace_bytes": [_i, _i, _i],
     "dq_bitlinear_workspace_bytes": [_i, _i, _i, _i],
     "dq_paged_attention_workspace_bytes": [_i] * 8,
+    "dq_experts_order_workspace_bytes": [_i] * 3,
+    "dq_experts_down_workspace_bytes": [_i] * 3,
 }
 
 

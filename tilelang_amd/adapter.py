@@ -100,7 +100,7 @@ class KernelAdapter:
 
     def _bind(self, result_idx):
         """The native call with the parameters of ``result_idx`` allocated by it; None where there is none."""
-        host = _lib.host_call() if self._native_spec is not None and _raw_stream is not None and len(result_idx) <= 1 else None
+        host = _lib.host_call() if self._native_spec is not None and _raw_stream is not None else None
         if host is None:
             return None
         entry, slots, ints, f, ws_bytes = self._native_spec

@@ -1,0 +1,398 @@
+// Routing: scores of a token's experts, the best top_k of them by score and bias, their weights; and the pairs (token, choice)
+// sorted by expert, for the experts' products.
+//
+// A wave has a token.  Its lane l holds experts l, l + 64, ...; a choice is the largest key left over the lanes, of equal ones the
+// lowest index.  Without a bias a key is the logit itself: softmax and logistic function only rise, so their order is the logits',
+// and nothing is lost where they saturate.  With a bias (and where groups count by the sum of their two best) keys are scores, and
+// fp32 does not tell all of them apart as they are in exact arithmetic: a token whose choices (or groups) lie closer together than
+// fp32's error is done again in 64 bits, so that who is chosen does not hang on how exp is rounded.
+//
+// The order is a counting sort that keeps the pairs' order within an expert: chunks of tokens are counted where they are routed,
+// and with all chunks' counts every workgroup knows where its pairs of an expert begin.  Nothing depends on timing: the only
+// atomics are counts in LDS.
+#include "dq_kv.h"
+
+#include <type_traits>
+
+namespace dq {
+
+namespace {
+
+constexpr int kMaxChunks = 256;
+constexpr int kWaves = 16;             // of a workgroup
+constexpr int kPlaceWorkgroups = 64;   // at most
+constexpr int kAlonePairs = 4096;      // up to here one workgroup sorts them all
+
+struct RouteArgs {
+  const void* Logits;
+  const float* Bias;
+  float* Weights;
+  int* Ids;
+  int tokens, experts, top_k, sigmoid, groups, top_groups, two, renormalize;
+  float factor;
+};
+
+struct OrderArgs {
+  const int* Ids;
+  int* Order;
+  int* Starts;
+  uint16_t* Counts;  // [chunks][experts]; nullptr: one workgroup has all pairs
+  int pairs, experts, first, chunk_pairs, chunks;
+};
+
+// The largest of the lanes' keys and, of the lanes that have it, the lowest index.
+template <class F>
+__device__ __forceinline__ void best_over_wave(F& key, int& index) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const F k = __shfl_xor(key, d, 64);
+    const int i = __shfl_xor(index, d, 64);
+    if (k > key || (k == key && i < index)) key = k, index = i;
+  }
+}
+
+template <class F>
+__device__ __forceinline__ F sum_over_wave(F v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, 64);
+  return v;
+}
+
+// Whether two keys in fp32 may be the other way round in exact arithmetic: a score's error is below 2^-19 (a sum of up to 1024
+// exponentials), a sum's rounding 2^-24 of it.
+__device__ __forceinline__ bool too_close(float a, float b) { return a - b <= 0x1p-17f + 0x1p-20f * (fabsf(a) + fabsf(b)); }
+
+template <class F>
+__device__ __forceinline__ F exp_of(F x) {
+  if constexpr (std::is_same<F, double>::value) return exp(x);
+  else return expf(x);
+}
+
+// One token's choices: lane j < top_k gets the j-th one and its score.  `keys`: the wave's LDS, an F an expert (groups alone).
+// Returns whether F is too narrow to tell (the same in every lane).  A NaN counts as the largest of all: it is chosen, and its
+// weight shows it.
+template <int V, class F>
+__device__ bool choose(const RouteArgs& a, const float (&x)[V], F* keys, int& my_id, float& my_score) {
+  const int lane = threadIdx.x & 63;
+  constexpr F kNone = -(F)__builtin_inff(), kMost = (F)__builtin_inff();
+  constexpr bool kNarrow = std::is_same<F, float>::value;
+  const bool by_score = a.Bias != nullptr;
+  bool close = false;
+
+  F score[V];
+  if (a.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const F t = exp_of<F>(-fabs((F)x[i]));
+      score[i] = (x[i] >= 0 ? (F)1 : t) / ((F)1 + t);
+    }
+  } else {
+    float largest = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i * 64 + lane < a.experts) largest = fmaxf(largest, x[i]);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) largest = fmaxf(largest, __shfl_xor(largest, d, 64));
+    if (largest == -__builtin_inff()) largest = 0.f;  // every expert is masked
+    F total = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      score[i] = i * 64 + lane < a.experts ? exp_of<F>((F)x[i] - (F)largest) : (F)0;
+      total += score[i];
+    }
+    total = sum_over_wave(total);
+#pragma unroll
+    for (int i = 0; i < V; ++i) score[i] = total == 0 ? (F)0 : score[i] / total;
+  }
+
+  F key[V];
+  bool open[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = i * 64 + lane;
+    open[i] = e < a.experts;
+    key[i] = by_score ? score[i] + (F)(open[i] ? a.Bias[e] : 0.f) : (F)x[i];
+    if (key[i] != key[i]) key[i] = kMost;
+  }
+
+  if (a.groups > 1) {
+    const int size = a.experts / a.groups;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (open[i]) {
+        F k = key[i];
+        if (a.two && !by_score) k = score[i] != score[i] ? kMost : score[i];
+        keys[i * 64 + lane] = k;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    F mine = kNone;
+    if (lane < a.groups) {
+      F best = kNone, next = kNone;
+      for (int i = 0; i < size; ++i) {
+        const F k = keys[lane * size + i];
+        if (k > best) next = best, best = k;
+        else if (k > next) next = k;
+      }
+      mine = a.two && size > 1 ? best + next : best;
+      if (mine != mine) mine = kMost;
+    }
+    __builtin_amdgcn_wave_barrier();
+    bool left = lane < a.groups;
+    F last = 0;
+    for (int r = 0; r < a.groups; ++r) {
+      F best = left ? mine : kNone;
+      int index = left ? lane : 64 + lane;  // (behind every group that is left, whatever its key)
+      best_over_wave(best, index);
+      if (kNarrow && r > 0 && (by_score || a.two) && too_close((float)last, (float)best)) close = true;
+      if (r == a.top_groups) break;
+      if (lane == index) left = false;
+      last = best;
+    }
+    const unsigned long long taken = ~__ballot(left);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = i * 64 + lane;
+      open[i] = open[i] && ((taken >> (e / size)) & 1);
+    }
+  }
+
+  F last = 0;
+  for (int r = 0; r < a.top_k + (by_score ? 1 : 0); ++r) {
+    F best = kNone;
+    int index = 1 << 20;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = i * 64 + lane;
+      if (open[i] && (key[i] > best || index == 1 << 20)) best = key[i], index = e;
+    }
+    best_over_wave(best, index);
+    if (kNarrow && by_score && r > 0 && index < 1 << 20 && too_close((float)last, (float)best)) close = true;
+    if (r == a.top_k) break;
+    last = best;
+    float found = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i * 64 + lane == index) open[i] = false, found = (float)score[i];
+    found = __shfl(found, index & 63, 64);
+    if (lane == r) my_id = index, my_score = found;
+  }
+  return close;
+}
+
+template <class T, int V>
+__device__ void route_token(const RouteArgs& a, long token, unsigned char* lds) {
+  const int lane = threadIdx.x & 63;
+  float x[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = i * 64 + lane;
+    x[i] = e < a.experts ? (float)((const T*)a.Logits)[token * a.experts + e] : 0.f;
+  }
+  int id = 0;
+  float score = 0.f;
+  if (choose<V, float>(a, x, (float*)lds, id, score)) choose<V, double>(a, x, (double*)lds, id, score);
+  const bool mine = lane < a.top_k;
+  if (!mine) score = 0.f;
+  if (a.renormalize) {
+    const float sum = sum_over_wave(score);
+    score = sum == 0.f ? 0.f : score / sum;
+  }
+  if (mine) {
+    a.Weights[token * a.top_k + lane] = score * a.factor;
+    a.Ids[token * a.top_k + lane] = id;
+  }
+}
+
+// ---- the order ------------------------------------------------------------------------------------------------------------
+
+// A chunk's pairs of every expert, counted by all threads of the workgroup.
+__device__ void count_chunk(const OrderArgs& o, int chunk, int* count) {
+  for (int e = threadIdx.x; e < o.experts; e += kWaves * 64) count[e] = 0;
+  __syncthreads();
+  const int p1 = min((chunk + 1) * o.chunk_pairs, o.pairs);
+  for (int p = chunk * o.chunk_pairs + threadIdx.x; p < p1; p += kWaves * 64) {
+    const int e = (int)((unsigned)o.Ids[p] - (unsigned)o.first);
+    if ((unsigned)e < (unsigned)o.experts) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < o.experts; e += kWaves * 64) o.Counts[(size_t)chunk * o.experts + e] = (uint16_t)count[e];
+}
+
+// The pairs of some chunks into their places.  `lds`: (kWaves + 1) experts + 64 ints.
+__device__ void place(const OrderArgs& o, int workgroup, int workgroups, int* lds) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = o.experts;
+  int* const mine = lds + wave * E;      // a wave's pairs of every expert; then where its next one goes
+  int* const total = lds + kWaves * E;   // all pairs of every expert
+  int* const sums = total + E;           // kWaves
+  const int per = (o.chunks + workgroups - 1) / workgroups;
+  const int c0 = min(workgroup * per, o.chunks), c1 = min(c0 + per, o.chunks);
+  const int p0 = min((long)c0 * o.chunk_pairs, (long)o.pairs), p1 = min((long)c1 * o.chunk_pairs, (long)o.pairs);
+  const int segment = ((p1 - p0 + kWaves * 64 - 1) / (kWaves * 64)) * 64;  // a wave's
+  const int w0 = min(p0 + wave * segment, p1), w1 = min(w0 + segment, p1);
+
+  for (int e = lane; e < E; e += 64) mine[e] = 0;
+  for (int p = w0 + lane; p < w1; p += 64) {
+    const int e = (int)((unsigned)o.Ids[p] - (unsigned)o.first);
+    if ((unsigned)e < (unsigned)E) atomicAdd(&mine[e], 1);
+  }
+  __syncthreads();
+  // one thread an expert: all pairs, those of earlier workgroups, and where every wave's begin among this one's
+  int before = 0, all = 0;
+  if (tid < E) {
+    if (o.Counts != nullptr) {
+#pragma unroll 8
+      for (int c = 0; c < o.chunks; ++c) {
+        const int n = o.Counts[(size_t)c * E + tid];
+        all += n;
+        before += c < c0 ? n : 0;
+      }
+    }
+    int run = before;
+    for (int w = 0; w < kWaves; ++w) {
+      const int n = lds[w * E + tid];
+      lds[w * E + tid] = run;
+      run += n;
+    }
+    if (o.Counts == nullptr) all = run;
+  }
+  // exclusive sum over the experts
+  int upto = all;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int n = __shfl_up(upto, d, 64);
+    if (lane >= d) upto += n;
+  }
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  int start = upto - all;
+  for (int w = 0; w < wave; ++w) start += sums[w];
+  int end = 0;
+  for (int w = 0; w < kWaves; ++w) end += sums[w];
+  if (tid < E) total[tid] = start;
+  if (workgroup == 0) {
+    if (tid < E) o.Starts[tid] = start;
+    if (tid == 0) o.Starts[E] = end;
+  }
+  __syncthreads();
+  // places that no pair has: pairs whose expert is not among these
+  for (int p = end + workgroup * (kWaves * 64) + tid; p < o.pairs; p += workgroups * (kWaves * 64)) o.Order[p] = -1;
+  const int bits = 32 - __builtin_clz(E);
+  for (int p = w0; p < w1; p += 64) {
+    const int e = p + lane < w1 ? (int)((unsigned)o.Ids[p + lane] - (unsigned)o.first) : -1;
+    const bool valid = (unsigned)e < (unsigned)E;
+    // the lanes that have the same expert
+    unsigned long long same = __ballot(valid);
+    for (int b = 0; b < bits; ++b) {
+      const unsigned long long set = __ballot((e >> b) & 1);
+      same &= ((e >> b) & 1) ? set : ~set;
+    }
+    if (valid) {
+      const int rank = __popcll(same & ((1ull << lane) - 1));
+      const int at = mine[e];
+      o.Order[total[e] + at + rank] = p + lane;
+      if (rank == 0) mine[e] = at + __popcll(same);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(kWaves * 64) void route_kernel(const RouteArgs a, const OrderArgs o) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int wave = threadIdx.x >> 6, chunk = blockIdx.x;
+  const int tokens = o.chunk_pairs / a.top_k;  // of a chunk
+  const long t1 = min((long)(chunk + 1) * tokens, (long)a.tokens);
+  for (long t = (long)chunk * tokens + wave; t < t1; t += kWaves) route_token<T, V>(a, t, smem + (size_t)wave * a.experts * 8);
+  __syncthreads();  // (the pairs that other waves wrote, and the LDS, which changes its use)
+  if (o.Counts != nullptr) count_chunk(o, chunk, (int*)smem);
+  else place(o, 0, 1, (int*)smem);
+}
+
+__global__ __launch_bounds__(kWaves * 64) void count_kernel(const OrderArgs o) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  count_chunk(o, blockIdx.x, (int*)smem);
+}
+
+__global__ __launch_bounds__(kWaves * 64) void place_kernel(const OrderArgs o) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  place(o, blockIdx.x, gridDim.x, (int*)smem);
+}
+
+int place_lds(int experts) { return ((kWaves + 1) * experts + 64) * 4; }
+
+// Whole tokens a chunk, at least a wave's worth, at most kMaxChunks chunks; 16-bit counts
+bool cut(OrderArgs& o, int tokens, int top_k) {
+  if (tokens * (long)top_k <= kAlonePairs && tokens <= 2 * kWaves) {
+    o.chunk_pairs = tokens * top_k, o.chunks = 1;
+    return false;
+  }
+  const int per = ((tokens + kMaxChunks - 1) / kMaxChunks + kWaves - 1) / kWaves * kWaves;
+  o.chunk_pairs = per * top_k, o.chunks = (tokens + per - 1) / per;
+  return true;
+}
+
+template <class T, int V>
+int launch_route(const RouteArgs& a, const OrderArgs& o, hipStream_t stream) {
+  constexpr int kMost = 16 * 1024 * 8 + 1024 * 4 + 256;
+  const int keys = kWaves * a.experts * 8, room = place_lds(a.experts);
+  const int lds = keys > room ? keys : room;
+  auto kern = route_kernel<T, V>;
+  static bool raised[kMaxDevices];
+  if (raise_lds_limit<kMost>(kern, raised)) return -1;
+  hipLaunchKernelGGL(kern, dim3(o.chunks), dim3(kWaves * 64), lds, stream, a, o);
+  DQ_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+template <class T>
+int route_experts_of(const RouteArgs& a, const OrderArgs& o, hipStream_t stream) {
+  if (a.experts <= 64) return launch_route<T, 1>(a, o, stream);
+  if (a.experts <= 128) return launch_route<T, 2>(a, o, stream);
+  if (a.experts <= 256) return launch_route<T, 4>(a, o, stream);
+  if (a.experts <= 512) return launch_route<T, 8>(a, o, stream);
+  return launch_route<T, 16>(a, o, stream);
+}
+
+int launch_place(const OrderArgs& o, hipStream_t stream) {
+  constexpr int kMost = (17 * 1024 + 64) * 4;
+  auto kern = place_kernel;
+  static bool raised[kMaxDevices];
+  if (raise_lds_limit<kMost>(kern, raised)) return -1;
+  const int workgroups = o.chunks < kPlaceWorkgroups ? o.chunks : kPlaceWorkgroups;
+  hipLaunchKernelGGL(kern, dim3(o.Counts ? workgroups : 1), dim3(kWaves * 64), place_lds(o.experts), stream, o);
+  DQ_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+}  // namespace
+
+size_t order_workspace_bytes(int tokens, int top_k, int experts) {
+  OrderArgs o{};
+  return cut(o, tokens, top_k) ? ((size_t)o.chunks * experts * 2 + 15) / 16 * 16 : 0;
+}
+
+int route_experts(const void* Logits, const float* Bias, float* Weights, int* Ids, int* Order, int* Starts, void* Workspace, int tokens,
+                  int experts, int top_k, int sigmoid, int groups, int top_groups, int two, int renormalize, int dtype, float factor,
+                  hipStream_t stream) {
+  const RouteArgs a{Logits, Bias, Weights, Ids, tokens, experts, top_k, sigmoid, groups, top_groups, two, renormalize, factor};
+  OrderArgs o{Ids, Order, Starts, nullptr, tokens * top_k, experts, 0, 0, 0};
+  const bool chunks = cut(o, tokens, top_k);
+  if (chunks) o.Counts = (uint16_t*)Workspace;
+  const int rc = dtype == 0 ? route_experts_of<half_t>(a, o, stream) : dtype == 1 ? route_experts_of<bf16_t>(a, o, stream) : route_experts_of<float>(a, o, stream);
+  return rc != 0 || !chunks ? rc : launch_place(o, stream);
+}
+
+int experts_order(const int* Ids, int* Order, int* Starts, void* Workspace, int tokens, int top_k, int experts, int first, hipStream_t stream) {
+  OrderArgs o{Ids, Order, Starts, nullptr, tokens * top_k, experts, first, 0, 0};
+  if (cut(o, tokens, top_k)) {
+    o.Counts = (uint16_t*)Workspace;
+    hipLaunchKernelGGL(count_kernel, dim3(o.chunks), dim3(kWaves * 64), (size_t)experts * 4, stream, o);
+    DQ_CHECK_HIP(hipGetLastError());
+  }
+  return launch_place(o, stream);
+}
+
+}  // namespace dq

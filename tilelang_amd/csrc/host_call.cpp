@@ -90,6 +90,26 @@ const Entry kEntries[] = {
      [](void* fn, const Args& a) {
        return DQ_CALL(call_paged_attention_decode)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.p[7], a.p[8], a.p[9], a.p[10], a.ws, a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.i[8], a.i[9], a.f, a.stream);
      }},
+    {"call_rms_norm", 6, 5,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_rms_norm)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.f, a.stream);
+     }},
+    {"call_route_experts", 7, 9,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_route_experts)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.ws, a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.i[8], a.f, a.stream);
+     }},
+    {"call_experts_order", 4, 4,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_experts_order)(a.p[0], a.p[1], a.p[2], a.p[3], a.ws, a.i[0], a.i[1], a.i[2], a.i[3], a.stream);
+     }},
+    {"call_experts_up", 8, 8,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_experts_up)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.p[7], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.stream);
+     }},
+    {"call_experts_down", 12, 8,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_experts_down)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.p[7], a.p[8], a.p[9], a.p[10], a.p[11], a.ws, a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.stream);
+     }},
 };
 #undef DQ_CALL
 
@@ -107,7 +127,7 @@ struct Call {
   void* fn;
   std::vector<Param>* params;
   int inputs;                 // parameters of role 0
-  int returned;               // the one that is returned, or -1
+  int returned;               // how many are returned: none, one as it is, several as a list
   int slot[kMaxPointers];     // pointer argument -> parameter, -1: NULL
   std::vector<int>* ints;
   float f;
@@ -166,8 +186,8 @@ PyObject* call_call(PyObject* self_, PyObject* args, PyObject* kwargs) {
   void* const stream = reinterpret_cast<void*>(PyLong_AsUnsignedLongLong(raw));
   Py_DECREF(raw);
   if (PyErr_Occurred()) return nullptr;
-  at::Tensor returned, scratch;
-  int rc;
+  at::Tensor returned[kMaxParams], scratch;
+  int rc, results = 0;
   {
     const WithoutInterpreter released;
     const at::Device dev(at::kCUDA, static_cast<c10::DeviceIndex>(device));
@@ -176,7 +196,7 @@ PyObject* call_call(PyObject* self_, PyObject* args, PyObject* kwargs) {
       if (p.role == 0) continue;
       at::Tensor t = at::empty(p.shape, at::TensorOptions().dtype(p.dtype).device(dev));
       pointers[k] = t.data_ptr();
-      (p.role == 1 ? returned : scratch) = std::move(t);
+      (p.role == 1 ? returned[results++] : scratch) = std::move(t);
     }
     Args a;
     for (int s = 0; s < self->entry->pointers; ++s) a.p[s] = self->slot[s] < 0 ? nullptr : pointers[self->slot[s]];
@@ -190,8 +210,18 @@ PyObject* call_call(PyObject* self_, PyObject* args, PyObject* kwargs) {
     PyErr_Format(PyExc_RuntimeError, "Kernel call failed: %s", g_last_error());
     return nullptr;
   }
-  if (self->returned < 0) Py_RETURN_NONE;
-  return THPVariable_Wrap(std::move(returned));
+  if (self->returned == 0) Py_RETURN_NONE;
+  if (self->returned == 1) return THPVariable_Wrap(std::move(returned[0]));
+  PyObject* const list = PyList_New(self->returned);
+  for (int i = 0; list && i < self->returned; ++i) {
+    PyObject* const t = THPVariable_Wrap(std::move(returned[i]));
+    if (!t) {
+      Py_DECREF(list);
+      return nullptr;
+    }
+    PyList_SET_ITEM(list, i, t);
+  }
+  return list;
   END_HANDLE_TH_ERRORS
 }
 
@@ -225,7 +255,7 @@ PyObject* bind(PyObject*, PyObject* args) {
   self->params = new std::vector<Param>();
   self->ints = new std::vector<int>();
   self->inputs = 0;
-  self->returned = -1;
+  self->returned = 0;
   self->f = f;
   self->ws = static_cast<size_t>(ws);
   bool good = true;
@@ -243,10 +273,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     good = good && (p.strides.empty() || p.strides.size() == p.shape.size());
     self->inputs += role == 0;
     workspaces += role == 2;
-    if (role == 1) {
-      good = self->returned < 0;
-      self->returned = static_cast<int>(k);
-    }
+    self->returned += role == 1;
     self->params->push_back(std::move(p));
   }
   good = good && workspaces <= 1;
