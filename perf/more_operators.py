@@ -312,7 +312,7 @@ def _kernel(state):
         return tl.route_experts(case["tokens"], case["experts"], case["top_k"], scores=case["scores"], bias=case["bias"], groups=case["groups"],
                                 top_groups=case["top_groups"], group_score=case["group_score"], renormalize=case["renormalize"],
                                 factor=case["factor"], dtype=case["dtype"])
-    sizes = dict(weight_format=case["weights"], group_size=case["group"], with_zeros=case["zeros"], with_bias=case["bias"])
+    sizes = dict(weight_format=case["weights"], group_size=case["group"] if case["weights"] == "uint4" else None, with_zeros=case["zeros"], with_bias=case["bias"])
     if case["kind"] == "up":
         return tl.experts_up(case["tokens"], case["experts"], case["top_k"], case["N"], case["K"], activation=case["activation"], **sizes)
     return tl.experts_down(case["tokens"], case["experts"], case["top_k"], case["N"], case["K"], residual=case["residual"], **sizes)
