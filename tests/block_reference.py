@@ -141,13 +141,15 @@ def down(h, w, order, starts, weights, tokens, residual):
     N = w.value.shape[1]
     out, size, slack = (torch.zeros((tokens, N), dtype=torch.float64) for _ in range(3))
     for e in range(len(starts) - 1):
-        for p in range(int(starts[e]), int(starts[e + 1])):
-            pair = int(order[p])
-            y, off = w.product(h[p : p + 1].cpu(), e)
-            y, off = y[0] * weights[pair], off[0] * weights[pair].abs()
-            out[pair // top_k] += y
-            size[pair // top_k] += y.abs()
-            slack[pair // top_k] += off
+        r = slice(int(starts[e]), int(starts[e + 1]))
+        if r.start == r.stop:
+            continue
+        pair = order[r].long()
+        y, off = w.product(h[r].cpu(), e)
+        # (an expert's rows may name a token twice)
+        out.index_add_(0, pair // top_k, y * weights[pair][:, None])
+        size.index_add_(0, pair // top_k, y.abs() * weights[pair].abs()[:, None])
+        slack.index_add_(0, pair // top_k, off * weights[pair].abs()[:, None])
     if residual is not None:
         out, size = out + residual.double().cpu(), size + residual.double().cpu().abs()
     return out, slack + (top_k + 2) * 2.0**-24 * size

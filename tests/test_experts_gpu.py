@@ -86,6 +86,16 @@ def test_sizes(cuda, tokens, experts, top_k, fmt, hidden, inter, whole):
     _both(cuda, tokens, experts, top_k, hidden, inter, whole=whole, **fmt)
 
 
+@pytest.mark.parametrize("fmt", FORMATS, ids=lambda f: "-".join(f"{k}={v}" for k, v in f.items()) or "uint4")
+@pytest.mark.parametrize("tokens,experts,top_k,how,hidden,inter", [
+    (1100, 2, 1, "even", 128, 256), (1024, 1, 1, "one", 256, 384), (700, 3, 1, "one", 384, 128), (3500, 70, 1, "skewed", 128, 128), (900, 5, 3, "padded", 256, 128),
+    (1400, 4, 2, "skewed", 640, 256),
+])
+def test_many_rows(cuda, tokens, experts, top_k, how, hidden, inter, fmt):
+    print(f"experts {tokens} of {experts} top {top_k} {how} {hidden} {inter} {fmt}", flush=True)
+    _both(cuda, tokens, experts, top_k, hidden, inter, how, residual=tokens % 4 == 0, **fmt)
+
+
 @pytest.mark.parametrize("weight_format", ["uint4", "mxfp4"])
 def test_nothing_to_do(cuda, weight_format):
     """No token has an expert here: h is left as it was, y is the residual."""

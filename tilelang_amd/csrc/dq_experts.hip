@@ -9,6 +9,8 @@
 
 namespace dq {
 
+int experts_tiles(const experts::Args& a, int mxfp4, bool up, int tile_rows, hipStream_t stream);
+
 namespace {
 
 using experts::Args;
@@ -146,22 +148,40 @@ __global__ __launch_bounds__(256) void sum_kernel(const Args a) {
   *reinterpret_cast<vec4*>((T*)a.Out + at) = o;
 }
 
+template <class T>
+int sum(const Args& a, hipStream_t stream) {
+  const size_t threads = (size_t)a.tokens * a.N / 4;
+  hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a);
+  DQ_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
 template <class W, bool UP>
 int product(const Args& a, hipStream_t stream) {
   constexpr int kWaves = 4;
   const int most = a.experts < a.pairs ? a.experts : a.pairs;  // experts that can have rows
   hipLaunchKernelGGL((rows_kernel<W, UP, kWaves>), dim3(a.N / (UP ? 16 : 32), most), dim3(kWaves * 64), 0, stream, a);
   DQ_CHECK_HIP(hipGetLastError());
-  if constexpr (!UP) {
-    const size_t threads = (size_t)a.tokens * a.N / 4;
-    hipLaunchKernelGGL((sum_kernel<typename W::T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a);
-    DQ_CHECK_HIP(hipGetLastError());
-  }
+  if constexpr (!UP) return sum<typename W::T>(a, stream);
   return 0;
+}
+
+// Rows of a tile of the matrix pipe's kernel, or 0: few rows an expert.
+int tile_rows(const Args& a, int mxfp4) {
+  if (a.K < 128) return 0;
+  const long mean = a.pairs / (a.experts < a.pairs ? a.experts : a.pairs);
+  if (mean < 48) return 0;
+  const bool tall = mxfp4 || a.group_shift > 5;
+  return tall && mean >= 512 ? 256 : 128;
 }
 
 template <bool UP>
 int by_format(const Args& a, int mxfp4, hipStream_t stream) {
+  if (const int rows = tile_rows(a, mxfp4)) {
+    if (const int rc = experts_tiles(a, mxfp4, UP, rows, stream)) return rc;
+    if constexpr (!UP) return mxfp4 ? sum<bf16_t>(a, stream) : sum<half_t>(a, stream);
+    return 0;
+  }
   if (mxfp4) return product<experts::Mxfp4, UP>(a, stream);
   return a.Z != nullptr ? product<experts::Uint4<true>, UP>(a, stream) : product<experts::Uint4<false>, UP>(a, stream);
 }

@@ -560,6 +560,24 @@ struct BFragments : std::false_type {};
 template <class P>
 struct BFragments<P, std::void_t<decltype(P::kBFragments)>> : std::integral_constant<bool, P::kBFragments> {};
 
+// A policy may declare `static constexpr bool kGrouped = true`: its problem is many, rows in groups that have weights of their own
+// (dq_experts_tiles.hip).  It brings
+//   params_t          derived from Params
+//   take_tile(p, bid, BM, m0, n0)   the tile of a workgroup: sets p.A, p.B, p.S, p.Z and p.M to those of its group; false: none
+//   a_row(p, m)       row of p.A of the group's row m (m0 on, of this tile)
+//   b_row(p, n0, row) weight row of the tile's row
+//   store<BLOCKS>(p, acc, smem, slab, lane, m0, n0, wn)   the epilogue of the wave of columns wn of the tile, over BLOCKS blocks of
+//                     32 rows from m0 on; slab: its number among the workgroup's waves
+// and is launched by its own code; direct-to-LDS variant only.
+template <class P, class = void>
+struct Grouped : std::false_type {
+  using params_t = Params;
+};
+template <class P>
+struct Grouped<P, std::void_t<decltype(P::kGrouped)>> : std::true_type {
+  using params_t = typename P::params_t;
+};
+
 // ---- direct-to-LDS variant ---------------------------------------------------------------------
 // For policies whose A needs no transform on its way to LDS (any per-fragment transform is P::fix_a,
 // applied after the fragment is read) and whose scales are absent, one byte per 32 k or one fp16 (plus
@@ -614,10 +632,11 @@ __device__ __forceinline__ void dma4_unless(int not_due, unsigned lds_addr, unsi
 // slower also where nothing is odd (MXFP4, M = 4096, N = K = 8192: 369 and 374 us; fp16 x uint4 at M = 2048, N = 4096,
 // K = 14336 203 and 206, at M = 2015, N = 24640, K = 2048 191 and 193; int8 x 2-bit, M = 2048, N = K = 8192: 109.7 and 110.2).
 template <class P, int kMBW, int kNBW, int kWavesM = 2, int kKHalves = 1, bool kOdd = false>
-__global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1) void gemm_kernel_dma(const Params p_in) {
-  Params p = p_in;
+__global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1) void gemm_kernel_dma(const typename Grouped<P>::params_t p_in) {
+  typename Grouped<P>::params_t p = p_in;
   int bid = blockIdx.x;
-  take_k_slice<P>(p, bid);
+  constexpr bool kGrouped = Grouped<P>::value;
+  if constexpr (!kGrouped) take_k_slice<P>(p, bid);
   extern __shared__ __align__(16) unsigned char smem[];
   static_assert(P::kBRowBytes == 32 || P::kBRowBytes == 64, "direct-to-LDS variant: 32 or 64 packed bytes per weight row per tile");
   static_assert(kWavesM == 2 ? (kMBW == 4 && kNBW == 4) : (kWavesM == 1 && (kMBW == 3 || kMBW == 4 || kMBW == 6 || kMBW == 8) && kNBW == 2), "one of the forms");
@@ -666,12 +685,24 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
   const int wave = kHalves ? dma_wave % kWaves : dma_wave;
   const int wm = wave / kWavesN, wn = wave % kWavesN;
   const int g = lane >> 5, r = lane & 31;
+  int m0, n0;
+  if constexpr (kGrouped) {
+    if (!P::take_tile(p, bid, BM, m0, n0)) return;
+  } else {
+    int tm, tn;
+    tile_of_block(bid, p.tiles_m, p.tiles_n, tm, tn);
+    m0 = tm * BM, n0 = tn * BN;
+  }
   const int M = p.M, N = p.N, K = p.K;
-
-  int tm, tn;
-  tile_of_block(bid, p.tiles_m, p.tiles_n, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BN;
   const int KB = K / P::kKPerBlock / kStageTiles;  // tiles, or stages of two of them
+  auto a_row = [&](int row) -> unsigned {
+    if constexpr (kGrouped) return P::a_row(p, min(m0 + row, M - 1));
+    else return (unsigned)min(m0 + row, M - 1);
+  };
+  auto b_row = [&](int row) -> unsigned {
+    if constexpr (kGrouped) return P::b_row(p, n0, row);
+    else return (unsigned)min(n0 + row, N - 1);
+  };
   const unsigned lds0 = (unsigned)(size_t)smem;  // LDS byte address of the dynamic segment
 
   // ---- per-lane source offsets: LDS chunk c (16 bytes) of a tile <- which global 16 bytes --------
@@ -680,7 +711,7 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
   for (int i = 0; i < kAOps; ++i) {
     const int c = (dma_wave * kAOps + i) * 64 + lane;  // A chunk: row c / 8 (of half c / 1024), physical piece c % 8
     const int row = (c >> 3) % BM, pp = c & 7;
-    a_voff[i] = (unsigned)min(m0 + row, M - 1) * (unsigned)(p.ldk * (kARowBytes / P::kKPerBlock)) + (unsigned)((pp ^ a_swz(row)) << 4) +
+    a_voff[i] = a_row(row) * (unsigned)(p.ldk * (kARowBytes / P::kKPerBlock)) + (unsigned)((pp ^ a_swz(row)) << 4) +
                 (unsigned)((c >> 3) / BM * kARowBytes);
   }
 #pragma unroll
@@ -688,7 +719,7 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
     const int c = (dma_wave * kBOps + i) * 64 + lane;  // B chunk: row c / pieces per row, physical piece c % pieces per row
     const int row = c / kBLoadPieces, pp = c % kBLoadPieces;
     // LDS position (piece + rotation) % pieces holds source piece `piece`
-    b_voff[i] = (unsigned)min(n0 + row, N - 1) * (unsigned)(p.ldk * P::kBRowBytes / P::kKPerBlock) +
+    b_voff[i] = b_row(row) * (unsigned)(p.ldk * P::kBRowBytes / P::kKPerBlock) +
                 (unsigned)(((pp - (row >> kBRot)) & (kBLoadPieces - 1)) << 4);
     if constexpr (kBFrag) {
       // instruction (wave, i) brings the 32-row block wave * kBOps + i of the tile: 1 KiB as stored, lane-linear
@@ -706,7 +737,7 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
   const int s_ps = s_gshift - 5;
   const bool s_odd = kOdd && P::kScaleDma != 0 && ((p.ldk >> s_gshift) & 1) != 0;
   const int s_ahead = s_odd ? -(lane & 1) : 0;  // rows of a tile start at an even one
-  const ScaleWalk walk((unsigned)min(n0 + (tid & 255), N - 1), (unsigned)(p.ldk >> s_gshift), s_odd);  // waves 4..7 repeat 0..3
+  const ScaleWalk walk(b_row(tid & 255), (unsigned)(p.ldk >> s_gshift), s_odd);  // waves 4..7 repeat 0..3
 
   // One tile = kSOps + kAOps + kBOps DMA instructions per thread: first the scale dword(s) (row tid) if one is due,
   // then the A chunks, then the packed-B chunks.  Two halves: waves 0 .. 3 bring the scales and waves 4 .. 7 the zeros.
@@ -1124,7 +1155,10 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
     }
     __syncthreads();  // the epilogue's slabs lie where the sums were handed over
     const int first_row = m0 + 32 * kOwn0 * kh, slab_wave = wave + kWaves * kh;
-    {
+    if constexpr (kGrouped) {
+      if (kh == 0) P::template store<kOwn0>(p, acc, smem, slab_wave, lane, first_row, n0, wn);
+      else P::template store<kOwn1>(p, acc, smem, slab_wave, lane, first_row, n0, wn);
+    } else {
       const int m0 = first_row, wave = slab_wave;
       if constexpr (kOwn0 == kOwn1) {
         DQ_GEMM_EPILOGUE_OF(kOwn0)
@@ -1134,6 +1168,8 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
         DQ_GEMM_EPILOGUE_OF(kOwn1)
       }
     }
+  } else if constexpr (kGrouped) {
+    P::template store<kMBW>(p, acc, smem, wave, lane, m0 + wm * (32 * kMBW), n0, wn);
   } else {
     DQ_GEMM_EPILOGUE
   }
