@@ -27,22 +27,25 @@ struct Args {
 };
 
 // Activations and weights of a product: uint4 codes x fp16, as the dense W4A16 kernels have them (rounded to fp16), and e2m1 x bf16.
-template <bool ZEROS>
+template <bool ZEROS, int SHIFT>
 struct Uint4 {
   using T = half_t;
   using frag = half8_t;
   static constexpr bool kZeros = ZEROS;
+  static constexpr int kShift = SHIFT, kScaleBytes = 2;  // 2 ^ kShift k share a scale
   static constexpr int MODE = ZEROS ? W4_ZEROS_ORIGINAL : W4_SCALE;
-  struct Raw { half_t s, z; };
   struct Scale { half_t s, addend; };
-  __device__ static __forceinline__ Raw fetch(const Args& a, size_t row, int k) {
-    const size_t at = row * (a.K >> a.group_shift) + (k >> a.group_shift);
-    Raw r{((const half_t*)a.S)[at], (half_t)0.f};
-    if constexpr (ZEROS) r.z = ((const half_t*)a.Z)[at];
-    return r;
+  // (the bits of a scale and a zero point)
+  __device__ static __forceinline__ Scale scale(unsigned s, unsigned z) {
+    const half_t f = __builtin_bit_cast(half_t, (unsigned short)s);
+    return {f, w4_cvt_addend<MODE>(f, __builtin_bit_cast(half_t, (unsigned short)z))};
   }
-  __device__ static __forceinline__ Scale scale(Raw r) { return {r.s, w4_cvt_addend<MODE>(r.s, r.z)}; }
-  __device__ static __forceinline__ frag decode(uint32_t w, const Scale& s) { return decode_w4_cvt<MODE, false, true>(w, s.s, s.addend); }
+  // eight activations in the order that a word's codes are decoded in
+  __device__ static __forceinline__ uint4_t order(uint4_t d) {
+    return {__builtin_amdgcn_perm(d[1], d[0], 0x05040100u), __builtin_amdgcn_perm(d[3], d[2], 0x05040100u),
+            __builtin_amdgcn_perm(d[1], d[0], 0x07060302u), __builtin_amdgcn_perm(d[3], d[2], 0x07060302u)};
+  }
+  __device__ static __forceinline__ frag decode(uint32_t w, const Scale& s) { return decode_w4_cvt<MODE, false, false>(w, s.s, s.addend); }
   __device__ static __forceinline__ float4_t mfma(frag a, frag b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
@@ -50,10 +53,10 @@ struct Mxfp4 {
   using T = bf16_t;
   using frag = bf16x8_t;
   static constexpr bool kZeros = false;
-  using Raw = int;
+  static constexpr int kShift = 5, kScaleBytes = 1;
   using Scale = float;
-  __device__ static __forceinline__ Raw fetch(const Args& a, size_t row, int k) { return ((const uint8_t*)a.S)[row * (a.K >> 5) + (k >> 5)]; }
-  __device__ static __forceinline__ Scale scale(Raw e) { return scale_to_f32(e, 0); }
+  __device__ static __forceinline__ Scale scale(unsigned e, unsigned) { return scale_to_f32((int)e, 0); }
+  __device__ static __forceinline__ uint4_t order(uint4_t d) { return d; }
   __device__ static __forceinline__ frag decode(uint32_t w, const Scale& s) { return cvt_e2m1x8(w, s); }
   __device__ static __forceinline__ float4_t mfma(frag a, frag b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };

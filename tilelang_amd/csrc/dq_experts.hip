@@ -1,11 +1,17 @@
 // The experts' products at a few rows an expert: a workgroup has 16 weight rows of the gate and the 16 of the up projection (or 32
 // weight rows) of one expert and multiplies them with up to 16 of its rows at a time.
 //
-// What bounds it is the weights' way out of memory: every expert that has rows is read once.  K is cut over the workgroup's waves,
-// whose sums meet in LDS.  A lane reads 16 bytes of a weight row at a time, 32 k; the matrix instruction's k are labelled
-// 32 g + 8 j + e for its lane group g and the j-th of four instructions, for both operands, so that the weights go into it as
-// they lie and the activations of a lane are 64 contiguous bytes.
+// What bounds it is the weights' way out of memory, every expert that has rows being read once, and the load unit of a CU, which
+// takes two cycles for 64 bytes or a piece of a row, whichever is less.  So loads are whole cache lines of neighbouring lanes: a
+// chunk of 256 k is 128 bytes of a weight row, eight rows a load, a step of 128 k is 256 bytes of an activation row, four rows a
+// load, and of those rows only the expert's own.  K is cut over the workgroup's waves.  A wave is a pipeline of its own: what it loads,
+// two chunks and two steps ahead, goes through LDS that it alone writes and reads into the order of the matrix instruction, whose
+// k are labelled 32 g + 8 j + e for its lane group g and the j-th of the step's four instructions, for both operands; its LDS
+// operations are carried out in their order, so there is no barrier.  The waves' sums meet in LDS at the end.
 #include "dq_experts.h"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace dq {
 
@@ -16,108 +22,352 @@ namespace {
 using experts::Args;
 
 constexpr int kStep = 128;  // k of a step: 32 a lane group
+constexpr int kWaves = 4;   // pipelines of a workgroup
 
-// The `nth` expert that has rows, or false.  Every wave finds it by itself.
-__device__ __forceinline__ bool nth_expert(const Args& a, int nth, int& expert, int& begin, int& end) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < a.experts; base += 64) {
-    int b = 0, e = 0;
-    if (base + lane < a.experts) experts::rows_of(a, base + lane, b, e);
-    unsigned long long has = __ballot(e > b);
-    const int count = __popcll(has);
-    if (nth < count) {
-      for (; nth > 0; --nth) has &= has - 1;
-      const int at = __builtin_ctzll(has);
-      expert = base + at;
-      begin = __builtin_amdgcn_readlane(b, at);
-      end = __builtin_amdgcn_readlane(e, at);
-      return true;
+// Work is counted in parts: up to `most` rows of an expert, the experts one behind the other.  Every wave counts and finds them for
+// itself: a lane holds the rows of experts lane, 64 + lane, ... of the first 256, all asked for at once; beyond, they are asked for
+// again.
+struct Part {
+  int expert, begin, end;  // rows begin .. end - 1
+};
+struct Parts {
+  static constexpr int kHeld = 4;
+  const Args& a;
+  const int most;
+  int begin[kHeld], end[kHeld];
+
+  __device__ __forceinline__ Parts(const Args& args, int rows) : a(args), most(rows) {
+    const int lane = threadIdx.x & 63;
+    int raw[kHeld][2];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int e = min(64 * i + lane, a.experts - 1);
+      raw[i][0] = a.Starts[e], raw[i][1] = a.Starts[e + 1];
     }
-    nth -= count;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      begin[i] = min(max(raw[i][0], 0), a.pairs);
+      end[i] = 64 * i + lane < a.experts ? min(max(raw[i][1], begin[i]), a.pairs) : begin[i];
+    }
   }
-  return false;
+  // f(first expert of 64, the lane's rows) until it is content
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (f(64 * i, begin[i], end[i])) return;
+    for (int base = 64 * kHeld; base < a.experts; base += 64) {
+      int b = 0, e = 0;
+      if (base + (int)(threadIdx.x & 63) < a.experts) experts::rows_of(a, base + (threadIdx.x & 63), b, e);
+      if (f(base, b, e)) return;
+    }
+  }
+  // inclusive sum of the lanes' parts, bit by bit of them (most experts have one); `all`: of all lanes
+  __device__ __forceinline__ int upto(int b, int e, int& all) const {
+    const int n = (e - b + most - 1) / most;
+    int sum = n;
+    all = 0;
+    for (int bit = 0;; ++bit) {
+      if (__ballot(n >> bit != 0) == 0) return sum;
+      const unsigned long long set = __ballot((n >> bit) & 1);
+      sum += (int)__builtin_amdgcn_mbcnt_hi((unsigned)(set >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)set, 0)) << bit;
+      all += __popcll(set) << bit;
+    }
+  }
+  __device__ __forceinline__ int count() const {
+    int all = 0;
+    each([&](int, int b, int e) {
+      int here;
+      upto(b, e, here);
+      all += here;
+      return false;
+    });
+    return all;
+  }
+  __device__ __forceinline__ Part nth(int n) const {  // (n below count())
+    Part found{0, 0, 0};
+    each([&](int base, int b, int e) {
+      int here;
+      const int sum = upto(b, e, here);
+      if (n >= here) {
+        n -= here;
+        return false;
+      }
+      const unsigned long long beyond = __ballot(sum > n);
+      const int at = __builtin_ctzll(beyond);
+      const int first = __builtin_amdgcn_readlane(b, at), last = __builtin_amdgcn_readlane(e, at);
+      const int before = __builtin_amdgcn_readlane(sum, at) - (last - first + most - 1) / most;
+      found.expert = base + at;
+      found.begin = first + (n - before) * most;
+      found.end = min(found.begin + most, last);
+      return true;
+    });
+    return found;
+  }
+};
+
+constexpr int kChunk = 256;       // k of a chunk: two steps, a cache line of a row
+constexpr int kWordsArea = 4096;  // a wave's LDS: 32 weight rows of 128 bytes,
+constexpr int kScalesArea = 512;  // and of up to 16 bytes of scales, and of zero points
+constexpr int kSumsArea = 2048;   // 32 sums of 16 rows, twice
+constexpr int kActsRoom = 120 * 1024;  // of a workgroup, at least
+constexpr int kDescriptor = 0x00027000, kNontemporal = 2;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bytes_at(const void* p, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, kDescriptor);
 }
 
-template <class W, bool UP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void rows_kernel(const Args a) {
-  using T = typename W::T;
-  typedef T vec __attribute__((ext_vector_type(8)));
-  __shared__ float4_t sums[WAVES][2][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int g = lane >> 4, c = lane & 15;
-  int expert, begin, end;
-  if (!nth_expert(a, blockIdx.y, expert, begin, end)) return;
-  const int rows = (UP ? 2 : 1) * a.N;  // weight rows of an expert
-  const int n0 = blockIdx.x * (UP ? 16 : 32);
-  size_t w_row[2];
-  w_row[0] = (size_t)expert * rows + n0 + c;
-  w_row[1] = w_row[0] + (UP ? a.N : 16);
-  const size_t row_bytes = (size_t)a.K >> 1;
+// Where 16-byte piece `piece` of a row lies in the wave's LDS: the lanes of one row number each, or of one piece, are in different banks.
+__device__ __forceinline__ int word_place(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) << 4); }
+__device__ __forceinline__ int act_place(int row, int piece, int stride) { return row * stride + ((piece ^ (row & 15)) << 4); }
 
-  for (int r0 = begin; r0 < end; r0 += 16) {
-    const int row = r0 + c;
-    const bool there = row < end;
-    const T* x = (const T*)a.A;
-    if (there) {
-      int at = row;
-      if constexpr (UP) at = min((unsigned)a.Order[row] / (unsigned)a.top_k, (unsigned)a.tokens - 1);
-      x += (size_t)at * a.K;
-    }
-    float4_t acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    for (int k0 = wave * kStep; k0 < a.K; k0 += WAVES * kStep) {
-      const int k = k0 + 32 * g;
-      const bool inside = k < a.K;  // (K is a multiple of 32)
-      vec xv[4];
-      uint4_t words[2];
-      typename W::Raw raw[2];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        xv[j] = vec{};
-        if (there && inside) xv[j] = *reinterpret_cast<const vec*>(x + k + 8 * j);
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        words[t] = uint4_t{};
-        const int ks = inside ? k : 0;
-        if (inside) words[t] = *reinterpret_cast<const uint4_t*>(a.B + w_row[t] * row_bytes + (k >> 1));
-        raw[t] = W::fetch(a, w_row[t], ks);
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const typename W::Scale s = W::scale(raw[t]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[t] = W::mfma(__builtin_bit_cast(typename W::frag, xv[j]), W::decode(words[t][j], s), acc[t]);
-      }
-    }
-    if (r0 != begin) __syncthreads();  // (the sums before are read)
-    sums[wave][0][lane] = acc[0];
-    sums[wave][1][lane] = acc[1];
-    __syncthreads();
-    // one value a thread: [tile][lane][4]
-    const float* const all = (const float*)sums;
-    if constexpr (UP) {
-      for (int i = threadIdx.x; i < 256; i += WAVES * 64) {
-        const int m = i >> 4, n = i & 15, at = ((m >> 2) * 16 + n) * 4 + (m & 3);
-        float v[2] = {0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) v[0] += all[w * 512 + at], v[1] += all[w * 512 + 256 + at];
-        if (a.Bias != nullptr) {
-          const T* bias = (const T*)a.Bias + (size_t)expert * rows + n0 + n;
-          v[0] += (float)bias[0];
-          v[1] += (float)bias[a.N];
-        }
-        if (r0 + m < end) ((T*)a.Out)[(size_t)(r0 + m) * a.N + n0 + n] = (T)(experts::activate(v[0], a.gelu) * v[1]);
-      }
+// A wave's part of the products of some rows of one expert, which lie in LDS, with a run of tiles of 32 weight rows: of every tile the
+// chunks c0 .. c1 - 1.  The chunks of all tiles are one sequence, whose weights are asked for DEPTH chunks ahead.  A load that is of
+// no use (behind the sequence, beyond K) names an offset beyond its descriptor's bytes, which reads zeros.
+// LINES: rows are whole cache lines, which are read once (nontemporal); otherwise two chunks share a line, and the one that comes second
+// is to find it in a cache.
+template <class W, int DEPTH, bool LINES>
+struct Pipeline {
+  static constexpr unsigned kNowhere = 0xFFFFFF00u;
+  const Args& a;
+  __amdgpu_buffer_rsrc_t w_rows, s_rows, z_rows;
+  unsigned w_at[4], s_at, tile_bytes, tile_scales;
+  int c0, c1, tile_end;
+  int w_tile, w_c;  // what is asked for next
+  bool idle;
+  unsigned char *words, *scales;
+  const unsigned char* acts;
+  int acts_stride;
+  uint4_t w_reg[DEPTH][4];
+  // a lane's half of the chunk's scales of its row (lane / 2): those of a step
+  static constexpr int kHalf = (kStep >> W::kShift) * W::kScaleBytes;  // bytes: 2, 4 or 8
+  static constexpr bool kPairs = W::kScaleBytes == 1 && !LINES;       // from where two bytes lie, not four
+  static constexpr int kRegs = kHalf == 8 || kPairs ? 2 : 1;
+  unsigned s_reg[DEPTH][kRegs], z_reg[DEPTH][kRegs];
+
+  __device__ __forceinline__ void ask_scales(unsigned (&to)[kRegs], __amdgpu_buffer_rsrc_t rows, unsigned at) const {
+    if constexpr (kPairs) {
+      to[0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rows, at, 0, 0);
+      to[1] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rows, at + 2, 0, 0);
+    } else if constexpr (kHalf == 2) {
+      to[0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rows, at, 0, 0);
+    } else if constexpr (kHalf == 4) {
+      to[0] = __builtin_amdgcn_raw_buffer_load_b32(rows, at, 0, 0);
     } else {
-      for (int i = threadIdx.x; i < 512; i += WAVES * 64) {
-        const int m = i >> 5, n = i & 31, at = (n >> 4) * 256 + ((m >> 2) * 16 + (n & 15)) * 4 + (m & 3);
-        float v = 0.f;
+      const uint2_t both = __builtin_bit_cast(uint2_t, __builtin_amdgcn_raw_buffer_load_b64(rows, at, 0, 0));
+      to[0] = both[0], to[1] = both[1];
+    }
+  }
+  __device__ __forceinline__ void put_scales(const unsigned (&from)[kRegs], unsigned char* area) const {
+    const int lane = threadIdx.x & 63;
+    unsigned char* const at = area + (lane >> 1) * 16 + (lane & 1) * kHalf;
+    if constexpr (kPairs) {
+      ((unsigned short*)at)[0] = (unsigned short)from[0];
+      ((unsigned short*)at)[1] = (unsigned short)from[1];
+    } else if constexpr (kHalf == 2) {
+      *(unsigned short*)at = (unsigned short)from[0];
+    } else if constexpr (kHalf == 4) {
+      *(unsigned*)at = from[0];
+    } else {
+      *(uint2_t*)at = uint2_t{from[0], from[1]};
+    }
+  }
+  __device__ __forceinline__ unsigned scale_of(const unsigned char* area, int row, int k) const {  // k of the chunk
+    const unsigned char* const at = area + row * 16 + (k >> W::kShift) * W::kScaleBytes;
+    if constexpr (W::kScaleBytes == 1) return *at;
+    else return *(const unsigned short*)at;
+  }
+
+  // (no condition but by arithmetic: a branch around a load would leave the compiler without its count of those in flight)
+  __device__ __forceinline__ void ask(int u) {
+    const int lane = threadIdx.x & 63;
+    const unsigned never = w_tile < tile_end ? 0u : kNowhere, first = w_tile * tile_bytes + w_c * (kChunk / 2);
+    const int left = a.K - w_c * kChunk;  // k
+    const unsigned beyond = never | ((lane & 7) * 32 < left ? 0u : kNowhere);
+    const unsigned at = (s_at + w_tile * tile_scales + ((unsigned)(w_c * kChunk) >> W::kShift) * W::kScaleBytes) | never | ((lane & 1) * kStep < left ? 0u : kNowhere);
+    ask_scales(s_reg[u], s_rows, at);
+    if constexpr (W::kZeros) ask_scales(z_reg[u], z_rows, at);
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) v += all[w * 512 + at];
-        if (a.Bias != nullptr) v += (float)((const T*)a.Bias)[(size_t)expert * rows + n0 + n];
-        if (r0 + m < end) {
-          const unsigned pair = a.Order[r0 + m];
-          if (pair < (unsigned)a.pairs) a.Parts[(size_t)pair * a.N + n0 + n] = v * a.Weights[pair];
+    for (int i = 0; i < 4; ++i)
+      w_reg[u][i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(w_rows, (w_at[i] + first) | beyond, 0, LINES ? kNontemporal : 0));
+    asm volatile("" ::: "memory");  // (chunk by chunk: loads come back in the order that they go out in)
+    const bool wraps = w_c + 1 == c1;
+    w_tile += wraps ? 1 : 0;
+    w_c = wraps ? c0 : w_c + 1;
+  }
+  // a chunk, c of its tile, out of its registers
+  __device__ __forceinline__ void chunk(int u, int c, float4_t (&acc)[2]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4_t*>(words + word_place(8 * i + (lane >> 3), lane & 7)) = w_reg[u][i];
+    put_scales(s_reg[u], scales);
+    if constexpr (W::kZeros) put_scales(z_reg[u], scales + kScalesArea);
+    asm volatile("" ::: "memory");  // (what is written here other lanes read)
+    ask(u);
+    if (!idle) {
+      // a step's operands are asked for before the first of them is used
+      uint4_t w[2][2];
+      typename W::Scale scale[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          w[h][t] = *reinterpret_cast<const uint4_t*>(words + word_place(16 * t + r, 4 * h + g));
+          const int k = h * kStep + 32 * g;
+          scale[h][t] = W::scale(scale_of(scales, 16 * t + r, k), W::kZeros ? scale_of(scales + kScalesArea, 16 * t + r, k) : 0u);
+        }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        typename W::frag x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const typename W::frag*>(acts + c * (2 * kChunk) + act_place(r, 16 * h + 4 * g + j, acts_stride));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) acc[t] = W::mfma(x[j], W::decode(w[h][t][j], scale[h][t]), acc[t]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    asm volatile("" ::: "memory");
+  }
+};
+
+template <class W>
+__host__ __device__ constexpr int wave_area() {
+  return kWordsArea + kScalesArea * (W::kZeros ? 2 : 1);
+}
+
+// Bytes of a row in LDS: whole chunks
+__host__ __device__ constexpr int acts_stride(int K) { return (K + kChunk - 1) / kChunk * (2 * kChunk); }
+
+// The workgroup's waves but the last are pipelines; the last adds their sums, a tile behind them, and is the only one that waits for
+// anything else than weights while they run (loads come back in the order that they go out in).
+template <class W, bool UP, int DEPTH, bool LINES>
+__global__ __launch_bounds__((kWaves + 1) * 64, DEPTH == 1 ? 4 : 2) void rows_kernel(const Args a, int pass_rows) {
+  using T = typename W::T;
+  extern __shared__ __align__(16) unsigned char smem[];
+  unsigned char* const sums = smem + kWaves * wave_area<W>();
+  unsigned char* const acts = sums + 2 * kWaves * kSumsArea;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c = lane & 15;
+  constexpr int kColumns = UP ? 16 : 32;                            // of the output, in a tile
+  const int rows = (UP ? 2 : 1) * a.N, second = UP ? a.N - 16 : 0;  // (weight row 16 on of a tile: so much further)
+  const unsigned row_bytes = (unsigned)a.K >> 1, row_scales = ((unsigned)a.K >> W::kShift) * W::kScaleBytes;
+  const int tiles_n = a.N / kColumns, stride = acts_stride(a.K);
+  const Parts parts(a, pass_rows);
+  // (fewer than 2^31: the entry point sees to it)
+  const unsigned tiles = (unsigned)parts.count() * tiles_n, share = tiles / gridDim.x, more = tiles % gridDim.x;
+  const unsigned t0 = blockIdx.x * share + min(blockIdx.x, more), t1 = t0 + share + (blockIdx.x < more ? 1 : 0);
+  // which run of the chunks a wave has turns with the workgroup, so that not all ask the same stretch of every row at once; one
+  // that would have none has a chunk that is nothing
+  const int turn = (wave + blockIdx.x) % kWaves, all = (a.K + kChunk - 1) / kChunk;
+  const int c0 = turn * all / kWaves, c1 = max((turn + 1) * all / kWaves, c0 + 1);
+  int done = 0;  // tiles, all waves alike: their sums go into two buffers in turn
+
+  for (unsigned at = t0; at < t1;) {
+    const Part part = parts.nth((int)(at / tiles_n));
+    const int tile0 = (int)(at % tiles_n), tile1 = min(tiles_n, tile0 + (int)(t1 - at));
+    const size_t first = (size_t)part.expert * rows;
+    const int r0 = part.begin, count = part.end - r0;
+    at += tile1 - tile0;
+    {
+      // lane m: row m's pair
+      const unsigned pairs = (unsigned)a.Order[r0 + min(c, count - 1)];
+      if (wave < kWaves) {
+        Pipeline<W, DEPTH, LINES> p{a};
+        p.words = smem + wave * wave_area<W>(), p.scales = p.words + kWordsArea, p.acts = acts, p.acts_stride = stride;
+        p.c0 = p.w_c = c0, p.c1 = c1, p.idle = (turn + 1) * all / kWaves == c0;
+        p.w_tile = p.idle ? tile1 : tile0, p.tile_end = tile1;
+        p.w_rows = bytes_at(a.B + first * row_bytes, (unsigned)rows * row_bytes);
+        p.s_rows = bytes_at((const uint8_t*)a.S + first * row_scales, (unsigned)rows * row_scales);
+        if constexpr (W::kZeros) p.z_rows = bytes_at((const uint8_t*)a.Z + first * row_scales, (unsigned)rows * row_scales);
+        p.tile_bytes = kColumns * row_bytes, p.tile_scales = kColumns * row_scales;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.w_at[i] = (unsigned)(8 * i + (lane >> 3) + (i < 2 ? 0 : second)) * row_bytes + 16 * (lane & 7);
+        p.s_at = (unsigned)((lane >> 1) + (lane < 32 ? 0 : second)) * row_scales + (lane & 1) * Pipeline<W, DEPTH, LINES>::kHalf;
+#pragma unroll
+        for (int u = 0; u < DEPTH; ++u) p.ask(u);
+        // the rows into LDS, a wave a row, zeros beyond K; places of rows that the pass does not have keep what was there: theirs of
+        // the result are not stored
+        for (int m = wave; m < count; m += kWaves) {
+          size_t row = r0 + m;
+          if constexpr (UP) row = min(__builtin_amdgcn_readlane(pairs, m) / (unsigned)a.top_k, (unsigned)a.tokens - 1);
+          const __amdgpu_buffer_rsrc_t x = bytes_at((const T*)a.A + row * a.K, (unsigned)a.K * 2);
+          for (int piece = lane; piece < stride >> 4; piece += 512) {
+            uint4_t v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(x, 16 * piece + 1024 * i, 0, 0));
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (piece + 64 * i < stride >> 4) *reinterpret_cast<uint4_t*>(acts + act_place(m, piece + 64 * i, stride)) = W::order(v[i]);
+          }
+        }
+        __syncthreads();
+        float4_t acc[2] = {};
+        int tile = tile0, at_c = c0;
+        // a tile ends where its last chunk does; one turn is a chunk of each set of registers, the last turn's spare ones are nothing
+        auto chunk = [&](int u) {
+          p.chunk(u, at_c, acc);
+          if (++at_c == c1) {
+            at_c = c0;
+            if (tile < tile1) {
+              float4_t* const to = (float4_t*)(sums + ((done & 1) * kWaves + wave) * kSumsArea);  // [block of 16][lane]
+              to[lane] = acc[0];
+              to[64 + lane] = acc[1];
+              acc[0] = acc[1] = float4_t{};
+              ++tile;
+              ++done;
+              __syncthreads();
+            }
+          }
+        };
+        const int turns = ((tile1 - tile0) * (c1 - c0) + DEPTH - 1) / DEPTH;
+        for (int i = 0; i < turns; ++i) {
+#pragma unroll
+          for (int u = 0; u < DEPTH; ++u) chunk(u);
+        }
+      } else {
+        // lane: column c of either block of 16, rows 4 g .. 4 g + 3
+        float weight[4];
+        unsigned pair[4];
+        if constexpr (!UP) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            pair[i] = __shfl(pairs, 4 * g + i, 64);
+            weight[i] = a.Weights[min(pair[i], (unsigned)a.pairs - 1)];
+          }
+        }
+        const T* const bias = a.Bias == nullptr ? nullptr : (const T*)a.Bias + first + c;
+        // (a tile's bias is asked for ahead of the stores of the tile before)
+        T ahead[2] = {};
+        if (bias != nullptr) ahead[0] = bias[tile0 * kColumns], ahead[1] = bias[tile0 * kColumns + 16 + second];
+        __syncthreads();
+        for (int tile = tile0; tile < tile1; ++tile) {
+          const float b[2] = {(float)ahead[0], (float)ahead[1]};
+          const int next = min(tile + 1, tile1 - 1) * kColumns;
+          if (bias != nullptr) ahead[0] = bias[next], ahead[1] = bias[next + 16 + second];
+          __syncthreads();
+          const float4_t* const from = (const float4_t*)(sums + (done++ & 1) * kWaves * kSumsArea);
+          float4_t part[kWaves][2];
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) part[w][0] = from[w * 128 + lane], part[w][1] = from[w * 128 + 64 + lane];
+          __builtin_amdgcn_sched_barrier(0);
+          float4_t v[2] = {part[0][0], part[0][1]};
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w) v[0] += part[w][0], v[1] += part[w][1];
+          const size_t n = (size_t)tile * kColumns + c;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (4 * g + i >= count) continue;
+            if constexpr (UP) {
+              ((T*)a.Out)[(size_t)(r0 + 4 * g + i) * a.N + n] = (T)(experts::activate(v[0][i] + b[0], a.gelu) * (v[1][i] + b[1]));
+            } else if (pair[i] < (unsigned)a.pairs) {
+              float* const to = a.Parts + (size_t)pair[i] * a.N + n;
+              to[0] = (v[0][i] + b[0]) * weight[i];
+              to[16] = (v[1][i] + b[1]) * weight[i];
+            }
+          }
         }
       }
     }
@@ -156,18 +406,47 @@ int sum(const Args& a, hipStream_t stream) {
   return 0;
 }
 
+// Bytes of LDS of a workgroup beside the rows that it holds
+template <class W>
+constexpr int pipes_area() {
+  return kWaves * (wave_area<W>() + 2 * kSumsArea);
+}
+
+template <class W, bool UP, int DEPTH, bool LINES>
+int launch_rows(const Args& a, int pass_rows, int workgroups, hipStream_t stream) {
+  constexpr int kMost = 160 * 1024 / (DEPTH == 1 ? 2 : 1);
+  auto kern = rows_kernel<W, UP, DEPTH, LINES>;
+  static bool raised[kMaxDevices];
+  if (raise_lds_limit<kMost>(kern, raised)) return -1;
+  hipLaunchKernelGGL(kern, dim3(workgroups), dim3((kWaves + 1) * 64), pipes_area<W>() + pass_rows * acts_stride(a.K), stream, a, pass_rows);
+  DQ_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+// Two workgroups a CU, each a chunk ahead, where what an expert is likely to have of rows leaves room for that (us, against one
+// workgroup that is two chunks ahead: one token, 8 of 128 experts, 1024 x 4096 10.5 and 11.7; 24 tokens, 4 of 64, 2048 x 1024 19.7 and
+// 25.8); else one, with as many rows as it can hold (64 tokens, 4 of 32, 2880 x 2880 MXFP4: 69.6 and 74.5).
 template <class W, bool UP>
 int product(const Args& a, hipStream_t stream) {
-  constexpr int kWaves = 4;
-  const int most = a.experts < a.pairs ? a.experts : a.pairs;  // experts that can have rows
-  hipLaunchKernelGGL((rows_kernel<W, UP, kWaves>), dim3(a.N / (UP ? 16 : 32), most), dim3(kWaves * 64), 0, stream, a);
-  DQ_CHECK_HIP(hipGetLastError());
+  const int stride = acts_stride(a.K), mean = a.pairs / std::min(a.experts, a.pairs);
+  const int both = (80 * 1024 - pipes_area<W>()) / stride, alone = (160 * 1024 - pipes_area<W>()) / stride;
+  const int likely = std::min(std::min(16, a.tokens), 3 * mean + 4);
+  const bool two = likely <= both;
+  const int pass_rows = std::min(std::min(16, a.tokens), two ? both : alone);
+  // tiles that there can be
+  const long most = (long)(a.pairs / pass_rows + std::min(a.experts, a.pairs)) * (a.N / (UP ? 16 : 32));
+  const int workgroups = (int)std::min(most, two ? 512l : 256l);
+  int rc;
+  if (a.K % kChunk == 0) rc = two ? launch_rows<W, UP, 1, true>(a, pass_rows, workgroups, stream) : launch_rows<W, UP, 2, true>(a, pass_rows, workgroups, stream);
+  else rc = two ? launch_rows<W, UP, 1, false>(a, pass_rows, workgroups, stream) : launch_rows<W, UP, 2, false>(a, pass_rows, workgroups, stream);
+  if (rc != 0) return rc;
   if constexpr (!UP) return sum<typename W::T>(a, stream);
   return 0;
 }
 
 // Rows of a tile of the matrix pipe's kernel, or 0: few rows an expert.
 int tile_rows(const Args& a, int mxfp4) {
+  if (acts_stride(a.K) > kActsRoom) return 128;  // (a row does not fit)
   if (a.K < 128) return 0;
   const long mean = a.pairs / (a.experts < a.pairs ? a.experts : a.pairs);
   if (mean < 48) return 0;
@@ -183,7 +462,9 @@ int by_format(const Args& a, int mxfp4, hipStream_t stream) {
     return 0;
   }
   if (mxfp4) return product<experts::Mxfp4, UP>(a, stream);
-  return a.Z != nullptr ? product<experts::Uint4<true>, UP>(a, stream) : product<experts::Uint4<false>, UP>(a, stream);
+#define DQ_UINT4(SHIFT_) (a.Z != nullptr ? product<experts::Uint4<true, SHIFT_>, UP>(a, stream) : product<experts::Uint4<false, SHIFT_>, UP>(a, stream))
+  return a.group_shift == 5 ? DQ_UINT4(5) : a.group_shift == 6 ? DQ_UINT4(6) : DQ_UINT4(7);
+#undef DQ_UINT4
 }
 
 }  // namespace
