@@ -121,26 +121,85 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t bytes_at(const void* p, unsign
 __device__ __forceinline__ int word_place(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) << 4); }
 __device__ __forceinline__ int act_place(int row, int piece, int stride) { return row * stride + ((piece ^ (row & 15)) << 4); }
 
-// A wave's part of the products of some rows of one expert, which lie in LDS, with a run of tiles of 32 weight rows: of every tile the
-// chunks c0 .. c1 - 1.  The chunks of all tiles are one sequence, whose weights are asked for DEPTH chunks ahead.  A load that is of
-// no use (behind the sequence, beyond K) names an offset beyond its descriptor's bytes, which reads zeros.
+constexpr unsigned kNowhere = 0xFFFFFF00u;  // an offset beyond the bytes of any descriptor
+
+// What a lane's half of a chunk's scales is, a step's: bytes, and from where
+template <class W>
+__host__ __device__ constexpr int half_scales() {
+  return (kStep >> W::kShift) * W::kScaleBytes;  // 2, 4 or 8
+}
+
+// Where a pipeline's two blocks of 16 weight rows come from, by their number in its sequence.
+// Of one expert: tile after tile of its columns.
+template <class W>
+struct TilesOf {
+  const uint8_t* words;
+  size_t tile_bytes, second_bytes;  // of words; to the second block
+  __amdgpu_buffer_rsrc_t scales, zeros;
+  unsigned lane_scales, tile_scales;
+  int end;
+
+  __device__ __forceinline__ TilesOf(const Args& a, int expert, int rows, int columns, int second, int end_) : end(end_) {
+    const int lane = threadIdx.x & 63;
+    const unsigned row_bytes = (unsigned)a.K >> 1, row_scales = ((unsigned)a.K >> W::kShift) * W::kScaleBytes;
+    const size_t first = (size_t)expert * rows;
+    words = a.B + first * row_bytes;
+    tile_bytes = (size_t)columns * row_bytes, second_bytes = (size_t)second * row_bytes;
+    scales = bytes_at((const uint8_t*)a.S + first * row_scales, (unsigned)rows * row_scales);
+    if constexpr (W::kZeros) zeros = bytes_at((const uint8_t*)a.Z + first * row_scales, (unsigned)rows * row_scales);
+    lane_scales = (unsigned)((lane >> 1) + (lane < 32 ? 0 : second - 16)) * row_scales + (lane & 1) * half_scales<W>();
+    tile_scales = columns * row_scales;
+  }
+  __device__ __forceinline__ const uint8_t* block(int tile, int t) const { return words + tile * tile_bytes + t * second_bytes; }
+  __device__ __forceinline__ bool on(int tile, int) const { return tile < end; }
+  __device__ __forceinline__ unsigned scale_at(int tile) const { return tile < end ? lane_scales + tile * tile_scales : kNowhere; }
+};
+
+// Of several experts the same 16 columns, two experts at a time.
+template <class W>
+struct ExpertsOf {
+  const uint8_t* words;
+  unsigned expert_scales, lane_scales;
+  size_t expert_bytes;
+  __amdgpu_buffer_rsrc_t scales, zeros;
+  int experts, count;  // experts: lane i has the i-th
+
+  __device__ __forceinline__ ExpertsOf(const Args& a, int n0, int experts_, int count_) : experts(experts_), count(count_) {
+    const int lane = threadIdx.x & 63;
+    const unsigned row_bytes = (unsigned)a.K >> 1, row_scales = ((unsigned)a.K >> W::kShift) * W::kScaleBytes;
+    words = a.B + (size_t)n0 * row_bytes;
+    expert_bytes = (size_t)a.N * row_bytes, expert_scales = (unsigned)a.N * row_scales;
+    scales = bytes_at(a.S, (unsigned)a.experts * expert_scales);
+    if constexpr (W::kZeros) zeros = bytes_at(a.Z, (unsigned)a.experts * expert_scales);
+    lane_scales = (unsigned)(n0 + ((lane >> 1) & 15)) * row_scales + (lane & 1) * half_scales<W>();
+  }
+  __device__ __forceinline__ int expert(int q, int t) const { return __builtin_amdgcn_readlane(experts, min(2 * q + t, count - 1)); }
+  __device__ __forceinline__ const uint8_t* block(int q, int t) const { return words + expert(q, t) * expert_bytes; }
+  __device__ __forceinline__ bool on(int q, int t) const { return 2 * q + t < count; }
+  __device__ __forceinline__ unsigned scale_at(int q) const {
+    const int t = (threadIdx.x & 63) >> 5;
+    return 2 * q + t < count ? lane_scales + (unsigned)(t ? expert(q, 1) : expert(q, 0)) * expert_scales : kNowhere;
+  }
+};
+
+// A wave's part of the products of some rows, which lie in LDS, with pairs of blocks of 16 weight rows, one pair after the other: of
+// each the chunks c0 .. c1 - 1.  The chunks of all pairs are one sequence, whose weights are asked for DEPTH chunks ahead.  A load that is
+// of no use (behind the sequence, beyond K) names an offset beyond its descriptor's bytes, which reads zeros.
 // LINES: rows are whole cache lines, which are read once (nontemporal); otherwise two chunks share a line, and the one that comes second
 // is to find it in a cache.
-template <class W, int DEPTH, bool LINES>
+template <class W, int DEPTH, bool LINES, class Source>
 struct Pipeline {
-  static constexpr unsigned kNowhere = 0xFFFFFF00u;
   const Args& a;
-  __amdgpu_buffer_rsrc_t w_rows, s_rows, z_rows;
-  unsigned w_at[4], s_at, tile_bytes, tile_scales;
-  int c0, c1, tile_end;
-  int w_tile, w_c;  // what is asked for next
+  const Source& from;
+  unsigned w_at[2];
+  int c0, c1;
+  int w_q, w_c;  // what is asked for next
   bool idle;
   unsigned char *words, *scales;
   const unsigned char* acts;
   int acts_stride;
   uint4_t w_reg[DEPTH][4];
-  // a lane's half of the chunk's scales of its row (lane / 2): those of a step
-  static constexpr int kHalf = (kStep >> W::kShift) * W::kScaleBytes;  // bytes: 2, 4 or 8
+  static constexpr int kHalf = half_scales<W>();
   static constexpr bool kPairs = W::kScaleBytes == 1 && !LINES;       // from where two bytes lie, not four
   static constexpr int kRegs = kHalf == 8 || kPairs ? 2 : 1;
   unsigned s_reg[DEPTH][kRegs], z_reg[DEPTH][kRegs];
@@ -178,24 +237,37 @@ struct Pipeline {
     else return *(const unsigned short*)at;
   }
 
+  __device__ __forceinline__ Pipeline(const Args& args, const Source& source, int first, int begin, int end, bool nothing, unsigned char* area,
+                                      const unsigned char* rows, int stride)
+      : a(args), from(source), c0(begin), c1(end), w_q(first), w_c(begin), idle(nothing), words(area), scales(area + kWordsArea), acts(rows), acts_stride(stride) {
+    const int lane = threadIdx.x & 63;
+    const unsigned row_bytes = (unsigned)a.K >> 1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w_at[i] = (unsigned)(8 * i + (lane >> 3)) * row_bytes + 16 * (lane & 7);
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) ask(u);
+  }
+
   // (no condition but by arithmetic: a branch around a load would leave the compiler without its count of those in flight)
   __device__ __forceinline__ void ask(int u) {
-    const int lane = threadIdx.x & 63;
-    const unsigned never = w_tile < tile_end ? 0u : kNowhere, first = w_tile * tile_bytes + w_c * (kChunk / 2);
-    const int left = a.K - w_c * kChunk;  // k
-    const unsigned beyond = never | ((lane & 7) * 32 < left ? 0u : kNowhere);
-    const unsigned at = (s_at + w_tile * tile_scales + ((unsigned)(w_c * kChunk) >> W::kShift) * W::kScaleBytes) | never | ((lane & 1) * kStep < left ? 0u : kNowhere);
-    ask_scales(s_reg[u], s_rows, at);
-    if constexpr (W::kZeros) ask_scales(z_reg[u], z_rows, at);
+    const int lane = threadIdx.x & 63, left = a.K - w_c * kChunk;  // k
+    const unsigned at = (from.scale_at(w_q) + ((unsigned)(w_c * kChunk) >> W::kShift) * W::kScaleBytes) | (!idle && (lane & 1) * kStep < left ? 0u : kNowhere);
+    ask_scales(s_reg[u], from.scales, at);
+    if constexpr (W::kZeros) ask_scales(z_reg[u], from.zeros, at);
+    const unsigned beyond = (lane & 7) * 32 < left ? 0u : kNowhere, bytes = 8u * (unsigned)a.K;  // 16 rows
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w_reg[u][i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(w_rows, (w_at[i] + first) | beyond, 0, LINES ? kNontemporal : 0));
+    for (int t = 0; t < 2; ++t) {
+      const __amdgpu_buffer_rsrc_t rows = bytes_at(from.block(w_q, t), !idle && from.on(w_q, t) ? bytes : 0u);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        w_reg[u][2 * t + i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(rows, (w_at[i] + w_c * (kChunk / 2)) | beyond, 0, LINES ? kNontemporal : 0));
+    }
     asm volatile("" ::: "memory");  // (chunk by chunk: loads come back in the order that they go out in)
     const bool wraps = w_c + 1 == c1;
-    w_tile += wraps ? 1 : 0;
+    w_q += wraps ? 1 : 0;
     w_c = wraps ? c0 : w_c + 1;
   }
-  // a chunk, c of its tile, out of its registers
+  // a chunk, c of its pair of blocks, out of its registers
   __device__ __forceinline__ void chunk(int u, int c, float4_t (&acc)[2]) {
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
 #pragma unroll
@@ -241,6 +313,75 @@ __host__ __device__ constexpr int wave_area() {
 // Bytes of a row in LDS: whole chunks
 __host__ __device__ constexpr int acts_stride(int K) { return (K + kChunk - 1) / kChunk * (2 * kChunk); }
 
+// A row of K activations into LDS, by one wave, zeros beyond K
+template <class W>
+__device__ __forceinline__ void put_row(const Args& a, size_t row, unsigned char* acts, int m, int stride) {
+  const __amdgpu_buffer_rsrc_t x = bytes_at((const typename W::T*)a.A + row * a.K, (unsigned)a.K * 2);
+  for (int piece = threadIdx.x & 63; piece < stride >> 4; piece += 512) {
+    uint4_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(x, 16 * piece + 1024 * i, 0, 0));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (piece + 64 * i < stride >> 4) *reinterpret_cast<uint4_t*>(acts + act_place(m, piece + 64 * i, stride)) = W::order(v[i]);
+  }
+}
+
+// A wave's chunks of a pair of blocks.  Which run of them a wave has turns with the workgroup, so that not all ask the same stretch of
+// every row at once; one that would have none has a chunk that is nothing.
+struct Share {
+  int c0, c1;
+  bool idle;
+  __device__ __forceinline__ Share(const Args& a, int wave) {
+    const int turn = (wave + blockIdx.x) % kWaves, all = (a.K + kChunk - 1) / kChunk;
+    c0 = turn * all / kWaves, c1 = (turn + 1) * all / kWaves;
+    idle = c0 == c1;
+    if (idle) ++c1;
+  }
+};
+
+// All of a pipeline's sequence, `blocks` pairs of blocks: a pair ends where its last chunk does, with the wave's sums in one of two
+// buffers and a barrier.  One turn is a chunk of each set of registers; the last turn's spare ones are nothing.
+template <int DEPTH, class P>
+__device__ __forceinline__ void run(P& p, int blocks, unsigned char* sums, int wave, int& done) {
+  const int lane = threadIdx.x & 63;
+  float4_t acc[2] = {};
+  int c = p.c0, left = blocks;
+  auto chunk = [&](int u) {
+    p.chunk(u, c, acc);
+    if (++c == p.c1) {
+      c = p.c0;
+      if (left > 0) {
+        float4_t* const to = (float4_t*)(sums + ((done & 1) * kWaves + wave) * kSumsArea);  // [block][lane]
+        to[lane] = acc[0];
+        to[64 + lane] = acc[1];
+        acc[0] = acc[1] = float4_t{};
+        --left;
+        ++done;
+        __syncthreads();
+      }
+    }
+  };
+  const int turns = (blocks * (p.c1 - p.c0) + DEPTH - 1) / DEPTH;
+  for (int i = 0; i < turns; ++i) {
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) chunk(u);
+  }
+}
+
+// The waves' sums of a pair of blocks: lane (g, c) has column c of either, rows 4 g .. 4 g + 3
+__device__ __forceinline__ void add_up(const unsigned char* sums, int done, float4_t (&v)[2]) {
+  const int lane = threadIdx.x & 63;
+  const float4_t* const from = (const float4_t*)(sums + (done & 1) * kWaves * kSumsArea);
+  float4_t part[kWaves][2];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) part[w][0] = from[w * 128 + lane], part[w][1] = from[w * 128 + 64 + lane];
+  __builtin_amdgcn_sched_barrier(0);
+  v[0] = part[0][0], v[1] = part[0][1];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) v[0] += part[w][0], v[1] += part[w][1];
+}
+
 // The workgroup's waves but the last are pipelines; the last adds their sums, a tile behind them, and is the only one that waits for
 // anything else than weights while they run (loads come back in the order that they go out in).
 template <class W, bool UP, int DEPTH, bool LINES>
@@ -251,122 +392,66 @@ __global__ __launch_bounds__((kWaves + 1) * 64, DEPTH == 1 ? 4 : 2) void rows_ke
   unsigned char* const acts = sums + 2 * kWaves * kSumsArea;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
-  constexpr int kColumns = UP ? 16 : 32;                            // of the output, in a tile
-  const int rows = (UP ? 2 : 1) * a.N, second = UP ? a.N - 16 : 0;  // (weight row 16 on of a tile: so much further)
-  const unsigned row_bytes = (unsigned)a.K >> 1, row_scales = ((unsigned)a.K >> W::kShift) * W::kScaleBytes;
+  constexpr int kColumns = UP ? 16 : 32;                       // of the output, in a tile
+  const int rows = (UP ? 2 : 1) * a.N, second = UP ? a.N : 16;  // weight rows of an expert; from a tile's first block to its second
   const int tiles_n = a.N / kColumns, stride = acts_stride(a.K);
   const Parts parts(a, pass_rows);
-  // (fewer than 2^31: the entry point sees to it)
+  // (fewer than 2^31: the launch sees to it)
   const unsigned tiles = (unsigned)parts.count() * tiles_n, share = tiles / gridDim.x, more = tiles % gridDim.x;
   const unsigned t0 = blockIdx.x * share + min(blockIdx.x, more), t1 = t0 + share + (blockIdx.x < more ? 1 : 0);
-  // which run of the chunks a wave has turns with the workgroup, so that not all ask the same stretch of every row at once; one
-  // that would have none has a chunk that is nothing
-  const int turn = (wave + blockIdx.x) % kWaves, all = (a.K + kChunk - 1) / kChunk;
-  const int c0 = turn * all / kWaves, c1 = max((turn + 1) * all / kWaves, c0 + 1);
+  const Share chunks(a, wave);
   int done = 0;  // tiles, all waves alike: their sums go into two buffers in turn
 
   for (unsigned at = t0; at < t1;) {
     const Part part = parts.nth((int)(at / tiles_n));
     const int tile0 = (int)(at % tiles_n), tile1 = min(tiles_n, tile0 + (int)(t1 - at));
-    const size_t first = (size_t)part.expert * rows;
     const int r0 = part.begin, count = part.end - r0;
     at += tile1 - tile0;
-    {
-      // lane m: row m's pair
-      const unsigned pairs = (unsigned)a.Order[r0 + min(c, count - 1)];
-      if (wave < kWaves) {
-        Pipeline<W, DEPTH, LINES> p{a};
-        p.words = smem + wave * wave_area<W>(), p.scales = p.words + kWordsArea, p.acts = acts, p.acts_stride = stride;
-        p.c0 = p.w_c = c0, p.c1 = c1, p.idle = (turn + 1) * all / kWaves == c0;
-        p.w_tile = p.idle ? tile1 : tile0, p.tile_end = tile1;
-        p.w_rows = bytes_at(a.B + first * row_bytes, (unsigned)rows * row_bytes);
-        p.s_rows = bytes_at((const uint8_t*)a.S + first * row_scales, (unsigned)rows * row_scales);
-        if constexpr (W::kZeros) p.z_rows = bytes_at((const uint8_t*)a.Z + first * row_scales, (unsigned)rows * row_scales);
-        p.tile_bytes = kColumns * row_bytes, p.tile_scales = kColumns * row_scales;
+    // lane m: row m's pair
+    const unsigned pairs = (unsigned)a.Order[r0 + min(c, count - 1)];
+    if (wave < kWaves) {
+      const TilesOf<W> source(a, part.expert, rows, kColumns, second, tile1);
+      Pipeline<W, DEPTH, LINES, TilesOf<W>> p(a, source, tile0, chunks.c0, chunks.c1, chunks.idle, smem + wave * wave_area<W>(), acts, stride);
+      // a wave a row; places of rows that the part does not have keep what was there: theirs of the result are not stored
+      for (int m = wave; m < count; m += kWaves) {
+        size_t row = r0 + m;
+        if constexpr (UP) row = min(__builtin_amdgcn_readlane(pairs, m) / (unsigned)a.top_k, (unsigned)a.tokens - 1);
+        put_row<W>(a, row, acts, m, stride);
+      }
+      __syncthreads();
+      run<DEPTH>(p, tile1 - tile0, sums, wave, done);
+    } else {
+      float weight[4];
+      unsigned pair[4];
+      if constexpr (!UP) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p.w_at[i] = (unsigned)(8 * i + (lane >> 3) + (i < 2 ? 0 : second)) * row_bytes + 16 * (lane & 7);
-        p.s_at = (unsigned)((lane >> 1) + (lane < 32 ? 0 : second)) * row_scales + (lane & 1) * Pipeline<W, DEPTH, LINES>::kHalf;
-#pragma unroll
-        for (int u = 0; u < DEPTH; ++u) p.ask(u);
-        // the rows into LDS, a wave a row, zeros beyond K; places of rows that the pass does not have keep what was there: theirs of
-        // the result are not stored
-        for (int m = wave; m < count; m += kWaves) {
-          size_t row = r0 + m;
-          if constexpr (UP) row = min(__builtin_amdgcn_readlane(pairs, m) / (unsigned)a.top_k, (unsigned)a.tokens - 1);
-          const __amdgpu_buffer_rsrc_t x = bytes_at((const T*)a.A + row * a.K, (unsigned)a.K * 2);
-          for (int piece = lane; piece < stride >> 4; piece += 512) {
-            uint4_t v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(x, 16 * piece + 1024 * i, 0, 0));
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (piece + 64 * i < stride >> 4) *reinterpret_cast<uint4_t*>(acts + act_place(m, piece + 64 * i, stride)) = W::order(v[i]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          pair[i] = __shfl(pairs, 4 * g + i, 64);
+          weight[i] = a.Weights[min(pair[i], (unsigned)a.pairs - 1)];
         }
+      }
+      const T* const bias = a.Bias == nullptr ? nullptr : (const T*)a.Bias + (size_t)part.expert * rows + c;
+      // (a tile's bias is asked for ahead of the stores of the tile before)
+      T ahead[2] = {};
+      if (bias != nullptr) ahead[0] = bias[tile0 * kColumns], ahead[1] = bias[tile0 * kColumns + second];
+      __syncthreads();
+      for (int tile = tile0; tile < tile1; ++tile) {
+        const float b[2] = {(float)ahead[0], (float)ahead[1]};
+        const int next = min(tile + 1, tile1 - 1) * kColumns;
+        if (bias != nullptr) ahead[0] = bias[next], ahead[1] = bias[next + second];
         __syncthreads();
-        float4_t acc[2] = {};
-        int tile = tile0, at_c = c0;
-        // a tile ends where its last chunk does; one turn is a chunk of each set of registers, the last turn's spare ones are nothing
-        auto chunk = [&](int u) {
-          p.chunk(u, at_c, acc);
-          if (++at_c == c1) {
-            at_c = c0;
-            if (tile < tile1) {
-              float4_t* const to = (float4_t*)(sums + ((done & 1) * kWaves + wave) * kSumsArea);  // [block of 16][lane]
-              to[lane] = acc[0];
-              to[64 + lane] = acc[1];
-              acc[0] = acc[1] = float4_t{};
-              ++tile;
-              ++done;
-              __syncthreads();
-            }
-          }
-        };
-        const int turns = ((tile1 - tile0) * (c1 - c0) + DEPTH - 1) / DEPTH;
-        for (int i = 0; i < turns; ++i) {
+        float4_t v[2];
+        add_up(sums, done++, v);
+        const size_t n = (size_t)tile * kColumns + c;
 #pragma unroll
-          for (int u = 0; u < DEPTH; ++u) chunk(u);
-        }
-      } else {
-        // lane: column c of either block of 16, rows 4 g .. 4 g + 3
-        float weight[4];
-        unsigned pair[4];
-        if constexpr (!UP) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            pair[i] = __shfl(pairs, 4 * g + i, 64);
-            weight[i] = a.Weights[min(pair[i], (unsigned)a.pairs - 1)];
-          }
-        }
-        const T* const bias = a.Bias == nullptr ? nullptr : (const T*)a.Bias + first + c;
-        // (a tile's bias is asked for ahead of the stores of the tile before)
-        T ahead[2] = {};
-        if (bias != nullptr) ahead[0] = bias[tile0 * kColumns], ahead[1] = bias[tile0 * kColumns + 16 + second];
-        __syncthreads();
-        for (int tile = tile0; tile < tile1; ++tile) {
-          const float b[2] = {(float)ahead[0], (float)ahead[1]};
-          const int next = min(tile + 1, tile1 - 1) * kColumns;
-          if (bias != nullptr) ahead[0] = bias[next], ahead[1] = bias[next + 16 + second];
-          __syncthreads();
-          const float4_t* const from = (const float4_t*)(sums + (done++ & 1) * kWaves * kSumsArea);
-          float4_t part[kWaves][2];
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) part[w][0] = from[w * 128 + lane], part[w][1] = from[w * 128 + 64 + lane];
-          __builtin_amdgcn_sched_barrier(0);
-          float4_t v[2] = {part[0][0], part[0][1]};
-#pragma unroll
-          for (int w = 1; w < kWaves; ++w) v[0] += part[w][0], v[1] += part[w][1];
-          const size_t n = (size_t)tile * kColumns + c;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (4 * g + i >= count) continue;
-            if constexpr (UP) {
-              ((T*)a.Out)[(size_t)(r0 + 4 * g + i) * a.N + n] = (T)(experts::activate(v[0][i] + b[0], a.gelu) * (v[1][i] + b[1]));
-            } else if (pair[i] < (unsigned)a.pairs) {
-              float* const to = a.Parts + (size_t)pair[i] * a.N + n;
-              to[0] = (v[0][i] + b[0]) * weight[i];
-              to[16] = (v[1][i] + b[1]) * weight[i];
-            }
+        for (int i = 0; i < 4; ++i) {
+          if (4 * g + i >= count) continue;
+          if constexpr (UP) {
+            ((T*)a.Out)[(size_t)(r0 + 4 * g + i) * a.N + n] = (T)(experts::activate(v[0][i] + b[0], a.gelu) * (v[1][i] + b[1]));
+          } else if (pair[i] < (unsigned)a.pairs) {
+            float* const to = a.Parts + (size_t)pair[i] * a.N + n;
+            to[0] = (v[0][i] + b[0]) * weight[i];
+            to[16] = (v[1][i] + b[1]) * weight[i];
           }
         }
       }
@@ -374,34 +459,129 @@ __global__ __launch_bounds__((kWaves + 1) * 64, DEPTH == 1 ? 4 : 2) void rows_ke
   }
 }
 
-// A token's pairs added, in the order of its choices, onto the residual.
+// "Down" for up to eight pairs, with nothing between the products and the tokens' sums: a workgroup has 16 columns of all experts that
+// have rows, two experts at a time, and all rows as those of its matrix instructions.  An expert's sums of other experts' rows are
+// left; every row's own are kept by the adding wave, and the tokens' sums, in the order of their choices, are its last step.
+constexpr int kFewPairs = 8;
+
+template <class W, bool LINES>
+__global__ __launch_bounds__((kWaves + 1) * 64, 4) void few_pairs_kernel(const Args a) {
+  using T = typename W::T;
+  extern __shared__ __align__(16) unsigned char smem[];
+  unsigned char* const sums = smem + kWaves * wave_area<W>();
+  unsigned char* const acts = sums + 2 * kWaves * kSumsArea;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c = lane & 15, n0 = blockIdx.x * 16, stride = acts_stride(a.K);
+  // the experts that have rows, the i-th in lane i
+  int experts = 0, begins = 0, ends = 0, count = 0;
+  Parts(a, 16).each([&](int base, int b, int e) {
+    const unsigned long long has = __ballot(e > b);
+    if (has == 0) return false;
+    const int rank = count + __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
+    const int here = __popcll(has), to = (e > b && rank < 16 ? rank : 63) * 4;  // (lane 63 takes what is nobody's)
+    const int x = __builtin_amdgcn_ds_permute(to, base + lane), y = __builtin_amdgcn_ds_permute(to, b), z = __builtin_amdgcn_ds_permute(to, e);
+    if (lane >= count && lane < min(count + here, 16)) experts = x, begins = y, ends = z;
+    count = min(count + here, 16);
+    return false;
+  });
+  const int rows = count > 0 ? __builtin_amdgcn_readlane(ends, count - 1) : 0;
+  const int blocks = (count + 1) / 2;
+  int done = 0;
+  if (wave < kWaves) {
+    const Share chunks(a, wave);
+    const ExpertsOf<W> source(a, n0, experts, max(count, 1));
+    Pipeline<W, 1, LINES, ExpertsOf<W>> p(a, source, 0, chunks.c0, chunks.c1, chunks.idle || count == 0, smem + wave * wave_area<W>(), acts, stride);
+    for (int m = wave; m < rows; m += kWaves) put_row<W>(a, m, acts, m, stride);
+    __syncthreads();
+    run<1>(p, blocks, sums, wave, done);
+  } else {
+    // (asked for now, for the last step)
+    float residual[4] = {0.f, 0.f, 0.f, 0.f};  // of tokens g, g + 4, ...
+    if (a.Residual != nullptr)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) residual[i] = (float)((const T*)a.Residual)[(size_t)min(g + 4 * i, a.tokens - 1) * a.N + n0 + c];
+    const int pair = a.Order[min(c, a.pairs - 1)];
+    const float weight = a.Weights[min((unsigned)pair, (unsigned)a.pairs - 1)];
+    const T* const bias = a.Bias == nullptr ? nullptr : (const T*)a.Bias + n0 + c;
+    auto bias_of = [&](int q, int t) { return bias[(size_t)__builtin_amdgcn_readlane(experts, min(2 * q + t, count - 1)) * a.N]; };
+    T ahead[2] = {};
+    if (bias != nullptr && count > 0) ahead[0] = bias_of(0, 0), ahead[1] = bias_of(0, 1);
+    __syncthreads();
+    float own[4] = {0.f, 0.f, 0.f, 0.f};  // row 4 g + i, column c
+    for (int q = 0; q < blocks; ++q) {
+      const float b[2] = {(float)ahead[0], (float)ahead[1]};
+      if (bias != nullptr) ahead[0] = bias_of(q + 1, 0), ahead[1] = bias_of(q + 1, 1);
+      __syncthreads();
+      float4_t v[2];
+      add_up(sums, done++, v);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (2 * q + t >= count) break;
+        const int first = __builtin_amdgcn_readlane(begins, 2 * q + t), last = __builtin_amdgcn_readlane(ends, 2 * q + t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * g + i >= first && 4 * g + i < last) own[i] = v[t][i] + b[t];
+      }
+    }
+    // rows to tokens, where the sums were: the last of them are read, and no pipeline writes more
+    float* const values = (float*)sums;  // [pair][column]
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) values[(4 * g + i) * 16 + c] = 0.f;
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 4 * g + i;
+      const unsigned to = (unsigned)__shfl(pair, row, 64);
+      const float w = __shfl(weight, row, 64);
+      if (row < rows && to < (unsigned)a.pairs) values[to * 16 + c] = own[i] * w;
+    }
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int token = g + 4 * i;
+      if (token >= a.tokens) break;
+      float sum = 0.f;
+      for (int j = 0; j < a.top_k; ++j) sum += values[(token * a.top_k + j) * 16 + c];
+      ((T*)a.Out)[(size_t)token * a.N + n0 + c] = (T)(sum + residual[i]);
+    }
+  }
+}
+
+// A token's pairs added, in the order of its choices, onto the residual: four columns a thread, eight choices asked for at once.
 template <class T>
 __global__ __launch_bounds__(256) void sum_kernel(const Args a) {
   typedef T vec4 __attribute__((ext_vector_type(4)));
-  const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  const size_t token = at / a.N;
-  const int n = (int)(at - token * a.N);
-  if (token >= (size_t)a.tokens) return;
+  const size_t token = (size_t)blockIdx.z * gridDim.y + blockIdx.y;
+  const int n = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
+  if (n >= a.N || token >= (size_t)a.tokens) return;
+  const size_t at = token * a.N + n;
+  vec4 r = {};
+  if (a.Residual != nullptr) r = *reinterpret_cast<const vec4*>((const T*)a.Residual + at);
   float4_t v = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < a.top_k; ++j) {
-    const size_t pair = token * a.top_k + j;
-    if ((unsigned)a.Ids[pair] - (unsigned)a.first < (unsigned)a.experts) v += *reinterpret_cast<const float4_t*>(a.Parts + pair * a.N + n);
-  }
-  if (a.Residual != nullptr) {
-    const vec4 r = *reinterpret_cast<const vec4*>((const T*)a.Residual + at);
+  for (int j0 = 0; j0 < a.top_k; j0 += 8) {
+    float4_t part[8];
+    unsigned id[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += (float)r[i];
+    for (int j = 0; j < 8; ++j) {
+      const size_t pair = token * a.top_k + min(j0 + j, a.top_k - 1);
+      id[j] = (unsigned)a.Ids[pair] - (unsigned)a.first;
+      part[j] = *reinterpret_cast<const float4_t*>(a.Parts + pair * a.N + n);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j0 + j < a.top_k && id[j] < (unsigned)a.experts) v += part[j];  // (nobody has written another's)
   }
   vec4 o;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = (T)v[i];
+  for (int i = 0; i < 4; ++i) o[i] = (T)(v[i] + (float)r[i]);
   *reinterpret_cast<vec4*>((T*)a.Out + at) = o;
 }
 
 template <class T>
 int sum(const Args& a, hipStream_t stream) {
-  const size_t threads = (size_t)a.tokens * a.N / 4;
-  hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a);
+  const int threads = a.N >= 1024 ? 256 : 64, tokens = std::min(a.tokens, 65535);
+  hipLaunchKernelGGL((sum_kernel<T>), dim3((a.N / 4 + threads - 1) / threads, tokens, (a.tokens + tokens - 1) / tokens), dim3(threads), 0, stream, a);
   DQ_CHECK_HIP(hipGetLastError());
   return 0;
 }
@@ -423,12 +603,30 @@ int launch_rows(const Args& a, int pass_rows, int workgroups, hipStream_t stream
   return 0;
 }
 
+template <class W, bool LINES>
+int launch_few(const Args& a, hipStream_t stream) {
+  constexpr int kMost = 160 * 1024;
+  auto kern = few_pairs_kernel<W, LINES>;
+  static bool raised[kMaxDevices];
+  if (raise_lds_limit<kMost>(kern, raised)) return -1;
+  hipLaunchKernelGGL(kern, dim3(a.N / 16), dim3((kWaves + 1) * 64), pipes_area<W>() + a.pairs * acts_stride(a.K), stream, a);
+  DQ_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
 // Two workgroups a CU, each a chunk ahead, where what an expert is likely to have of rows leaves room for that (us, against one
 // workgroup that is two chunks ahead: one token, 8 of 128 experts, 1024 x 4096 10.5 and 11.7; 24 tokens, 4 of 64, 2048 x 1024 19.7 and
 // 25.8); else one, with as many rows as it can hold (64 tokens, 4 of 32, 2880 x 2880 MXFP4: 69.6 and 74.5).
 template <class W, bool UP>
 int product(const Args& a, hipStream_t stream) {
   const int stride = acts_stride(a.K), mean = a.pairs / std::min(a.experts, a.pairs);
+  if constexpr (!UP) {
+    const size_t scales = (size_t)a.experts * a.N * (a.K >> W::kShift) * W::kScaleBytes;
+    // (us, against parts of every expert's rows and the sums behind them: 4096 x 1024, 8 pairs 9.0 and 13.1, 2048 x 768, 8 8.4 and 11.0,
+    // 8192 x 4096 MXFP4, 2 10.6 and 12.2; 4096 x 1536, 16 pairs 19.7 and 18.7, 2048 x 1024, 16 12.1 and 9.3)
+    if (a.pairs <= kFewPairs && pipes_area<W>() + a.pairs * stride <= 160 * 1024 && scales < kNowhere)
+      return a.K % kChunk == 0 ? launch_few<W, true>(a, stream) : launch_few<W, false>(a, stream);
+  }
   const int both = (80 * 1024 - pipes_area<W>()) / stride, alone = (160 * 1024 - pipes_area<W>()) / stride;
   const int likely = std::min(std::min(16, a.tokens), 3 * mean + 4);
   const bool two = likely <= both;

@@ -186,7 +186,9 @@ int tiles(const Args& a, int tile_rows, hipStream_t stream) {
   p.tiles_n = (a.N + P::kColumns - 1) / P::kColumns;
   // every expert's last tile may be a part of one
   const long row_tiles = a.pairs / tile_rows + (a.experts < a.pairs ? a.experts : a.pairs);
-  const int workgroups = (int)((row_tiles * p.tiles_n + 7) / 8 * 8);
+  const long all = (row_tiles * p.tiles_n + 7) / 8 * 8;
+  if (all >= 1l << 23) DQ_FAIL("experts: %d rows of %d columns: more tiles than a launch takes", a.pairs, a.N);  // (2^32 threads)
+  const int workgroups = (int)all;
   const bool odd = (a.K / 64) % 2 != 0 || (Base::kScaleDma >= 2 && ((a.K >> a.group_shift) & 1) != 0);
   if (tile_rows == 256) {
     if constexpr (gemm::TallWaves<Base>::value) return odd ? launch_tiles<P, 8, 2, 1, 1, true>(p, workgroups, stream) : launch_tiles<P, 8, 2, 1, 1, false>(p, workgroups, stream);

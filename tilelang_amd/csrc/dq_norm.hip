@@ -46,7 +46,7 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void norm_kernel(const T
   constexpr int kRows = LANES <= 64 ? 256 / LANES : 1;  // a workgroup's
   __shared__ float slots[4][16];
   const int lane = threadIdx.x % LANES;
-  const long row = (long)blockIdx.x * kRows + threadIdx.x / LANES;
+  const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * kRows + threadIdx.x / LANES;
   if (row >= rows) return;  // (one row a workgroup where there is a barrier)
   const int pieces = dim >> 3;
 
@@ -154,7 +154,8 @@ struct NormArgs {
 template <class T, int LANES, int NV, bool RESIDUAL, bool INT8>
 int launch(const NormArgs& a) {
   constexpr int kRows = LANES <= 64 ? 256 / LANES : 1;
-  hipLaunchKernelGGL((norm_kernel<T, LANES, NV, RESIDUAL, INT8>), dim3((a.rows + kRows - 1) / kRows), dim3(LANES <= 64 ? 256 : LANES), 0, a.stream,
+  const unsigned blocks = ((unsigned)a.rows + kRows - 1) / kRows, wide = blocks < (1u << 20) ? blocks : 1u << 20;  // (a launch takes 2^32 threads a dimension)
+  hipLaunchKernelGGL((norm_kernel<T, LANES, NV, RESIDUAL, INT8>), dim3(wide, (blocks + wide - 1) / wide), dim3(LANES <= 64 ? 256 : LANES), 0, a.stream,
                      (const T*)a.X, (const T*)a.Residual, (const T*)a.Weight, a.Y, (T*)a.Sum, a.Scale, a.rows, a.dim, a.row_stride, a.eps);
   DQ_CHECK_HIP(hipGetLastError());
   return 0;
