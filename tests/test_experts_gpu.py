@@ -89,7 +89,8 @@ def test_sizes(cuda, tokens, experts, top_k, fmt, hidden, inter, whole):
 @pytest.mark.parametrize("fmt", FORMATS, ids=lambda f: "-".join(f"{k}={v}" for k, v in f.items()) or "uint4")
 @pytest.mark.parametrize("tokens,experts,top_k,how,hidden,inter", [
     (1100, 2, 1, "even", 128, 256), (1024, 1, 1, "one", 256, 384), (700, 3, 1, "one", 384, 128), (3500, 70, 1, "skewed", 128, 128), (900, 5, 3, "padded", 256, 128),
-    (1400, 4, 2, "skewed", 640, 256),
+    (1400, 4, 2, "skewed", 640, 256), (100, 5, 2, "skewed", 256, 384), (3500, 70, 1, "padded", 128, 256), (2500, 70, 2, "skewed", 384, 128),
+    (40, 2, 2, "one", 640, 128), (130, 300, 2, "even", 128, 128), (600, 300, 8, "even", 128, 128),
 ])
 def test_many_rows(cuda, tokens, experts, top_k, how, hidden, inter, fmt):
     print(f"experts {tokens} of {experts} top {top_k} {how} {hidden} {inter} {fmt}", flush=True)

@@ -633,6 +633,7 @@ int product(const Args& a, hipStream_t stream) {
   const int pass_rows = std::min(std::min(16, a.tokens), two ? both : alone);
   // tiles that there can be
   const long most = (long)(a.pairs / pass_rows + std::min(a.experts, a.pairs)) * (a.N / (UP ? 16 : 32));
+  if (most >= 1l << 31) DQ_FAIL("experts: %d rows of %d columns: more tiles than a call counts", a.pairs, a.N);
   const int workgroups = (int)std::min(most, two ? 512l : 256l);
   int rc;
   if (a.K % kChunk == 0) rc = two ? launch_rows<W, UP, 1, true>(a, pass_rows, workgroups, stream) : launch_rows<W, UP, 2, true>(a, pass_rows, workgroups, stream);
@@ -642,14 +643,21 @@ int product(const Args& a, hipStream_t stream) {
   return 0;
 }
 
-// Rows of a tile of the matrix pipe's kernel, or 0: few rows an expert.
+// Rows of a tile of the matrix pipe's kernel (dq_experts_tiles.hip), or 0: few rows an expert.  By the mean number of rows, of E experts
+// with N x K (us, "up", rows as here / tiles of 64 / of 128):
+//   uint4 8 of 4096 x 4096, 32 of 2880 x 2816, 128 of 1024 x 4096: 8 rows 38, 75, 121 here, 68, 121, 220 in tiles of 128;
+//     16 rows 48 / 47 / 64, 92 / 85 / 117, 179 / 158 / 232; 96 rows 186 / 81 / 99, 371 / 163 / 167, 768 / 329 / 347;
+//     128 rows 244 / 111 / 107, 486 / 208 / 208, 992 / 401 / 398; 512 rows 960 / 329 / 284, 1797 / 631 / 536
+//   MXFP4 (decoded with less): 16 rows 41 / 43 / 57, 82 / 117 / 111, 153 / 181 / 219; 32 rows 66 / 62 / 60, 123 / 125 / 131,
+//     262 / 205 / 249; 64 rows 115 / 72 / 64, 209 / 157 / 155, 454 / 268 / 270; 128 rows 202 / 107 / 99, 385 / 241 / 194
+// Tiles of 96 rows are between their neighbours everywhere, tiles of 256 ahead by 1 % at best (4096 tokens, two of 8 experts of
+// 14336 x 4096: 1719 and 1740) and eight waves on a tile of 128 nowhere.
 int tile_rows(const Args& a, int mxfp4) {
-  if (acts_stride(a.K) > kActsRoom) return 128;  // (a row does not fit)
   if (a.K < 128) return 0;
-  const long mean = a.pairs / (a.experts < a.pairs ? a.experts : a.pairs);
-  if (mean < 48) return 0;
-  const bool tall = mxfp4 || a.group_shift > 5;
-  return tall && mean >= 512 ? 256 : 128;
+  if (acts_stride(a.K) > kActsRoom) return 128;  // (a row does not fit)
+  const long mean = a.pairs / std::min(a.experts, a.pairs);
+  if (mxfp4) return mean < 28 ? 0 : mean < 64 ? 64 : 128;
+  return mean < 16 ? 0 : mean < 112 ? 64 : 128;
 }
 
 template <bool UP>

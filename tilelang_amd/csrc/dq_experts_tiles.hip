@@ -1,4 +1,4 @@
-// The experts' products at many rows an expert: the direct-to-LDS GEMM of dq_gemm_core.h on tiles of 256 or 128 rows of one expert
+// The experts' products at many rows an expert: the direct-to-LDS GEMM of dq_gemm_core.h on tiles of 64 or 128 rows of one expert
 // by 256 of its weight rows (up: 128 of the gate and the 128 of the up projection that go with them, in blocks of 32, so that a
 // lane has both sums of a value).
 //
@@ -160,18 +160,16 @@ struct ExpertsPolicy : Base {
   }
 };
 
-template <class P, int kMBW, int kNBW, int kWavesM, int kKHalves, bool kOdd>
+template <class P, int kMBW, bool kOdd>
 int launch_tiles(const TileParams& p, int workgroups, hipStream_t stream) {
-  constexpr int kTileM = 32 * kMBW * kWavesM;
-  constexpr bool kPairB = P::kBRowBytes == 32 && kTileM == 256;  // as in the kernel: a fourth B slot
-  constexpr int kPipe = 3 * (kKHalves == 2 ? 2 : 1) * (kTileM * gemm::kARowBytes + gemm::BN * P::kBRowBytes) + (kPairB ? gemm::BN * P::kBRowBytes : 0) + 8 * 1024;
-  constexpr int kSlabs = kKHalves == 1 ? 4 * 32 * 36 * 4 : 128 * 1024;  // the epilogue's, or the accumulators handed over before it
+  // three stages of rows and weights and the rings of scales, or the epilogue's slabs
+  constexpr int kPipe = 3 * (32 * kMBW * gemm::kARowBytes + gemm::BN * P::kBRowBytes) + 8 * 1024, kSlabs = 4 * 32 * 36 * 4;
   constexpr int kLds = kPipe > kSlabs ? kPipe : kSlabs;
-  static_assert(P::kBRowBytes == 32 && kLds <= 160 * 1024, "LDS budget");
-  auto kern = gemm::gemm_kernel_dma<P, kMBW, kNBW, kWavesM, kKHalves, kOdd>;
+  static_assert(P::kBRowBytes == 32 && kLds <= 80 * 1024, "LDS budget of two workgroups a CU");
+  auto kern = gemm::gemm_kernel_dma<P, kMBW, 2, 1, 1, kOdd>;
   static bool raised[kMaxDevices];
   if (raise_lds_limit<kLds>(kern, raised)) return -1;
-  hipLaunchKernelGGL(kern, dim3(workgroups), dim3(256 * kKHalves), kLds, stream, p);
+  hipLaunchKernelGGL(kern, dim3(workgroups), dim3(256), kLds, stream, p);
   DQ_CHECK_HIP(hipGetLastError());
   return 0;
 }
@@ -190,16 +188,14 @@ int tiles(const Args& a, int tile_rows, hipStream_t stream) {
   if (all >= 1l << 23) DQ_FAIL("experts: %d rows of %d columns: more tiles than a launch takes", a.pairs, a.N);  // (2^32 threads)
   const int workgroups = (int)all;
   const bool odd = (a.K / 64) % 2 != 0 || (Base::kScaleDma >= 2 && ((a.K >> a.group_shift) & 1) != 0);
-  if (tile_rows == 256) {
-    if constexpr (gemm::TallWaves<Base>::value) return odd ? launch_tiles<P, 8, 2, 1, 1, true>(p, workgroups, stream) : launch_tiles<P, 8, 2, 1, 1, false>(p, workgroups, stream);
-    else return odd ? launch_tiles<P, 4, 4, 2, 1, true>(p, workgroups, stream) : launch_tiles<P, 4, 4, 2, 1, false>(p, workgroups, stream);
-  }
-  return odd ? launch_tiles<P, 4, 2, 1, 1, true>(p, workgroups, stream) : launch_tiles<P, 4, 2, 1, 1, false>(p, workgroups, stream);
+#define DQ_TILES(BLOCKS_) (odd ? launch_tiles<P, BLOCKS_, true>(p, workgroups, stream) : launch_tiles<P, BLOCKS_, false>(p, workgroups, stream))
+  return tile_rows == 64 ? DQ_TILES(2) : DQ_TILES(4);
+#undef DQ_TILES
 }
 
 }  // namespace
 
-// Tiles of 256 or 128 rows; groups of 32 k of fp16 scales come with every tile, which the kernel has for 128 rows.
+// Tiles of 64 or 128 rows.
 int experts_tiles(const Args& a, int mxfp4, bool up, int tile_rows, hipStream_t stream) {
   if (mxfp4) return up ? tiles<MxPolicy<FP4_E2M1, false>, true>(a, tile_rows, stream) : tiles<MxPolicy<FP4_E2M1, false>, false>(a, tile_rows, stream);
   if (a.Z != nullptr)

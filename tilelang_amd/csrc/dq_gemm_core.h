@@ -608,7 +608,7 @@ __device__ __forceinline__ void dma4_unless(int not_due, unsigned lds_addr, unsi
   asm volatile("s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lnot_due%=\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, %3\n.Lnot_due%=:" ::"s"(__builtin_amdgcn_readfirstlane(not_due)), "s"(lds_addr), "v"(voff), "s"(sbase) : "memory", "scc");
 }
 
-// Five forms, on a tile of 256 columns:
+// The forms, on a tile of 256 columns:
 // * kMBW = 4, kNBW = 4, kWavesM = 2: 256 rows on 2 x 2 waves of 128 x 128, one workgroup per CU.
 // * kMBW = 8, kNBW = 2, kWavesM = 1: 256 rows on four waves side by side, each 256 rows x 64 columns.  A wave then
 //   decodes only the 64 weight rows it alone multiplies (with two rows of waves every packed word is decoded twice per
@@ -618,6 +618,7 @@ __device__ __forceinline__ void dma4_unless(int not_due, unsigned lds_addr, unsi
 //   of 256 rows.  With kKHalves = 2 on eight waves, two per SIMD: waves 4 .. 7 multiply the other half of every stage
 //   (a second k-block, or with 64-byte rows of B the other two steps of the one k-block) into accumulators of their own,
 //   and the two halves exchange sums through LDS before the epilogue, of which each does half.
+// * kMBW = 2, kNBW = 2, kWavesM = 1: 64 rows on four waves, for the groups of few rows of dq_experts_tiles.hip.
 // * kMBW = 3 and 6, kNBW = 2, kWavesM = 1: 96 rows, on four waves or (kKHalves = 2) eight, and 192 rows on four, as the two above:
 //   for the policies with P::kRowCosts, where such tiles fill their rounds better.
 // What bounds the 128-row form is the CU's load unit, which takes about two cycles per 64 bytes or per row piece, if that
@@ -639,7 +640,7 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
   if constexpr (!kGrouped) take_k_slice<P>(p, bid);
   extern __shared__ __align__(16) unsigned char smem[];
   static_assert(P::kBRowBytes == 32 || P::kBRowBytes == 64, "direct-to-LDS variant: 32 or 64 packed bytes per weight row per tile");
-  static_assert(kWavesM == 2 ? (kMBW == 4 && kNBW == 4) : (kWavesM == 1 && (kMBW == 3 || kMBW == 4 || kMBW == 6 || kMBW == 8) && kNBW == 2), "one of the forms");
+  static_assert(kWavesM == 2 ? (kMBW == 4 && kNBW == 4) : (kWavesM == 1 && (kMBW == 2 || kMBW == 3 || kMBW == 4 || kMBW == 6 || kMBW == 8) && kNBW == 2), "one of the forms");
   static_assert(kKHalves == 1 || (kKHalves == 2 && kWavesM == 1 && kMBW <= 4), "two halves of a stage: 96 or 128 rows");
   constexpr int kWavesN = 8 / kNBW;            // waves across the 256 tile columns
   constexpr int kWaves = 4;                    // of one half

@@ -40,15 +40,22 @@ struct OrderArgs {
   int pairs, experts, first, chunk_pairs, chunks;
 };
 
-// The largest of the lanes' keys and, of the lanes that have it, the lowest index.
-template <class F>
-__device__ __forceinline__ void best_over_wave(F& key, int& index) {
+// The largest of the lanes' values, in every lane.  fp32 goes through the register file: neighbours, rows of 16, then from row to row.
+__device__ __forceinline__ float max_over_wave(float v) {
+  v = fmaxf(v, dpp_move<0xB1>(v));   // lane ^ 1
+  v = fmaxf(v, dpp_move<0x4E>(v));   // lane ^ 2
+  v = fmaxf(v, dpp_move<0x124>(v));  // rotated by 4 in its row
+  v = fmaxf(v, dpp_move<0x128>(v));  // by 8
+  const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 0));
+  const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 16));
+  const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 32));
+  const float d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 48));
+  return fmaxf(fmaxf(a, b), fmaxf(c, d));
+}
+__device__ __forceinline__ double max_over_wave(double v) {
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const F k = __shfl_xor(key, d, 64);
-    const int i = __shfl_xor(index, d, 64);
-    if (k > key || (k == key && i < index)) key = k, index = i;
-  }
+  for (int d = 1; d < 64; d *= 2) v = fmax(v, __shfl_xor(v, d, 64));
+  return v;
 }
 
 template <class F>
@@ -91,8 +98,7 @@ __device__ bool choose(const RouteArgs& a, const float (&x)[V], F* keys, int& my
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i * 64 + lane < a.experts) largest = fmaxf(largest, x[i]);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) largest = fmaxf(largest, __shfl_xor(largest, d, 64));
+    largest = max_over_wave(largest);
     if (largest == -__builtin_inff()) largest = 0.f;  // every expert is masked
     F total = 0;
 #pragma unroll
@@ -128,30 +134,40 @@ __device__ bool choose(const RouteArgs& a, const float (&x)[V], F* keys, int& my
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-    F mine = kNone;
-    if (lane < a.groups) {
-      F best = kNone, next = kNone;
-      for (int i = 0; i < size; ++i) {
-        const F k = keys[lane * size + i];
-        if (k > best) next = best, best = k;
-        else if (k > next) next = k;
+    // a group's two largest, by as many lanes as there are for it
+    int each = 64;
+    for (int n = 1; n < a.groups; n *= 2) each /= 2;
+    const int group = lane / each;
+    F mine = kNone, next = kNone;
+    if (group < a.groups) {
+#pragma unroll 4
+      for (int i = lane % each; i < size; i += each) {
+        const F k = keys[group * size + i];
+        next = k > mine ? mine : k > next ? k : next;
+        mine = k > mine ? k : mine;
       }
-      mine = a.two && size > 1 ? best + next : best;
-      if (mine != mine) mine = kMost;
     }
+    for (int d = 1; d < each; d *= 2) {
+      const F o = __shfl_xor(mine, d, 64), p = __shfl_xor(next, d, 64);
+      const F less = o < mine ? o : mine, more = p > next ? p : next;
+      mine = o > mine ? o : mine;
+      next = less > more ? less : more;
+    }
+    if (a.two && size > 1) mine += next;
+    if (mine != mine) mine = kMost;
     __builtin_amdgcn_wave_barrier();
-    bool left = lane < a.groups;
+    bool left = group < a.groups && lane % each == 0;
+    unsigned long long taken = 0;  // a bit a group
     F last = 0;
     for (int r = 0; r < a.groups; ++r) {
-      F best = left ? mine : kNone;
-      int index = left ? lane : 64 + lane;  // (behind every group that is left, whatever its key)
-      best_over_wave(best, index);
+      const F best = max_over_wave(left ? mine : kNone);
       if (kNarrow && r > 0 && (by_score || a.two) && too_close((float)last, (float)best)) close = true;
       if (r == a.top_groups) break;
-      if (lane == index) left = false;
+      const int at = __builtin_ctzll(__ballot(left && mine == best));  // (of equal groups the first)
+      if (lane == at) left = false;
+      taken |= 1ull << (at / each);
       last = best;
     }
-    const unsigned long long taken = ~__ballot(left);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int e = i * 64 + lane;
@@ -162,28 +178,35 @@ __device__ bool choose(const RouteArgs& a, const float (&x)[V], F* keys, int& my
   F last = 0;
   for (int r = 0; r < a.top_k + (by_score ? 1 : 0); ++r) {
     F best = kNone;
-    int index = 1 << 20;
+    bool any = false;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = i * 64 + lane;
-      if (open[i] && (key[i] > best || index == 1 << 20)) best = key[i], index = e;
+      best = open[i] && key[i] > best ? key[i] : best;
+      any = any || open[i];
     }
-    best_over_wave(best, index);
-    if (kNarrow && by_score && r > 0 && index < 1 << 20 && too_close((float)last, (float)best)) close = true;
+    best = max_over_wave(best);
+    if (kNarrow && by_score && r > 0 && __ballot(any) != 0 && too_close((float)last, (float)best)) close = true;
     if (r == a.top_k) break;
     last = best;
+    // the lowest index of those that have it: expert 64 i + lane
+    int index = 0;
+#pragma unroll
+    for (int i = V - 1; i >= 0; --i) {
+      const unsigned long long has = __ballot(open[i] && key[i] == best);
+      index = has != 0 ? i * 64 + __builtin_ctzll(has) : index;
+    }
     float found = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i * 64 + lane == index) open[i] = false, found = (float)score[i];
-    found = __shfl(found, index & 63, 64);
+    found = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, found), index & 63));
     if (lane == r) my_id = index, my_score = found;
   }
   return close;
 }
 
 template <class T, int V>
-__device__ void route_token(const RouteArgs& a, long token, unsigned char* lds) {
+__device__ __forceinline__ int route_token(const RouteArgs& a, long token, unsigned char* lds) {
   const int lane = threadIdx.x & 63;
   float x[V];
 #pragma unroll
@@ -204,9 +227,30 @@ __device__ void route_token(const RouteArgs& a, long token, unsigned char* lds) 
     a.Weights[token * a.top_k + lane] = score * a.factor;
     a.Ids[token * a.top_k + lane] = id;
   }
+  return id;
 }
 
 // ---- the order ------------------------------------------------------------------------------------------------------------
+
+constexpr int kFewPairs = 64;
+
+// Up to 64 pairs, a lane each, by one wave: a pair's place is how many have a lower expert, or its own and come earlier.
+__device__ void place_few(const OrderArgs& o, int id) {
+  const int lane = threadIdx.x & 63;
+  const unsigned e = lane < o.pairs ? (unsigned)id - (unsigned)o.first : ~0u, mine = e < (unsigned)o.experts ? e : (unsigned)o.experts;
+  int at = 0;
+  for (int p = 0; p < o.pairs; ++p) {
+    const unsigned other = (unsigned)__builtin_amdgcn_readlane((int)mine, p);
+    at += other < mine || (other == mine && p < lane) ? 1 : 0;
+  }
+  // (pairs of other experts come behind all others: their places hold -1)
+  if (lane < o.pairs) o.Order[at] = mine < (unsigned)o.experts ? lane : -1;
+  for (int first = 0; first <= o.experts; first += 64) {
+    int start = 0;
+    for (int p = 0; p < o.pairs; ++p) start += __builtin_amdgcn_readlane((int)mine, p) < first + lane ? 1 : 0;
+    if (first + lane <= o.experts) o.Starts[first + lane] = start;
+  }
+}
 
 // A chunk's pairs of every expert, counted by all threads of the workgroup.
 __device__ void count_chunk(const OrderArgs& o, int chunk, int* count) {
@@ -221,7 +265,7 @@ __device__ void count_chunk(const OrderArgs& o, int chunk, int* count) {
   for (int e = threadIdx.x; e < o.experts; e += kWaves * 64) o.Counts[(size_t)chunk * o.experts + e] = (uint16_t)count[e];
 }
 
-// The pairs of some chunks into their places.  `lds`: (kWaves + 1) experts + 64 ints.
+// The pairs of some chunks into their places.  `lds`: (kWaves + 2) experts + 64 ints.
 __device__ void place(const OrderArgs& o, int workgroup, int workgroups, int* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = o.experts;
   int* const mine = lds + wave * E;      // a wave's pairs of every expert; then where its next one goes
@@ -241,15 +285,30 @@ __device__ void place(const OrderArgs& o, int workgroup, int workgroups, int* ld
   __syncthreads();
   // one thread an expert: all pairs, those of earlier workgroups, and where every wave's begin among this one's
   int before = 0, all = 0;
-  if (tid < E) {
-    if (o.Counts != nullptr) {
-#pragma unroll 8
-      for (int c = 0; c < o.chunks; ++c) {
-        const int n = o.Counts[(size_t)c * E + tid];
-        all += n;
-        before += c < c0 ? n : 0;
+  if (o.Counts != nullptr) {
+    // the chunks' counts by as many threads an expert as there are, their parts added where the totals go later
+    int wide = 64;
+    while (wide < E) wide *= 2;
+    const int e = tid & (wide - 1), slices = kWaves * 64 / wide;
+    int part = 0, early = 0;
+    if (e < E) {
+#pragma unroll 16
+      for (int c = tid / wide; c < o.chunks; c += slices) {
+        const int n = o.Counts[(size_t)c * E + e];
+        part += n;
+        early += c < c0 ? n : 0;
       }
     }
+    if (tid < E) total[tid] = 0, sums[64 + tid] = 0;
+    __syncthreads();
+    if (e < E) {
+      atomicAdd(&total[e], part);
+      atomicAdd(&sums[64 + e], early);
+    }
+    __syncthreads();
+    if (tid < E) all = total[tid], before = sums[64 + tid];
+  }
+  if (tid < E) {
     int run = before;
     for (int w = 0; w < kWaves; ++w) {
       const int n = lds[w * E + tid];
@@ -302,13 +361,22 @@ __device__ void place(const OrderArgs& o, int workgroup, int workgroups, int* ld
 template <class T, int V>
 __global__ __launch_bounds__(kWaves * 64) void route_kernel(const RouteArgs a, const OrderArgs o) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const int wave = threadIdx.x >> 6, chunk = blockIdx.x;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, chunk = blockIdx.x;
   const int tokens = o.chunk_pairs / a.top_k;  // of a chunk
   const long t1 = min((long)(chunk + 1) * tokens, (long)a.tokens);
-  for (long t = (long)chunk * tokens + wave; t < t1; t += kWaves) route_token<T, V>(a, t, smem + (size_t)wave * a.experts * 8);
+  unsigned char* const keys = smem + kFewPairs * 4 + (size_t)wave * a.experts * 8;
+  for (long t = (long)chunk * tokens + wave; t < t1; t += kWaves) {
+    const int id = route_token<T, V>(a, t, keys);
+    if (o.pairs <= kFewPairs && lane < a.top_k) ((int*)smem)[t * a.top_k + lane] = id;
+  }
   __syncthreads();  // (the pairs that other waves wrote, and the LDS, which changes its use)
-  if (o.Counts != nullptr) count_chunk(o, chunk, (int*)smem);
-  else place(o, 0, 1, (int*)smem);
+  if (o.pairs <= kFewPairs) {
+    if (wave == 0) place_few(o, ((const int*)smem)[min(lane, o.pairs - 1)]);
+  } else if (o.Counts != nullptr) {
+    count_chunk(o, chunk, (int*)smem);
+  } else {
+    place(o, 0, 1, (int*)smem);
+  }
 }
 
 __global__ __launch_bounds__(kWaves * 64) void count_kernel(const OrderArgs o) {
@@ -318,10 +386,14 @@ __global__ __launch_bounds__(kWaves * 64) void count_kernel(const OrderArgs o) {
 
 __global__ __launch_bounds__(kWaves * 64) void place_kernel(const OrderArgs o) {
   extern __shared__ __align__(16) unsigned char smem[];
+  if (o.pairs <= kFewPairs) {
+    if (threadIdx.x < 64) place_few(o, o.Ids[min((int)threadIdx.x, o.pairs - 1)]);
+    return;
+  }
   place(o, blockIdx.x, gridDim.x, (int*)smem);
 }
 
-int place_lds(int experts) { return ((kWaves + 1) * experts + 64) * 4; }
+int place_lds(int experts) { return ((kWaves + 2) * experts + 64) * 4; }
 
 // Whole tokens a chunk, at least a wave's worth, at most kMaxChunks chunks; 16-bit counts
 bool cut(OrderArgs& o, int tokens, int top_k) {
@@ -336,8 +408,8 @@ bool cut(OrderArgs& o, int tokens, int top_k) {
 
 template <class T, int V>
 int launch_route(const RouteArgs& a, const OrderArgs& o, hipStream_t stream) {
-  constexpr int kMost = 16 * 1024 * 8 + 1024 * 4 + 256;
-  const int keys = kWaves * a.experts * 8, room = place_lds(a.experts);
+  constexpr int kMost = kFewPairs * 4 + kWaves * 1024 * 8;
+  const int keys = kFewPairs * 4 + kWaves * a.experts * 8, room = place_lds(a.experts);
   const int lds = keys > room ? keys : room;
   auto kern = route_kernel<T, V>;
   static bool raised[kMaxDevices];
@@ -357,7 +429,7 @@ int route_experts_of(const RouteArgs& a, const OrderArgs& o, hipStream_t stream)
 }
 
 int launch_place(const OrderArgs& o, hipStream_t stream) {
-  constexpr int kMost = (17 * 1024 + 64) * 4;
+  constexpr int kMost = (18 * 1024 + 64) * 4;
   auto kern = place_kernel;
   static bool raised[kMaxDevices];
   if (raise_lds_limit<kMost>(kern, raised)) return -1;
