@@ -40,22 +40,36 @@ struct OrderArgs {
   int pairs, experts, first, chunk_pairs, chunks;
 };
 
-// The largest of the lanes' values, in every lane.  fp32 goes through the register file: neighbours, rows of 16, then from row to row.
-__device__ __forceinline__ float max_over_wave(float v) {
-  v = fmaxf(v, dpp_move<0xB1>(v));   // lane ^ 1
-  v = fmaxf(v, dpp_move<0x4E>(v));   // lane ^ 2
-  v = fmaxf(v, dpp_move<0x124>(v));  // rotated by 4 in its row
-  v = fmaxf(v, dpp_move<0x128>(v));  // by 8
-  const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 0));
-  const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 16));
-  const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 32));
-  const float d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 48));
-  return fmaxf(fmaxf(a, b), fmaxf(c, d));
+// The largest of the lanes' values, in every lane; a NaN counts for nothing, and is what comes back where all are.  fp32 goes through
+// the register file: neighbours, rows of 16, a row's last lane to the next row, lane 31 to the upper half.
+template <int CTRL>
+__device__ __forceinline__ float max_with(float v) {
+  const int b = __builtin_bit_cast(int, v);
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, b, CTRL, 0xF, 0xF, false)));
 }
-__device__ __forceinline__ double max_over_wave(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v = fmax(v, __shfl_xor(v, d, 64));
-  return v;
+template <int CTRL>
+__device__ __forceinline__ double max_with(double v) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const int l = (int)b, h = (int)(b >> 32);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(l, l, CTRL, 0xF, 0xF, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(h, h, CTRL, 0xF, 0xF, false);
+  return fmax(v, __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo));
+}
+template <class F>
+__device__ __forceinline__ F max_over_wave(F v) {
+  v = max_with<0xB1>(v);   // lane ^ 1
+  v = max_with<0x4E>(v);   // lane ^ 2
+  v = max_with<0x124>(v);  // rotated by 4 in its row
+  v = max_with<0x128>(v);  // by 8
+  v = max_with<0x142>(v);
+  v = max_with<0x143>(v);
+  if constexpr (std::is_same<F, float>::value) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+  } else {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)b, 63), hi = (unsigned)__builtin_amdgcn_readlane((int)(b >> 32), 63);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+  }
 }
 
 template <class F>
@@ -65,9 +79,11 @@ __device__ __forceinline__ F sum_over_wave(F v) {
   return v;
 }
 
-// Whether two keys in fp32 may be the other way round in exact arithmetic: a score's error is below 2^-19 (a sum of up to 1024
-// exponentials), a sum's rounding 2^-24 of it.
-__device__ __forceinline__ bool too_close(float a, float b) { return a - b <= 0x1p-17f + 0x1p-20f * (fabsf(a) + fabsf(b)); }
+// Whether two keys in fp32 may be the other way round in exact arithmetic.  `slack` is at least twice what the scores in both are off
+// by, four scores where a key is a group's sum of two: a logistic score has three roundings and exp's, below 2^-22 together; a share
+// is off by less than 2^-18.8 of the largest share (22 additions, exp's error and its argument's), nearly all of it by a factor that
+// every share has.  The keys' own roundings are 2^-24 of each.
+__device__ __forceinline__ bool too_close(float a, float b, float slack) { return a - b <= slack + 0x1p-21f * (fabsf(a) + fabsf(b)); }
 
 template <class F>
 __device__ __forceinline__ F exp_of(F x) {
@@ -75,133 +91,160 @@ __device__ __forceinline__ F exp_of(F x) {
   else return expf(x);
 }
 
-// One token's choices: lane j < top_k gets the j-th one and its score.  `keys`: the wave's LDS, an F an expert (groups alone).
-// Returns whether F is too narrow to tell (the same in every lane).  A NaN counts as the largest of all: it is chosen, and its
-// weight shows it.
-template <int V, class F>
-__device__ bool choose(const RouteArgs& a, const float (&x)[V], F* keys, int& my_id, float& my_score) {
+// One token's choices: lane j < top_k gets the j-th one and its score.  V > 0: logits and keys in registers, in fp32, V a lane.  V = 0,
+// in 64 bits: logits from memory and keys in LDS, so that what few tokens need takes no registers from all others.  `keys`: the wave's
+// LDS, an F an expert.  Returns whether F is too narrow to tell (the same in every lane).  A NaN counts as the largest of all: it is
+// chosen, and its weight shows it.
+template <class T, int V, class F>
+__device__ __forceinline__ bool choose(const RouteArgs& a, const T* logits, const float (&held)[V ? V : 1], F* keys, int& my_id, float& my_score) {
   const int lane = threadIdx.x & 63;
-  constexpr F kNone = -(F)__builtin_inff(), kMost = (F)__builtin_inff();
-  constexpr bool kNarrow = std::is_same<F, float>::value;
+  constexpr F kNone = -(F)__builtin_inff(), kMost = (F)__builtin_inff(), kGone = (F)__builtin_nanf("");
+  constexpr bool kNarrow = V > 0;
+  constexpr int kUnroll = V ? V : 1;
+  const int n = V ? V : (a.experts + 63) / 64;  // experts a lane
   const bool by_score = a.Bias != nullptr;
   bool close = false;
+  const auto x = [&](int i) -> float {
+    if constexpr (V) return held[i];
+    else return i * 64 + lane < a.experts ? (float)logits[i * 64 + lane] : 0.f;
+  };
 
-  F score[V];
-  if (a.sigmoid) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const F t = exp_of<F>(-fabs((F)x[i]));
-      score[i] = (x[i] >= 0 ? (F)1 : t) / ((F)1 + t);
-    }
-  } else {
-    float largest = -__builtin_inff();
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i * 64 + lane < a.experts) largest = fmaxf(largest, x[i]);
-    largest = max_over_wave(largest);
-    if (largest == -__builtin_inff()) largest = 0.f;  // every expert is masked
-    F total = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      score[i] = i * 64 + lane < a.experts ? exp_of<F>((F)x[i] - (F)largest) : (F)0;
-      total += score[i];
-    }
+  F largest = 0, total = 1;
+  if (!a.sigmoid) {
+    float l = -__builtin_inff();
+#pragma unroll kUnroll
+    for (int i = 0; i < n; ++i)
+      if (i * 64 + lane < a.experts) l = fmaxf(l, x(i));
+    l = max_over_wave(l);
+    largest = l == -__builtin_inff() ? (F)0 : (F)l;  // (every expert is masked)
+    total = 0;
+#pragma unroll kUnroll
+    for (int i = 0; i < n; ++i) total += i * 64 + lane < a.experts ? exp_of<F>((F)x(i) - largest) : (F)0;
     total = sum_over_wave(total);
-#pragma unroll
-    for (int i = 0; i < V; ++i) score[i] = total == 0 ? (F)0 : score[i] / total;
   }
-
-  F key[V];
-  bool open[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
+  const auto score_of = [&](float v) -> F {
+    if (a.sigmoid) {
+      const F t = exp_of<F>(-fabs((F)v));
+      return (v >= 0 ? (F)1 : t) / ((F)1 + t);
+    }
+    return total == 0 ? (F)0 : exp_of<F>((F)v - largest) / total;
+  };
+  const float slack = a.sigmoid ? 0x1p-19f : total == 0 ? 0.f : 0x1p-17f / (float)total;
+  // what an expert is chosen by, and what its group counts by
+  const auto key_of = [&](int i) -> F {
     const int e = i * 64 + lane;
-    open[i] = e < a.experts;
-    key[i] = by_score ? score[i] + (F)(open[i] ? a.Bias[e] : 0.f) : (F)x[i];
-    if (key[i] != key[i]) key[i] = kMost;
-  }
+    F k = (F)x(i);
+    if (by_score) k = score_of(x(i)) + (F)(e < a.experts ? a.Bias[e] : 0.f);
+    return k != k ? kMost : k;
+  };
+  const auto group_key_of = [&](int i, F key) -> F {
+    if (!a.two || by_score) return key;
+    const F k = score_of(x(i));
+    return k != k ? kMost : k;
+  };
+  // a key that is not to be chosen (any more) is NaN
+  F key[kUnroll];
+  const auto at = [&](int i) -> F {
+    if constexpr (V) return key[i];
+    else return i * 64 + lane < a.experts ? keys[i * 64 + lane] : kGone;
+  };
+  const auto put = [&](int i, F k) {
+    if constexpr (V) key[i] = k;
+    else if (i * 64 + lane < a.experts) keys[i * 64 + lane] = k;
+  };
+#pragma unroll kUnroll
+  for (int i = 0; i < n; ++i) put(i, i * 64 + lane < a.experts ? key_of(i) : kGone);
 
   if (a.groups > 1) {
     const int size = a.experts / a.groups;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (open[i]) {
-        F k = key[i];
-        if (a.two && !by_score) k = score[i] != score[i] ? kMost : score[i];
-        keys[i * 64 + lane] = k;
-      }
-    }
+#pragma unroll kUnroll
+    for (int i = 0; i < n; ++i)
+      if (i * 64 + lane < a.experts) keys[i * 64 + lane] = group_key_of(i, at(i));
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
     // a group's two largest, by as many lanes as there are for it
-    int each = 64;
-    for (int n = 1; n < a.groups; n *= 2) each /= 2;
-    const int group = lane / each;
+    int each = 6;
+    for (int g = 1; g < a.groups; g *= 2) --each;
+    const int group = lane >> each, first = lane & ((1 << each) - 1);
     F mine = kNone, next = kNone;
     if (group < a.groups) {
 #pragma unroll 4
-      for (int i = lane % each; i < size; i += each) {
+      for (int i = first; i < size; i += 1 << each) {
         const F k = keys[group * size + i];
-        next = k > mine ? mine : k > next ? k : next;
-        mine = k > mine ? k : mine;
+        next = fmax(next, fmin(k, mine));
+        mine = fmax(mine, k);
       }
     }
-    for (int d = 1; d < each; d *= 2) {
+    for (int d = 1; d < 1 << each; d *= 2) {
       const F o = __shfl_xor(mine, d, 64), p = __shfl_xor(next, d, 64);
-      const F less = o < mine ? o : mine, more = p > next ? p : next;
-      mine = o > mine ? o : mine;
-      next = less > more ? less : more;
+      next = fmax(fmin(o, mine), fmax(next, p));
+      mine = fmax(mine, o);
     }
     if (a.two && size > 1) mine += next;
     if (mine != mine) mine = kMost;
+    if (group >= a.groups || first != 0) mine = kGone;
     __builtin_amdgcn_wave_barrier();
-    bool left = group < a.groups && lane % each == 0;
     unsigned long long taken = 0;  // a bit a group
     F last = 0;
     for (int r = 0; r < a.groups; ++r) {
-      const F best = max_over_wave(left ? mine : kNone);
-      if (kNarrow && r > 0 && (by_score || a.two) && too_close((float)last, (float)best)) close = true;
+      const F best = max_over_wave(mine);
+      if (kNarrow && r > 0 && (by_score || a.two) && too_close((float)last, (float)best, slack)) close = true;
       if (r == a.top_groups) break;
-      const int at = __builtin_ctzll(__ballot(left && mine == best));  // (of equal groups the first)
-      if (lane == at) left = false;
-      taken |= 1ull << (at / each);
+      const int l = __builtin_ctzll(__ballot(mine == best));  // (of equal groups the first)
+      if (lane == l) mine = kGone;
+      taken |= 1ull << (l >> each);
       last = best;
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = i * 64 + lane;
-      open[i] = open[i] && ((taken >> (e / size)) & 1);
+    // (exact: the quotient is off by less than 2^-12 / size, and no nearer than 1 / (2 size) to a whole number)
+    const float inverse = 1.f / (float)size;
+#pragma unroll kUnroll
+    for (int i = 0; i < n; ++i) {
+      const int g = (int)(((float)(i * 64 + lane) + 0.5f) * inverse);
+      F k = kGone;
+      if (i * 64 + lane < a.experts && ((taken >> (g & 63)) & 1)) k = V || by_score || !a.two ? at(i) : key_of(i);
+      put(i, k);
     }
   }
 
   F last = 0;
   for (int r = 0; r < a.top_k + (by_score ? 1 : 0); ++r) {
-    F best = kNone;
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      best = open[i] && key[i] > best ? key[i] : best;
-      any = any || open[i];
+    F best = kGone;
+    int own = 0;  // (V = 0 alone: which of the lane's experts that is, the first)
+#pragma unroll kUnroll
+    for (int i = 0; i < n; ++i) {
+      const F k = at(i);
+      if constexpr (V) best = fmax(best, k);
+      else if (k > best || !(best == best)) best = k, own = i;
     }
+    const F most = best;
     best = max_over_wave(best);
-    if (kNarrow && by_score && r > 0 && __ballot(any) != 0 && too_close((float)last, (float)best)) close = true;
+    if (kNarrow && by_score && r > 0 && too_close((float)last, (float)best, slack)) close = true;
     if (r == a.top_k) break;
     last = best;
     // the lowest index of those that have it: expert 64 i + lane
     int index = 0;
+    if constexpr (V) {
 #pragma unroll
-    for (int i = V - 1; i >= 0; --i) {
-      const unsigned long long has = __ballot(open[i] && key[i] == best);
-      index = has != 0 ? i * 64 + __builtin_ctzll(has) : index;
+      for (int i = V - 1; i >= 0; --i) {
+        const unsigned long long has = __ballot(key[i] == best);
+        index = has != 0 ? i * 64 + __builtin_ctzll(has) : index;
+      }
+      const bool mine = lane == (index & 63);
+#pragma unroll
+      for (int i = 0; i < V; ++i) key[i] = mine && i == index >> 6 ? kGone : key[i];
+    } else {
+      for (int i = 0; i < n; ++i) {
+        const unsigned long long has = __ballot(most == best && own == i);
+        if (has == 0) continue;
+        index = i * 64 + __builtin_ctzll(has);
+        break;
+      }
+      if (lane == (index & 63)) keys[index] = kGone;
     }
-    float found = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i * 64 + lane == index) open[i] = false, found = (float)score[i];
-    found = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, found), index & 63));
-    if (lane == r) my_id = index, my_score = found;
+    if (lane == r) my_id = index;
   }
+  my_score = lane < a.top_k ? (float)score_of((float)logits[my_id]) : 0.f;
   return close;
 }
 
@@ -216,9 +259,12 @@ __device__ __forceinline__ int route_token(const RouteArgs& a, long token, unsig
   }
   int id = 0;
   float score = 0.f;
-  if (choose<V, float>(a, x, (float*)lds, id, score)) choose<V, double>(a, x, (double*)lds, id, score);
+  const T* const logits = (const T*)a.Logits + token * a.experts;
+  if (choose<T, V, float>(a, logits, x, (float*)lds, id, score)) {
+    const float none[1] = {0.f};
+    choose<T, 0, double>(a, logits, none, (double*)lds, id, score);
+  }
   const bool mine = lane < a.top_k;
-  if (!mine) score = 0.f;
   if (a.renormalize) {
     const float sum = sum_over_wave(score);
     score = sum == 0.f ? 0.f : score / sum;
@@ -397,7 +443,8 @@ int place_lds(int experts) { return ((kWaves + 2) * experts + 64) * 4; }
 
 // Whole tokens a chunk, at least a wave's worth, at most kMaxChunks chunks; 16-bit counts
 bool cut(OrderArgs& o, int tokens, int top_k) {
-  if (tokens * (long)top_k <= kAlonePairs && tokens <= 2 * kWaves) {
+  const long pairs = tokens * (long)top_k;
+  if (pairs <= kFewPairs || (pairs <= kAlonePairs && tokens <= 2 * kWaves)) {
     o.chunk_pairs = tokens * top_k, o.chunks = 1;
     return false;
   }
