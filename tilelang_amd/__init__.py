@@ -44,6 +44,7 @@ from .block_kernels import (  # noqa: F401
 from .bitlinear import BitLinear  # noqa: F401
 from .w4linear import W4A16Linear  # noqa: F401
 from .attention import PagedKVCache, W4Attention  # noqa: F401
+from .experts import RMSNorm, W4Experts  # noqa: F401
 from .profiler import Profiler, TensorSupplyType, do_bench  # noqa: F401
 
 __version__ = "0.1.0"

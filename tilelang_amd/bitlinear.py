@@ -105,7 +105,23 @@ class BitLinear(nn.Module):
             self._kernels[M] = k
         return k
 
-    def forward(self, input: torch.Tensor) -> torch.Tensor:
+    def _codes_forward(self, codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+        M = codes.numel() // self.in_features
+        k = self._kernels.get((M, "codes"))
+        if k is None:
+            k = kernels.bitlinear_int8xint2(M, self.out_features, self.in_features, self._sw_value, interleaved=self.interleave,
+                                            weight_fragments=self.prefill_fragments)
+            self._kernels[(M, "codes")] = k
+        out = k(codes.reshape(M, self.in_features).contiguous(), self.qweight, scale.reshape(M).contiguous())
+        if self.bias is not None:
+            out += self.bias.view(1, -1).expand_as(out)
+        return out.reshape(*codes.shape[:-1], self.out_features)
+
+    def forward(self, input: torch.Tensor, scale: torch.Tensor | None = None) -> torch.Tensor:
+        """``scale``: ``input`` has int8 codes already, and this is the scale of each of its rows, as an int8
+        :class:`~tilelang_amd.experts.RMSNorm` returns them."""
+        if scale is not None:
+            return self._codes_forward(input, scale)
         flat = input.dim() == 2 and input.shape[1] == self.in_features
         x = input if flat else input.reshape(-1, self.in_features)
         if x.dtype != torch.float16:

@@ -29,6 +29,8 @@ EXPERTS_UINT4, EXPERTS_MXFP4 = 0, 1
 MAX_NORM_DIM, MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 32768, 1024, 32, 64
 #: (token, choice) pairs that a call takes
 MAX_PAIRS = 2**23
+#: elements of the tokens' rows
+MAX_ELEMENTS = 2**30
 
 
 def _one_of(fn: str, name: str, value, values: dict) -> int:
@@ -183,7 +185,7 @@ class _Weights:
 
 
 def _activations(fn: str, rows: int, width: int) -> None:
-    if rows * width > 2**30:
+    if rows * width > MAX_ELEMENTS:
         raise ValueError(f"{fn}: {rows} tokens of {width} elements: at most 2^30 elements")
 
 
