@@ -39,6 +39,11 @@ def _one_of(fn: str, name: str, value, values: dict) -> int:
     return values[value]
 
 
+def _first(fn: str, first: int, experts: int) -> None:
+    if not 0 <= first <= 2**31 - 1 - experts:
+        raise ValueError(f"{fn}: first={first} must be from 0 to 2^31 - 1 - experts={experts}")
+
+
 def rms_norm(rows: int, dim: int, eps: float = 1e-6, dtype="float16", residual: bool = False, int8: bool = False,
              row_stride: int | None = None) -> KernelAdapter:
     """Root-mean-square norm: ``y = kernel(x, Weight)``, ``y = Weight * x / sqrt(mean(x ** 2) + eps)`` over rows ``[rows, dim]``.
@@ -55,8 +60,10 @@ def rms_norm(rows: int, dim: int, eps: float = 1e-6, dtype="float16", residual: 
         raise ValueError(f"{fn}: dim={dim} must be a multiple of 8, at most {MAX_NORM_DIM}")
     t = _type16(fn, dtype)
     stride = dim if row_stride is None else row_stride
-    if stride < dim or stride % 8:
-        raise ValueError(f"{fn}: row_stride={stride} must be a multiple of 8 and at least dim={dim}")
+    if stride < dim or stride % 8 or stride > 2**31 - 8:
+        raise ValueError(f"{fn}: row_stride={stride} must be a multiple of 8 and at least dim={dim}, below 2^31")
+    if rows >= 2**31:
+        raise ValueError(f"{fn}: rows={rows} must be below 2^31")
     eps = float(eps)
     if not (eps > 0 and math.isfinite(eps)):
         raise ValueError(f"{fn}: eps must be positive and finite (got {eps})")
@@ -137,8 +144,7 @@ def experts_order(tokens: int, top_k: int, experts: int, first: int = 0) -> Kern
     """
     fn = "experts_order"
     _pairs(fn, tokens, experts, top_k)
-    if first < 0:
-        raise ValueError(f"{fn}: first={first} must not be negative")
+    _first(fn, first, experts)
     params = [KernelParam("ids", torch.int32, (tokens, top_k)), KernelParam("order", torch.int32, (tokens * top_k,)),
               KernelParam("starts", torch.int32, (experts + 1,))]
     room = int(_lib.load_library().dq_experts_order_workspace_bytes(tokens, top_k, experts))
@@ -225,8 +231,7 @@ def experts_down(tokens: int, experts: int, top_k: int, N: int, K: int, weight_f
     fn = "experts_down"
     _pairs(fn, tokens, experts, top_k)
     w = _Weights(fn, experts, N, N, K, weight_format, group_size, with_zeros, with_bias)
-    if first < 0:
-        raise ValueError(f"{fn}: first={first} must not be negative")
+    _first(fn, first, experts)
     _activations(fn, tokens, K)
     params = [KernelParam("h", w.dtype, (tokens * top_k, K)), *w.params]
     n = len(params)

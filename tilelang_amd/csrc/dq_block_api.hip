@@ -3,6 +3,7 @@
 #include "../../include/dqgemm.h"
 #include "dq_experts.h"
 
+#include <limits.h>
 #include <math.h>
 
 namespace dq {
@@ -112,7 +113,7 @@ extern "C" int call_experts_order(const void* Ids, void* Order, void* Starts, vo
                                   int experts, int first, dq_stream_t stream) {
   const char* const fn = "call_experts_order";
   if (check_pairs(fn, tokens, experts, top_k) != 0) return -1;
-  if (first < 0) DQ_FAIL("%s: first must not be negative (got %d)", fn, first);
+  if (first < 0 || first > INT_MAX - experts) DQ_FAIL("%s: first must be from 0 to 2^31 - 1 - experts=%d (got %d)", fn, experts, first);
   if (!Ids || !Order || !Starts) DQ_FAIL("%s: Ids, Order and Starts are expected to have non-NULL data pointers", fn);
   if (!on(Ids, 4) || !on(Order, 4) || !on(Starts, 4)) DQ_FAIL("%s: Ids, Order and Starts must be 4-byte aligned", fn);
   if (check_workspace(fn, Workspace, workspace_bytes, order_workspace_bytes(tokens, top_k, experts)) != 0) return -1;
@@ -143,7 +144,7 @@ extern "C" int call_experts_down(const void* H, const void* B, const void* Scale
                                  dq_stream_t stream) {
   const char* const fn = "call_experts_down";
   if (check_product(fn, H, B, Scale, Zeros, Bias, Order, Starts, C, tokens, experts, top_k, N, K, group_size, format) != 0) return -1;
-  if (first < 0) DQ_FAIL("%s: first must not be negative (got %d)", fn, first);
+  if (first < 0 || first > INT_MAX - experts) DQ_FAIL("%s: first must be from 0 to 2^31 - 1 - experts=%d (got %d)", fn, experts, first);
   if (!Ids || !Weights) DQ_FAIL("%s: Ids and Weights are expected to have non-NULL data pointers", fn);
   if (!on(Ids, 4) || !on(Weights, 4) || !on(Residual, 16)) DQ_FAIL("%s: Ids and Weights must be 4-byte and Residual 16-byte aligned", fn);
   if (check_workspace(fn, Workspace, workspace_bytes, dq_experts_down_workspace_bytes(tokens, top_k, N)) != 0) return -1;
