@@ -197,7 +197,7 @@ struct Pipeline {
   bool idle;
   unsigned char *words, *scales;
   const unsigned char* acts;
-  int acts_stride;
+  int acts_stride, act_row;
   uint4_t w_reg[DEPTH][4];
   static constexpr int kHalf = half_scales<W>();
   static constexpr bool kPairs = W::kScaleBytes == 1 && !LINES;       // from where two bytes lie, not four
@@ -238,10 +238,11 @@ struct Pipeline {
   }
 
   __device__ __forceinline__ Pipeline(const Args& args, const Source& source, int first, int begin, int end, bool nothing, unsigned char* area,
-                                      const unsigned char* rows, int stride)
+                                      const unsigned char* rows, int held, int stride)
       : a(args), from(source), c0(begin), c1(end), w_q(first), w_c(begin), idle(nothing), words(area), scales(area + kWordsArea), acts(rows), acts_stride(stride) {
     const int lane = threadIdx.x & 63;
     const unsigned row_bytes = (unsigned)a.K >> 1;
+    act_row = min(lane & 15, held - 1);  // (of the rows beyond those that LDS has room for, the last)
 #pragma unroll
     for (int i = 0; i < 2; ++i) w_at[i] = (unsigned)(8 * i + (lane >> 3)) * row_bytes + 16 * (lane & 7);
 #pragma unroll
@@ -292,7 +293,7 @@ struct Pipeline {
       for (int h = 0; h < 2; ++h) {
         typename W::frag x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const typename W::frag*>(acts + c * (2 * kChunk) + act_place(r, 16 * h + 4 * g + j, acts_stride));
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const typename W::frag*>(acts + c * (2 * kChunk) + act_place(act_row, 16 * h + 4 * g + j, acts_stride));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -411,7 +412,7 @@ __global__ __launch_bounds__((kWaves + 1) * 64, DEPTH == 1 ? 4 : 2) void rows_ke
     const unsigned pairs = (unsigned)a.Order[r0 + min(c, count - 1)];
     if (wave < kWaves) {
       const TilesOf<W> source(a, part.expert, rows, kColumns, second, tile1);
-      Pipeline<W, DEPTH, LINES, TilesOf<W>> p(a, source, tile0, chunks.c0, chunks.c1, chunks.idle, smem + wave * wave_area<W>(), acts, stride);
+      Pipeline<W, DEPTH, LINES, TilesOf<W>> p(a, source, tile0, chunks.c0, chunks.c1, chunks.idle, smem + wave * wave_area<W>(), acts, pass_rows, stride);
       // a wave a row; places of rows that the part does not have keep what was there: theirs of the result are not stored
       for (int m = wave; m < count; m += kWaves) {
         size_t row = r0 + m;
@@ -490,7 +491,7 @@ __global__ __launch_bounds__((kWaves + 1) * 64, 4) void few_pairs_kernel(const A
   if (wave < kWaves) {
     const Share chunks(a, wave);
     const ExpertsOf<W> source(a, n0, experts, max(count, 1));
-    Pipeline<W, 1, LINES, ExpertsOf<W>> p(a, source, 0, chunks.c0, chunks.c1, chunks.idle || count == 0, smem + wave * wave_area<W>(), acts, stride);
+    Pipeline<W, 1, LINES, ExpertsOf<W>> p(a, source, 0, chunks.c0, chunks.c1, chunks.idle || count == 0, smem + wave * wave_area<W>(), acts, a.pairs, stride);
     for (int m = wave; m < rows; m += kWaves) put_row<W>(a, m, acts, m, stride);
     __syncthreads();
     run<1>(p, blocks, sums, wave, done);
