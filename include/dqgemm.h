@@ -466,7 +466,7 @@ int call_experts_up(const void* X, const void* B, const void* Scale, const void*
  * [tokens][top_k]; B [experts][N][K / 2] and so on as above.  Pairs whose id is not one of first .. first + experts - 1 add
  * nothing.  Sums in fp32, a token's choices in their order whatever the timing.
  * Workspace: dq_experts_down_workspace_bytes(...) bytes, as above. */
-size_t dq_experts_down_workspace_bytes(int tokens, int top_k, int N);
+size_t dq_experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int group_size, int format);
 int call_experts_down(const void* H, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,
                       const void* Starts, const void* Ids, const void* Weights, const void* Residual, void* C, void* Workspace,
                       size_t workspace_bytes, int tokens, int experts, int top_k, int N, int K, int group_size, int format, int first,

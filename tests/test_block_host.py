@@ -170,7 +170,10 @@ def test_workspaces_are_named_without_a_gpu():
     assert order(1, 8, 128) == order(32, 8, 128) == order(64, 1, 8) == 0  # one workgroup has them all
     assert order(65, 1, 8) >= 5 * 8 * 2 and order(2**18, 32, 1024) <= 256 * 1024 * 2
     assert order(0, 8, 128) == order(2**30, 8, 128) == order(-1, 8, 128) == 0
-    assert down(4096, 2, 4096) == 4096 * 2 * 4096 * 4 and down(0, 2, 64) == 0 and down(2**30, 2, 64) == 0
+    # a value a pair, and slices of K where there are few tiles
+    assert down(4096, 8, 2, 4096, 14336, 128, EXPERTS_UINT4) == 4096 * 2 * 4096 * 4
+    assert down(64, 8, 2, 4096, 14336, 128, EXPERTS_UINT4) in (2 * 64 * 2 * 4096 * 4, 4 * 64 * 2 * 4096 * 4)
+    assert down(0, 8, 2, 64, 256, 128, EXPERTS_UINT4) == 0 and down(2**30, 8, 2, 64, 256, 32, EXPERTS_MXFP4) == 0
 
 
 def test_results_of_a_kernel_object():

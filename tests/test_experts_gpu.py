@@ -7,6 +7,7 @@ import torch
 
 import block_reference as ref
 import tilelang_amd as tl
+from tilelang_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -95,6 +96,20 @@ def test_sizes(cuda, tokens, experts, top_k, fmt, hidden, inter, whole):
 def test_many_rows(cuda, tokens, experts, top_k, how, hidden, inter, fmt):
     print(f"experts {tokens} of {experts} top {top_k} {how} {hidden} {inter} {fmt}", flush=True)
     _both(cuda, tokens, experts, top_k, hidden, inter, how, residual=tokens % 4 == 0, **fmt)
+
+
+@pytest.mark.parametrize("fmt,inter", [
+    (dict(), 4096), (dict(group_size=64, with_bias=True), 4224), (dict(group_size=32, with_zeros=True), 2176), (dict(with_zeros=True, with_bias=True), 8192),
+    (dict(weight_format="mxfp4"), 4096), (dict(weight_format="mxfp4", with_bias=True), 4224),
+], ids=str)
+@pytest.mark.parametrize("tokens,experts,top_k,how,hidden", [(500, 2, 1, "even", 1152), (330, 3, 2, "skewed", 1024), (520, 3, 1, "padded", 1152), (300, 2, 2, "one", 1152)])
+def test_slices_of_k(cuda, tokens, experts, top_k, how, hidden, fmt, inter):
+    """Few experts and columns: "down" cuts K into slices, of units of 256 and what is left."""
+    print(f"experts slices {tokens} of {experts} top {top_k} {how} {hidden} {inter} {fmt}", flush=True)
+    mx = fmt.get("weight_format") == "mxfp4"
+    room = _lib.load_library().dq_experts_down_workspace_bytes(tokens, experts, top_k, hidden, inter, fmt.get("group_size") or (32 if mx else 128), int(mx))
+    assert room in (2 * tokens * top_k * hidden * 4, 4 * tokens * top_k * hidden * 4)
+    _both(cuda, tokens, experts, top_k, hidden, inter, how, residual=tokens % 40 == 0, **fmt)
 
 
 @pytest.mark.parametrize("weight_format", ["uint4", "mxfp4"])

@@ -74,7 +74,7 @@ SIZE_QUERIES = {
     "dq_bitlinear_workspace_bytes": [_i, _i, _i, _i],
     "dq_paged_attention_workspace_bytes": [_i] * 8,
     "dq_experts_order_workspace_bytes": [_i] * 3,
-    "dq_experts_down_workspace_bytes": [_i] * 3,
+    "dq_experts_down_workspace_bytes": [_i] * 7,
 }
 
 

@@ -241,7 +241,7 @@ def experts_down(tokens: int, experts: int, top_k: int, N: int, K: int, weight_f
         params.append(KernelParam("Residual", w.dtype, (tokens, N)))
     out = len(params)
     params.append(KernelParam("y", w.dtype, (tokens, N)))
-    room = int(_lib.load_library().dq_experts_down_workspace_bytes(tokens, top_k, N))
+    room = int(_lib.load_library().dq_experts_down_workspace_bytes(tokens, experts, top_k, N, K, *w.ints))
     if room:
         params.append(KernelParam("Workspace", torch.uint8, (room,)))
     slots = (0, *w.slots(1), n, n + 1, n + 2, n + 3, n + 4 if residual else None, out, out + 1 if room else None)

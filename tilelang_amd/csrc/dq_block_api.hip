@@ -15,7 +15,7 @@ int route_experts(const void* Logits, const float* Bias, float* Weights, int* Id
                   int experts, int top_k, int sigmoid, int groups, int top_groups, int two, int renormalize, int dtype, float factor,
                   hipStream_t stream);
 int experts_order(const int* Ids, int* Order, int* Starts, void* Workspace, int tokens, int top_k, int experts, int first, hipStream_t stream);
-size_t experts_down_workspace_bytes(int tokens, int top_k, int N);
+size_t experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int mxfp4, int group_shift);
 int experts_up(const experts::Args& a, int mxfp4, hipStream_t stream);
 int experts_down(const experts::Args& a, int mxfp4, hipStream_t stream);
 
@@ -133,9 +133,9 @@ extern "C" int call_experts_up(const void* X, const void* B, const void* Scale, 
   return experts_up(a, format == DQ_EXPERTS_MXFP4, (hipStream_t)stream);
 }
 
-extern "C" size_t dq_experts_down_workspace_bytes(int tokens, int top_k, int N) {
-  if (tokens <= 0 || top_k <= 0 || N <= 0 || (long)tokens * top_k > kMaxPairs) return 0;
-  return experts_down_workspace_bytes(tokens, top_k, N);
+extern "C" size_t dq_experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int group_size, int format) {
+  if (tokens <= 0 || experts <= 0 || top_k <= 0 || N <= 0 || K < 64 || (long)tokens * top_k > kMaxPairs) return 0;
+  return experts_down_workspace_bytes(tokens, experts, top_k, N, K, format == DQ_EXPERTS_MXFP4, log2_of(group_size));
 }
 
 extern "C" int call_experts_down(const void* H, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,
@@ -147,7 +147,7 @@ extern "C" int call_experts_down(const void* H, const void* B, const void* Scale
   if (first < 0 || first > INT_MAX - experts) DQ_FAIL("%s: first must be from 0 to 2^31 - 1 - experts=%d (got %d)", fn, experts, first);
   if (!Ids || !Weights) DQ_FAIL("%s: Ids and Weights are expected to have non-NULL data pointers", fn);
   if (!on(Ids, 4) || !on(Weights, 4) || !on(Residual, 16)) DQ_FAIL("%s: Ids and Weights must be 4-byte and Residual 16-byte aligned", fn);
-  if (check_workspace(fn, Workspace, workspace_bytes, dq_experts_down_workspace_bytes(tokens, top_k, N)) != 0) return -1;
+  if (check_workspace(fn, Workspace, workspace_bytes, dq_experts_down_workspace_bytes(tokens, experts, top_k, N, K, group_size, format)) != 0) return -1;
   experts::Args a{};
   a.A = H, a.B = (const uint8_t*)B, a.S = Scale, a.Z = Zeros, a.Bias = Bias, a.Order = (const int*)Order, a.Starts = (const int*)Starts, a.Out = C;
   a.Ids = (const int*)Ids, a.Weights = (const float*)Weights, a.Residual = Residual, a.Parts = (float*)Workspace;

@@ -22,8 +22,8 @@ struct Args {
   const float* Weights;  // down: [pairs]
   const void* Residual;  // down: [tokens][N], or nullptr
   void* Out;           // up: [pairs][N]; down: [tokens][N]
-  float* Parts;        // down: fp32 [pairs][N], a pair's product
-  int tokens, experts, top_k, pairs, N, K, group_shift, gelu, first;
+  float* Parts;        // down: fp32 [slices][pairs][N], a pair's product, of a slice of K
+  int tokens, experts, top_k, pairs, N, K, group_shift, gelu, first, slices;
 };
 
 // Activations and weights of a product: uint4 codes x fp16, as the dense W4A16 kernels have them (rounded to fp16), and e2m1 x bf16.
@@ -73,6 +73,9 @@ __device__ __forceinline__ void rows_of(const Args& a, int e, int& begin, int& e
   begin = min(max(a.Starts[e], 0), a.pairs);
   end = min(max(a.Starts[e + 1], begin), a.pairs);
 }
+
+// K that is an odd number of blocks of 64, or a row's scales that are: rows of scales begin between dwords
+inline bool odd_rows(int mxfp4, int K, int group_shift) { return (K / 64) % 2 != 0 || (!mxfp4 && ((K >> group_shift) & 1) != 0); }
 
 }  // namespace experts
 }  // namespace dq

@@ -10,6 +10,8 @@
 // operations are carried out in their order, so there is no barrier.  The waves' sums meet in LDS at the end.
 #include "dq_experts.h"
 
+#include <math.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -549,8 +551,9 @@ __global__ __launch_bounds__((kWaves + 1) * 64, 4) void few_pairs_kernel(const A
   }
 }
 
-// A token's pairs added, in the order of its choices, onto the residual: four columns a thread, eight choices asked for at once.
-template <class T>
+// A token's pairs added, in the order of its choices and, of a choice's eight, of the slices, onto the residual: four columns a thread,
+// eight choices asked for at once.  (A loop over one slice cost a third: 4096 tokens, two choices, 4096 columns 31 -> 43 us.)
+template <class T, bool SLICES>
 __global__ __launch_bounds__(256) void sum_kernel(const Args a) {
   typedef T vec4 __attribute__((ext_vector_type(4)));
   const size_t token = (size_t)blockIdx.z * gridDim.y + blockIdx.y;
@@ -561,17 +564,19 @@ __global__ __launch_bounds__(256) void sum_kernel(const Args a) {
   if (a.Residual != nullptr) r = *reinterpret_cast<const vec4*>((const T*)a.Residual + at);
   float4_t v = {0.f, 0.f, 0.f, 0.f};
   for (int j0 = 0; j0 < a.top_k; j0 += 8) {
-    float4_t part[8];
-    unsigned id[8];
+    for (int z = 0; z < (SLICES ? a.slices : 1); ++z) {
+      float4_t part[8];
+      unsigned id[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const size_t pair = token * a.top_k + min(j0 + j, a.top_k - 1);
-      id[j] = (unsigned)a.Ids[pair] - (unsigned)a.first;
-      part[j] = *reinterpret_cast<const float4_t*>(a.Parts + pair * a.N + n);
+      for (int j = 0; j < 8; ++j) {
+        const size_t pair = token * a.top_k + min(j0 + j, a.top_k - 1);
+        id[j] = (unsigned)a.Ids[pair] - (unsigned)a.first;
+        part[j] = *reinterpret_cast<const float4_t*>(a.Parts + (SLICES ? (size_t)z * a.pairs * a.N : 0) + pair * a.N + n);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < a.top_k && id[j] < (unsigned)a.experts) v += part[j];  // (nobody has written another's)
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j0 + j < a.top_k && id[j] < (unsigned)a.experts) v += part[j];  // (nobody has written another's)
   }
   vec4 o;
 #pragma unroll
@@ -582,7 +587,8 @@ __global__ __launch_bounds__(256) void sum_kernel(const Args a) {
 template <class T>
 int sum(const Args& a, hipStream_t stream) {
   const int threads = a.N >= 1024 ? 256 : 64, tokens = std::min(a.tokens, 65535);
-  hipLaunchKernelGGL((sum_kernel<T>), dim3((a.N / 4 + threads - 1) / threads, tokens, (a.tokens + tokens - 1) / tokens), dim3(threads), 0, stream, a);
+  const auto kern = a.slices > 1 ? sum_kernel<T, true> : sum_kernel<T, false>;
+  hipLaunchKernelGGL(kern, dim3((a.N / 4 + threads - 1) / threads, tokens, (a.tokens + tokens - 1) / tokens), dim3(threads), 0, stream, a);
   DQ_CHECK_HIP(hipGetLastError());
   return 0;
 }
@@ -644,27 +650,52 @@ int product(const Args& a, hipStream_t stream) {
   return 0;
 }
 
-// Rows of a tile of the matrix pipe's kernel (dq_experts_tiles.hip), or 0: few rows an expert.  By the mean number of rows, of E experts
-// with N x K (us, "up", rows as here / tiles of 64 / of 128):
-//   uint4 8 of 4096 x 4096, 32 of 2880 x 2816, 128 of 1024 x 4096: 8 rows 38, 75, 121 here, 68, 121, 220 in tiles of 128;
-//     16 rows 48 / 47 / 64, 92 / 85 / 117, 179 / 158 / 232; 96 rows 186 / 81 / 99, 371 / 163 / 167, 768 / 329 / 347;
-//     128 rows 244 / 111 / 107, 486 / 208 / 208, 992 / 401 / 398; 512 rows 960 / 329 / 284, 1797 / 631 / 536
-//   MXFP4 (decoded with less): 16 rows 41 / 43 / 57, 82 / 117 / 111, 153 / 181 / 219; 32 rows 66 / 62 / 60, 123 / 125 / 131,
-//     262 / 205 / 249; 64 rows 115 / 72 / 64, 209 / 157 / 155, 454 / 268 / 270; 128 rows 202 / 107 / 99, 385 / 241 / 194
-// Tiles of 96 rows are between their neighbours everywhere, tiles of 256 ahead by 1 % at best (4096 tokens, two of 8 experts of
-// 14336 x 4096: 1719 and 1740) and eight waves on a tile of 128 nowhere.
-int tile_rows(const Args& a, int mxfp4) {
-  if (a.K < 128) return 0;
-  if (acts_stride(a.K) > kActsRoom) return 128;  // (a row does not fit)
-  const long mean = a.pairs / std::min(a.experts, a.pairs);
-  if (mxfp4) return mean < 28 ? 0 : mean < 64 ? 64 : 128;
-  return mean < 16 ? 0 : mean < 112 ? 64 : 128;
+// Which kernel has a product: this file's, or that of tiles of 64 or 128 rows (dq_experts_tiles.hip), and "down" of the latter in how
+// many slices of K.  What each would take is estimated from what bounds it, with experts that have the mean number of rows, and the
+// least is taken; the number of an expert's parts is one up to 0.7 of what a part holds, beyond that half a part more than the mean's.
+// * rows_kernel: the weights once a part, at 4.3 TB/s (uint4) and 5.2 (MXFP4, decoded with less);
+// * tiles: 7.5 and 12.5 ns a k of a tile that has its CU for itself, and all of them 43 and 66 ps a k (MXFP4 40 and 54); slices, down
+//   to 1024 k, while there are fewer than 256 workgroups, each with its results' way out and back (10 bytes at 5 TB/s a value).
+// Measured, us, rows_kernel / tiles of 64 / of 128 [in 2, 4 slices]:
+//   up uint4 8 experts of 4096 x 4096, 16 rows each: 48 / 47 / 64; 128 rows: 244 / 111 / 107; 128 of 1024 x 4096, 8 rows: 121 / - / 220;
+//     4 of 2048 x 8192, 32 rows: 77 / 67 / 91, 256 rows: 499 / 88 / 107; 8 of 1024 x 4096, 32 rows: 28 / 38 / 51
+//   down uint4 8 of 4096 x 14336, 2 rows: 64 / 121 / -; 32 rows: 391 / 132 [88, 84] / 176 [120, 118]; 128 rows: 1458 / 230 [208, 203] /
+//     211 [199, 192]; 384 rows: - / 529 / 413 [430, 445]; 16 of 8192 x 4096, 32 rows: 180 / 100 [101, 119] / 138
+//   down MXFP4 8 of 4096 x 14336, 4 rows: 64 / - [72, -]; 32 rows: 354 / 142 [84, 92] / 155; 96 rows: 980 / 164 [156, 160] / 185 [128, 130]
+// Over 120 such products the choice is 3 % behind the best of these on average.  Tiles of 96 rows are between their neighbours
+// everywhere, tiles of 256 ahead by 1 % at best (4096 tokens, two of 8 experts of 14336 x 4096: 1719 and 1740) and eight waves on a tile
+// of 128 nowhere.
+struct Plan {
+  int rows, slices;  // of a tile, 0: rows_kernel
+};
+Plan plan(long pairs, int experts, int N, int K, int mxfp4, int group_shift, bool zeros, bool up) {
+  const double live = std::min((long)experts, pairs), mean = pairs / live;
+  auto parts = [&](int rows) { return live * (mean <= 0.7 * rows ? 1.0 : mean / rows + 0.5); };
+  const double weights = (up ? 2.0 : 1.0) * N * K;
+  const int held = std::min(16, kActsRoom / acts_stride(K));  // rows of a part
+  Plan best{0, 1};
+  double least = INFINITY;
+  if (held > 0) least = parts(held) * weights * (0.5 + (mxfp4 ? 1 : zeros ? 4 : 2) / (double)(1 << group_shift)) / (mxfp4 ? 5.2e6 : 4.3e6);
+  if (K < 128) return best;  // (a tile takes two blocks of k)
+  for (const bool tall : {false, true}) {
+    const int rows = tall ? 128 : 64;
+    const double tiles = parts(rows) * ((N + (up ? 127 : 255)) / (up ? 128 : 256));
+    int slices = 1;
+    if (!up && !experts::odd_rows(mxfp4, K, group_shift))
+      while (slices < 4 && tiles * slices < 256 && K / (2 * slices) >= 1024) slices *= 2;
+    const double pipe = tiles * (mxfp4 ? (tall ? 54e-6 : 40e-6) : (tall ? 66e-6 : 43e-6)), alone = (tall ? 12.5e-3 : 7.5e-3) / slices;
+    const double us = K * std::max(pipe, alone) + (up ? 0.0 : slices * (double)pairs * N * 2e-6);
+    if (us < least) least = us, best = {rows, slices};
+  }
+  return best;
 }
 
 template <bool UP>
-int by_format(const Args& a, int mxfp4, hipStream_t stream) {
-  if (const int rows = tile_rows(a, mxfp4)) {
-    if (const int rc = experts_tiles(a, mxfp4, UP, rows, stream)) return rc;
+int by_format(Args a, int mxfp4, hipStream_t stream) {
+  const Plan by = plan(a.pairs, a.experts, a.N, a.K, mxfp4, a.group_shift, a.Z != nullptr, UP);
+  a.slices = by.slices;
+  if (by.rows != 0) {
+    if (const int rc = experts_tiles(a, mxfp4, UP, by.rows, stream)) return rc;
     if constexpr (!UP) return mxfp4 ? sum<bf16_t>(a, stream) : sum<half_t>(a, stream);
     return 0;
   }
@@ -676,7 +707,12 @@ int by_format(const Args& a, int mxfp4, hipStream_t stream) {
 
 }  // namespace
 
-size_t experts_down_workspace_bytes(int tokens, int top_k, int N) { return (size_t)tokens * top_k * N * 4; }
+// (with zero points or without: the same)
+size_t experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int mxfp4, int group_shift) {
+  const long pairs = (long)tokens * top_k;
+  const int slices = std::max(plan(pairs, experts, N, K, mxfp4, group_shift, false, false).slices, plan(pairs, experts, N, K, mxfp4, group_shift, true, false).slices);
+  return (size_t)slices * pairs * N * 4;
+}
 
 int experts_up(const Args& a, int mxfp4, hipStream_t stream) { return by_format<true>(a, mxfp4, stream); }
 int experts_down(const Args& a, int mxfp4, hipStream_t stream) { return by_format<false>(a, mxfp4, stream); }

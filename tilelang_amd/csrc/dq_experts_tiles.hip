@@ -1,6 +1,7 @@
 // The experts' products at many rows an expert: the direct-to-LDS GEMM of dq_gemm_core.h on tiles of 64 or 128 rows of one expert
 // by 256 of its weight rows (up: 128 of the gate and the 128 of the up projection that go with them, in blocks of 32, so that a
-// lane has both sums of a value).
+// lane has both sums of a value; down: or a slice of K of them, each slice with fp32 results of its own, which the sums of the tokens
+// add in their order).
 //
 // How many tiles there are is known on the device alone.  The grid has as many workgroups as there can be, every one counts the
 // experts' tiles and those beyond them end; the others go over the XCDs in runs, expert by expert, so that an XCD finds an expert's
@@ -18,7 +19,7 @@ using experts::Args;
 
 struct TileParams : gemm::Params {
   Args a;
-  int begin, expert;  // of the tile
+  int begin, expert, slice;  // of the tile
 };
 
 template <class Base, bool UP>
@@ -44,11 +45,12 @@ struct ExpertsPolicy : Base {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d, 64);
     // runs of tiles an XCD (workgroup id mod 8)
-    const int tiles = __builtin_amdgcn_readfirstlane(all) * p.tiles_n;
+    const int tiles_n = p.tiles_n * (UP ? 1 : a.slices);  // and slices of K
+    const int tiles = __builtin_amdgcn_readfirstlane(all) * tiles_n;
     const int x = bid & 7, i = bid >> 3, share = tiles >> 3, more = tiles & 7;
     if (i >= share + (x < more ? 1 : 0)) return false;
     const int pid = x * share + min(x, more) + i;
-    int row_tile = pid / p.tiles_n, before = 0;
+    int row_tile = pid / tiles_n, before = 0;
     for (int base = 0;; base += 64) {
       const int n = tiles_of(base + lane, begin, rows);
       int upto = n;
@@ -65,20 +67,37 @@ struct ExpertsPolicy : Base {
         p.M = __builtin_amdgcn_readlane(rows, at);
         const int tiles_m = __builtin_amdgcn_readlane(n, at);
         // the expert's tiles in bands of four tile rows, column by column inside a band
-        const int local = pid - (before + __builtin_amdgcn_readlane(upto, at) - tiles_m) * p.tiles_n;
-        const int band = 4 * p.tiles_n, first = local / band * 4, in_band = local % band, high = min(tiles_m - first, 4);
+        const int local = pid - (before + __builtin_amdgcn_readlane(upto, at) - tiles_m) * tiles_n;
+        const int band = 4 * tiles_n, first = local / band * 4, in_band = local % band, high = min(tiles_m - first, 4);
         m0 = (first + in_band % high) * tile_rows;
-        n0 = in_band / high * kColumns;
+        n0 = in_band / high;
         break;
       }
       before += __builtin_amdgcn_readlane(upto, 63);
     }
+    p.slice = 0;
+    if constexpr (!UP) {
+      p.slice = n0 % a.slices;
+      n0 /= a.slices;
+    }
+    n0 *= kColumns;
     const size_t weight_rows = (size_t)p.expert * p.N;
     p.B = (const unsigned char*)p.B + weight_rows * (a.K >> 1);
     const size_t scales = weight_rows * (a.K >> a.group_shift) * (Base::kScaleDma == 1 ? 1 : 2);
     p.S = (const unsigned char*)p.S + scales;
     if constexpr (Base::kScaleDma == 3) p.Z = (const unsigned char*)p.Z + scales;
     if constexpr (!UP) p.A = (const unsigned char*)p.A + ((size_t)p.begin + m0) * a.K * 2;
+    if constexpr (!UP) {
+      // whole units of 256 k: a row's scales of one begin at a dword, whatever its groups
+      const int units = a.K >> 8, k0 = units * p.slice / a.slices << 8;
+      if (p.slice + 1 < a.slices) p.K = units * (p.slice + 1) / a.slices << 8;
+      p.K -= k0;
+      p.A = (const unsigned char*)p.A + (size_t)k0 * 2;
+      p.B = (const unsigned char*)p.B + (k0 >> 1);
+      const int groups = Base::kScaleDma == 1 ? k0 >> 5 : k0 >> a.group_shift << 1;  // bytes
+      p.S = (const unsigned char*)p.S + groups;
+      if constexpr (Base::kScaleDma == 3) p.Z = (const unsigned char*)p.Z + groups;
+    }
     p.tiles_m = m0;
     return true;
   }
@@ -143,7 +162,7 @@ struct ExpertsPolicy : Base {
         for (int nb = 0; nb < NB; ++nb) {
           const int n = n0 + (wn * NB + nb) * 32;
           if (n >= a.N) break;
-          const float add = bias == nullptr ? 0.f : (float)bias[n + r];
+          const float add = bias == nullptr || p.slice != 0 ? 0.f : (float)bias[n + r];
 #pragma unroll
           for (int i = 0; i < 16; ++i) slab[(8 * (i >> 2) + 4 * g + (i & 3)) * kStride + r] = acc[mb][nb][i] + add;
           __builtin_amdgcn_wave_barrier();
@@ -151,7 +170,7 @@ struct ExpertsPolicy : Base {
           for (int it = 0; it < 4; ++it) {
             const int row = (lane + 64 * it) >> 3, piece = lane & 7;
             const float4_t v = *reinterpret_cast<const float4_t*>(slab + row * kStride + piece * 4);
-            if (pair[it] < (unsigned)a.pairs) *reinterpret_cast<float4_t*>(a.Parts + (size_t)pair[it] * a.N + n + piece * 4) = v * weight[it];
+            if (pair[it] < (unsigned)a.pairs) *reinterpret_cast<float4_t*>(a.Parts + ((size_t)p.slice * a.pairs + pair[it]) * a.N + n + piece * 4) = v * weight[it];
           }
           __builtin_amdgcn_wave_barrier();
         }
@@ -184,10 +203,10 @@ int tiles(const Args& a, int tile_rows, hipStream_t stream) {
   p.tiles_n = (a.N + P::kColumns - 1) / P::kColumns;
   // every expert's last tile may be a part of one
   const long row_tiles = a.pairs / tile_rows + (a.experts < a.pairs ? a.experts : a.pairs);
-  const long all = (row_tiles * p.tiles_n + 7) / 8 * 8;
+  const long all = (row_tiles * p.tiles_n * (UP ? 1 : a.slices) + 7) / 8 * 8;
   if (all >= 1l << 23) DQ_FAIL("experts: %d rows of %d columns: more tiles than a launch takes", a.pairs, a.N);  // (2^32 threads)
   const int workgroups = (int)all;
-  const bool odd = (a.K / 64) % 2 != 0 || (Base::kScaleDma >= 2 && ((a.K >> a.group_shift) & 1) != 0);
+  const bool odd = experts::odd_rows(Base::kScaleDma == 1, a.K, a.group_shift);
 #define DQ_TILES(BLOCKS_) (odd ? launch_tiles<P, BLOCKS_, true>(p, workgroups, stream) : launch_tiles<P, BLOCKS_, false>(p, workgroups, stream))
   return tile_rows == 64 ? DQ_TILES(2) : DQ_TILES(4);
 #undef DQ_TILES
