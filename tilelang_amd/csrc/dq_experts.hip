@@ -8,6 +8,10 @@
 // two chunks and two steps ahead, goes through LDS that it alone writes and reads into the order of the matrix instruction, whose
 // k are labelled 32 g + 8 j + e for its lane group g and the j-th of the step's four instructions, for both operands; its LDS
 // operations are carried out in their order, so there is no barrier.  The waves' sums meet in LDS at the end.
+//
+// Measured: one token, 8 of 128 experts, 1024 x 4096 uint4 "up" 10 us (3.4 TB/s; 17 with words straight into registers), 4096 x 1024 "down"
+// 9; 64 tokens, 4 of 32 experts, 2880 x 2880 MXFP4 61 to 68 and 37 us (4.3 and 3.9 TB/s: rows end inside cache lines, where lines are whole
+// it reaches 5.7).
 #include "dq_experts.h"
 
 #include <math.h>

@@ -566,9 +566,8 @@ struct BFragments<P, std::void_t<decltype(P::kBFragments)>> : std::integral_cons
 //   take_tile(p, bid, BM, m0, n0)   the tile of a workgroup: sets p.A, p.B, p.S, p.Z and p.M to those of its group; false: none
 //   a_row(p, m)       row of p.A of the group's row m (m0 on, of this tile)
 //   b_row(p, n0, row) weight row of the tile's row
-//   store<BLOCKS>(p, acc, smem, slab, lane, m0, n0, wn)   the epilogue of the wave of columns wn of the tile, over BLOCKS blocks of
-//                     32 rows from m0 on; slab: its number among the workgroup's waves
-// and is launched by its own code; direct-to-LDS variant only.
+//   store(p, acc, smem, wave, lane, m0, n0, wn)   the epilogue of the wave of columns wn of the tile, rows from m0 on
+// and is launched by its own code; direct-to-LDS variant only, one half.
 template <class P, class = void>
 struct Grouped : std::false_type {
   using params_t = Params;
@@ -637,6 +636,7 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
   typename Grouped<P>::params_t p = p_in;
   int bid = blockIdx.x;
   constexpr bool kGrouped = Grouped<P>::value;
+  static_assert(!kGrouped || kKHalves == 1, "groups: one half");
   if constexpr (!kGrouped) take_k_slice<P>(p, bid);
   extern __shared__ __align__(16) unsigned char smem[];
   static_assert(P::kBRowBytes == 32 || P::kBRowBytes == 64, "direct-to-LDS variant: 32 or 64 packed bytes per weight row per tile");
@@ -1156,10 +1156,7 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
     }
     __syncthreads();  // the epilogue's slabs lie where the sums were handed over
     const int first_row = m0 + 32 * kOwn0 * kh, slab_wave = wave + kWaves * kh;
-    if constexpr (kGrouped) {
-      if (kh == 0) P::template store<kOwn0>(p, acc, smem, slab_wave, lane, first_row, n0, wn);
-      else P::template store<kOwn1>(p, acc, smem, slab_wave, lane, first_row, n0, wn);
-    } else {
+    {
       const int m0 = first_row, wave = slab_wave;
       if constexpr (kOwn0 == kOwn1) {
         DQ_GEMM_EPILOGUE_OF(kOwn0)
@@ -1170,7 +1167,7 @@ __global__ __launch_bounds__(256 * kKHalves, 32 * kMBW * kWavesM <= 128 ? 2 : 1)
       }
     }
   } else if constexpr (kGrouped) {
-    P::template store<kMBW>(p, acc, smem, wave, lane, m0 + wm * (32 * kMBW), n0, wn);
+    P::store(p, acc, smem, wave, lane, m0 + wm * (32 * kMBW), n0, wn);
   } else {
     DQ_GEMM_EPILOGUE
   }

@@ -10,6 +10,9 @@
 // The order is a counting sort that keeps the pairs' order within an expert: chunks of tokens are counted where they are routed,
 // and with all chunks' counts every workgroup knows where its pairs of an expert begin.  Nothing depends on timing: the only
 // atomics are counts in LDS.
+//
+// What bounds it is instructions, a choice after the other.  Measured: one token, 8 of 128 5.6 us in one launch; 1021 tokens, 4 of 60 6.3 us and 5.6 for
+// the order; 8192 tokens, 8 of 256 in 4 of 8 groups with biases 28 and 10 (27 in all without biases, where nothing is done in 64 bits).
 #include "dq_kv.h"
 
 #include <type_traits>
