@@ -421,6 +421,11 @@ int call_paged_attention_decode(const void* Q, const void* KCache, const void* V
 int call_rms_norm(const void* X, const void* Residual, const void* Weight, void* Y, void* Sum, void* Scale, int rows, int dim,
                   int row_stride, int int8, int dtype, float eps, dq_stream_t stream);
 
+/* A router's logits: Logits [tokens][experts] fp32 = X [tokens][K] . W [experts][K]^T + Bias [experts] (or NULL), all three of dtype
+ * (DQ_DT_F16 or DQ_DT_BF16), sums in fp32.  K a multiple of 32, experts at most 1024, tokens at most 2^23. */
+int call_router_logits(const void* X, const void* W, const void* Bias, void* Logits, int tokens, int experts, int K, int dtype,
+                       dq_stream_t stream);
+
 enum dq_scores { DQ_SCORES_SOFTMAX = 0, DQ_SCORES_SIGMOID = 1 };
 enum dq_group_score { DQ_GROUP_MAX = 0, DQ_GROUP_SUM2 = 1 /* the sum of a group's two largest */ };
 

@@ -26,6 +26,10 @@ ROUTE, PRODUCT = dict(tokens=5, experts=16, top_k=2), dict(tokens=5, experts=16,
     (lambda: tl.rms_norm(2, 64, row_stride=56), "row_stride=56"),
     (lambda: tl.rms_norm(2, 64, row_stride=68), "row_stride=68"),
     (lambda: tl.rms_norm(2, 64, row_stride=2**31), "row_stride="),
+    (lambda: tl.router_logits(0, 16, 64), "tokens"),
+    (lambda: tl.router_logits(1, 1025, 64), "experts"),
+    (lambda: tl.router_logits(1, 16, 48), "K=48"),
+    (lambda: tl.router_logits(1, 16, 64, "float32"), "dtype must be"),
     (lambda: tl.route_experts(**ROUTE | {"tokens": 0}), "tokens"),
     (lambda: tl.route_experts(**ROUTE | {"experts": 1025}), "experts"),
     (lambda: tl.route_experts(**ROUTE | {"top_k": 33}), "top_k"),
@@ -66,7 +70,7 @@ def _operands(kernel, device="cpu"):
 
 
 @pytest.mark.parametrize("kernel", [
-    tl.rms_norm(3, 64), tl.rms_norm(3, 64, residual=True, int8=True), tl.route_experts(**ROUTE, bias=True), tl.route_experts(500, 16, 2), tl.experts_order(500, 2, 16),
+    tl.router_logits(3, 8, 64, with_bias=True), tl.rms_norm(3, 64), tl.rms_norm(3, 64, residual=True, int8=True), tl.route_experts(**ROUTE, bias=True), tl.route_experts(500, 16, 2), tl.experts_order(500, 2, 16),
     tl.experts_up(**PRODUCT, with_zeros=True, with_bias=True), tl.experts_down(**PRODUCT, weight_format="mxfp4", residual=True),
 ], ids=lambda k: k.name)
 def test_kernel_objects_refuse(kernel):
@@ -91,6 +95,7 @@ def _entry(name, **changed):
     sizes = dict(tokens=4, experts=8, top_k=2, N=64, K=256, group_size=64, format=EXPERTS_UINT4)
     args = {
         "call_rms_norm": dict(X=p, Residual=p, Weight=p, Y=p, Sum=p, Scale=p, rows=2, dim=64, row_stride=64, int8=1, dtype=DT_F16, eps=1e-6),
+        "call_router_logits": dict(X=p, W=p, Bias=None, Logits=p, tokens=2, experts=8, K=64, dtype=DT_F16),
         "call_route_experts": dict(Logits=p, Bias=p, Weights=p, Ids=p, Order=p, Starts=p, Workspace=None, bytes=0, tokens=4, experts=8, top_k=2, scores=0, groups=2,
                                    top_groups=1, group_score=1, renormalize=1, dtype=DT_F32, factor=1.0),
         "call_experts_order": dict(Ids=p, Order=p, Starts=p, Workspace=None, bytes=0, tokens=4, top_k=2, experts=8, first=0),
@@ -122,6 +127,15 @@ ODD = ctypes.c_void_p((1 << 20) + 2)
     ("call_rms_norm", dict(row_stride=56), "row_stride must be"),
     ("call_rms_norm", dict(dtype=DT_F32), "dtype must be"),
     ("call_rms_norm", dict(eps=-1.0), "eps must be"),
+    ("call_router_logits", dict(tokens=0), "tokens must be"),
+    ("call_router_logits", dict(tokens=(1 << 23) + 1), "at most"),
+    ("call_router_logits", dict(experts=1025), "experts must be"),
+    ("call_router_logits", dict(K=0), "K must be"),
+    ("call_router_logits", dict(K=40), "K must be"),
+    ("call_router_logits", dict(dtype=DT_F32), "dtype must be"),
+    ("call_router_logits", dict(Logits=None), "non-NULL"),
+    ("call_router_logits", dict(W=ODD), "16-byte"),
+    ("call_router_logits", dict(Bias=ctypes.c_void_p((1 << 20) + 1)), "2-byte"),
     ("call_route_experts", dict(tokens=0), "tokens must be"),
     ("call_route_experts", dict(tokens=1 << 30), "pairs in a call"),
     ("call_route_experts", dict(experts=2000), "experts must be"),

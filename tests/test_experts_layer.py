@@ -30,6 +30,8 @@ def _filled(gen, device="cpu", **more):
     args = dict(hidden=256, width=128, experts=6, top_k=2) | more
     layer = tl.W4Experts(**args)
     layer.router.copy_(torch.randn(layer.router.shape, generator=gen) / 16)
+    if layer.router_bias is not None:
+        layer.router_bias.copy_(torch.rand(layer.router_bias.shape, generator=gen))
     if layer.score_bias is not None:
         layer.score_bias.copy_(torch.rand(layer.score_bias.shape, generator=gen) / 4)
     for e in range(layer.held):
@@ -152,7 +154,7 @@ FORMATS = [dict(), dict(with_zeros=True, bias=True, group_size=64, activation="g
 @pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [1, 5, 150])
 @pytest.mark.parametrize("more", FORMATS, ids=["uint4", "zeros", "mxfp4"])
-@pytest.mark.parametrize("routing", [dict(), dict(scores="sigmoid", score_bias=True, groups=3, top_groups=2, group_score="sum2", factor=2.5)], ids=["softmax", "groups"])
+@pytest.mark.parametrize("routing", [dict(), dict(scores="sigmoid", router_bias=True, score_bias=True, groups=3, top_groups=2, group_score="sum2", factor=2.5)], ids=["softmax", "groups"])
 def test_layer(cuda, tokens, more, routing):
     """The layer's steps, each against the formulas on what the one before gave, and the whole against the steps."""
     print(f"layer {tokens} {more} {routing}", flush=True)
@@ -161,10 +163,12 @@ def test_layer(cuda, tokens, more, routing):
     dtype = layer.router.dtype
     x, r = (torch.randn((tokens, 256), generator=gen).to(dtype).to(cuda) for _ in range(2))
     product, route, sort, up, down, down_onto = layer._make(tokens)
-    logits = product(x, layer.router)
+    logits = product(x, layer.router, *([] if layer.router_bias is None else [layer.router_bias]))
     exact = x.cpu().double() @ layer.router.cpu().double().t()
+    if layer.router_bias is not None:
+        exact = exact + layer.router_bias.cpu().double()
     size = x.cpu().double().abs() @ layer.router.cpu().double().abs().t()
-    assert sort is None and ((logits.cpu().double() - exact).abs() <= 264 * 2.0**-24 * size).all()
+    assert sort is None and ((logits.cpu().double() - exact).abs() <= 274 * 2.0**-24 * (size + 1)).all()
     weights, ids, order, starts = route(logits) if layer.score_bias is None else route(logits, layer.score_bias)
     how = layer._routing
     want, shares = ref.route(logits, layer.score_bias, layer.top_k, how["scores"], how["groups"], how["top_groups"] or how["groups"], how["group_score"], how["renormalize"], how["factor"])
@@ -176,6 +180,20 @@ def test_layer(cuda, tokens, more, routing):
     assert ref.agrees(got, *ref.down(h, _held(layer, "down"), order, starts, weights, tokens, r), dtype)
     assert ref.agrees(plain, *ref.down(h, _held(layer, "down"), order, starts, weights, tokens, None), dtype)
     assert torch.equal(plain, given)
+
+
+@pytest.mark.gpu
+def test_many_logits_go_to_the_tiled_product(cuda, monkeypatch):
+    """From some number of logits on the layer's router is the tiled GEMM: the same sums in another order."""
+    gen = torch.Generator().manual_seed(6)
+    layer = _filled(gen, cuda)
+    x = torch.randn((90, 256), generator=gen).half().to(cuda)
+    few = layer._make(90)[0](x, layer.router)
+    monkeypatch.setattr(layers, "TILED_LOGITS", 512)
+    product = layer._make(90)[0]
+    size = x.cpu().double().abs() @ layer.router.cpu().double().abs().t()
+    assert product.name == "matmul" and ((product(x, layer.router) - few).cpu().double().abs() <= 2 * 264 * 2.0**-24 * size).all()
+    assert torch.isfinite(layer(x)).all()
 
 
 @pytest.mark.gpu

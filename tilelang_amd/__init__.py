@@ -40,6 +40,7 @@ from .block_kernels import (  # noqa: F401
     experts_up,
     rms_norm,
     route_experts,
+    router_logits,
 )
 from .bitlinear import BitLinear  # noqa: F401
 from .w4linear import W4A16Linear  # noqa: F401

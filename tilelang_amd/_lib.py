@@ -57,6 +57,7 @@ SIGNATURES = {
     "call_kv_cache_read": [_vp] * 7 + [_i] * 9 + [_vp],
     "call_paged_attention_decode": [_vp] * 11 + [ctypes.c_size_t] + [_i] * 10 + [ctypes.c_float, _vp],
     "call_rms_norm": [_vp] * 6 + [_i] * 5 + [ctypes.c_float, _vp],
+    "call_router_logits": [_vp] * 4 + [_i] * 4 + [_vp],
     "call_route_experts": [_vp] * 7 + [ctypes.c_size_t] + [_i] * 9 + [ctypes.c_float, _vp],
     "call_experts_order": [_vp] * 4 + [ctypes.c_size_t] + [_i] * 4 + [_vp],
     "call_experts_up": [_vp] * 8 + [_i] * 8 + [_vp],

@@ -4,7 +4,7 @@ experts' products.
 As in :mod:`kernels`, a factory takes sizes and types and returns a :class:`~tilelang_amd.adapter.KernelAdapter` bound to an
 entry point of ``libdqgemm.so`` (``include/dqgemm.h``); its call checks every operand and launches on torch's current stream.
 
-A layer of experts is four calls: ``weights, ids, order, starts = route_experts(...)(logits)`` chooses the experts of every token and
+A layer of experts is five calls: ``logits = router_logits(...)(x, W)``, ``weights, ids, order, starts = route_experts(...)(logits)`` chooses the experts of every token and
 sorts the pairs (token, choice) by expert, ``h = experts_up(...)(x, ..., order, starts)`` has a row for every pair in that order, and
 ``y = experts_down(...)(h, ..., order, starts, ids, weights)`` one for every token again.
 """
@@ -88,6 +88,22 @@ def _pairs(fn: str, tokens: int, experts: int, top_k: int) -> None:
         raise ValueError(f"{fn}: at most {MAX_EXPERTS} experts and top_k={MAX_TOP_K} (got {experts} and {top_k})")
     if tokens * top_k > MAX_PAIRS:
         raise ValueError(f"{fn}: {top_k} choices of {tokens} tokens: at most {MAX_PAIRS} pairs in a call")
+
+
+def router_logits(tokens: int, experts: int, K: int, dtype="float16", with_bias: bool = False) -> KernelAdapter:
+    """A router's logits: ``logits = kernel(x, W[, Bias])`` fp32 ``[tokens, experts]`` ``= x @ W.T (+ Bias)`` for ``x`` ``[tokens, K]``, ``W`` ``[experts, K]``
+    and ``Bias`` ``[experts]`` in fp16 or bf16; sums are fp32, ``K`` is a multiple of 32."""
+    fn = "router_logits"
+    _pairs(fn, tokens, experts, 1)
+    if K <= 0 or K % 32:
+        raise ValueError(f"{fn}: K={K} must be a positive multiple of 32")
+    held = _type16(fn, dtype)
+    params = [KernelParam("x", held, (tokens, K)), KernelParam("W", held, (experts, K))]
+    if with_bias:
+        params.append(KernelParam("Bias", held, (experts,)))
+    out = len(params)
+    params.append(KernelParam("logits", torch.float32, (tokens, experts)))
+    return _kernel(fn, "call_router_logits", params, [out], (0, 1, 2 if with_bias else None, out), (tokens, experts, K, DT_BF16 if held == torch.bfloat16 else DT_F16))
 
 
 def route_experts(tokens: int, experts: int, top_k: int, scores: str = "softmax", bias: bool = False, groups: int = 1, top_groups: int | None = None,

@@ -10,6 +10,7 @@ namespace dq {
 
 int rms_norm(const void* X, const void* Residual, const void* Weight, void* Y, void* Sum, float* Scale, int rows, int dim, long row_stride,
              int int8, int bf16, float eps, hipStream_t stream);
+int router_logits(const void* X, const void* W, const void* Bias, float* Logits, int tokens, int experts, int K, int bf16, hipStream_t stream);
 size_t order_workspace_bytes(int tokens, int top_k, int experts);
 int route_experts(const void* Logits, const float* Bias, float* Weights, int* Ids, int* Order, int* Starts, void* Workspace, int tokens,
                   int experts, int top_k, int sigmoid, int groups, int top_groups, int two, int renormalize, int dtype, float factor,
@@ -80,6 +81,17 @@ extern "C" int call_rms_norm(const void* X, const void* Residual, const void* We
   if (!on(X, 16) || !on(Residual, 16) || !on(Weight, 16) || !on(Y, 16) || !on(Sum, 16) || !on(Scale, 4))
     DQ_FAIL("%s: X, Residual, Weight, Y and Sum must be 16-byte and Scale 4-byte aligned", fn);
   return rms_norm(X, Residual, Weight, Y, Sum, (float*)Scale, rows, dim, row_stride, int8 != 0, dtype == DQ_DT_BF16, eps, (hipStream_t)stream);
+}
+
+extern "C" int call_router_logits(const void* X, const void* W, const void* Bias, void* Logits, int tokens, int experts, int K, int dtype,
+                                  dq_stream_t stream) {
+  const char* const fn = "call_router_logits";
+  if (check_pairs(fn, tokens, experts, 1) != 0) return -1;
+  if (K <= 0 || K % 32 != 0) DQ_FAIL("%s: K must be a positive multiple of 32 (got %d)", fn, K);
+  if (dtype != DQ_DT_F16 && dtype != DQ_DT_BF16) DQ_FAIL("%s: dtype must be DQ_DT_F16 or DQ_DT_BF16 (got %d)", fn, dtype);
+  if (!X || !W || !Logits) DQ_FAIL("%s: X, W and Logits are expected to have non-NULL data pointers", fn);
+  if (!on(X, 16) || !on(W, 16) || !on(Bias, 2) || !on(Logits, 4)) DQ_FAIL("%s: X and W must be 16-byte, Bias 2-byte and Logits 4-byte aligned", fn);
+  return router_logits(X, W, Bias, (float*)Logits, tokens, experts, K, dtype == DQ_DT_BF16, (hipStream_t)stream);
 }
 
 extern "C" size_t dq_experts_order_workspace_bytes(int tokens, int top_k, int experts) {

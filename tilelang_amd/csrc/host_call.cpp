@@ -94,6 +94,10 @@ const Entry kEntries[] = {
      [](void* fn, const Args& a) {
        return DQ_CALL(call_rms_norm)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.f, a.stream);
      }},
+    {"call_router_logits", 4, 4,
+     [](void* fn, const Args& a) {
+       return DQ_CALL(call_router_logits)(a.p[0], a.p[1], a.p[2], a.p[3], a.i[0], a.i[1], a.i[2], a.i[3], a.stream);
+     }},
     {"call_route_experts", 7, 9,
      [](void* fn, const Args& a) {
        return DQ_CALL(call_route_experts)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.ws, a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.i[8], a.f, a.stream);

@@ -17,6 +17,8 @@ from .w4linear import quantize_w4
 MAX_KERNELS = 64
 #: tokens that go through the experts at once; more go in parts, so that the rows between the two products take bounded memory
 MAX_TOKENS = 65536
+#: from this many logits on the tiled GEMM is ahead (4096 tokens, 256 experts, 7168 wide 57 us and 77; 16384, 32 of 2880 25 and 21)
+TILED_LOGITS = 2**20
 
 
 def _kept(held: dict, key, make):
@@ -90,7 +92,7 @@ class W4Experts(nn.Module):
     with the router's weights.
 
     ``hidden`` and ``width`` are the sizes outside and inside of an expert.  ``weight_format``, ``group_size``, ``with_zeros``, ``activation`` and
-    ``bias`` are as for :func:`experts_up`; ``scores``, ``score_bias``, ``groups``, ``top_groups``, ``group_score``, ``renormalize`` and ``factor`` as for
+    ``bias`` are as for :func:`experts_up`; the logits are ``x @ router.T``, with ``router_bias`` ``+ router_bias``; ``scores``, ``score_bias``, ``groups``, ``top_groups``, ``group_score``, ``renormalize`` and ``factor`` as for
     :func:`route_experts`.  Activations are fp16 with ``"uint4"`` weights, bf16 with ``"mxfp4"``; logits are fp32.
 
     ``first`` and ``held``: this layer has only the experts from ``first`` on, ``held`` of them (a rank of several that share a layer): its output
@@ -98,7 +100,7 @@ class W4Experts(nn.Module):
     """
 
     def __init__(self, hidden: int, width: int, experts: int, top_k: int, weight_format: str = "uint4", group_size: int | None = None,
-                 with_zeros: bool = False, activation: str = "silu", bias: bool = False, scores: str = "softmax", score_bias: bool = False,
+                 with_zeros: bool = False, activation: str = "silu", bias: bool = False, scores: str = "softmax", router_bias: bool = False, score_bias: bool = False,
                  groups: int = 1, top_groups: int | None = None, group_score: str = "max", renormalize: bool = True, factor: float = 1.0,
                  first: int = 0, held: int | None = None):
         super().__init__()
@@ -110,7 +112,7 @@ class W4Experts(nn.Module):
         mx = weight_format == "mxfp4"
         self.group_size = (32 if mx else 128) if group_size is None else group_size
         self._format = dict(weight_format=weight_format, group_size=self.group_size, with_zeros=with_zeros)
-        self._activation, self._bias = activation, bias
+        self._activation, self._bias, self._router_bias = activation, bias, router_bias
         self._routing = dict(scores=scores, bias=score_bias, groups=groups, top_groups=top_groups, group_score=group_score, renormalize=renormalize,
                              factor=factor)
         self._kernels: dict = {}
@@ -125,6 +127,7 @@ class W4Experts(nn.Module):
             self.register_buffer(name + "_bias", torch.zeros((held, rows), dtype=dtype) if bias else None)
 
         self.register_buffer("router", torch.zeros((experts, hidden), dtype=dtype))
+        self.register_buffer("router_bias", torch.zeros((experts,), dtype=dtype) if router_bias else None)
         self.register_buffer("score_bias", torch.zeros((experts,), dtype=torch.float32) if score_bias else None)
         packed("up", 2 * width, hidden)
         packed("down", hidden, width)
@@ -166,7 +169,11 @@ class W4Experts(nn.Module):
         """The kernel objects of a number of tokens: logits, choices, the order of this layer's experts where that is another, both products."""
         sizes = (tokens, self.held, self.top_k)
         dtype = "bfloat16" if self._format["weight_format"] == "mxfp4" else "float16"
-        return (kernels.matmul(tokens, self.experts, self.hidden, in_dtype=dtype, out_dtype="float32"),
+        if tokens * self.experts < TILED_LOGITS or self._router_bias:
+            logits = block_kernels.router_logits(tokens, self.experts, self.hidden, dtype, self._router_bias)
+        else:
+            logits = kernels.matmul(tokens, self.experts, self.hidden, in_dtype=dtype, out_dtype="float32")
+        return (logits,
                 block_kernels.route_experts(tokens, self.experts, self.top_k, **self._routing),
                 None if self.held == self.experts else block_kernels.experts_order(tokens, self.top_k, self.held, self.first),
                 block_kernels.experts_up(*sizes, self.width, self.hidden, activation=self._activation, with_bias=self._bias, **self._format),
@@ -175,7 +182,7 @@ class W4Experts(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, logits: torch.Tensor | None = None) -> torch.Tensor:
         """``x`` ``[..., hidden]`` -> the same; ``residual`` of that shape is added in the same launch.  ``logits`` fp32 ``[..., experts]``: in place of
-        ``x @ router.T``."""
+        the router's."""
         dtype = self.router.dtype
         rows = _whole(x.to(dtype).reshape(-1, self.hidden))
         r = None if residual is None else _whole(residual.to(dtype).reshape(-1, self.hidden))
@@ -190,7 +197,7 @@ class W4Experts(nn.Module):
     def _pass(self, x, residual, logits):
         product, route, sort, up, down, down_onto = _kept(self._kernels, x.shape[0], lambda: self._make(x.shape[0]))
         if logits is None:
-            logits = product(x, self.router)
+            logits = product(x, self.router, *(() if self.router_bias is None else (self.router_bias,)))
         weights, ids, order, starts = route(logits) if self.score_bias is None else route(logits, self.score_bias)
         if sort is not None:
             order, starts = sort(ids)
