@@ -4,9 +4,9 @@ experts' products.
 As in :mod:`kernels`, a factory takes sizes and types and returns a :class:`~tilelang_amd.adapter.KernelAdapter` bound to an
 entry point of ``libdqgemm.so`` (``include/dqgemm.h``); its call checks every operand and launches on torch's current stream.
 
-A layer of experts is five calls: ``logits = router_logits(...)(x, W)``, ``weights, ids, order, starts = route_experts(...)(logits)`` chooses the experts of every token and
-sorts the pairs (token, choice) by expert, ``h = experts_up(...)(x, ..., order, starts)`` has a row for every pair in that order, and
-``y = experts_down(...)(h, ..., order, starts, ids, weights)`` one for every token again.
+A layer of experts is four calls: ``logits = router_logits(...)(x, W)``; ``weights, ids, order, starts = route_experts(...)(logits)`` chooses
+the experts of every token and sorts the pairs (token, choice) by expert; ``h = experts_up(...)(x, ..., order, starts)`` has a row for
+every pair in that order, and ``y = experts_down(...)(h, ..., order, starts, ids, weights)`` one for every token again.
 """
 
 from __future__ import annotations

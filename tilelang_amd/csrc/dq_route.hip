@@ -39,7 +39,7 @@ struct OrderArgs {
   const int* Ids;
   int* Order;
   int* Starts;
-  uint16_t* Counts;  // [chunks][experts]; nullptr: one workgroup has all pairs
+  uint16_t* Counts;  // [chunks][experts, rounded up to four]; nullptr: one workgroup has all pairs
   int pairs, experts, first, chunk_pairs, chunks;
 };
 
@@ -283,6 +283,8 @@ __device__ __forceinline__ int route_token(const RouteArgs& a, long token, unsig
 
 constexpr int kFewPairs = 64;
 
+__host__ __device__ constexpr int counts_stride(int experts) { return (experts + 3) & ~3; }
+
 // Up to 64 pairs, a lane each, by one wave: a pair's place is how many have a lower expert, or its own and come earlier.
 __device__ void place_few(const OrderArgs& o, int id) {
   const int lane = threadIdx.x & 63;
@@ -311,7 +313,7 @@ __device__ void count_chunk(const OrderArgs& o, int chunk, int* count) {
     if ((unsigned)e < (unsigned)o.experts) atomicAdd(&count[e], 1);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < o.experts; e += kWaves * 64) o.Counts[(size_t)chunk * o.experts + e] = (uint16_t)count[e];
+  for (int e = threadIdx.x; e < o.experts; e += kWaves * 64) o.Counts[(size_t)chunk * counts_stride(o.experts) + e] = (uint16_t)count[e];
 }
 
 // The pairs of some chunks into their places.  `lds`: (kWaves + 2) experts + 64 ints.
@@ -335,24 +337,38 @@ __device__ void place(const OrderArgs& o, int workgroup, int workgroups, int* ld
   // one thread an expert: all pairs, those of earlier workgroups, and where every wave's begin among this one's
   int before = 0, all = 0;
   if (o.Counts != nullptr) {
-    // the chunks' counts by as many threads an expert as there are, their parts added where the totals go later
-    int wide = 64;
-    while (wide < E) wide *= 2;
-    const int e = tid & (wide - 1), slices = kWaves * 64 / wide;
-    int part = 0, early = 0;
+    // the chunks' counts by as many threads to four experts as there are, their parts added where the totals go later
+    int wide = 16;
+    while (wide * 4 < E) wide *= 2;
+    const int e = (tid & (wide - 1)) * 4, slices = kWaves * 64 / wide;
+    int part[4] = {0, 0, 0, 0}, early[4] = {0, 0, 0, 0};
     if (e < E) {
-#pragma unroll 16
-      for (int c = tid / wide; c < o.chunks; c += slices) {
-        const int n = o.Counts[(size_t)c * E + e];
-        part += n;
-        early += c < c0 ? n : 0;
+      const uint16_t* const counts = o.Counts + e;
+      auto add = [&](uint2_t four, int c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = (int)((four[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+          part[i] += n;
+          early[i] += c < c0 ? n : 0;
+        }
+      };
+      int c = tid / wide;
+      for (; c + 15 * slices < o.chunks; c += 16 * slices) {  // (all of them on their way at once)
+        uint2_t four[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) four[u] = *reinterpret_cast<const uint2_t*>(counts + (size_t)(c + u * slices) * counts_stride(E));
+#pragma unroll
+        for (int u = 0; u < 16; ++u) add(four[u], c + u * slices);
       }
+      for (; c < o.chunks; c += slices) add(*reinterpret_cast<const uint2_t*>(counts + (size_t)c * counts_stride(E)), c);
     }
     if (tid < E) total[tid] = 0, sums[64 + tid] = 0;
     __syncthreads();
-    if (e < E) {
-      atomicAdd(&total[e], part);
-      atomicAdd(&sums[64 + e], early);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (e + i >= E) break;
+      atomicAdd(&total[e + i], part[i]);
+      atomicAdd(&sums[64 + e + i], early[i]);
     }
     __syncthreads();
     if (tid < E) all = total[tid], before = sums[64 + tid];
@@ -493,7 +509,7 @@ int launch_place(const OrderArgs& o, hipStream_t stream) {
 
 size_t order_workspace_bytes(int tokens, int top_k, int experts) {
   OrderArgs o{};
-  return cut(o, tokens, top_k) ? ((size_t)o.chunks * experts * 2 + 15) / 16 * 16 : 0;
+  return cut(o, tokens, top_k) ? ((size_t)o.chunks * counts_stride(experts) * 2 + 15) / 16 * 16 : 0;
 }
 
 int route_experts(const void* Logits, const float* Bias, float* Weights, int* Ids, int* Order, int* Starts, void* Workspace, int tokens,
