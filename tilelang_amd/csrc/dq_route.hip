@@ -12,7 +12,8 @@
 // atomics are counts in LDS.
 //
 // What bounds it is instructions, a choice after the other.  Measured: one token, 8 of 128 5.6 us in one launch; 1021 tokens, 4 of 60 6.3 us and 5.6 for
-// the order; 8192 tokens, 8 of 256 in 4 of 8 groups with biases 28 and 10 (27 in all without biases, where nothing is done in 64 bits).
+// the order; 8192 tokens, 8 of 256 in 4 of 8 groups with biases 28 and 8.2 (25 in all without biases, where nothing is done in 64 bits: one token
+// that is adds 7, being the last).
 #include "dq_kv.h"
 
 #include <type_traits>
