@@ -11,9 +11,9 @@
 // and with all chunks' counts every workgroup knows where its pairs of an expert begin.  Nothing depends on timing: the only
 // atomics are counts in LDS.
 //
-// What bounds it is instructions, a choice after the other.  Measured: one token, 8 of 128 5.6 us in one launch; 1021 tokens, 4 of 60 6.3 us and 5.6 for
-// the order; 8192 tokens, 8 of 256 in 4 of 8 groups with biases 28 and 8.2 (25 in all without biases, where nothing is done in 64 bits: one token
-// that is adds 7, being the last).
+// What bounds it is instructions, a choice after the other.  Measured: one token, 8 of 128 5.6 us in one launch; 1021 tokens, 4 of 60
+// 5.8 us and 5.5 for the order; 8192 tokens, 8 of 256 in 4 of 8 groups with biases 24 and 8.2 (25 in all without biases, where nothing
+// is done in 64 bits: one token that is adds 3, being the last).
 #include "dq_kv.h"
 
 #include <type_traits>
@@ -95,21 +95,22 @@ __device__ __forceinline__ F exp_of(F x) {
   else return expf(x);
 }
 
-// One token's choices: lane j < top_k gets the j-th one and its score.  V > 0: logits and keys in registers, in fp32, V a lane.  V = 0,
-// in 64 bits: logits from memory and keys in LDS, so that what few tokens need takes no registers from all others.  `keys`: the wave's
-// LDS, an F an expert.  Returns whether F is too narrow to tell (the same in every lane).  A NaN counts as the largest of all: it is
+// One token's choices: lane j < top_k gets the j-th one and its score.  In fp32 logits and keys are in registers, V a lane; in 64 bits
+// logits come from memory and keys are made in LDS, one after the other, so that what few tokens need takes no registers from all
+// others, and chosen among in registers where that is no more than V = 4 (0: in LDS).  `keys`: the wave's LDS, an F an expert.  Returns whether F is too narrow to tell (the same in every lane).  A NaN counts as the largest of all: it is
 // chosen, and its weight shows it.
 template <class T, int V, class F>
-__device__ __forceinline__ bool choose(const RouteArgs& a, const T* logits, const float (&held)[V ? V : 1], F* keys, int& my_id, float& my_score) {
+__device__ __forceinline__ bool choose(const RouteArgs& a, const T* logits, const float* held, F* keys, int& my_id, float& my_score) {
   const int lane = threadIdx.x & 63;
   constexpr F kNone = -(F)__builtin_inff(), kMost = (F)__builtin_inff(), kGone = (F)__builtin_nanf("");
-  constexpr bool kNarrow = V > 0;
-  constexpr int kUnroll = V ? V : 1;
-  const int n = V ? V : (a.experts + 63) / 64;  // experts a lane
+  constexpr bool kNarrow = std::is_same<F, float>::value;
+  static_assert(V > 0 || !kNarrow, "fp32 keys are in registers");
+  constexpr int kUnroll = kNarrow ? V : 1, kRounds = V ? V : 1;
+  const int n = kNarrow ? V : (a.experts + 63) / 64;  // experts a lane
   const bool by_score = a.Bias != nullptr;
   bool close = false;
   const auto x = [&](int i) -> float {
-    if constexpr (V) return held[i];
+    if constexpr (kNarrow) return held[i];
     else return i * 64 + lane < a.experts ? (float)logits[i * 64 + lane] : 0.f;
   };
 
@@ -135,29 +136,39 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* logits, cons
   };
   const float slack = a.sigmoid ? 0x1p-19f : total == 0 ? 0.f : 0x1p-17f / (float)total;
   // what an expert is chosen by, and what its group counts by
-  const auto key_of = [&](int i) -> F {
-    const int e = i * 64 + lane;
-    F k = (F)x(i);
-    if (by_score) k = score_of(x(i)) + (F)(e < a.experts ? a.Bias[e] : 0.f);
+  const auto bias = [&](int i) -> float { return by_score && i * 64 + lane < a.experts ? a.Bias[i * 64 + lane] : 0.f; };
+  const auto key_from = [&](float v, float add) -> F {
+    const F k = by_score ? score_of(v) + (F)add : (F)v;
     return k != k ? kMost : k;
   };
+  const auto key_of = [&](int i) -> F { return key_from(x(i), bias(i)); };
   const auto group_key_of = [&](int i, F key) -> F {
     if (!a.two || by_score) return key;
     const F k = score_of(x(i));
     return k != k ? kMost : k;
   };
   // a key that is not to be chosen (any more) is NaN
-  F key[kUnroll];
+  F key[kRounds];
   const auto at = [&](int i) -> F {
-    if constexpr (V) return key[i];
+    if constexpr (kNarrow) return key[i];
     else return i * 64 + lane < a.experts ? keys[i * 64 + lane] : kGone;
   };
   const auto put = [&](int i, F k) {
-    if constexpr (V) key[i] = k;
+    if constexpr (kNarrow) key[i] = k;
     else if (i * 64 + lane < a.experts) keys[i * 64 + lane] = k;
   };
-#pragma unroll kUnroll
-  for (int i = 0; i < n; ++i) put(i, i * 64 + lane < a.experts ? key_of(i) : kGone);
+  if constexpr (kNarrow) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) put(i, i * 64 + lane < a.experts ? key_of(i) : kGone);
+  } else {
+    // (the next one's operands on their way)
+    float v = x(0), add = bias(0);
+    for (int i = 0; i < n; ++i) {
+      const float next_v = x(i + 1), next_add = bias(i + 1);
+      put(i, key_from(v, add));
+      v = next_v, add = next_add;
+    }
+  }
 
   if (a.groups > 1) {
     const int size = a.experts / a.groups;
@@ -206,20 +217,28 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* logits, cons
     for (int i = 0; i < n; ++i) {
       const int g = (int)(((float)(i * 64 + lane) + 0.5f) * inverse);
       F k = kGone;
-      if (i * 64 + lane < a.experts && ((taken >> (g & 63)) & 1)) k = V || by_score || !a.two ? at(i) : key_of(i);
+      if (i * 64 + lane < a.experts && ((taken >> (g & 63)) & 1)) k = kNarrow || by_score || !a.two ? at(i) : key_of(i);
       put(i, k);
     }
   }
 
+  if constexpr (!kNarrow && V > 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = at(i);
+  }
+
   F last = 0;
-  for (int r = 0; r < a.top_k + (by_score ? 1 : 0); ++r) {
+  for (int r = 0; r < a.top_k + (kNarrow && by_score ? 1 : 0); ++r) {
     F best = kGone;
     int own = 0;  // (V = 0 alone: which of the lane's experts that is, the first)
-#pragma unroll kUnroll
-    for (int i = 0; i < n; ++i) {
-      const F k = at(i);
-      if constexpr (V) best = fmax(best, k);
-      else if (k > best || !(best == best)) best = k, own = i;
+    if constexpr (V) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) best = fmax(best, key[i]);
+    } else {
+      for (int i = 0; i < n; ++i) {
+        const F k = at(i);
+        if (k > best || !(best == best)) best = k, own = i;
+      }
     }
     const F most = best;
     best = max_over_wave(best);
@@ -265,8 +284,7 @@ __device__ __forceinline__ int route_token(const RouteArgs& a, long token, unsig
   float score = 0.f;
   const T* const logits = (const T*)a.Logits + token * a.experts;
   if (choose<T, V, float>(a, logits, x, (float*)lds, id, score)) {
-    const float none[1] = {0.f};
-    choose<T, 0, double>(a, logits, none, (double*)lds, id, score);
+    choose<T, V <= 4 ? V : 0, double>(a, logits, nullptr, (double*)lds, id, score);
   }
   const bool mine = lane < a.top_k;
   if (a.renormalize) {
