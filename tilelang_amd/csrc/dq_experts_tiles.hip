@@ -7,7 +7,7 @@
 // experts' tiles and those beyond them end; the others go over the XCDs in runs, expert by expert, so that an XCD finds an expert's
 // rows and weights in its own L2 cache.  Rows of "up" are gathered where they are loaded: a lane's source address is its row's own.
 // What bounds it is the matrix pipe: 4096 tokens, two of 8 experts, uint4, 14336 x 4096 "up" 1.75 ms, 1.1 PFLOP/s, 4096 x 14336 "down"
-// 1.02 ms, 0.94 (1088 tiles on the 512 places of two workgroups a CU: the third round is a short one).
+// 1.02 ms, 0.94 (1088 tiles on the 512 places of two workgroups a CU: the last 64 have the chip for themselves).
 #include "dq_experts.h"
 #include "dq_gemm_mx.h"
 #include "dq_gemm_w4.h"
