@@ -460,22 +460,23 @@ enum dq_activation { DQ_ACT_SILU = 0, DQ_ACT_GELU = 1 /* the tanh form */ };
  * low nibble; Scale [experts][2 N][K / group_size]; Bias [experts][2 N] or NULL.
  * DQ_EXPERTS_UINT4: fp16; weights as call_dequantize_gemv_w4a16's, fp16((q - 8) * s), or with Zeros (fp16, as Scale)
  * fp16(fp16(q - z) * s); group_size 32, 64 or 128; K % 128 == 0.  DQ_EXPERTS_MXFP4: bf16; e2m1 codes times 2^(Scale - 127), Scale
- * uint8, group_size 32; K % 64 == 0.  N % 32 == 0.  Sums in fp32.  Order and Starts are what the calls above write; whatever they
+ * uint8, group_size 32; K % 64 == 0.  N % 32 == 0.  Sums in fp32.  routed: of how many experts the ids are, experts or
+ * more where this GPU has some of them; which kernel is taken goes by it, and nothing else.  Order and Starts are what the calls above write; whatever they
  * hold, nothing outside of the buffers is read or written. */
 int call_experts_up(const void* X, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,
                     const void* Starts, void* H, int tokens, int experts, int top_k, int N, int K, int group_size, int format,
-                    int activation, dq_stream_t stream);
+                    int activation, int routed, dq_stream_t stream);
 
 /* The way back: C[t] = Residual[t] + sum over the token's choices j of Weights[t][j] * (H[p] . D_e^T + bias), p the pair's row in
  * the sorted order and e its expert.  H [tokens * top_k][K], C [tokens][N], Residual [tokens][N] or NULL, Weights fp32 and Ids
  * [tokens][top_k]; B [experts][N][K / 2] and so on as above.  Pairs whose id is not one of first .. first + experts - 1 add
  * nothing.  Sums in fp32, a token's choices in their order whatever the timing.
  * Workspace: dq_experts_down_workspace_bytes(...) bytes, as above. */
-size_t dq_experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int group_size, int format);
+size_t dq_experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int group_size, int format, int routed);
 int call_experts_down(const void* H, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,
                       const void* Starts, const void* Ids, const void* Weights, const void* Residual, void* C, void* Workspace,
                       size_t workspace_bytes, int tokens, int experts, int top_k, int N, int K, int group_size, int format, int first,
-                      dq_stream_t stream);
+                      int routed, dq_stream_t stream);
 
 /* ---- diagnostics ------------------------------------------------------------------------------------- */
 

@@ -57,6 +57,8 @@ ROUTE, PRODUCT = dict(tokens=5, experts=16, top_k=2), dict(tokens=5, experts=16,
     (lambda: tl.experts_up(**PRODUCT, weight_format="mxfp4", with_zeros=True), "zero points"),
     (lambda: tl.experts_up(**PRODUCT, activation="relu"), "activation must be"),
     (lambda: tl.experts_down(**PRODUCT, first=-3), "first=-3"),
+    (lambda: tl.experts_up(**PRODUCT, routed=15), "routed=15"),
+    (lambda: tl.experts_down(**PRODUCT, routed=2**31), "routed="),
     (lambda: tl.experts_down(**PRODUCT | {"K": 0}), "K=0"),
 ])
 def test_factories_refuse(make, match):
@@ -99,8 +101,8 @@ def _entry(name, **changed):
         "call_route_experts": dict(Logits=p, Bias=p, Weights=p, Ids=p, Order=p, Starts=p, Workspace=None, bytes=0, tokens=4, experts=8, top_k=2, scores=0, groups=2,
                                    top_groups=1, group_score=1, renormalize=1, dtype=DT_F32, factor=1.0),
         "call_experts_order": dict(Ids=p, Order=p, Starts=p, Workspace=None, bytes=0, tokens=4, top_k=2, experts=8, first=0),
-        "call_experts_up": dict(X=p, **product, H=p, **sizes, activation=0),
-        "call_experts_down": dict(H=p, **product, Ids=p, Weights=p, Residual=p, C=p, Workspace=p, bytes=1 << 30, **sizes, first=0),
+        "call_experts_up": dict(X=p, **product, H=p, **sizes, activation=0, routed=8),
+        "call_experts_down": dict(H=p, **product, Ids=p, Weights=p, Residual=p, C=p, Workspace=p, bytes=1 << 30, **sizes, first=0, routed=8),
     }[name]
     assert set(changed) <= set(args)
     args |= changed
@@ -167,6 +169,8 @@ ODD = ctypes.c_void_p((1 << 20) + 2)
     ("call_experts_up", dict(Bias=ODD), "16-byte"),
     ("call_experts_up", dict(Order=ctypes.c_void_p((1 << 20) + 1)), "4-byte"),
     ("call_experts_up", dict(activation=2), "unknown activation"),
+    ("call_experts_up", dict(routed=7), "routed must be"),
+    ("call_experts_down", dict(routed=0), "routed must be"),
     ("call_experts_down", dict(Weights=None), "non-NULL"),
     ("call_experts_down", dict(Residual=ODD), "16-byte"),
     ("call_experts_down", dict(first=-1), "first must be"),
@@ -185,9 +189,10 @@ def test_workspaces_are_named_without_a_gpu():
     assert order(65, 1, 8) >= 5 * 8 * 2 and order(2**18, 32, 1024) <= 256 * 1024 * 2
     assert order(0, 8, 128) == order(2**30, 8, 128) == order(-1, 8, 128) == 0
     # a value a pair, and slices of K where there are few tiles
-    assert down(4096, 8, 2, 4096, 14336, 128, EXPERTS_UINT4) == 4096 * 2 * 4096 * 4
-    assert down(64, 8, 2, 4096, 14336, 128, EXPERTS_UINT4) in (2 * 64 * 2 * 4096 * 4, 4 * 64 * 2 * 4096 * 4)
-    assert down(0, 8, 2, 64, 256, 128, EXPERTS_UINT4) == 0 and down(2**30, 8, 2, 64, 256, 32, EXPERTS_MXFP4) == 0
+    assert down(4096, 8, 2, 4096, 14336, 128, EXPERTS_UINT4, 8) == 4096 * 2 * 4096 * 4
+    assert down(64, 8, 2, 4096, 14336, 128, EXPERTS_UINT4, 8) in (2 * 64 * 2 * 4096 * 4, 4 * 64 * 2 * 4096 * 4)
+    assert down(0, 8, 2, 64, 256, 128, EXPERTS_UINT4, 8) == 0 and down(2**30, 8, 2, 64, 256, 32, EXPERTS_MXFP4, 8) == 0
+    assert down(64, 8, 2, 4096, 14336, 128, EXPERTS_UINT4, 64) == 64 * 2 * 4096 * 4  # (two rows an expert: no tiles)
 
 
 def test_results_of_a_kernel_object():

@@ -107,7 +107,7 @@ def test_slices_of_k(cuda, tokens, experts, top_k, how, hidden, fmt, inter):
     """Few experts and columns: "down" cuts K into slices, of units of 256 and what is left."""
     print(f"experts slices {tokens} of {experts} top {top_k} {how} {hidden} {inter} {fmt}", flush=True)
     mx = fmt.get("weight_format") == "mxfp4"
-    room = _lib.load_library().dq_experts_down_workspace_bytes(tokens, experts, top_k, hidden, inter, fmt.get("group_size") or (32 if mx else 128), int(mx))
+    room = _lib.load_library().dq_experts_down_workspace_bytes(tokens, experts, top_k, hidden, inter, fmt.get("group_size") or (32 if mx else 128), int(mx), experts)
     assert room in (2 * tokens * top_k * hidden * 4, 4 * tokens * top_k * hidden * 4)
     _both(cuda, tokens, experts, top_k, hidden, inter, how, residual=tokens % 40 == 0, **fmt)
 

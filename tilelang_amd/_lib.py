@@ -60,8 +60,8 @@ SIGNATURES = {
     "call_router_logits": [_vp] * 4 + [_i] * 4 + [_vp],
     "call_route_experts": [_vp] * 7 + [ctypes.c_size_t] + [_i] * 9 + [ctypes.c_float, _vp],
     "call_experts_order": [_vp] * 4 + [ctypes.c_size_t] + [_i] * 4 + [_vp],
-    "call_experts_up": [_vp] * 8 + [_i] * 8 + [_vp],
-    "call_experts_down": [_vp] * 12 + [ctypes.c_size_t] + [_i] * 8 + [_vp],
+    "call_experts_up": [_vp] * 8 + [_i] * 9 + [_vp],
+    "call_experts_down": [_vp] * 12 + [ctypes.c_size_t] + [_i] * 9 + [_vp],
     "call_gemm_mxfp4_mxfp4": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
 }
 
@@ -75,7 +75,7 @@ SIZE_QUERIES = {
     "dq_bitlinear_workspace_bytes": [_i, _i, _i, _i],
     "dq_paged_attention_workspace_bytes": [_i] * 8,
     "dq_experts_order_workspace_bytes": [_i] * 3,
-    "dq_experts_down_workspace_bytes": [_i] * 7,
+    "dq_experts_down_workspace_bytes": [_i] * 8,
 }
 
 

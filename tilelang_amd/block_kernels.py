@@ -206,13 +206,20 @@ class _Weights:
         return (first, first + 1, None if self.zeros is None else first + self.zeros, None if self.bias is None else first + self.bias)
 
 
+def _routed(fn: str, routed: int | None, experts: int) -> int:
+    routed = experts if routed is None else routed
+    if not experts <= routed < 2**31:
+        raise ValueError(f"{fn}: routed={routed} must be at least experts={experts}")
+    return routed
+
+
 def _activations(fn: str, rows: int, width: int) -> None:
     if rows * width > MAX_ELEMENTS:
         raise ValueError(f"{fn}: {rows} tokens of {width} elements: at most 2^30 elements")
 
 
 def experts_up(tokens: int, experts: int, top_k: int, N: int, K: int, weight_format: str = "uint4", group_size: int | None = None,
-               with_zeros: bool = False, activation: str = "silu", with_bias: bool = False) -> KernelAdapter:
+               with_zeros: bool = False, activation: str = "silu", with_bias: bool = False, routed: int | None = None) -> KernelAdapter:
     """The experts' gate and up projections: ``h = kernel(x, B, Scale[, Zeros][, Bias], order, starts)``, ``x`` ``[tokens, K]``, ``h`` ``[tokens *
     top_k, N]``: row ``p`` is ``act(x[t] @ gate.T + gate_bias) * (x[t] @ up.T + up_bias)`` for token ``t = order[p] // top_k`` and the expert
     whose rows are about ``p``.  Rows behind ``starts[experts]`` are not written.
@@ -221,33 +228,36 @@ def experts_up(tokens: int, experts: int, top_k: int, N: int, K: int, weight_for
     activations and the weights of :func:`dequantize_gemv` with ``source_format="int"`` (``Scale`` fp16 ``[experts, 2 N, K / group_size]``,
     groups of 32, 64 or 128) or, ``with_zeros``, ``"uint"`` codes with fp16 zero points; or ``"mxfp4"``, bf16 activations and the weights of
     :func:`matmul_bf16_mxfp4` with ``weight_format="e2m1"`` and ``scale_bias=127``.  ``activation``: ``"silu"`` or ``"gelu"`` (the tanh form).
-    ``K`` is a multiple of 128 (mxfp4: 64), ``N`` of 32.  Sums are fp32.
+    ``K`` is a multiple of 128 (mxfp4: 64), ``N`` of 32.  Sums are fp32.  ``routed``: of how many experts the ids are, where these are some of
+    them: which kernel is taken goes by it, and nothing else.
     """
     fn = "experts_up"
     _pairs(fn, tokens, experts, top_k)
     w = _Weights(fn, experts, 2 * N, N, K, weight_format, group_size, with_zeros, with_bias)
     act = _one_of(fn, "activation", activation, ACTIVATIONS)
+    routed = _routed(fn, routed, experts)
     _activations(fn, tokens, K)
     params = [KernelParam("x", w.dtype, (tokens, K)), *w.params]
     n = len(params)
     params += [KernelParam("order", torch.int32, (tokens * top_k,)), KernelParam("starts", torch.int32, (experts + 1,)),
                KernelParam("h", w.dtype, (tokens * top_k, N))]
-    return _kernel(fn, "call_experts_up", params, [n + 2], (0, *w.slots(1), n, n + 1, n + 2), (tokens, experts, top_k, N, K, *w.ints, act))
+    return _kernel(fn, "call_experts_up", params, [n + 2], (0, *w.slots(1), n, n + 1, n + 2), (tokens, experts, top_k, N, K, *w.ints, act, routed))
 
 
 def experts_down(tokens: int, experts: int, top_k: int, N: int, K: int, weight_format: str = "uint4", group_size: int | None = None,
-                 with_zeros: bool = False, with_bias: bool = False, residual: bool = False, first: int = 0) -> KernelAdapter:
+                 with_zeros: bool = False, with_bias: bool = False, residual: bool = False, first: int = 0, routed: int | None = None) -> KernelAdapter:
     """The way back from the experts: ``y = kernel(h, B, Scale[, Zeros][, Bias], order, starts, ids, weights[, Residual])``, ``h`` ``[tokens *
     top_k, K]`` in the sorted order, ``y`` ``[tokens, N]``: a token's choices, each ``h[p] @ down.T + bias`` times its weight, added in their
     order, onto ``Residual`` ``[tokens, N]`` (``residual``).
 
     ``B`` ``[experts, N, K / 2]``, ``Bias`` ``[experts, N]``, formats as for :func:`experts_up`.  ``first``: the id of the first of these experts,
-    as for :func:`experts_order`; choices of other ids add nothing.  Sums are fp32; a call gives the same bits every time.
+    as for :func:`experts_order`, ``routed`` as for :func:`experts_up`; choices of other ids add nothing.  Sums are fp32; a call gives the same bits every time.
     """
     fn = "experts_down"
     _pairs(fn, tokens, experts, top_k)
     w = _Weights(fn, experts, N, N, K, weight_format, group_size, with_zeros, with_bias)
     _first(fn, first, experts)
+    routed = _routed(fn, routed, experts)
     _activations(fn, tokens, K)
     params = [KernelParam("h", w.dtype, (tokens * top_k, K)), *w.params]
     n = len(params)
@@ -257,8 +267,8 @@ def experts_down(tokens: int, experts: int, top_k: int, N: int, K: int, weight_f
         params.append(KernelParam("Residual", w.dtype, (tokens, N)))
     out = len(params)
     params.append(KernelParam("y", w.dtype, (tokens, N)))
-    room = int(_lib.load_library().dq_experts_down_workspace_bytes(tokens, experts, top_k, N, K, *w.ints))
+    room = int(_lib.load_library().dq_experts_down_workspace_bytes(tokens, experts, top_k, N, K, *w.ints, routed))
     if room:
         params.append(KernelParam("Workspace", torch.uint8, (room,)))
     slots = (0, *w.slots(1), n, n + 1, n + 2, n + 3, n + 4 if residual else None, out, out + 1 if room else None)
-    return _kernel(fn, "call_experts_down", params, [out], slots, (tokens, experts, top_k, N, K, *w.ints, first), None, room, [out + 1] if room else [])
+    return _kernel(fn, "call_experts_down", params, [out], slots, (tokens, experts, top_k, N, K, *w.ints, first, routed), None, room, [out + 1] if room else [])

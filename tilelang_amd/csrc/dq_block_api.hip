@@ -16,7 +16,7 @@ int route_experts(const void* Logits, const float* Bias, float* Weights, int* Id
                   int experts, int top_k, int sigmoid, int groups, int top_groups, int two, int renormalize, int dtype, float factor,
                   hipStream_t stream);
 int experts_order(const int* Ids, int* Order, int* Starts, void* Workspace, int tokens, int top_k, int experts, int first, hipStream_t stream);
-size_t experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int mxfp4, int group_shift);
+size_t experts_down_workspace_bytes(int tokens, int experts, int routed, int top_k, int N, int K, int mxfp4, int group_shift);
 int experts_up(const experts::Args& a, int mxfp4, hipStream_t stream);
 int experts_down(const experts::Args& a, int mxfp4, hipStream_t stream);
 
@@ -42,8 +42,9 @@ int check_workspace(const char* fn, const void* Workspace, size_t have, size_t n
 }
 
 int check_product(const char* fn, const void* A, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,
-                  const void* Starts, const void* Out, int tokens, int experts, int top_k, int N, int K, int group_size, int format) {
+                  const void* Starts, const void* Out, int tokens, int experts, int top_k, int N, int K, int group_size, int format, int routed) {
   if (check_pairs(fn, tokens, experts, top_k) != 0) return -1;
+  if (routed < experts) DQ_FAIL("%s: routed must be at least experts=%d (got %d)", fn, experts, routed);
   if (format != DQ_EXPERTS_UINT4 && format != DQ_EXPERTS_MXFP4) DQ_FAIL("%s: unknown weight format %d", fn, format);
   const int unit = format == DQ_EXPERTS_UINT4 ? 128 : 64;
   if (K <= 0 || K % unit != 0) DQ_FAIL("%s: K must be a positive multiple of %d (got %d)", fn, unit, K);
@@ -134,36 +135,36 @@ extern "C" int call_experts_order(const void* Ids, void* Order, void* Starts, vo
 
 extern "C" int call_experts_up(const void* X, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,
                                const void* Starts, void* H, int tokens, int experts, int top_k, int N, int K, int group_size, int format,
-                               int activation, dq_stream_t stream) {
+                               int activation, int routed, dq_stream_t stream) {
   const char* const fn = "call_experts_up";
-  if (check_product(fn, X, B, Scale, Zeros, Bias, Order, Starts, H, tokens, experts, top_k, N, K, group_size, format) != 0) return -1;
+  if (check_product(fn, X, B, Scale, Zeros, Bias, Order, Starts, H, tokens, experts, top_k, N, K, group_size, format, routed) != 0) return -1;
   if (activation != DQ_ACT_SILU && activation != DQ_ACT_GELU) DQ_FAIL("%s: unknown activation %d", fn, activation);
   experts::Args a{};
   a.A = X, a.B = (const uint8_t*)B, a.S = Scale, a.Z = Zeros, a.Bias = Bias, a.Order = (const int*)Order, a.Starts = (const int*)Starts, a.Out = H;
   a.tokens = tokens, a.experts = experts, a.top_k = top_k, a.pairs = tokens * top_k, a.N = N, a.K = K, a.group_shift = log2_of(group_size);
-  a.gelu = activation == DQ_ACT_GELU;
+  a.gelu = activation == DQ_ACT_GELU, a.routed = routed;
   return experts_up(a, format == DQ_EXPERTS_MXFP4, (hipStream_t)stream);
 }
 
-extern "C" size_t dq_experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int group_size, int format) {
-  if (tokens <= 0 || experts <= 0 || top_k <= 0 || N <= 0 || K < 64 || (long)tokens * top_k > kMaxPairs) return 0;
-  return experts_down_workspace_bytes(tokens, experts, top_k, N, K, format == DQ_EXPERTS_MXFP4, log2_of(group_size));
+extern "C" size_t dq_experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int group_size, int format, int routed) {
+  if (tokens <= 0 || experts <= 0 || routed < experts || top_k <= 0 || N <= 0 || K < 64 || (long)tokens * top_k > kMaxPairs) return 0;
+  return experts_down_workspace_bytes(tokens, experts, routed, top_k, N, K, format == DQ_EXPERTS_MXFP4, log2_of(group_size));
 }
 
 extern "C" int call_experts_down(const void* H, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,
                                  const void* Starts, const void* Ids, const void* Weights, const void* Residual, void* C, void* Workspace,
                                  size_t workspace_bytes, int tokens, int experts, int top_k, int N, int K, int group_size, int format, int first,
-                                 dq_stream_t stream) {
+                                 int routed, dq_stream_t stream) {
   const char* const fn = "call_experts_down";
-  if (check_product(fn, H, B, Scale, Zeros, Bias, Order, Starts, C, tokens, experts, top_k, N, K, group_size, format) != 0) return -1;
+  if (check_product(fn, H, B, Scale, Zeros, Bias, Order, Starts, C, tokens, experts, top_k, N, K, group_size, format, routed) != 0) return -1;
   if (first < 0 || first > INT_MAX - experts) DQ_FAIL("%s: first must be from 0 to 2^31 - 1 - experts=%d (got %d)", fn, experts, first);
   if (!Ids || !Weights) DQ_FAIL("%s: Ids and Weights are expected to have non-NULL data pointers", fn);
   if (!on(Ids, 4) || !on(Weights, 4) || !on(Residual, 16)) DQ_FAIL("%s: Ids and Weights must be 4-byte and Residual 16-byte aligned", fn);
-  if (check_workspace(fn, Workspace, workspace_bytes, dq_experts_down_workspace_bytes(tokens, experts, top_k, N, K, group_size, format)) != 0) return -1;
+  if (check_workspace(fn, Workspace, workspace_bytes, dq_experts_down_workspace_bytes(tokens, experts, top_k, N, K, group_size, format, routed)) != 0) return -1;
   experts::Args a{};
   a.A = H, a.B = (const uint8_t*)B, a.S = Scale, a.Z = Zeros, a.Bias = Bias, a.Order = (const int*)Order, a.Starts = (const int*)Starts, a.Out = C;
   a.Ids = (const int*)Ids, a.Weights = (const float*)Weights, a.Residual = Residual, a.Parts = (float*)Workspace;
   a.tokens = tokens, a.experts = experts, a.top_k = top_k, a.pairs = tokens * top_k, a.N = N, a.K = K, a.group_shift = log2_of(group_size);
-  a.first = first;
+  a.first = first, a.routed = routed;
   return experts_down(a, format == DQ_EXPERTS_MXFP4, (hipStream_t)stream);
 }

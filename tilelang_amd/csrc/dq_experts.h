@@ -24,6 +24,7 @@ struct Args {
   void* Out;           // up: [pairs][N]; down: [tokens][N]
   float* Parts;        // down: fp32 [slices][pairs][N], a pair's product, of a slice of K
   int tokens, experts, top_k, pairs, N, K, group_shift, gelu, first, slices;
+  int routed;  // choices are of so many experts, of which these are some: what to expect here, no more
 };
 
 // Activations and weights of a product: uint4 codes x fp16, as the dense W4A16 kernels have them (rounded to fp16), and e2m1 x bf16.

@@ -597,6 +597,9 @@ int sum(const Args& a, hipStream_t stream) {
   return 0;
 }
 
+// The pairs that fall to these experts where choices are spread evenly, one at least
+double expected(long pairs, int experts, int routed) { return std::max(1.0, (double)pairs * experts / std::max(experts, routed)); }
+
 // Bytes of LDS of a workgroup beside the rows that it holds
 template <class W>
 constexpr int pipes_area() {
@@ -630,7 +633,7 @@ int launch_few(const Args& a, hipStream_t stream) {
 // 25.8); else one, with as many rows as it can hold (64 tokens, 4 of 32, 2880 x 2880 MXFP4: 69.6 and 74.5).
 template <class W, bool UP>
 int product(const Args& a, hipStream_t stream) {
-  const int stride = acts_stride(a.K), mean = a.pairs / std::min(a.experts, a.pairs);
+  const int stride = acts_stride(a.K), mean = (int)std::max(1.0, expected(a.pairs, a.experts, a.routed) / std::min(a.experts, a.pairs));
   if constexpr (!UP) {
     const size_t scales = (size_t)a.experts * a.N * (a.K >> W::kShift) * W::kScaleBytes;
     // (us, against parts of every expert's rows and the sums behind them: 4096 x 1024, 8 pairs 9.0 and 13.1, 2048 x 768, 8 8.4 and 11.0,
@@ -672,8 +675,8 @@ int product(const Args& a, hipStream_t stream) {
 struct Plan {
   int rows, slices;  // of a tile, 0: rows_kernel
 };
-Plan plan(long pairs, int experts, int N, int K, int mxfp4, int group_shift, bool zeros, bool up) {
-  const double live = std::min((long)experts, pairs), mean = pairs / live;
+Plan plan(long all, int experts, int routed, int N, int K, int mxfp4, int group_shift, bool zeros, bool up) {
+  const double pairs = expected(all, experts, routed), live = std::min((double)experts, pairs), mean = pairs / live;
   auto parts = [&](int rows) { return live * (mean <= 0.7 * rows ? 1.0 : mean / rows + 0.5); };
   const double weights = (up ? 2.0 : 1.0) * N * K;
   const int held = std::min(16, kActsRoom / acts_stride(K));  // rows of a part
@@ -688,7 +691,7 @@ Plan plan(long pairs, int experts, int N, int K, int mxfp4, int group_shift, boo
     if (!up && !experts::odd_rows(mxfp4, K, group_shift))
       while (slices < 4 && tiles * slices < 256 && K / (2 * slices) >= 1024) slices *= 2;
     const double pipe = tiles * (mxfp4 ? (tall ? 54e-6 : 40e-6) : (tall ? 66e-6 : 43e-6)), alone = (tall ? 12.5e-3 : 7.5e-3) / slices;
-    const double us = K * std::max(pipe, alone) + (up ? 0.0 : slices * (double)pairs * N * 2e-6);
+    const double us = K * std::max(pipe, alone) + (up ? 0.0 : slices * (double)all * N * 2e-6);
     if (us < least) least = us, best = {rows, slices};
   }
   return best;
@@ -696,7 +699,7 @@ Plan plan(long pairs, int experts, int N, int K, int mxfp4, int group_shift, boo
 
 template <bool UP>
 int by_format(Args a, int mxfp4, hipStream_t stream) {
-  const Plan by = plan(a.pairs, a.experts, a.N, a.K, mxfp4, a.group_shift, a.Z != nullptr, UP);
+  const Plan by = plan(a.pairs, a.experts, a.routed, a.N, a.K, mxfp4, a.group_shift, a.Z != nullptr, UP);
   a.slices = by.slices;
   if (by.rows != 0) {
     if (const int rc = experts_tiles(a, mxfp4, UP, by.rows, stream)) return rc;
@@ -712,9 +715,9 @@ int by_format(Args a, int mxfp4, hipStream_t stream) {
 }  // namespace
 
 // (with zero points or without: the same)
-size_t experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int mxfp4, int group_shift) {
+size_t experts_down_workspace_bytes(int tokens, int experts, int routed, int top_k, int N, int K, int mxfp4, int group_shift) {
   const long pairs = (long)tokens * top_k;
-  const int slices = std::max(plan(pairs, experts, N, K, mxfp4, group_shift, false, false).slices, plan(pairs, experts, N, K, mxfp4, group_shift, true, false).slices);
+  const int slices = std::max(plan(pairs, experts, routed, N, K, mxfp4, group_shift, false, false).slices, plan(pairs, experts, routed, N, K, mxfp4, group_shift, true, false).slices);
   return (size_t)slices * pairs * N * 4;
 }
 

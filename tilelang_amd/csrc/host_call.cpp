@@ -106,13 +106,13 @@ const Entry kEntries[] = {
      [](void* fn, const Args& a) {
        return DQ_CALL(call_experts_order)(a.p[0], a.p[1], a.p[2], a.p[3], a.ws, a.i[0], a.i[1], a.i[2], a.i[3], a.stream);
      }},
-    {"call_experts_up", 8, 8,
+    {"call_experts_up", 8, 9,
      [](void* fn, const Args& a) {
-       return DQ_CALL(call_experts_up)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.p[7], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.stream);
+       return DQ_CALL(call_experts_up)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.p[7], a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.i[8], a.stream);
      }},
-    {"call_experts_down", 12, 8,
+    {"call_experts_down", 12, 9,
      [](void* fn, const Args& a) {
-       return DQ_CALL(call_experts_down)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.p[7], a.p[8], a.p[9], a.p[10], a.p[11], a.ws, a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.stream);
+       return DQ_CALL(call_experts_down)(a.p[0], a.p[1], a.p[2], a.p[3], a.p[4], a.p[5], a.p[6], a.p[7], a.p[8], a.p[9], a.p[10], a.p[11], a.ws, a.i[0], a.i[1], a.i[2], a.i[3], a.i[4], a.i[5], a.i[6], a.i[7], a.i[8], a.stream);
      }},
 };
 #undef DQ_CALL

@@ -176,8 +176,10 @@ class W4Experts(nn.Module):
         return (logits,
                 block_kernels.route_experts(tokens, self.experts, self.top_k, **self._routing),
                 None if self.held == self.experts else block_kernels.experts_order(tokens, self.top_k, self.held, self.first),
-                block_kernels.experts_up(*sizes, self.width, self.hidden, activation=self._activation, with_bias=self._bias, **self._format),
-                *(block_kernels.experts_down(*sizes, self.hidden, self.width, with_bias=self._bias, residual=residual, first=self.first, **self._format)
+                block_kernels.experts_up(*sizes, self.width, self.hidden, activation=self._activation, with_bias=self._bias, routed=self.experts,
+                                         **self._format),
+                *(block_kernels.experts_down(*sizes, self.hidden, self.width, with_bias=self._bias, residual=residual, first=self.first, routed=self.experts,
+                                             **self._format)
                   for residual in (False, True)))
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, logits: torch.Tensor | None = None) -> torch.Tensor:
