@@ -86,7 +86,8 @@ __device__ __forceinline__ F sum_over_wave(F v) {
 // Whether two keys in fp32 may be the other way round in exact arithmetic.  `slack` is at least twice what the scores in both are off
 // by, four scores where a key is a group's sum of two: a logistic score has three roundings and exp's, below 2^-22 together; a share
 // is off by less than 2^-18.8 of the largest share (22 additions, exp's error and its argument's), nearly all of it by a factor that
-// every share has.  The keys' own roundings are 2^-24 of each.
+// every share has.  The keys' own roundings are 2^-24 of each: of an expert's key, and where two are added, of both and of their sum,
+// whose magnitudes can be far beyond the sum's (biases of either sign).
 __device__ __forceinline__ bool too_close(float a, float b, float slack) { return a - b <= slack + 0x1p-21f * (fabsf(a) + fabsf(b)); }
 
 template <class F>
@@ -196,20 +197,27 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* logits, cons
       next = fmax(fmin(o, mine), fmax(next, p));
       mine = fmax(mine, o);
     }
-    if (a.two && size > 1) mine += next;
+    // (halves: of two finite keys it is finite)
+    F size_of = fabs(mine) * (F)0.5;
+    if (a.two && size > 1) size_of += fabs(next) * (F)0.5, mine += next;
     if (mine != mine) mine = kMost;
     if (group >= a.groups || first != 0) mine = kGone;
+    const F group_key = mine;
     __builtin_amdgcn_wave_barrier();
     unsigned long long taken = 0;  // a bit a group
-    F last = 0;
-    for (int r = 0; r < a.groups; ++r) {
+    for (int r = 0; r < a.top_groups; ++r) {
       const F best = max_over_wave(mine);
-      if (kNarrow && r > 0 && (by_score || a.two) && too_close((float)last, (float)best, slack)) close = true;
-      if (r == a.top_groups) break;
       const int l = __builtin_ctzll(__ballot(mine == best));  // (of equal groups the first)
       if (lane == l) mine = kGone;
       taken |= 1ull << (l >> each);
-      last = best;
+    }
+    if (kNarrow && (by_score || a.two) && a.top_groups < a.groups) {
+      // whether the least that a taken group may count by is above the most that another may; what each is off by goes with the
+      // magnitudes of its own keys, so neighbours in the order alone would not tell
+      const float off = size_of < (F)__builtin_inff() ? 0.5f * slack + 0x1p-20f * (float)size_of : 0.f;
+      const bool in = (taken >> group) & 1;
+      const float least = -max_over_wave(in ? off - (float)group_key : __builtin_nanf("")), most = max_over_wave(in ? __builtin_nanf("") : (float)group_key + off);
+      close = least <= most;
     }
     // (exact: the quotient is off by less than 2^-12 / size, and no nearer than 1 / (2 size) to a whole number)
     const float inverse = 1.f / (float)size;
