@@ -46,13 +46,14 @@ __global__ __launch_bounds__(WAVES * 64) void router_kernel(const T* __restrict_
 #pragma unroll
   for (int j = 0; j < NB; ++j) b[j] = W + (size_t)min(e0 + 16 * j + r, e1 - 1) * K + 8 * g;
   float4_t acc[MB][NB] = {};
-  for (int k0 = wave * kBlock; k0 < K; k0 += WAVES * kBlock) {
+  // (unsigned: with K next to 2^31 the step beyond it passes that)
+  for (unsigned k0 = wave * kBlock; k0 < (unsigned)K; k0 += WAVES * kBlock) {
     frag x[4][MB], w[4][NB];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       // (K is a multiple of 32: a step is there as a whole or not at all)
-      const int k = k0 + 32 * s;
-      if (k < K) {
+      const unsigned k = k0 + 32 * s;
+      if (k < (unsigned)K) {
 #pragma unroll
         for (int i = 0; i < MB; ++i) x[s][i] = *reinterpret_cast<const frag*>(a[i] + k);
 #pragma unroll
