@@ -435,7 +435,8 @@ enum dq_group_score { DQ_GROUP_MAX = 0, DQ_GROUP_SUM2 = 1 /* the sum of a group'
  * (fp32), or without one (NULL) the logit; of equal keys the lowest index comes first.  groups > 1: of the groups of
  * experts / groups neighbours only the top_groups best count, by the largest key of each or the sum of its two largest (without a
  * bias: scores).  Weights are scores (without the bias), renormalize: divided by their sum over the token's choices (a sum of zero
- * leaves zeros), times factor.  Logits of -inf mask experts: score 0, chosen last.  A NaN counts as the largest, and shows in the
+ * leaves zeros), times factor.  A logit of -inf: score 0, and without a bias chosen last; with one its key is its Bias, and who is
+ * never to be chosen ahead of others has a Bias of -inf.  A NaN counts as the largest, and shows in the
  * weights.  Choices do not depend on how an exponential is rounded: where fp32 cannot tell two scores apart, 64 bits do.
  * experts at most 1024, top_k at most 32, groups at most 64, tokens * top_k at most 2^23.
  * Workspace: dq_experts_order_workspace_bytes(...) bytes, 16-byte aligned (0: none), contents undefined before and after, not to

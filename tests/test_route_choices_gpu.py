@@ -1,8 +1,11 @@
-"""Who is chosen where 32 bits cannot tell: groups whose biases all but cancel, more experts than a wave has in registers."""
+"""Who is chosen where 32 bits cannot tell: groups whose biases all but cancel, more experts than a wave has in registers; and masks."""
+
+import math
 
 import pytest
 import torch
 
+import block_reference as ref
 import tilelang_amd as tl
 from test_route_gpu import _check
 
@@ -60,3 +63,41 @@ def test_near_ties_of_many_experts(cuda, experts, groups, top_groups, group_scor
     logits = row.expand(36, experts).clone()
     logits[18:] = torch.randn((18, experts), generator=gen)
     _check(logits, (1 - score).float(), 10, scores=scores, groups=groups, top_groups=top_groups, group_score=group_score)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts", [4, 300])
+def test_masks(cuda, experts, scores):
+    """Without a bias a logit of -inf is chosen last.  With one its key is its bias, score 0; a bias of -inf is chosen last."""
+    inf = math.inf
+    logits = torch.full((3, experts), -inf)
+    logits[0, 1:4] = torch.tensor([-2.0, -3.0, 0.0])
+    logits[1, 2] = 5.0
+    route = lambda bias: tl.route_experts(3, experts, 2, scores=scores, bias=bias is not None)(logits.cuda(), *(() if bias is None else (bias.cuda(),)))
+    share = (torch.sigmoid if scores == "sigmoid" else lambda v: torch.exp(v))(torch.tensor([0.0, -2.0], dtype=torch.float64))
+    share = (share / share.sum()).tolist()
+
+    weights, ids, _, _ = route(None)
+    assert ids.tolist() == [[3, 1], [2, 0], [0, 1]]
+    assert torch.allclose(weights.cpu().double(), torch.tensor([share, [1, 0], [0, 0]], dtype=torch.float64), rtol=2e-6, atol=0)
+
+    # scores are at most 1: what is masked with a bias of 2 goes first, with a weight of 0
+    bias = torch.zeros(experts)
+    bias[0] = 2.0
+    weights, ids, _, _ = route(bias)
+    assert ids.tolist() == [[0, 3], [0, 2], [0, 1]]
+    assert torch.equal(weights.cpu(), torch.tensor([[0.0, 1.0], [0.0, 1.0], [0.0, 0.0]]))
+
+    bias = torch.full((experts,), -inf)
+    bias[1:3] = 0.0
+    weights, ids, _, _ = route(bias)
+    assert ids.tolist() == [[1, 2], [2, 1], [1, 2]]
+    assert (weights[0] > 0).all() and torch.equal(weights[1:].cpu(), torch.tensor([[1.0, 0.0], [0.0, 0.0]]))
+
+
+def test_masked_expert_by_its_bias(cuda):
+    """Logistic scores 0, .119, .047, .5: keys .5, .02, -.05, .5."""
+    logits, bias = torch.tensor([[-math.inf, -2.0, -3.0, 0.0]]), torch.tensor([0.5, -0.1, -0.1, 0.0])
+    ids, weights = _check(logits, bias, 2, scores="sigmoid")
+    assert ids.tolist() == [[0, 3]] and weights.tolist() == [[0.0, 1.0]]
+    assert torch.equal(ids, ref.route(logits, bias, 2, "sigmoid")[0])

@@ -116,7 +116,8 @@ def route_experts(tokens: int, experts: int, top_k: int, scores: str = "softmax"
     (``bias``; it balances the experts' load and is no part of the weights), or else the logit.  ``groups``: the experts are that many
     groups of neighbours, and only the ``top_groups`` best of them count, by the largest key of each (``group_score="max"``) or the
     sum of its two largest (``"sum2"``; without a bias: of scores).  ``weights`` fp32 ``[tokens, top_k]`` are the chosen scores, divided
-    by their sum (``renormalize``), times ``factor``.  Logits of -inf mask experts; a NaN is chosen first and shows in the weights.
+    by their sum (``renormalize``), times ``factor``.  A logit of -inf has a score of 0 and without a bias is chosen last; with one its key is
+    its bias, and a bias of -inf is chosen last.  A NaN is chosen first and shows in the weights.
     Choices do not depend on how an exponential is rounded: where 32 bits cannot tell two scores apart, 64 do.
 
     ``order`` and ``starts`` are :func:`experts_order`'s of the same ids.
