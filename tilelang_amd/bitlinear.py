@@ -106,6 +106,8 @@ class BitLinear(nn.Module):
         return k
 
     def _codes_forward(self, codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+        if codes.numel() == 0:  # (a batch of no tokens: nothing to launch)
+            return codes.new_empty((*codes.shape[:-1], self.out_features), dtype=torch.float16)
         M = codes.numel() // self.in_features
         k = self._kernels.get((M, "codes"))
         if k is None:

@@ -55,13 +55,17 @@ class RMSNorm(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
         lead, dtype = x.shape[:-1], self.weight.dtype
-        rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        rows = x if x.dim() == 2 else x.reshape(lead.numel(), x.shape[-1])
         if rows.dtype != dtype:
             rows = rows.to(dtype)
         stride = rows.stride(0) if rows.shape[0] > 1 else self.dim
         if rows.stride(1) != 1 or stride < self.dim or stride % 8 or rows.data_ptr() % 16:
             rows, stride = _whole(rows), self.dim
         n = rows.shape[0]
+        if n == 0 and rows.shape[1] == self.dim:  # (a batch of no tokens: nothing to launch)
+            out = [rows.new_empty(x.shape, dtype=torch.int8), rows.new_empty(lead, dtype=torch.float32)] if self.int8 else [rows.new_empty(x.shape)]
+            out += [] if residual is None else [rows.new_empty(x.shape)]
+            return out[0] if len(out) == 1 else tuple(out)
         kern = _kept(self._kernels, (n, stride, residual is not None, dtype),
                      lambda: block_kernels.rms_norm(n, self.dim, self.eps, dtype, residual is not None, self.int8, stride))
         if residual is None:
@@ -186,6 +190,8 @@ class W4Experts(nn.Module):
         """``x`` ``[..., hidden]`` -> the same; ``residual`` of that shape is added in the same launch.  ``logits`` fp32 ``[..., experts]``: in place of
         the router's."""
         dtype = self.router.dtype
+        if x.numel() == 0:  # (a batch of no tokens: nothing to launch)
+            return x.new_empty(x.shape, dtype=dtype)
         rows = _whole(x.to(dtype).reshape(-1, self.hidden))
         r = None if residual is None else _whole(residual.to(dtype).reshape(-1, self.hidden))
         given = None if logits is None else _whole(logits.float().reshape(-1, self.experts))
