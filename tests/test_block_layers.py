@@ -4,6 +4,8 @@ import pytest
 import torch
 
 import tilelang_amd as tl
+from tilelang_amd import _lib
+from tilelang_amd import experts as layers
 
 
 @pytest.mark.parametrize("lead", [(0,), (0, 5), (3, 0)])
@@ -33,3 +35,24 @@ def test_experts_of_no_tokens(lead, weight_format):
     x = torch.zeros((*lead, 256))
     for out in (layer(x), layer(x, x), layer(x, logits=torch.zeros((*lead, 4)))):
         assert out.shape == x.shape and out.dtype == layer.router.dtype
+
+
+@pytest.mark.parametrize("hidden,width,top_k,tokens", [(7168, 2048, 8, 70000), (16384, 16384, 32, 65536), (4096, 14336, 2, 65536), (2560, 2560, 4, 65536), (128, 128, 1, 200000)])
+def test_parts_take_bounded_memory(monkeypatch, hidden, width, top_k, tokens):
+    """What goes through the experts at once: the rows between the two products and the sums' workspace stay below a bound."""
+    with torch.device("meta"):
+        layer = tl.W4Experts(hidden, width, 64, top_k)
+        x = torch.empty((tokens, hidden), dtype=torch.float16)
+    parts = []
+
+    def one(rows, residual, logits):
+        parts.append(rows.shape[0])
+        return torch.empty_like(rows)
+
+    monkeypatch.setattr(layer, "_pass", one)
+    assert layer(x).shape == x.shape and sum(parts) == tokens
+    for n in set(parts):
+        room = _lib.load_library().dq_experts_down_workspace_bytes(n, 64, top_k, hidden, width, 128, 0, 64)
+        assert room + n * top_k * width * 2 <= layers.PART_BYTES and n <= layers.MAX_TOKENS
+    # no more parts than that takes
+    assert len(parts) <= 2 + tokens // layers.MAX_TOKENS + tokens * top_k * (4 * hidden + 2 * width) // layers.PART_BYTES

@@ -15,8 +15,10 @@ from .w4linear import quantize_w4
 
 #: kernel objects (sets of them) that a layer keeps: prompts come in any number of rows
 MAX_KERNELS = 64
-#: tokens that go through the experts at once; more go in parts, so that the rows between the two products take bounded memory
+#: tokens that go through the experts at once, and bytes of the rows between the two products and of "down"'s workspace that these take
+#: at most; more go in parts
 MAX_TOKENS = 65536
+PART_BYTES = 2**33
 #: from this many logits on the tiled GEMM is ahead (4096 tokens, 256 experts, 7168 wide 57 us and 77; 16384, 32 of 2880 25 and 21)
 TILED_LOGITS = 2**20
 
@@ -195,7 +197,9 @@ class W4Experts(nn.Module):
         rows = _whole(x.to(dtype).reshape(-1, self.hidden))
         r = None if residual is None else _whole(residual.to(dtype).reshape(-1, self.hidden))
         given = None if logits is None else _whole(logits.float().reshape(-1, self.experts))
-        n, most = rows.shape[0], min(MAX_TOKENS, block_kernels.MAX_ELEMENTS // max(self.hidden, self.width))
+        # (a pair's row of h, and its product in fp32: slices of K, which have one each, are only where there are few pairs)
+        pair = 2 * self.width + 4 * self.hidden
+        n, most = rows.shape[0], max(1, min(MAX_TOKENS, block_kernels.MAX_ELEMENTS // max(self.hidden, self.width), PART_BYTES // (self.top_k * pair)))
         if n <= most:
             out = self._pass(rows, r, given)
         else:
