@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import tilelang_amd as tl
-from tilelang_amd import _lib
+from tilelang_amd import _lib, bitlinear
 from tilelang_amd import experts as layers
 
 
@@ -56,3 +56,24 @@ def test_parts_take_bounded_memory(monkeypatch, hidden, width, top_k, tokens):
         assert room + n * top_k * width * 2 <= layers.PART_BYTES and n <= layers.MAX_TOKENS
     # no more parts than that takes
     assert len(parts) <= 2 + tokens // layers.MAX_TOKENS + tokens * top_k * (4 * hidden + 2 * width) // layers.PART_BYTES
+
+
+def test_bitlinear_keeps_the_kernels_of_its_last_sizes(monkeypatch):
+    """Prompts come in any number of rows: kernel objects are kept for the last ones, of either kind of rows."""
+    made = []
+
+    def make(M, N, K, *args, **more):
+        made.append(M)
+        return lambda x, weight, *scale: torch.zeros((M, N), dtype=torch.float16)
+
+    monkeypatch.setattr(bitlinear.kernels, "bitlinear_int8xint2", make)
+    monkeypatch.setattr(bitlinear.kernels, "bitlinear_fp16", make)
+    layer = tl.BitLinear(128, 32)
+    for M in range(1, 200):
+        assert layer(torch.zeros((M, 128), dtype=torch.int8), torch.ones(M)).shape == (M, 32)
+        assert layer(torch.zeros((M, 128), dtype=torch.float16)).shape == (M, 32)
+        layer(torch.zeros((7, 128), dtype=torch.int8), torch.ones(7))
+    assert len(layer._kernels) == len(layer._codes_kernels) == bitlinear.MAX_KERNELS
+    assert made.count(7) == 2  # (one of a kind: in use, it stays; the fp16 rows' goes by when it was made)
+    layer.load_packed_weight(layer.qweight, 2.0)
+    assert not layer._kernels and not layer._codes_kernels

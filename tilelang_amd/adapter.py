@@ -62,6 +62,17 @@ def _unbound(*inputs):
     return NotImplemented
 
 
+def kept(held: dict, key, make, most: int):
+    """``make()``, made once for a key; the last ``most`` used are kept: prompts come in any number of rows."""
+    found = held.pop(key, None)
+    if found is None:
+        found = make()
+        while len(held) >= most:
+            del held[next(iter(held))]
+    held[key] = found  # (the last in the order)
+    return found
+
+
 class KernelAdapter:
     def __init__(
         self,

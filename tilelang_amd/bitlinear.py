@@ -14,6 +14,10 @@ import torch
 from torch import nn
 
 from . import kernels, quantize
+from .adapter import kept
+
+#: kernel objects that a layer keeps of either kind: fp16 rows, whose call is the shortest, by when they were made, int8 rows by their last use
+MAX_KERNELS = 64
 
 
 def weight_quant(weight: torch.Tensor) -> torch.Tensor:
@@ -55,7 +59,7 @@ class BitLinear(nn.Module):
         self.register_buffer("sw", torch.ones((), dtype=torch.float32))
         self._sw_value = 1.0
         self.bias = None
-        self._kernels = {}
+        self._kernels, self._codes_kernels = {}, {}
 
     @classmethod
     def from_bit_linear(cls, bitlinear, interleave: bool = True, prefill_fragments: bool = False) -> "BitLinear":
@@ -84,6 +88,7 @@ class BitLinear(nn.Module):
         self._sw_value = float(self.sw)
         self.bias = None if bias is None else bias.detach().to(self.qweight.device)
         self._kernels.clear()
+        self._codes_kernels.clear()
 
     def rowmajor_weight(self) -> torch.Tensor:
         """The packed words ``[out, in/4]`` whatever order the layer holds them in."""
@@ -96,24 +101,20 @@ class BitLinear(nn.Module):
         # the weight scale is baked into the kernels as a number
         self._sw_value = float(self.sw)
         self._kernels.clear()
+        self._codes_kernels.clear()
 
     def _get_kernel(self, M: int):
-        k = self._kernels.get(M)
-        if k is None:
-            k = kernels.bitlinear_fp16(M, self.out_features, self.in_features, self._sw_value, interleaved=self.interleave,
-                                       weight_fragments=self.prefill_fragments)
-            self._kernels[M] = k
-        return k
+        return kept(self._kernels, M, lambda: kernels.bitlinear_fp16(M, self.out_features, self.in_features, self._sw_value,
+                                                                     interleaved=self.interleave,
+                                                                     weight_fragments=self.prefill_fragments), MAX_KERNELS)
 
     def _codes_forward(self, codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
         if codes.numel() == 0:  # (a batch of no tokens: nothing to launch)
             return codes.new_empty((*codes.shape[:-1], self.out_features), dtype=torch.float16)
         M = codes.numel() // self.in_features
-        k = self._kernels.get((M, "codes"))
-        if k is None:
-            k = kernels.bitlinear_int8xint2(M, self.out_features, self.in_features, self._sw_value, interleaved=self.interleave,
-                                            weight_fragments=self.prefill_fragments)
-            self._kernels[(M, "codes")] = k
+        k = kept(self._codes_kernels, M, lambda: kernels.bitlinear_int8xint2(M, self.out_features, self.in_features, self._sw_value,
+                                                                             interleaved=self.interleave,
+                                                                             weight_fragments=self.prefill_fragments), MAX_KERNELS)
         out = k(codes.reshape(M, self.in_features).contiguous(), self.qweight, scale.reshape(M).contiguous())
         if self.bias is not None:
             out += self.bias.view(1, -1).expand_as(out)

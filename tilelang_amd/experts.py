@@ -11,6 +11,7 @@ import torch
 from torch import nn
 
 from . import block_kernels, kernels, quantize
+from .adapter import kept
 from .w4linear import quantize_w4
 
 #: kernel objects (sets of them) that a layer keeps: prompts come in any number of rows
@@ -24,14 +25,7 @@ TILED_LOGITS = 2**20
 
 
 def _kept(held: dict, key, make):
-    """``make()``, made once for a key; the last :data:`MAX_KERNELS` used are kept."""
-    found = held.pop(key, None)
-    if found is None:
-        found = make()
-        while len(held) >= MAX_KERNELS:
-            del held[next(iter(held))]
-    held[key] = found  # (the last in the order)
-    return found
+    return kept(held, key, make, MAX_KERNELS)
 
 
 def _whole(t: torch.Tensor) -> torch.Tensor:
