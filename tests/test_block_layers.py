@@ -77,3 +77,29 @@ def test_bitlinear_keeps_the_kernels_of_its_last_sizes(monkeypatch):
     assert made.count(7) == 2  # (one of a kind: in use, it stays; the fp16 rows' goes by when it was made)
     layer.load_packed_weight(layer.qweight, 2.0)
     assert not layer._kernels and not layer._codes_kernels
+
+
+def test_rows_that_are_not_x_s_are_refused(monkeypatch):
+    """A residual or logits of as many elements as x but of other rows, and an x of other rows than the layer's."""
+    norm, layer = tl.RMSNorm(64), tl.W4Experts(256, 128, 4, 2)
+    monkeypatch.setattr(layer, "_pass", lambda rows, residual, logits: torch.empty_like(rows))
+    monkeypatch.setattr(layers.block_kernels, "rms_norm", lambda *a: lambda x, *r: [torch.empty_like(x) for _ in range(1 + (len(r) == 2))])
+    x = torch.zeros((2, 3, 64))
+    for shape in ((3, 2, 64), (2, 64, 3), (6, 32), (5, 64), (64,), (1, 3, 64), (2, 3, 128)):
+        with pytest.raises(ValueError, match="RMSNorm: residual is"):
+            norm(x, torch.zeros(shape))
+    assert norm(x, torch.zeros((6, 64)))[1].shape == x.shape and norm(x[0], torch.zeros((1, 3, 64)))[0].shape == (3, 64)
+    x = torch.zeros((2, 3, 256))
+    for bad in (torch.zeros((2, 6, 128)), torch.zeros((2, 512)), torch.zeros((5, 0)), torch.zeros(512)):
+        with pytest.raises(ValueError, match="W4Experts: x is"):
+            layer(bad)
+    for shape in ((3, 2, 256), (6, 128), (5, 256), (256,), (2, 256, 3)):
+        with pytest.raises(ValueError, match="W4Experts: residual is"):
+            layer(x, torch.zeros(shape))
+    for shape in ((3, 2, 4), (6, 8), (7, 4), (2, 4, 3), (2, 3, 5)):
+        with pytest.raises(ValueError, match="W4Experts: logits is"):
+            layer(x, logits=torch.zeros(shape))
+    with pytest.raises(ValueError, match="W4Experts: residual is"):
+        layer(x[:0], x)
+    assert layer(x, torch.zeros((6, 256)), torch.zeros((6, 4))).shape == x.shape
+    assert layer(x[0, 0], x[0, 0], torch.zeros(4)).shape == (256,)

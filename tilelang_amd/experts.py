@@ -34,6 +34,15 @@ def _whole(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _check_rows(fn: str, name: str, t: torch.Tensor, x: torch.Tensor, width: int) -> None:
+    """That ``t`` has a row of ``width`` for each of ``x``'s: the same leading sizes, or one of the two flat."""
+    if t.shape[:-1] == x.shape[:-1] and t.shape[-1] == width:
+        return
+    flat = (t.dim() == 2 or x.dim() == 2) and t.shape[-1:] == (width,) and t.shape[:-1].numel() == x.shape[:-1].numel()
+    if not flat:
+        raise ValueError(f"{fn}: {name} is {tuple(t.shape)}, not a row of {width} for each of x, {tuple(x.shape)}")
+
+
 class RMSNorm(nn.Module):
     """``weight * x / sqrt(mean(x ** 2) + eps)`` over rows of fp16 or bf16.
 
@@ -51,6 +60,8 @@ class RMSNorm(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
         lead, dtype = x.shape[:-1], self.weight.dtype
+        if residual is not None:
+            _check_rows("RMSNorm", "residual", residual, x, self.dim)
         rows = x if x.dim() == 2 else x.reshape(lead.numel(), x.shape[-1])
         if rows.dtype != dtype:
             rows = rows.to(dtype)
@@ -186,6 +197,9 @@ class W4Experts(nn.Module):
         """``x`` ``[..., hidden]`` -> the same; ``residual`` of that shape is added in the same launch.  ``logits`` fp32 ``[..., experts]``: in place of
         the router's."""
         dtype = self.router.dtype
+        for name, t, width in (("x", x, self.hidden), ("residual", residual, self.hidden), ("logits", logits, self.experts)):
+            if t is not None:
+                _check_rows("W4Experts", name, t, x, width)
         if x.numel() == 0:  # (a batch of no tokens: nothing to launch)
             return x.new_empty(x.shape, dtype=dtype)
         rows = _whole(x.to(dtype).reshape(-1, self.hidden))
