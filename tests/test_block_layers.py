@@ -103,3 +103,18 @@ def test_rows_that_are_not_x_s_are_refused(monkeypatch):
         layer(x[:0], x)
     assert layer(x, torch.zeros((6, 256)), torch.zeros((6, 4))).shape == x.shape
     assert layer(x[0, 0], x[0, 0], torch.zeros(4)).shape == (256,)
+
+
+@pytest.mark.parametrize("apart", [2**31 - 8, 2**31, 2**33])
+def test_norm_of_rows_far_apart(monkeypatch, apart):
+    """Rows of x further apart than a kernel's row stride goes are copied together."""
+    rms_norm, strides = layers.block_kernels.rms_norm, []
+
+    def make(rows, dim, eps, dtype, residual, int8, stride):
+        strides.append(rms_norm(rows, dim, eps, dtype, residual, int8, stride).params[0].strides)
+        return lambda x, weight: torch.empty_like(x)
+
+    norm = tl.RMSNorm(64)
+    monkeypatch.setattr(layers.block_kernels, "rms_norm", make)
+    x = torch.empty_strided((2, 64), (apart, 1), dtype=torch.float16, device="meta")
+    assert norm(x).shape == (2, 64) and strides == [(apart, 1) if apart < 2**31 else None]

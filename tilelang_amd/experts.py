@@ -66,7 +66,7 @@ class RMSNorm(nn.Module):
         if rows.dtype != dtype:
             rows = rows.to(dtype)
         stride = rows.stride(0) if rows.shape[0] > 1 else self.dim
-        if rows.stride(1) != 1 or stride < self.dim or stride % 8 or rows.data_ptr() % 16:
+        if rows.stride(1) != 1 or not self.dim <= stride < 2**31 or stride % 8 or rows.data_ptr() % 16:
             rows, stride = _whole(rows), self.dim
         n = rows.shape[0]
         if n == 0 and rows.shape[1] == self.dim:  # (a batch of no tokens: nothing to launch)
