@@ -471,7 +471,8 @@ int call_experts_up(const void* X, const void* B, const void* Scale, const void*
 /* The way back: C[t] = Residual[t] + sum over the token's choices j of Weights[t][j] * (H[p] . D_e^T + bias), p the pair's row in
  * the sorted order and e its expert.  H [tokens * top_k][K], C [tokens][N], Residual [tokens][N] or NULL, Weights fp32 and Ids
  * [tokens][top_k]; B [experts][N][K / 2] and so on as above.  Pairs whose id is not one of first .. first + experts - 1 add
- * nothing.  Sums in fp32, a token's choices in their order whatever the timing.
+ * nothing.  Sums in fp32, a token's choices in their order whatever the timing.  128 rows of H (all, where there are fewer) have at
+ * most 2^31 elements.
  * Workspace: dq_experts_down_workspace_bytes(...) bytes, as above. */
 size_t dq_experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int group_size, int format, int routed);
 int call_experts_down(const void* H, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,

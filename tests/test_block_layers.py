@@ -1,11 +1,14 @@
 """RMSNorm, W4Experts and BitLinear on int8 rows: batches of no tokens, and what a call is checked for before it goes to a kernel."""
 
+import ctypes
+
 import pytest
 import torch
 
 import tilelang_amd as tl
 from tilelang_amd import _lib, bitlinear
 from tilelang_amd import experts as layers
+from tilelang_amd.block_kernels import EXPERTS_MXFP4
 
 
 @pytest.mark.parametrize("lead", [(0,), (0, 5), (3, 0)])
@@ -118,3 +121,14 @@ def test_norm_of_rows_far_apart(monkeypatch, apart):
     monkeypatch.setattr(layers.block_kernels, "rms_norm", make)
     x = torch.empty_strided((2, 64), (apart, 1), dtype=torch.float16, device="meta")
     assert norm(x).shape == (2, 64) and strides == [(apart, 1) if apart < 2**31 else None]
+
+
+def test_down_refuses_rows_beyond_32_bit_offsets():
+    """All choices of 16 tokens may be one expert's: 128 rows of 2^26 elements are 16 GiB from a tile's first to its last."""
+    entry = dict(tokens=16, experts=2, top_k=32, N=32, K=2**26, group_size=32, format=EXPERTS_MXFP4, first=0, routed=2)
+    assert tl.experts_down(16, 2, 2, 32, 2**26, "mxfp4").name == "experts_down"
+    with pytest.raises(ValueError, match="128 rows of h"):
+        tl.experts_down(16, 2, 32, 32, 2**26, "mxfp4")
+    lib, p = _lib.load_library(), ctypes.c_void_p(1 << 20)  # (never followed: the checks come first)
+    rc = lib.call_experts_down(p, p, p, None, None, p, p, p, p, None, p, p, 1 << 40, *entry.values(), None)
+    assert rc == -1 and "128 rows of H" in lib.get_last_error().decode()

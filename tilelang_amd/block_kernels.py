@@ -260,6 +260,8 @@ def experts_down(tokens: int, experts: int, top_k: int, N: int, K: int, weight_f
     _first(fn, first, experts)
     routed = _routed(fn, routed, experts)
     _activations(fn, tokens, K)
+    if min(tokens * top_k, 128) * K > 2**31:
+        raise ValueError(f"{fn}: K={K}: at most 2^31 elements of 128 rows of h, or of all where they are fewer")
     params = [KernelParam("h", w.dtype, (tokens * top_k, K)), *w.params]
     n = len(params)
     params += [KernelParam("order", torch.int32, (tokens * top_k,)), KernelParam("starts", torch.int32, (experts + 1,)),

@@ -158,6 +158,9 @@ extern "C" int call_experts_down(const void* H, const void* B, const void* Scale
   const char* const fn = "call_experts_down";
   if (check_product(fn, H, B, Scale, Zeros, Bias, Order, Starts, C, tokens, experts, top_k, N, K, group_size, format, routed) != 0) return -1;
   if (first < 0 || first > INT_MAX - experts) DQ_FAIL("%s: first must be from 0 to 2^31 - 1 - experts=%d (got %d)", fn, experts, first);
+  // (and so they are in the rows of a tile of H: beyond tokens rows of an expert, where ids name it several times for a token)
+  const long tile = (long)tokens * top_k < 128 ? (long)tokens * top_k : 128;
+  if (tile * K > 1l << 31) DQ_FAIL("%s: at most 2^31 elements of 128 rows of H, or of all where they are fewer (got K=%d)", fn, K);
   if (!Ids || !Weights) DQ_FAIL("%s: Ids and Weights are expected to have non-NULL data pointers", fn);
   if (!on(Ids, 4) || !on(Weights, 4) || !on(Residual, 16)) DQ_FAIL("%s: Ids and Weights must be 4-byte and Residual 16-byte aligned", fn);
   if (check_workspace(fn, Workspace, workspace_bytes, dq_experts_down_workspace_bytes(tokens, experts, top_k, N, K, group_size, format, routed)) != 0) return -1;
