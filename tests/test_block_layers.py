@@ -1,6 +1,9 @@
 """RMSNorm, W4Experts and BitLinear on int8 rows: batches of no tokens, and what a call is checked for before it goes to a kernel."""
 
 import ctypes
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -132,3 +135,12 @@ def test_down_refuses_rows_beyond_32_bit_offsets():
     lib, p = _lib.load_library(), ctypes.c_void_p(1 << 20)  # (never followed: the checks come first)
     rc = lib.call_experts_down(p, p, p, None, None, p, p, p, p, None, p, p, 1 << 40, *entry.values(), None)
     assert rc == -1 and "128 rows of H" in lib.get_last_error().decode()
+
+
+def test_no_workspace_for_sizes_that_calls_refuse():
+    """In a process of its own: a quotient of the first's sizes ended it."""
+    asked = [("down", (64, 8, 2, 64, 2**31 - 255, 128, 0, 8)), ("down", (64, 8, 2, 2**31 - 32, 2**31 - 128, 128, 0, 8)), ("down", (64, 2000, 2, 64, 256, 128, 0, 2000)),
+             ("down", (64, 8, 33, 64, 256, 128, 0, 8)), ("order", (500, 2, 2**31 - 1)), ("order", (500, 33, 64))]
+    code = "from tilelang_amd import _lib; lib = _lib.load_library(); print(" + ", ".join(f"lib.dq_experts_{name}_workspace_bytes(*{sizes})" for name, sizes in asked) + ")"
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=pathlib.Path(__file__).parent.parent)
+    assert done.returncode == 0 and done.stdout.split() == ["0"] * len(asked), (done.returncode, done.stdout, done.stderr)

@@ -26,6 +26,12 @@ bool on(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) 
 
 constexpr int kMaxNormDim = 32768, kMaxExperts = 1024, kMaxTopK = 32;
 constexpr long kMaxPairs = 1l << 23;  // counted in 16 bits a chunk, 256 chunks
+constexpr long kMaxWeights = 1l << 31;  // of an expert and projection: byte offsets are 32-bit
+
+// The sizes that check_pairs lets through: what a workspace is asked for of others is nothing
+bool takes_pairs(int tokens, int experts, int top_k) {
+  return tokens > 0 && experts > 0 && experts <= kMaxExperts && top_k > 0 && top_k <= kMaxTopK && (long)tokens * top_k <= kMaxPairs;
+}
 
 int check_pairs(const char* fn, int tokens, int experts, int top_k) {
   if (tokens <= 0) DQ_FAIL("%s: tokens must be positive (got %d)", fn, tokens);
@@ -53,7 +59,7 @@ int check_product(const char* fn, const void* A, const void* B, const void* Scal
     DQ_FAIL("%s: group_size must be 32, 64 or 128, with MXFP4 32 (got %d)", fn, group_size);
   if (format == DQ_EXPERTS_MXFP4 && Zeros) DQ_FAIL("%s: MXFP4 weights have no zero points", fn);
   // (byte offsets in an expert's weights and in the activations are 32-bit)
-  if ((long)N * K > 1l << 31 || (long)tokens * K > 1l << 30 || (long)tokens * top_k * (N > K ? N : K) > 1l << 40)
+  if ((long)N * K > kMaxWeights || (long)tokens * K > 1l << 30 || (long)tokens * top_k * (N > K ? N : K) > 1l << 40)
     DQ_FAIL("%s: at most 2^31 weights an expert and projection, and 2^30 elements of %d tokens (got N=%d, K=%d)", fn, tokens, N, K);
   if (!A || !B || !Scale || !Order || !Starts || !Out) DQ_FAIL("%s: an operand is NULL that is expected to have a non-NULL data pointer", fn);
   if (!on(A, 16) || !on(B, 16) || !on(Out, 16) || !on(Bias, 16)) DQ_FAIL("%s: activations, weights, bias and output must be 16-byte aligned", fn);
@@ -96,7 +102,7 @@ extern "C" int call_router_logits(const void* X, const void* W, const void* Bias
 }
 
 extern "C" size_t dq_experts_order_workspace_bytes(int tokens, int top_k, int experts) {
-  if (tokens <= 0 || top_k <= 0 || experts <= 0 || (long)tokens * top_k > kMaxPairs) return 0;
+  if (!takes_pairs(tokens, experts, top_k)) return 0;
   return order_workspace_bytes(tokens, top_k, experts);
 }
 
@@ -147,7 +153,7 @@ extern "C" int call_experts_up(const void* X, const void* B, const void* Scale, 
 }
 
 extern "C" size_t dq_experts_down_workspace_bytes(int tokens, int experts, int top_k, int N, int K, int group_size, int format, int routed) {
-  if (tokens <= 0 || experts <= 0 || routed < experts || top_k <= 0 || N <= 0 || K < 64 || (long)tokens * top_k > kMaxPairs) return 0;
+  if (!takes_pairs(tokens, experts, top_k) || routed < experts || N <= 0 || K < 64 || (long)N * K > kMaxWeights) return 0;
   return experts_down_workspace_bytes(tokens, experts, routed, top_k, N, K, format == DQ_EXPERTS_MXFP4, log2_of(group_size));
 }
 
