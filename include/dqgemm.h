@@ -461,7 +461,7 @@ enum dq_activation { DQ_ACT_SILU = 0, DQ_ACT_GELU = 1 /* the tanh form */ };
  * low nibble; Scale [experts][2 N][K / group_size]; Bias [experts][2 N] or NULL.
  * DQ_EXPERTS_UINT4: fp16; weights as call_dequantize_gemv_w4a16's, fp16((q - 8) * s), or with Zeros (fp16, as Scale)
  * fp16(fp16(q - z) * s); group_size 32, 64 or 128; K % 128 == 0.  DQ_EXPERTS_MXFP4: bf16; e2m1 codes times 2^(Scale - 127), Scale
- * uint8, group_size 32; K % 64 == 0.  N % 32 == 0.  Sums in fp32.  routed: of how many experts the ids are, experts or
+ * uint8 (255 counts as 254), group_size 32; K % 64 == 0.  N % 32 == 0.  Sums in fp32.  routed: of how many experts the ids are, experts or
  * more where this GPU has some of them; which kernel is taken goes by it, and nothing else.  Order and Starts are what the calls above write; whatever they
  * hold, nothing outside of the buffers is read or written. */
 int call_experts_up(const void* X, const void* B, const void* Scale, const void* Zeros, const void* Bias, const void* Order,

@@ -1,5 +1,5 @@
 """The experts' products and the order at the edges of what a call takes: up to eight pairs in every form, many choices a token, the
-most pairs."""
+most pairs, scales of every size."""
 
 import math
 
@@ -91,3 +91,20 @@ def test_route_of_the_most_pairs(cuda):
     assert torch.equal(ids, best.int())
     assert torch.equal(order, best.flatten().argsort(stable=True).int())
     assert torch.equal(starts[1:].long(), torch.bincount(best.flatten(), minlength=experts).cumsum(0))
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 2000])
+@pytest.mark.parametrize("byte", [0, 1, 127, 254, 255])
+def test_scales_of_every_size(cuda, tokens, byte):
+    """An MXFP4 scale is 2^(byte - 127), 2^127 at most; powers of two multiply without rounding."""
+    N, K = 32, 128
+    x = 2.0 ** (127 - byte + 3)
+    for code, value in ((1, 0.5), (2, 1.0), (3, 1.5)):
+        packed = torch.full((1, N, K // 2), code | code << 4, dtype=torch.uint8, device=cuda)
+        scale = torch.full((1, N, K // 32), byte, dtype=torch.uint8, device=cuda)
+        h = torch.zeros((tokens, K), dtype=torch.bfloat16, device=cuda)
+        h[:, 70] = x
+        ids = torch.zeros((tokens, 1), dtype=torch.int32, device=cuda)
+        order, starts = tl.experts_order(tokens, 1, 1)(ids)
+        y = tl.experts_down(tokens, 1, 1, N, K, "mxfp4")(h, packed, scale, order, starts, ids, torch.ones((tokens, 1), device=cuda))
+        assert (y == value * 2.0 ** (min(byte, 254) - 127) * x).all()
