@@ -144,3 +144,17 @@ def test_no_workspace_for_sizes_that_calls_refuse():
     code = "from tilelang_amd import _lib; lib = _lib.load_library(); print(" + ", ".join(f"lib.dq_experts_{name}_workspace_bytes(*{sizes})" for name, sizes in asked) + ")"
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=pathlib.Path(__file__).parent.parent)
     assert done.returncode == 0 and done.stdout.split() == ["0"] * len(asked), (done.returncode, done.stdout, done.stderr)
+
+
+def test_scales_that_are_not_the_codes_are_refused(monkeypatch):
+    monkeypatch.setattr(bitlinear.kernels, "bitlinear_int8xint2", lambda M, N, K, *args, **more: lambda x, weight, scale: torch.zeros((M, N), dtype=torch.float16))
+    layer = tl.BitLinear(128, 32)
+    codes = torch.zeros((2, 3, 128), dtype=torch.int8)
+    for shape in ((3, 2), (2, 3, 2), (5,), (), (2, 1, 3)):
+        with pytest.raises(ValueError, match="BitLinear: scale is"):
+            layer(codes, torch.ones(shape))
+    for bad in (torch.zeros((2, 3, 64), dtype=torch.int8), torch.zeros((2, 384), dtype=torch.int8)):
+        with pytest.raises(ValueError, match="BitLinear: codes are"):
+            layer(bad, torch.ones(bad.shape[:-1]))
+    for shape in ((2, 3), (2, 3, 1), (6,), (6, 1)):
+        assert layer(codes, torch.ones(shape)).shape == (2, 3, 32)

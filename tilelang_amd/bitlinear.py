@@ -109,16 +109,21 @@ class BitLinear(nn.Module):
                                                                      weight_fragments=self.prefill_fragments), MAX_KERNELS)
 
     def _codes_forward(self, codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+        lead = codes.shape[:-1]
+        if codes.shape[-1:] != (self.in_features,):
+            raise ValueError(f"BitLinear: codes are {tuple(codes.shape)}, not rows of {self.in_features}")
+        if scale.shape not in (lead, (*lead, 1), (lead.numel(),), (lead.numel(), 1)):
+            raise ValueError(f"BitLinear: scale is {tuple(scale.shape)}, not one for each row of codes, {tuple(codes.shape)}")
         if codes.numel() == 0:  # (a batch of no tokens: nothing to launch)
-            return codes.new_empty((*codes.shape[:-1], self.out_features), dtype=torch.float16)
-        M = codes.numel() // self.in_features
+            return codes.new_empty((*lead, self.out_features), dtype=torch.float16)
+        M = lead.numel()
         k = kept(self._codes_kernels, M, lambda: kernels.bitlinear_int8xint2(M, self.out_features, self.in_features, self._sw_value,
                                                                              interleaved=self.interleave,
                                                                              weight_fragments=self.prefill_fragments), MAX_KERNELS)
         out = k(codes.reshape(M, self.in_features).contiguous(), self.qweight, scale.reshape(M).contiguous())
         if self.bias is not None:
             out += self.bias.view(1, -1).expand_as(out)
-        return out.reshape(*codes.shape[:-1], self.out_features)
+        return out.reshape(*lead, self.out_features)
 
     def forward(self, input: torch.Tensor, scale: torch.Tensor | None = None) -> torch.Tensor:
         """``scale``: ``input`` has int8 codes already, and this is the scale of each of its rows, as an int8
