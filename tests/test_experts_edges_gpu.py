@@ -96,15 +96,15 @@ def test_route_of_the_most_pairs(cuda):
 @pytest.mark.parametrize("tokens", [1, 20, 2000])
 @pytest.mark.parametrize("byte", [0, 1, 127, 254, 255])
 def test_scales_of_every_size(cuda, tokens, byte):
-    """An MXFP4 scale is 2^(byte - 127), 2^127 at most; powers of two multiply without rounding."""
+    """An MXFP4 scale is 2^(byte - 127), 2^127 at most; powers of two multiply without rounding.  (2^130 is an infinity in bf16.)"""
     N, K = 32, 128
-    x = 2.0 ** (127 - byte + 3)
-    for code, value in ((1, 0.5), (2, 1.0), (3, 1.5)):
-        packed = torch.full((1, N, K // 2), code | code << 4, dtype=torch.uint8, device=cuda)
-        scale = torch.full((1, N, K // 32), byte, dtype=torch.uint8, device=cuda)
-        h = torch.zeros((tokens, K), dtype=torch.bfloat16, device=cuda)
-        h[:, 70] = x
-        ids = torch.zeros((tokens, 1), dtype=torch.int32, device=cuda)
-        order, starts = tl.experts_order(tokens, 1, 1)(ids)
-        y = tl.experts_down(tokens, 1, 1, N, K, "mxfp4")(h, packed, scale, order, starts, ids, torch.ones((tokens, 1), device=cuda))
-        assert (y == value * 2.0 ** (min(byte, 254) - 127) * x).all()
+    ids = torch.zeros((tokens, 1), dtype=torch.int32, device=cuda)
+    order, starts = tl.experts_order(tokens, 1, 1)(ids)
+    for x in (2.0 ** (127 - byte + 3), 2.0 ** round(0.75 * (127 - byte))):
+        for code, value in ((1, 0.5), (2, 1.0), (3, 1.5)):
+            packed = torch.full((1, N, K // 2), code | code << 4, dtype=torch.uint8, device=cuda)
+            scale = torch.full((1, N, K // 32), byte, dtype=torch.uint8, device=cuda)
+            h = torch.zeros((tokens, K), dtype=torch.bfloat16, device=cuda)
+            h[:, 70] = x
+            y = tl.experts_down(tokens, 1, 1, N, K, "mxfp4")(h, packed, scale, order, starts, ids, torch.ones((tokens, 1), device=cuda))
+            assert (y.double() == value * 2.0 ** (min(byte, 254) - 127) * float(h[0, 70])).all()
