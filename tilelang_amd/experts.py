@@ -60,7 +60,7 @@ class RMSNorm(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
         lead, dtype = x.shape[:-1], self.weight.dtype
-        if residual is not None:
+        if residual is not None and residual.shape != x.shape:
             _check_rows("RMSNorm", "residual", residual, x, self.dim)
         rows = x if x.dim() == 2 else x.reshape(lead.numel(), x.shape[-1])
         if rows.dtype != dtype:
@@ -197,9 +197,12 @@ class W4Experts(nn.Module):
         """``x`` ``[..., hidden]`` -> the same; ``residual`` of that shape is added in the same launch.  ``logits`` fp32 ``[..., experts]``: in place of
         the router's."""
         dtype = self.router.dtype
-        for name, t, width in (("x", x, self.hidden), ("residual", residual, self.hidden), ("logits", logits, self.experts)):
-            if t is not None:
-                _check_rows("W4Experts", name, t, x, width)
+        if x.shape[-1] != self.hidden:
+            _check_rows("W4Experts", "x", x, x, self.hidden)
+        if residual is not None and residual.shape != x.shape:
+            _check_rows("W4Experts", "residual", residual, x, self.hidden)
+        if logits is not None:
+            _check_rows("W4Experts", "logits", logits, x, self.experts)
         if x.numel() == 0:  # (a batch of no tokens: nothing to launch)
             return x.new_empty(x.shape, dtype=dtype)
         rows = _whole(x.to(dtype).reshape(-1, self.hidden))
