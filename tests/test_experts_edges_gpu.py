@@ -108,3 +108,25 @@ def test_scales_of_every_size(cuda, tokens, byte):
             h[:, 70] = x
             y = tl.experts_down(tokens, 1, 1, N, K, "mxfp4")(h, packed, scale, order, starts, ids, torch.ones((tokens, 1), device=cuda))
             assert (y.double() == value * 2.0 ** (min(byte, 254) - 127) * float(h[0, 70])).all()
+
+
+@pytest.mark.parametrize("weight_format", ["uint4", "mxfp4"])
+@pytest.mark.parametrize("tokens", [1, 9, 40, 700])
+@pytest.mark.parametrize("N", [32, 96, 160, 288, 416])
+def test_columns_in_blocks_of_32(cuda, N, tokens, weight_format):
+    """N that is an odd number of blocks of 32: a tile's last blocks are not there."""
+    print(f"experts {tokens} N={N} {weight_format}", flush=True)
+    gen = torch.Generator().manual_seed(N + tokens)
+    experts, top_k, K = 5, 2, 384
+    ids = torch.rand((tokens, experts), generator=gen).argsort(dim=1)[:, :top_k].int().contiguous()
+    order, starts = ref.order(ids, experts)
+    got = order.to(cuda), starts.to(cuda)
+    w = ref.Weights(gen, experts, 2 * N, K, weight_format, with_bias=True, device=cuda)
+    x = torch.randn((tokens, K), generator=gen).to(w.dtype)
+    h = tl.experts_up(tokens, experts, top_k, N, K, weight_format, activation="gelu", with_bias=True)(x.to(cuda), *w.on_device, *got)
+    assert ref.agrees(h, *ref.up(x, w, order, starts, top_k, N, "gelu"), w.dtype)
+    d = ref.Weights(gen, experts, N, K, weight_format, with_bias=True, device=cuda)
+    h = torch.randn((tokens * top_k, K), generator=gen).to(d.dtype)
+    weights, r = torch.rand((tokens, top_k), generator=gen), torch.randn((tokens, N), generator=gen).to(d.dtype)
+    y = tl.experts_down(tokens, experts, top_k, N, K, weight_format, with_bias=True, residual=True)(h.to(cuda), *d.on_device, *got, ids.to(cuda), weights.to(cuda), r.to(cuda))
+    assert ref.agrees(y, *ref.down(h, d, order, starts, weights, tokens, r), d.dtype)
