@@ -68,7 +68,7 @@ def kept(held: dict, key, make, most: int):
     if found is None:
         found = make()
         while len(held) >= most:
-            del held[next(iter(held))]
+            held.pop(next(iter(held)), None)  # (None: another thread has been here)
     held[key] = found  # (the last in the order)
     return found
 
