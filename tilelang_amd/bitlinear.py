@@ -127,7 +127,7 @@ class BitLinear(nn.Module):
 
     def forward(self, input: torch.Tensor, scale: torch.Tensor | None = None) -> torch.Tensor:
         """``scale``: ``input`` has int8 codes already, and this is the scale of each of its rows, as an int8
-        :class:`~tilelang_amd.experts.RMSNorm` returns them."""
+        :class:`~tilelang_amd.experts.RMSNorm` returns them (of no rows: no rows)."""
         if scale is not None:
             return self._codes_forward(input, scale)
         flat = input.dim() == 2 and input.shape[1] == self.in_features

@@ -10,8 +10,8 @@
 // operations are carried out in their order, so there is no barrier.  The waves' sums meet in LDS at the end.
 //
 // Measured: one token, 8 of 128 experts, 1024 x 4096 uint4 "up" 10 us (3.4 TB/s; 17 with words straight into registers), 4096 x 1024 "down"
-// 9; 64 tokens, 4 of 32 experts, 2880 x 2880 MXFP4 61 to 68 and 37 us (4.3 and 3.9 TB/s: rows end inside cache lines, where lines are whole
-// it reaches 5.7).
+// 9; 64 tokens, 4 of 32 experts, 2880 x 2880 MXFP4 61 to 72 and 38 to 41 us (4.0 to 4.6 and 3.5 to 3.7 TB/s: rows end inside cache lines,
+// where lines are whole it reaches 5.7).
 #include "dq_experts.h"
 
 #include <math.h>

@@ -7,7 +7,7 @@
 // and no barrier, or all of a workgroup of 256 or 1024, whose waves meet in LDS once a reduction.
 //
 // Measured: 7999 x 5120 bf16 with a residual 63 us, 5.2 TB/s, what a copy reaches here; 2048 x 8192 fp16 with a residual to int8 23.5 us,
-// 5.0 TB/s; one row of 4096 2.8 us, of which an empty launch is 2.0.
+// 5.0 TB/s; one row of 4096 2.3 to 2.5 us, of which an empty launch is 2.0.
 #include "dq_kv.h"
 
 namespace dq {

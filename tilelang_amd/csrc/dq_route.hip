@@ -12,7 +12,7 @@
 // atomics are counts in LDS.
 //
 // What bounds it is instructions, a choice after the other.  Measured: one token, 8 of 128 5.6 us in one launch; 1021 tokens, 4 of 60
-// 5.8 us and 5.5 for the order; 8192 tokens, 8 of 256 in 4 of 8 groups with biases 24 and 8.2 (25 in all without biases, where nothing
+// 5.8 us and 5.5 for the order; 8192 tokens, 8 of 256 in 4 of 8 groups with biases 23 to 24 and 7.9 (25 in all without biases, where nothing
 // is done in 64 bits: one token that is adds 3, being the last).
 #include "dq_kv.h"
 

@@ -48,7 +48,8 @@ class RMSNorm(nn.Module):
 
     ``norm(x)`` is ``y``; ``norm(x, residual)`` is ``(y, x + residual)``, the norm that of the sum before it is rounded.  ``int8``: in place of ``y``
     come ``(codes, scale)``, which :class:`~tilelang_amd.bitlinear.BitLinear` takes: ``norm(x)`` is ``(codes, scale)``, ``norm(x, residual)``
-    ``(codes, scale, x + residual)``.  Rows of ``x`` may lie apart (a slice of a wider projection's columns).
+    ``(codes, scale, x + residual)``.  Rows of ``x`` may lie apart (a slice of a wider projection's columns).  ``residual`` has ``x``'s shape, or one
+    of them is flat, a row a token.  A batch of no tokens has results of no rows.
     """
 
     def __init__(self, dim: int, eps: float = 1e-6, dtype=torch.float16, int8: bool = False):
@@ -195,7 +196,7 @@ class W4Experts(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, logits: torch.Tensor | None = None) -> torch.Tensor:
         """``x`` ``[..., hidden]`` -> the same; ``residual`` of that shape is added in the same launch.  ``logits`` fp32 ``[..., experts]``: in place of
-        the router's."""
+        the router's.  (Either may be flat, a row a token.)  A batch of no tokens has a result of no rows."""
         dtype = self.router.dtype
         if x.shape[-1] != self.hidden:
             _check_rows("W4Experts", "x", x, x, self.hidden)
